@@ -5,7 +5,7 @@ this package is the Python mirror of the reference's operator surface
 (crates/burn_automata_kernels and NpaModel / run_rollout of crates/burn_automata).
 """
 
-from .config import (Boundary, EquivarianceMode, GaussianDecodeConfig, GaussianDecodeMode,
+from .config import (Activation, Boundary, EquivarianceMode, GaussianDecodeConfig, GaussianDecodeMode,
                      HashGridConfig, HashGridMode, KernelError, NpaConfig, PerceptionOptions,
                      Splat2dConfig,
                      feature_dims)
@@ -13,6 +13,8 @@ from .kernels import (DevicePerception, Gaussian3d, HashGridSnapshot, Perception
                       decode_gaussians_3d, decode_gaussians_3d_records, euler_step, perceive,
                       perceive_adjoint_with_options, perceive_state_adjoint_with_options,
                       perceive_with_options, splat_particles_2d)
+from .layers import (LayerNormGradients, LayerNormOutput, LinearGradients, LinearOutput,
+                     layer_norm, layer_norm_backward, linear, linear_backward)
 from .model import (CudaAutomataExecutor, NpaModel, NpaWeights, RolloutConfig, RolloutTrace,
                     StepOutput, rollout_update_masks, run_rollout_from_particles)
 from . import bpk
@@ -25,5 +27,7 @@ __all__ = [
     "decode_gaussians_3d", "decode_gaussians_3d_records", "euler_step", "perceive",
     "perceive_with_options", "CudaAutomataExecutor", "NpaModel", "NpaWeights", "RolloutConfig",
     "RolloutTrace", "StepOutput", "rollout_update_masks", "run_rollout_from_particles",
+    "Activation", "LayerNormGradients", "LayerNormOutput", "LinearGradients", "LinearOutput",
+    "layer_norm", "layer_norm_backward", "linear", "linear_backward",
     "build_library", "load_library",
 ]

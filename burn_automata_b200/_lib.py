@@ -147,6 +147,22 @@ SIGNATURES = [
     ("npa_dev_model_step", c_i32,
      [vp, P(GridConfigC), vp, vp, c_i64, c_i64, c_f32, vp, vp, vp, vp, vp, vp, vp, vp,
       ctypes.c_size_t, vp]),
+    ("npa_dev_layer_norm", c_i32,
+     [c_i32, vp, c_i64, vp, vp, c_i64, c_i64, c_f32, vp, c_i64, vp, vp, vp]),
+    ("npa_dev_layer_norm_backward_workspace_size", c_i32,
+     [c_i32, c_i64, c_i64, P(ctypes.c_size_t)]),
+    ("npa_dev_layer_norm_backward", c_i32,
+     [c_i32, vp, c_i64, vp, c_i64, vp, vp, vp, vp, c_i64, c_i64, c_i64, vp, c_i64, vp, vp, vp,
+      ctypes.c_size_t, vp]),
+    ("npa_dev_linear_workspace_size", c_i32, [c_i32, c_i64, c_i64, c_i64, P(ctypes.c_size_t)]),
+    ("npa_dev_linear", c_i32,
+     [c_i32, c_i32, vp, c_i64, vp, c_i64, vp, vp, c_i64, c_i64, c_i64, c_i64, vp, c_i64, vp,
+      c_i64, vp, ctypes.c_size_t, vp]),
+    ("npa_dev_linear_backward_workspace_size", c_i32,
+     [c_i32, c_i32, c_i64, c_i64, c_i64, P(ctypes.c_size_t)]),
+    ("npa_dev_linear_backward", c_i32,
+     [c_i32, c_i32, vp, c_i64, vp, c_i64, vp, c_i64, vp, c_i64, c_i64, c_i64, c_i64, vp, c_i64,
+      vp, vp, vp, ctypes.c_size_t, vp]),
     ("npa_executor_create", c_i32, [vp, P(GridConfigC), c_i64, c_i64, P(vp)]),
     ("npa_executor_destroy", None, [vp]),
     ("npa_executor_upload_state", c_i32, [vp, f32p, f32p]),

@@ -41,6 +41,17 @@ class GaussianDecodeMode(enum.IntEnum):
     GaussianSh0Oriented = 3
 
 
+class Activation(enum.IntEnum):
+    """Activations of the linear operator (layers.py); no counterpart in the
+    reference, whose update MLP is relu only."""
+
+    Identity = 0
+    Relu = 1
+    Gelu = 2
+    GeluTanh = 3
+    Silu = 4
+
+
 # Status codes of the C ABI (include/npa_b200.h); 1..9 map 1:1 onto KernelError /
 # AutomataError variants of the reference.
 STATUS_NAMES = {

@@ -33,9 +33,7 @@ npa_status fail(npa_status st, const std::string& msg) {
   return st;
 }
 
-// fail() with the payload the reference's KernelError variant carries.
-npa_status fail_with(npa_status st, const std::string& msg, int64_t a, int64_t b = 0,
-                     float eps = 0.0f) {
+npa_status fail_with(npa_status st, const std::string& msg, int64_t a, int64_t b, float eps) {
   set_error(msg);
   g_last_detail = npa_error_detail{st, eps, a, b};
   return st;

@@ -1,0 +1,116 @@
+// layers.h -- storage types, activations and launchers of the normalised-linear
+// operators (layer_norm.cu, linear.cu; entry points in capi_layers.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "npa_internal.h"
+
+namespace npa {
+
+template <class T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Results are rounded to the storage type once, to nearest even.
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// VEC consecutive values, loaded and stored as one access.
+template <class T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+inline size_t dtype_bytes(int dtype) { return dtype == NPA_DTYPE_F32 ? 4 : 2; }
+
+struct LayerNormArgs {
+  const void* x;
+  int64_t x_stride;
+  const void* weight;  // optional
+  const void* bias;    // optional
+  int64_t rows;
+  int dims;
+  float eps;
+  void* y;
+  int64_t y_stride;
+  float* mean;  // optional
+  float* rstd;  // optional
+};
+npa_status launch_layer_norm(int dtype, const LayerNormArgs& a, cudaStream_t stream);
+
+struct LayerNormBackwardArgs {
+  const void* dy;
+  int64_t dy_stride;
+  const void* x;
+  int64_t x_stride;
+  const float* mean;
+  const float* rstd;
+  const void* weight;    // optional
+  const void* residual;  // optional: added to dx
+  int64_t residual_stride;
+  int64_t rows;
+  int dims;
+  void* dx;  // optional
+  int64_t dx_stride;
+  void* dweight;  // optional
+  void* dbias;    // optional
+  float* partials;
+};
+size_t layer_norm_backward_workspace(int64_t rows, int dims);
+npa_status launch_layer_norm_backward(int dtype, const LayerNormBackwardArgs& a,
+                                      cudaStream_t stream);
+
+struct LinearArgs {
+  const void* x;
+  int64_t x_stride;
+  const void* weight;
+  int64_t weight_stride;
+  const void* bias;      // optional
+  const void* residual;  // optional
+  int64_t residual_stride;
+  int64_t rows;
+  int inputs, outputs;
+  void* y;
+  int64_t y_stride;
+  void* z;  // optional
+  int64_t z_stride;
+  int activation;
+};
+size_t linear_workspace(int dtype, int64_t rows, int inputs, int outputs);
+npa_status launch_linear(int dtype, const LinearArgs& a, void* workspace, cudaStream_t stream);
+
+struct LinearBackwardArgs {
+  const void* dy;
+  int64_t dy_stride;
+  const void* x;
+  int64_t x_stride;
+  const void* weight;
+  int64_t weight_stride;
+  const void* z;  // null for the identity
+  int64_t z_stride;
+  int64_t rows;
+  int inputs, outputs;
+  void* dx;  // optional
+  int64_t dx_stride;
+  void* dweight;  // optional
+  void* dbias;    // optional
+  int activation;
+};
+size_t linear_backward_workspace(int dtype, int activation, int64_t rows, int inputs, int outputs);
+npa_status launch_linear_backward(int dtype, const LinearBackwardArgs& a, void* workspace,
+                                  cudaStream_t stream);
+
+}  // namespace npa

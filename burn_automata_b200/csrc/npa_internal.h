@@ -15,6 +15,9 @@ namespace npa {
 // Thread-local last-error text (npa_last_error_message).
 void set_error(const std::string& msg);
 npa_status fail(npa_status st, const std::string& msg);
+// fail() with the payload the reference's KernelError variant carries.
+npa_status fail_with(npa_status st, const std::string& msg, int64_t a, int64_t b = 0,
+                     float eps = 0.0f);
 // Maps a CUDA error to NPA_ERR_CUDA / NPA_ERR_OUT_OF_MEMORY with its text.
 npa_status cuda_fail(cudaError_t err, const char* what);
 // Counts kernel launches (npa_kernel_launch_count) and checks the launch.

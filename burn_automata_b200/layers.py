@@ -1,0 +1,292 @@
+"""Layer norm and the linear layer with its epilogue, forward and backward.
+
+The layers of a per-particle update block on torch CUDA tensors (float32,
+float16 or bfloat16), enqueued on the current torch stream of the tensors'
+device through the npa_dev_* entry points.  They have no counterpart in the
+reference, whose update MLP is a fixed relu pair of at most 256 hidden units
+(NpaModel); they take any width.
+
+Inputs are [..., width]; leading axes are rows.  A 2-D column range of a wider
+tensor is read in place; other layouts are copied to rows first.  A caller that
+hands over tensors allocated on another stream orders the streams itself, as
+for any torch operation.  Gradients are explicit calls (as training.py's);
+autograd does not see them.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+from . import _lib
+from .config import Activation, InvalidArgument
+
+
+@dataclass
+class LayerNormOutput:
+    """y as the input's shape; mean and rstd are float32 [rows...]."""
+
+    y: "torch.Tensor"
+    mean: "torch.Tensor"
+    rstd: "torch.Tensor"
+
+
+@dataclass
+class LayerNormGradients:
+    """Gradients of layer_norm's x, weight and bias (None where not needed)."""
+
+    x: Optional["torch.Tensor"]
+    weight: Optional["torch.Tensor"]
+    bias: Optional["torch.Tensor"]
+
+
+@dataclass
+class LinearOutput:
+    """y and, when it was asked for, the pre-activation z."""
+
+    y: "torch.Tensor"
+    pre_activation: Optional["torch.Tensor"]
+
+
+@dataclass
+class LinearGradients:
+    """Gradients of linear's x, weight and bias (None where not needed).  The
+    residual's gradient is dy itself."""
+
+    x: Optional["torch.Tensor"]
+    weight: Optional["torch.Tensor"]
+    bias: Optional["torch.Tensor"]
+
+
+_torch = None
+_dtypes = {}
+
+
+def _t():
+    global _torch
+    if _torch is None:
+        import torch
+
+        _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        _torch = torch
+    return _torch
+
+
+def _dtype(x, name: str) -> int:
+    """The C ABI's storage type of a CUDA tensor."""
+    torch = _t()
+    if not isinstance(x, torch.Tensor):
+        raise InvalidArgument(f"{name} must be a torch tensor")
+    code = _dtypes.get(x.dtype)
+    if code is None:
+        raise InvalidArgument(f"{name} must be float32, float16 or bfloat16, got {x.dtype}")
+    if not x.is_cuda:
+        raise InvalidArgument(f"{name} must be a CUDA tensor")
+    if x.dim() < 1:
+        raise InvalidArgument(f"{name} needs at least one axis")
+    return code
+
+
+def _like(t, x, name: str):
+    if not isinstance(t, type(x)) and not isinstance(t, _t().Tensor):
+        raise InvalidArgument(f"{name} must be a torch tensor")
+    if t.dtype != x.dtype or t.device != x.device:
+        raise InvalidArgument(f"{name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
+
+
+def _rows(t):
+    """(tensor, row stride) with unit stride inside rows: the tensor itself for
+    a contiguous tensor or a 2-D column range, else a contiguous copy."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t, t.stride(0)
+    return t.contiguous(), t.shape[-1]
+
+
+def _matrix(t, x, shape, name: str):
+    _like(t, x, name)
+    if t.shape != shape:
+        raise InvalidArgument(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return _rows(t)
+
+
+def _vector(t, x, size: int, name: str):
+    if t is None:
+        return None
+    _like(t, x, name)
+    if t.dim() != 1 or t.shape[0] != size:
+        raise InvalidArgument(f"{name} has shape {tuple(t.shape)}, expected ({size},)")
+    return t.contiguous()
+
+
+def _statistic(t, x, name: str):
+    if not isinstance(t, _t().Tensor) or t.dtype != _torch.float32 or t.device != x.device:
+        raise InvalidArgument(f"{name} must be a float32 tensor on {x.device}")
+    if t.shape != x.shape[:-1]:
+        raise InvalidArgument(f"{name} has shape {tuple(t.shape)}, expected "
+                              f"{tuple(x.shape[:-1])}")
+    return t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _needs(needs, weight_given: bool = True):
+    want = set(needs)
+    if not want <= {"x", "weight", "bias"}:
+        raise InvalidArgument(f"needs may name x, weight and bias, got {sorted(want)}")
+    return want
+
+
+class _on_device:
+    """The launching thread's current device for one call."""
+
+    def __init__(self, device):
+        self.device = device
+        self.guard = None
+
+    def __enter__(self):
+        torch = _torch
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> LayerNormOutput:
+    """(x - mean) * rstd * weight + bias over the last axis, with the mean and
+    rstd that layer_norm_backward takes."""
+    code = _dtype(x, "x")
+    torch = _torch
+    dims = x.shape[-1]
+    w, b = _vector(weight, x, dims, "weight"), _vector(bias, x, dims, "bias")
+    xr, xs = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    with _on_device(x.device) as stream:
+        _lib.check(_lib.lib().npa_dev_layer_norm(
+            code, xr.data_ptr(), xs, _ptr(w), _ptr(b), mean.numel(), dims, float(eps),
+            y.data_ptr(), dims, mean.data_ptr(), rstd.data_ptr(), stream), "layer_norm")
+    return LayerNormOutput(y, mean, rstd)
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, residual_gradient=None,
+                        needs=None) -> LayerNormGradients:
+    """The gradients of layer_norm given dy and its saved statistics.
+    residual_gradient, the gradient that reaches x over a skip connection, is
+    added to x's on the way.  `needs` names the gradients to compute: x,
+    weight and bias by default, x alone when there is no weight."""
+    code = _dtype(x, "x")
+    torch = _torch
+    dims = x.shape[-1]
+    want = _needs(needs if needs is not None else
+                  (("x", "weight", "bias") if weight is not None else ("x",)))
+    w = _vector(weight, x, dims, "weight")
+    dyr, dys = _matrix(dy, x, x.shape, "dy")
+    xr, xs = _rows(x)
+    m, r = _statistic(mean, x, "mean"), _statistic(rstd, x, "rstd")
+    rr, rs = (None, 0) if residual_gradient is None else _matrix(
+        residual_gradient, x, x.shape, "residual_gradient")
+    if rr is not None and "x" not in want:
+        raise InvalidArgument("residual_gradient is added to x's gradient, which is not needed")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if "x" in want else None
+    dw = torch.empty(dims, dtype=x.dtype, device=x.device) if "weight" in want else None
+    db = torch.empty(dims, dtype=x.dtype, device=x.device) if "bias" in want else None
+    rows = m.numel()
+    L = _lib.lib()
+    with _on_device(x.device) as stream:
+        ws, ws_bytes = None, 0
+        if dw is not None or db is not None:
+            need = ctypes.c_size_t(0)
+            _lib.check(L.npa_dev_layer_norm_backward_workspace_size(
+                code, rows, dims, ctypes.byref(need)), "layer_norm_backward")
+            ws_bytes = need.value
+            ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=x.device)
+        _lib.check(L.npa_dev_layer_norm_backward(
+            code, dyr.data_ptr(), dys, xr.data_ptr(), xs, m.data_ptr(), r.data_ptr(), _ptr(w),
+            _ptr(rr), rs, rows, dims, _ptr(dx), dims, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes,
+            stream), "layer_norm_backward")
+    return LayerNormGradients(dx, dw, db)
+
+
+def _layer_shape(x, weight):
+    if not isinstance(weight, _t().Tensor) or weight.dim() != 2:
+        raise InvalidArgument("weight must be a 2-D tensor [outputs, inputs]")
+    if weight.shape[1] != x.shape[-1]:
+        raise InvalidArgument(f"weight has {weight.shape[1]} inputs, x has {x.shape[-1]}")
+    return weight.shape[1], weight.shape[0]
+
+
+def linear(x, weight, bias=None, residual=None, activation: Activation = Activation.Identity,
+           save_pre_activation: bool = False) -> LinearOutput:
+    """activation(x weight^T + bias) + residual, weight [outputs, inputs].
+    save_pre_activation also returns z = x weight^T + bias, which
+    linear_backward reads for every activation but the identity."""
+    code = _dtype(x, "x")
+    torch = _torch
+    inputs, outputs = _layer_shape(x, weight)
+    out_shape = x.shape[:-1] + (outputs,)
+    wr, wstride = _matrix(weight, x, weight.shape, "weight")
+    b = _vector(bias, x, outputs, "bias")
+    rr, rs = (None, 0) if residual is None else _matrix(residual, x, out_shape, "residual")
+    xr, xs = _rows(x)
+    rows = x.numel() // inputs if inputs else 0
+    y = torch.empty(out_shape, dtype=x.dtype, device=x.device)
+    z = torch.empty_like(y) if save_pre_activation else None
+    L = _lib.lib()
+    with _on_device(x.device) as stream:
+        need = ctypes.c_size_t(0)
+        _lib.check(L.npa_dev_linear_workspace_size(code, rows, inputs, outputs,
+                                                   ctypes.byref(need)), "linear")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
+        _lib.check(L.npa_dev_linear(
+            code, int(activation), xr.data_ptr(), xs, wr.data_ptr(), wstride, _ptr(b), _ptr(rr),
+            rs, rows, inputs, outputs, y.data_ptr(), outputs, _ptr(z), outputs, _ptr(ws),
+            need.value, stream), "linear")
+    return LinearOutput(y, z)
+
+
+def linear_backward(dy, x, weight, pre_activation=None,
+                    activation: Activation = Activation.Identity,
+                    needs=("x", "weight", "bias")) -> LinearGradients:
+    """The gradients of linear given dy and (for every activation but the
+    identity) its saved pre-activation.  `needs` names the gradients to
+    compute."""
+    code = _dtype(x, "x")
+    torch = _torch
+    inputs, outputs = _layer_shape(x, weight)
+    out_shape = x.shape[:-1] + (outputs,)
+    want = _needs(needs)
+    wr, wstride = _matrix(weight, x, weight.shape, "weight")
+    dyr, dys = _matrix(dy, x, out_shape, "dy")
+    zr, zs = None, 0
+    if int(activation) != Activation.Identity:
+        if pre_activation is None:
+            raise InvalidArgument("this activation's gradient needs pre_activation")
+        zr, zs = _matrix(pre_activation, x, out_shape, "pre_activation")
+    xr, xs = _rows(x)
+    rows = x.numel() // inputs if inputs else 0
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if "x" in want else None
+    dw = (torch.empty(weight.shape, dtype=x.dtype, device=x.device) if "weight" in want
+          else None)
+    db = torch.empty(outputs, dtype=x.dtype, device=x.device) if "bias" in want else None
+    L = _lib.lib()
+    with _on_device(x.device) as stream:
+        need = ctypes.c_size_t(0)
+        _lib.check(L.npa_dev_linear_backward_workspace_size(
+            code, int(activation), rows, inputs, outputs, ctypes.byref(need)), "linear_backward")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
+        _lib.check(L.npa_dev_linear_backward(
+            code, int(activation), dyr.data_ptr(), dys, xr.data_ptr(), xs, wr.data_ptr(), wstride,
+            _ptr(zr), zs, rows, inputs, outputs, _ptr(dx), inputs, _ptr(dw), _ptr(db), _ptr(ws),
+            need.value, stream), "linear_backward")
+    return LinearGradients(dx, dw, db)

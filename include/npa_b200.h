@@ -520,6 +520,94 @@ npa_status npa_dev_model_step(npa_model* model, const npa_grid_config* grid,
                               void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* Normalised-linear operators: layer norm and matrix product           */
+/* ------------------------------------------------------------------ */
+
+/* The two layers of a per-particle update block, forward and backward, on
+ * device buffers.  They stand beside the f32 MLP of npa_model_step (whose
+ * operation order is the reference's and whose hidden width ends at 256): any
+ * width, three storage types, and no claim on the reference's rounding.
+ *
+ * Matrices are row-major; `*_stride` is the distance between rows in elements
+ * (at least the row's width), so a column range of a wider buffer may be
+ * passed.  Every matrix and vector of a call has the storage type `dtype`;
+ * sums, statistics and products are held in 32 bits and results are rounded
+ * once.  NULL leaves an optional buffer out.  Outputs must not overlap inputs
+ * or each other.  rows = 0 is valid (gradients over rows are then zero).
+ * Results do not depend on timing: no sum goes through atomics. */
+enum { NPA_DTYPE_F32 = 0, NPA_DTYPE_F16 = 1, NPA_DTYPE_BF16 = 2 };
+
+/* identity; max(z, 0); z Phi(z); the tanh form of z Phi(z); z / (1 + e^-z). */
+enum {
+  NPA_ACTIVATION_IDENTITY = 0,
+  NPA_ACTIVATION_RELU = 1,
+  NPA_ACTIVATION_GELU = 2,
+  NPA_ACTIVATION_GELU_TANH = 3,
+  NPA_ACTIVATION_SILU = 4
+};
+
+/* y = (x - mean) * rstd * weight + bias for each of `rows` rows of `dims`
+ * values, mean = sum(x) / dims, rstd = 1 / sqrt(sum((x - mean)^2) / dims + eps).
+ * weight, bias [dims], mean and rstd [rows] (f32) are optional.  eps must be
+ * finite and positive (NPA_ERR_INVALID_EPS). */
+npa_status npa_dev_layer_norm(int32_t dtype, const void* d_x, int64_t x_stride,
+                              const void* d_weight, const void* d_bias, int64_t rows, int64_t dims,
+                              float eps, void* d_y, int64_t y_stride, float* d_mean, float* d_rstd,
+                              void* stream);
+
+/* Workspace bytes of npa_dev_layer_norm_backward (with parameter gradients). */
+npa_status npa_dev_layer_norm_backward_workspace_size(int32_t dtype, int64_t rows, int64_t dims,
+                                                      size_t* bytes);
+/* The gradients of npa_dev_layer_norm from dy and the saved mean and rstd.
+ * With xhat = (x - mean) * rstd and g = dy * weight:
+ *   dx      = rstd * (g - sum(g) / dims - xhat * sum(g * xhat) / dims)
+ *             + residual_gradient
+ *   dweight = sum over rows of dy * xhat,  dbias = sum over rows of dy.
+ * residual_gradient (the gradient that reaches x past the norm, over a skip
+ * connection) and each output are optional. */
+npa_status npa_dev_layer_norm_backward(int32_t dtype, const void* d_dy, int64_t dy_stride,
+                                       const void* d_x, int64_t x_stride, const float* d_mean,
+                                       const float* d_rstd, const void* d_weight,
+                                       const void* d_residual_gradient,
+                                       int64_t residual_gradient_stride, int64_t rows, int64_t dims,
+                                       void* d_dx, int64_t dx_stride, void* d_dweight,
+                                       void* d_dbias, void* d_workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* Workspace bytes of npa_dev_linear. */
+npa_status npa_dev_linear_workspace_size(int32_t dtype, int64_t rows, int64_t inputs,
+                                         int64_t outputs, size_t* bytes);
+/* z = x weight^T + bias, y = activation(z) + residual: x [rows][inputs],
+ * weight [outputs][inputs] (as w1 / w2 of npa_model_create), y, residual and
+ * pre_activation (z) [rows][outputs].  bias, residual and pre_activation are
+ * optional. */
+npa_status npa_dev_linear(int32_t dtype, int32_t activation, const void* d_x, int64_t x_stride,
+                          const void* d_weight, int64_t weight_stride, const void* d_bias,
+                          const void* d_residual, int64_t residual_stride, int64_t rows,
+                          int64_t inputs, int64_t outputs, void* d_y, int64_t y_stride,
+                          void* d_pre_activation, int64_t pre_activation_stride,
+                          void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of npa_dev_linear_backward. */
+npa_status npa_dev_linear_backward_workspace_size(int32_t dtype, int32_t activation, int64_t rows,
+                                                  int64_t inputs, int64_t outputs, size_t* bytes);
+/* The gradients of npa_dev_linear from dy [rows][outputs] and the saved z.
+ * With dz = dy * activation'(z) (dz = dy for the identity, where
+ * pre_activation is not read):
+ *   dx = dz weight,  dweight = dz^T x [outputs][inputs],  dbias = sum over
+ *   rows of dz.  The residual's gradient is dy itself.
+ * Each output is optional; weight is read for dx only and x for dweight only.
+ * 16-bit types round dz to the storage type for the two products (their sums
+ * stay in 32 bits); dbias sums dz unrounded. */
+npa_status npa_dev_linear_backward(int32_t dtype, int32_t activation, const void* d_dy,
+                                   int64_t dy_stride, const void* d_x, int64_t x_stride,
+                                   const void* d_weight, int64_t weight_stride,
+                                   const void* d_pre_activation, int64_t pre_activation_stride,
+                                   int64_t rows, int64_t inputs, int64_t outputs, void* d_dx,
+                                   int64_t dx_stride, void* d_dweight, void* d_dbias,
+                                   void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Executor: resident rollout state (the CUDA counterpart of            */
 /* WgpuAutomataExecutor, crates/burn_automata/src/gpu/executor/*)      */
 /* ------------------------------------------------------------------ */
