@@ -17,7 +17,7 @@
 #include <string>
 #include <vector>
 
-#include "npa_internal.h"
+#include "layers.h"
 
 namespace npa {
 
@@ -529,7 +529,9 @@ npa_status npa_last_error_detail(npa_error_detail* out) {
 
 uint64_t npa_kernel_launch_count(void) { return g_launches.load(); }
 
-uint64_t npa_bulk_copy_timeouts(void) { return bulk_copy_timeouts() + ws_step_timeouts(); }
+uint64_t npa_bulk_copy_timeouts(void) {
+  return bulk_copy_timeouts() + ws_step_timeouts() + linear_timeouts();
+}
 
 npa_status npa_prepare_host_tables(int64_t* ln_1p_exceptions) {
   NPA_TRY(prepare_host_log1p());

@@ -89,6 +89,8 @@ struct LinearArgs {
   int64_t z_stride;
   int activation;
 };
+// Bounded waits of the product kernels that gave up on the current device.
+uint64_t linear_timeouts();
 size_t linear_workspace(int dtype, int64_t rows, int inputs, int outputs);
 npa_status launch_linear(int dtype, const LinearArgs& a, void* workspace, cudaStream_t stream);
 

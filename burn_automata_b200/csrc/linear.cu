@@ -3,198 +3,320 @@
 //
 //   z = x W^T + b,  y = act(z) + r;  dz = dy act'(z),
 //   dx = dz W,  dW = dz^T x,  db = sum over rows of dz.
+// The three products run on product_kernel (linear_product.cuh); the sums over
+// rows that give db, and dz itself, come from slope_kernel.
 #include <algorithm>
 
-#include "layers.h"
+#include "linear_product.cuh"
 
 namespace npa {
 namespace {
 
-__device__ __forceinline__ float activate(float z, int act) {
-  switch (act) {
-    case NPA_ACTIVATION_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-    case NPA_ACTIVATION_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case NPA_ACTIVATION_GELU_TANH:
-      return 0.5f * z * (1.0f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
-    case NPA_ACTIVATION_SILU: return z / (1.0f + expf(-z));
-    default: return z;
-  }
-}
+using linear_tc::Operand;
+using linear_tc::Product;
 
-__device__ __forceinline__ float activation_slope(float z, int act) {
-  switch (act) {
-    case NPA_ACTIVATION_RELU: return z <= 0.0f ? 0.0f : 1.0f;
-    case NPA_ACTIVATION_GELU:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-             z * 0.39894228040143268f * expf(-0.5f * z * z);
-    case NPA_ACTIVATION_GELU_TANH: {
-      const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
-      return 0.5f * (1.0f + t) +
-             0.5f * z * (1.0f - t * t) * 0.79788456080286536f * (1.0f + 0.134145f * z * z);
-    }
-    case NPA_ACTIVATION_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
-      return s * (1.0f + z * (1.0f - s));
-    }
-    default: return 1.0f;
-  }
-}
-
-// One operand of a product: value (i, k) at i * si + k * sk.
-struct Operand {
-  const void* p;
-  int64_t si, sk;
-};
-struct Product {
-  Operand a, b;  // a: [m][k], b: [n][k]
-  int64_t m, n, k;
-  int64_t k_split;  // k values per grid layer
-  float* partials;  // [splits][m][n] when split, else null
-  const void* bias;
-  const void* residual;
-  int64_t residual_stride;
-  void* y;
-  int64_t y_stride;
-  void* z;
-  int64_t z_stride;
-  int act;
-};
-
+// ---- the split product's layers, summed in order, with the epilogue ----
+// A thread has four columns of a row.
 template <class T>
-__device__ __forceinline__ void finish(const Product& p, int64_t i, int64_t j, float z) {
-  if (p.bias) z += to_f32(static_cast<const T*>(p.bias)[j]);
-  if (p.z) static_cast<T*>(p.z)[i * p.z_stride + j] = from_f32<T>(z);
-  float y = activate(z, p.act);
-  if (p.residual) y += to_f32(static_cast<const T*>(p.residual)[i * p.residual_stride + j]);
-  static_cast<T*>(p.y)[i * p.y_stride + j] = from_f32<T>(y);
-}
-
-template <class T>
-__global__ void __launch_bounds__(256) product_kernel(Product p) {
-  __shared__ float as[16][65], bs[16][65];
-  const int64_t m0 = int64_t(blockIdx.x) * 64, n0 = int64_t(blockIdx.y) * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t kb = blockIdx.z * p.k_split;
-  const int64_t ke = kb + p.k_split < p.k ? kb + p.k_split : p.k;
-  float acc[4][4] = {};
-  for (int64_t k0 = kb; k0 < ke; k0 += 16) {
-    for (int e = threadIdx.x; e < 1024; e += 256) {
-      // the axis with unit stride runs over neighbouring threads
-      const int ka = p.a.sk == 1 ? e & 15 : e >> 6, ia = p.a.sk == 1 ? e >> 4 : e & 63;
-      const int kc = p.b.sk == 1 ? e & 15 : e >> 6, ib = p.b.sk == 1 ? e >> 4 : e & 63;
-      as[ka][ia] = m0 + ia < p.m && k0 + ka < ke
-                       ? to_f32(static_cast<const T*>(p.a.p)[(m0 + ia) * p.a.si + (k0 + ka) * p.a.sk])
-                       : 0.0f;
-      bs[kc][ib] = n0 + ib < p.n && k0 + kc < ke
-                       ? to_f32(static_cast<const T*>(p.b.p)[(n0 + ib) * p.b.si + (k0 + kc) * p.b.sk])
-                       : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += as[k][ty + 16 * i] * bs[k][tx + 16 * j];
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = m0 + ty + 16 * i, c = n0 + tx + 16 * j;
-      if (r >= p.m || c >= p.n) continue;
-      if (p.partials)
-        p.partials[(blockIdx.z * p.m + r) * p.n + c] = acc[i][j];
-      else
-        finish<T>(p, r, c, acc[i][j]);
-    }
-}
-
-// The split product's layers summed in order.
-template <class T>
-__global__ void __launch_bounds__(256) product_reduce_kernel(Product p, int splits) {
+__global__ void __launch_bounds__(256) product_reduce_kernel(const __grid_constant__ Product p) {
+  const int64_t quads = (p.n + 3) / 4;
   const int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (e >= p.m * p.n) return;
-  float s = 0.0f;
-  for (int k = 0; k < splits; ++k) s += p.partials[k * p.m * p.n + e];
-  finish<T>(p, e / p.n, e % p.n, s);
-}
-
-// dz = dy act'(z) as contiguous rows, and per-block column sums of the
-// unrounded dz.
-template <class T>
-__global__ void __launch_bounds__(256) slope_kernel(const T* dy, int64_t dy_stride, const T* z,
-                                                    int64_t z_stride, int64_t rows, int outputs,
-                                                    int64_t rows_per_block, int act, T* dz,
-                                                    float* partials) {
-  const int col = blockIdx.x * blockDim.x + threadIdx.x;
-  if (col >= outputs) return;
-  const int64_t begin = blockIdx.y * rows_per_block;
-  const int64_t end = begin + rows_per_block < rows ? begin + rows_per_block : rows;
-  float s = 0.0f;
-  for (int64_t r = begin; r < end; ++r) {
-    float d = to_f32(dy[r * dy_stride + col]);
-    if (z) d *= activation_slope(to_f32(z[r * z_stride + col]), act);
-    s += d;
-    if (dz) dz[r * outputs + col] = from_f32<T>(d);
+  if (e >= int64_t(p.m) * quads) return;
+  const int64_t row = e / quads, col = e % quads * 4;
+  const int64_t layer = int64_t(p.m_tiles) * linear_tc::kBM * p.partial_pitch;
+  const float* at = p.partials + row * p.partial_pitch + col;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < p.splits; ++s, at += layer) {
+    const float4 f = *reinterpret_cast<const float4*>(at);
+    v[0] += f.x;
+    v[1] += f.y;
+    v[2] += f.z;
+    v[3] += f.w;
   }
-  partials[int64_t(blockIdx.y) * outputs + col] = s;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (col + j >= p.n) break;
+    float z = v[j];
+    if (p.bias) z += to_f32(static_cast<const T*>(p.bias)[col + j]);
+    if (p.z) static_cast<T*>(p.z)[row * p.z_stride + col + j] = from_f32<T>(z);
+    float y = linear_tc::activation(p.act, z);
+    if (p.residual)
+      y += to_f32(static_cast<const T*>(p.residual)[row * p.residual_stride + col + j]);
+    static_cast<T*>(p.y)[row * p.y_stride + col + j] = from_f32<T>(y);
+  }
+}
+
+// ---- dz and the bias gradient ----
+struct SlopeArgs {
+  const void* dy;
+  int64_t dy_stride;
+  const void* z;  // null: dz = dy
+  int64_t z_stride;
+  int64_t rows;
+  int outputs;
+  int64_t rows_per_block;
+  int act;
+  void* dz;  // optional
+  int64_t dz_stride;
+  float* partials;  // [gridDim.y][outputs]
+  int tx;           // column groups per block, a power of two
+};
+// dz = dy act'(z) rounded to the storage type, and each block's column sums of
+// the unrounded values.  A thread has VEC columns of every (256 / tx)th row.
+template <class T, int VEC>
+__global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ SlopeArgs a) {
+  __shared__ float sums[256 * VEC];
+  const int tx = threadIdx.x & (a.tx - 1), ty = threadIdx.x / a.tx, rows_at_once = 256 / a.tx;
+  const int64_t col = (int64_t(blockIdx.x) * a.tx + tx) * VEC;
+  const bool mine = col < a.outputs;
+  const int64_t begin = int64_t(blockIdx.y) * a.rows_per_block;
+  const int64_t end = min(begin + a.rows_per_block, a.rows);
+  float s[VEC] = {};
+  if (mine) {
+#pragma unroll 4
+    for (int64_t r = begin + ty; r < end; r += rows_at_once) {
+      const Pack<T, VEC> g =
+          *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + r * a.dy_stride + col);
+      Pack<T, VEC> zz, out;
+      if (a.z)
+        zz = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.z) + r * a.z_stride + col);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float d = to_f32(g.v[j]);
+        if (a.z) d *= linear_tc::activation_slope(a.act, to_f32(zz.v[j]));
+        s[j] += d;
+        out.v[j] = from_f32<T>(d);
+      }
+      if (a.dz)
+        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dz) + r * a.dz_stride + col) = out;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sums[j * 256 + threadIdx.x] = s[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.tx * VEC; c += 256) {
+    const int64_t at = int64_t(blockIdx.x) * a.tx * VEC + c;
+    if (at >= a.outputs) continue;
+    float t = 0.0f;
+    for (int q = 0; q < rows_at_once; ++q) t += sums[(c % VEC) * 256 + q * a.tx + c / VEC];
+    a.partials[int64_t(blockIdx.y) * a.outputs + at] = t;
+  }
 }
 template <class T>
-__global__ void __launch_bounds__(256) bias_reduce_kernel(const float* partials, int count,
-                                                          int outputs, T* dbias) {
-  const int col = blockIdx.x * blockDim.x + threadIdx.x;
-  if (col >= outputs) return;
+__global__ void __launch_bounds__(256) bias_reduce_kernel(const float* __restrict__ partials,
+                                                          int count, int outputs, T* dbias) {
+  __shared__ float acc[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + tx;
   float s = 0.0f;
-  for (int p = 0; p < count; ++p) s += partials[int64_t(p) * outputs + col];
-  dbias[col] = from_f32<T>(s);
+  if (col < outputs)
+    for (int p = ty; p < count; p += 8) s += partials[int64_t(p) * outputs + col];
+  acc[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && col < outputs)
+    dbias[col] = from_f32<T>(((acc[0][tx] + acc[1][tx]) + (acc[2][tx] + acc[3][tx])) +
+                             ((acc[4][tx] + acc[5][tx]) + (acc[6][tx] + acc[7][tx])));
 }
 
-constexpr int kBiasSplits = 256;
+// ---- host side ----
+constexpr int kSms = 148;             // the plans' block count: B200's SMs
+constexpr int kBiasBlocks = 4 * kSms;  // blocks of slope_kernel at most
 
-int weight_splits(int64_t rows, int inputs, int outputs) {
-  const int64_t tiles = int64_t((inputs + 63) / 64) * ((outputs + 63) / 64);
-  const int64_t want = std::max<int64_t>(1, 592 / tiles);
-  return int(std::max<int64_t>(1, std::min<int64_t>(want, rows / 256)));
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) !=
+            cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      p = nullptr;
+    }
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+template <class T>
+constexpr CUtensorMapDataType tma_type() {
+  return sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : (std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+}
+
+// Rows that TMA can address: 16-byte aligned starts, strides below 2^40 bytes.
+bool tma_rows(const void* p, int64_t stride, int64_t rows, size_t size) {
+  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  return rows <= 1 || (stride * int64_t(size) % 16 == 0 && stride * int64_t(size) < (int64_t(1) << 40));
+}
+
+// A map of `rows` rows of `width` values in boxes of box_rows x 128 bytes,
+// 128-byte swizzled; values outside read as zero and are not written.
+template <class T>
+npa_status make_map(CUtensorMap* map, const void* p, int64_t width, int64_t rows, int64_t stride,
+                    int box_rows) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return fail(NPA_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[2] = {cuuint64_t(width), cuuint64_t(rows)};
+  const cuuint64_t pitch =
+      rows <= 1 ? cuuint64_t((width * sizeof(T) + 15) / 16 * 16) : cuuint64_t(stride * sizeof(T));
+  const cuuint32_t box[2] = {cuuint32_t(128 / sizeof(T)), cuuint32_t(box_rows)};
+  const cuuint32_t step[2] = {1, 1};
+  const CUresult r = encode(map, tma_type<T>(), 2, const_cast<void*>(p), dims, &pitch, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(NPA_ERR_CUDA, "cuTensorMapEncodeTiled failed with " + std::to_string(int(r)));
+  return NPA_OK;
+}
+
+int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
+
+// Tile width and k splits of an m x n x k product.
+struct Plan {
+  int bn;
+  int m_tiles, n_tiles, k_blocks, splits, split_blocks;
+  size_t partial_bytes() const {
+    return splits > 1 ? size_t(splits) * m_tiles * linear_tc::kBM * partial_pitch * 4 : 0;
+  }
+  int64_t partial_pitch;
+};
+Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
+  Plan p{};
+  p.m_tiles = ceil_div(m, linear_tc::kBM);
+  // The widest tile moves the fewest operand bytes; narrower ones only where
+  // the widest would leave SMs idle or columns empty.
+  p.bn = size == 2 && tma ? 256 : 128;
+  while (p.bn > 64 && (p.bn / 2 >= n || int64_t(p.m_tiles) * ceil_div(n, p.bn) < kSms)) p.bn /= 2;
+  p.n_tiles = ceil_div(n, p.bn);
+  p.k_blocks = ceil_div(k, linear_tc::kBK);
+  const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles;
+  // Few tiles over a long sum: layers of at least four k blocks each.
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(kSms / tiles, p.k_blocks / 4)));
+  p.split_blocks = ceil_div(p.k_blocks, p.splits);
+  p.splits = ceil_div(p.k_blocks, p.split_blocks);
+  p.partial_pitch = (n + 3) / 4 * 4;
+  return p;
+}
+size_t product_workspace(size_t size, int64_t m, int64_t n, int64_t k) {
+  return std::max(plan_product(size, true, m, n, k).partial_bytes(),
+                  plan_product(size, false, m, n, k).partial_bytes());
+}
+
+template <class T>
+int vector_width(const void* p, int64_t stride, int64_t rows) {
+  int vec = 16 / int(sizeof(T));
+  while (vec > 1 && (reinterpret_cast<uintptr_t>(p) % (vec * sizeof(T)) ||
+                     (rows > 1 && stride % vec)))
+    vec /= 2;
+  return vec;
+}
+
+template <class T, bool LOADER, int BN>
+npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, cudaStream_t stream) {
+  using C = linear_tc::Config<T, LOADER, BN>;
+  const auto kernel = linear_tc::product_kernel<T, LOADER, BN>;
+  int per_sm = 0, sms = 0;
+  NPA_TRY(kernel_occupancy(reinterpret_cast<const void*>(kernel), C::kThreads, C::kSmemBytes,
+                           &per_sm, &sms));
+  if (per_sm < 1) return fail(NPA_ERR_UNSUPPORTED, "linear kernel cannot be resident");
+  const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles * p.splits;
+  kernel<<<unsigned(std::min<int64_t>(tiles, sms)), C::kThreads, C::kSmemBytes, stream>>>(
+      maps[0], maps[1], maps[2], maps[3], p);
+  return after_launch("linear product_kernel");
+}
+
+// Runs the product; p holds operands, sizes and the epilogue's buffers.
+template <class T>
+npa_status run_product(Product p, float* partials, cudaStream_t stream) {
+  constexpr bool kSplitParts = sizeof(T) == 4;
+  // rows of an operand as it lies in memory
+  const int64_t a_rows = p.a.mn_major ? p.k : p.m, b_rows = p.b.mn_major ? p.k : p.n;
+  const bool tma = !kSplitParts && tma_rows(p.a.p, p.a.ld, a_rows, sizeof(T)) &&
+                   tma_rows(p.b.p, p.b.ld, b_rows, sizeof(T));
+  const Plan plan = plan_product(sizeof(T), tma, p.m, p.n, p.k);
+  p.m_tiles = plan.m_tiles;
+  p.n_tiles = plan.n_tiles;
+  p.k_blocks = plan.k_blocks;
+  p.splits = plan.splits;
+  p.split_blocks = plan.split_blocks;
+  p.partial_pitch = plan.partial_pitch;
+  p.partials = plan.splits > 1 ? partials : nullptr;
+  p.idesc = tc::instruction_desc(!std::is_same<T, __half>::value, p.a.mn_major, p.b.mn_major,
+                                 linear_tc::kBM, plan.bn);
+  p.a_vec = vector_width<T>(p.a.p, p.a.ld, a_rows);
+  p.b_vec = vector_width<T>(p.b.p, p.b.ld, b_rows);
+  p.y_tma = tma_rows(p.y, p.y_stride, p.m, sizeof(T));
+  p.z_tma = p.z && tma_rows(p.z, p.z_stride, p.m, sizeof(T));
+  p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
+  p.residual_vec = p.residual && tma_rows(p.residual, p.residual_stride, p.m, sizeof(T));
+  CUtensorMap maps[4] = {};
+  if (tma) {
+    NPA_TRY(p.a.mn_major ? make_map<T>(&maps[0], p.a.p, p.m, p.k, p.a.ld, linear_tc::kBK)
+                         : make_map<T>(&maps[0], p.a.p, p.k, p.m, p.a.ld, linear_tc::kBM));
+    NPA_TRY(p.b.mn_major ? make_map<T>(&maps[1], p.b.p, p.n, p.k, p.b.ld, linear_tc::kBK)
+                         : make_map<T>(&maps[1], p.b.p, p.k, p.n, p.b.ld, plan.bn));
+  }
+  if (p.partials)
+    NPA_TRY(make_map<float>(&maps[2], p.partials, p.n,
+                            int64_t(p.splits) * p.m_tiles * linear_tc::kBM, p.partial_pitch, 32));
+  else if (p.y_tma)
+    NPA_TRY(make_map<T>(&maps[2], p.y, p.n, p.m, p.y_stride, 32));
+  if (p.z_tma && !p.partials) NPA_TRY(make_map<T>(&maps[3], p.z, p.n, p.m, p.z_stride, 32));
+  if constexpr (kSplitParts) {
+    NPA_TRY(plan.bn == 128 ? (launch_product<T, true, 128>(maps, p, stream))
+                           : (launch_product<T, true, 64>(maps, p, stream)));
+  } else if (tma) {
+    NPA_TRY(plan.bn == 256   ? (launch_product<T, false, 256>(maps, p, stream))
+            : plan.bn == 128 ? (launch_product<T, false, 128>(maps, p, stream))
+                             : (launch_product<T, false, 64>(maps, p, stream)));
+  } else {
+    NPA_TRY(plan.bn == 128 ? (launch_product<T, true, 128>(maps, p, stream))
+                           : (launch_product<T, true, 64>(maps, p, stream)));
+  }
+  if (!p.partials) return NPA_OK;
+  product_reduce_kernel<T>
+      <<<grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 256), 256, 0, stream>>>(p);
+  return after_launch("product_reduce_kernel");
 }
 
 struct BackwardCarve {
   void* dz;
+  int64_t dz_stride;
   float* bias_partials;
-  float* weight_partials;
+  float* product_partials;
   size_t bytes;
 };
 BackwardCarve carve_backward(void* ws, int dtype, int activation, int64_t rows, int inputs,
                              int outputs) {
+  const size_t size = dtype_bytes(dtype);
   Carve c(ws, 0);
   BackwardCarve b{};
+  b.dz_stride = (int64_t(outputs) + 7) / 8 * 8;  // rows of 16-byte multiples
   b.dz = activation != NPA_ACTIVATION_IDENTITY
-             ? static_cast<void*>(c.take<char>(size_t(rows) * outputs * dtype_bytes(dtype)))
+             ? static_cast<void*>(c.take<char>(size_t(rows) * b.dz_stride * size))
              : nullptr;
-  b.bias_partials = c.take<float>(size_t(kBiasSplits) * outputs);
-  const int splits = weight_splits(rows, inputs, outputs);
-  b.weight_partials = splits > 1 ? c.take<float>(size_t(splits) * inputs * outputs) : nullptr;
+  b.bias_partials = c.take<float>(size_t(kBiasBlocks) * outputs);
+  const size_t partial = std::max(product_workspace(size, rows, inputs, outputs),
+                                  product_workspace(size, outputs, inputs, rows));
+  b.product_partials = c.take<float>(partial / 4);
   b.bytes = c.used;
   return b;
 }
 
 template <class T>
-npa_status run_product(const Product& p, int splits, cudaStream_t s) {
-  const dim3 grid(unsigned((p.m + 63) / 64), unsigned((p.n + 63) / 64), unsigned(splits));
-  product_kernel<T><<<grid, 256, 0, s>>>(p);
-  NPA_TRY(after_launch("product_kernel"));
-  if (!p.partials) return NPA_OK;
-  product_reduce_kernel<T><<<grid_for(uint64_t(p.m * p.n), 256), 256, 0, s>>>(p, splits);
-  return after_launch("product_reduce_kernel");
-}
-
-template <class T>
-npa_status forward_typed(const LinearArgs& a, cudaStream_t s) {
+npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
   Product p{};
-  p.a = {a.x, a.x_stride, 1};
-  p.b = {a.weight, a.weight_stride, 1};
-  p.m = a.rows;
+  p.a = {a.x, a.x_stride, 0};
+  p.b = {a.weight, a.weight_stride, 0};
+  p.m = int(a.rows);
   p.n = a.outputs;
-  p.k = p.k_split = a.inputs;
+  p.k = a.inputs;
   p.bias = a.bias;
   p.residual = a.residual;
   p.residual_stride = a.residual_stride;
@@ -203,7 +325,22 @@ npa_status forward_typed(const LinearArgs& a, cudaStream_t s) {
   p.z = a.z;
   p.z_stride = a.z_stride;
   p.act = a.activation;
-  return run_product<T>(p, 1, s);
+  return run_product<T>(p, static_cast<float*>(workspace), s);
+}
+
+template <class T, int VEC>
+npa_status launch_slope(SlopeArgs s, int* parts, cudaStream_t stream) {
+  const int groups = ceil_div(s.outputs, VEC);
+  s.tx = 1;
+  while (s.tx < 32 && s.tx < groups) s.tx *= 2;
+  const int grid_x = ceil_div(groups, s.tx);
+  const int64_t at_once = 256 / s.tx;
+  const int64_t most = std::max(1, kBiasBlocks / grid_x);
+  *parts = int(std::max<int64_t>(1, std::min<int64_t>(most, (s.rows + at_once * 4 - 1) / (at_once * 4))));
+  s.rows_per_block = (s.rows + *parts - 1) / *parts;
+  *parts = int((s.rows + s.rows_per_block - 1) / s.rows_per_block);
+  slope_kernel<T, VEC><<<dim3(unsigned(grid_x), unsigned(*parts)), 256, 0, stream>>>(s);
+  return after_launch("slope_kernel");
 }
 
 template <class T>
@@ -219,61 +356,70 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   const T* dz = static_cast<const T*>(a.dy);
   int64_t dz_stride = a.dy_stride;
   if (a.dbias || (a.z && (a.dx || a.dweight))) {
-    int parts = int(std::min<int64_t>(kBiasSplits, (a.rows + 63) / 64));
-    const int64_t per = (a.rows + parts - 1) / parts;
-    parts = int((a.rows + per - 1) / per);
-    slope_kernel<T><<<dim3(unsigned((a.outputs + 255) / 256), unsigned(parts)), 256, 0, s>>>(
-        dz, dz_stride, static_cast<const T*>(a.z), a.z_stride, a.rows, a.outputs, per,
-        a.activation, static_cast<T*>(a.z ? ws.dz : nullptr), ws.bias_partials);
-    NPA_TRY(after_launch("slope_kernel"));
+    SlopeArgs g{};
+    g.dy = a.dy;
+    g.dy_stride = a.dy_stride;
+    g.z = a.z;
+    g.z_stride = a.z_stride;
+    g.rows = a.rows;
+    g.outputs = a.outputs;
+    g.act = a.activation;
+    g.dz = a.z && (a.dx || a.dweight) ? ws.dz : nullptr;
+    g.dz_stride = ws.dz_stride;
+    g.partials = ws.bias_partials;
+    int parts = 0;
+    constexpr int kVec = 16 / int(sizeof(T));
+    if (a.outputs % kVec == 0 && vector_width<T>(a.dy, a.dy_stride, a.rows) == kVec &&
+        (!a.z || vector_width<T>(a.z, a.z_stride, a.rows) == kVec))
+      NPA_TRY((launch_slope<T, kVec>(g, &parts, s)));
+    else
+      NPA_TRY((launch_slope<T, 1>(g, &parts, s)));
     if (a.dbias) {
-      bias_reduce_kernel<T><<<grid_for(a.outputs, 256), 256, 0, s>>>(
+      bias_reduce_kernel<T><<<grid_for(a.outputs, 32), 256, 0, s>>>(
           ws.bias_partials, parts, a.outputs, static_cast<T*>(a.dbias));
       NPA_TRY(after_launch("bias_reduce_kernel"));
     }
-    if (a.z) {
+    if (g.dz) {
       dz = static_cast<const T*>(ws.dz);
-      dz_stride = a.outputs;
+      dz_stride = ws.dz_stride;
     }
   }
   if (a.dx) {
     Product p{};
-    p.a = {dz, dz_stride, 1};
-    p.b = {a.weight, 1, a.weight_stride};
-    p.m = a.rows;
+    p.a = {dz, dz_stride, 0};
+    p.b = {a.weight, a.weight_stride, 1};
+    p.m = int(a.rows);
     p.n = a.inputs;
-    p.k = p.k_split = a.outputs;
+    p.k = a.outputs;
     p.y = a.dx;
     p.y_stride = a.dx_stride;
-    NPA_TRY(run_product<T>(p, 1, s));
+    NPA_TRY(run_product<T>(p, ws.product_partials, s));
   }
   if (a.dweight) {
     Product p{};
-    p.a = {dz, 1, dz_stride};
-    p.b = {a.x, 1, a.x_stride};
+    p.a = {dz, dz_stride, 1};
+    p.b = {a.x, a.x_stride, 1};
     p.m = a.outputs;
     p.n = a.inputs;
-    p.k = a.rows;
-    int splits = weight_splits(a.rows, a.inputs, a.outputs);
-    p.k_split = (a.rows + splits - 1) / splits;
-    splits = int((a.rows + p.k_split - 1) / p.k_split);
-    p.partials = splits > 1 ? ws.weight_partials : nullptr;
+    p.k = int(a.rows);
     p.y = a.dweight;
     p.y_stride = a.inputs;
-    NPA_TRY(run_product<T>(p, splits, s));
+    NPA_TRY(run_product<T>(p, ws.product_partials, s));
   }
   return NPA_OK;
 }
 
 }  // namespace
 
-size_t linear_workspace(int, int64_t, int, int) { return 0; }
+size_t linear_workspace(int dtype, int64_t rows, int inputs, int outputs) {
+  return rows == 0 ? 0 : product_workspace(dtype_bytes(dtype), rows, outputs, inputs);
+}
 
-npa_status launch_linear(int dtype, const LinearArgs& a, void*, cudaStream_t stream) {
+npa_status launch_linear(int dtype, const LinearArgs& a, void* workspace, cudaStream_t stream) {
   switch (dtype) {
-    case NPA_DTYPE_F32: return forward_typed<float>(a, stream);
-    case NPA_DTYPE_F16: return forward_typed<__half>(a, stream);
-    default: return forward_typed<__nv_bfloat16>(a, stream);
+    case NPA_DTYPE_F32: return forward_typed<float>(a, workspace, stream);
+    case NPA_DTYPE_F16: return forward_typed<__half>(a, workspace, stream);
+    default: return forward_typed<__nv_bfloat16>(a, workspace, stream);
   }
 }
 
@@ -285,12 +431,22 @@ size_t linear_backward_workspace(int dtype, int activation, int64_t rows, int in
 npa_status launch_linear_backward(int dtype, const LinearBackwardArgs& a, void* workspace,
                                   cudaStream_t stream) {
   const BackwardCarve ws =
-      carve_backward(workspace, dtype, a.activation, a.rows, a.inputs, a.outputs);
+      a.rows == 0 ? BackwardCarve{}
+                  : carve_backward(workspace, dtype, a.activation, a.rows, a.inputs, a.outputs);
   switch (dtype) {
     case NPA_DTYPE_F32: return backward_typed<float>(a, ws, stream);
     case NPA_DTYPE_F16: return backward_typed<__half>(a, ws, stream);
     default: return backward_typed<__nv_bfloat16>(a, ws, stream);
   }
+}
+
+uint64_t linear_timeouts() {
+  unsigned long long v = 0;
+  if (cudaMemcpyFromSymbol(&v, linear_tc::g_timeouts, sizeof(v)) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return v;
 }
 
 }  // namespace npa

@@ -1,0 +1,705 @@
+// linear_product.cuh -- the tensor-core product of the linear operator and its
+// backward pass: C = A B^T over tiles of 128 rows, with the layer's epilogue.
+//
+// A block has one tile at a time and walks them in a grid-stride loop.  Its
+// warps have roles: producers fill a ring of operand stages (64 values of k),
+// one thread issues the tensor-core products into one of two accumulator
+// buffers in TMEM, and eight epilogue warps read the other one, so a tile's
+// epilogue runs under the next tile's products.
+//
+// Operands come in two ways.  16-bit operands whose rows start on 16 bytes are
+// copied by TMA into the 128-byte swizzle.  Everything else (f32, odd widths)
+// goes through eight loader warps that read rows with plain loads of whatever
+// alignment they have and write the same swizzled tiles.
+//
+// f32 values are split into three bf16 parts, x = x0 + x1 + x2 exactly but for
+// 2^-24 |x|, and six of the nine part products are summed in f32:
+//   x w ~ x0 w0 + (x0 w1 + x1 w0 + x1 w1 + x0 w2 + x2 w0),
+// the rest is below 2^-24 |x w|.  The tensor core truncates as it accumulates,
+// so the leading products and the five small ones have accumulators of their
+// own, and every 256 values of k the epilogue warps move both into rounded
+// f32 sums in registers.  An infinite value has no such parts (its rest is
+// NaN): outputs that come out NaN are recomputed from their rows.
+#pragma once
+
+#include "layers.h"
+#include "tcgen05.cuh"
+
+namespace npa {
+namespace linear_tc {
+
+constexpr int kBM = 128;                 // rows of a tile: the tensor core's M
+constexpr int kBK = 64;                  // k values per stage: one 128-byte swizzle row
+constexpr int kEpilogueWarps = 8;        // two per 32 TMEM lanes
+constexpr int kLoaderWarps = 8;
+constexpr int kChunkBlocks = 4;          // k blocks between f32 moves out of TMEM
+constexpr int kSmemLimit = 227 * 1024;
+
+// One operand: value (i, k) at i * ld + k, or at k * ld + i when MN-major.
+struct Operand {
+  const void* p;
+  int64_t ld;
+  int mn_major;
+};
+
+struct Product {
+  Operand a, b;  // [m][k] and [n][k]
+  int m, n, k;
+  int m_tiles, n_tiles, splits;
+  int k_blocks, split_blocks;  // 64-value blocks in all and per split
+  uint32_t idesc;
+  int a_vec, b_vec;  // values per plain load (loader warps)
+  const void* bias;
+  const void* residual;
+  int64_t residual_stride;
+  void* y;
+  int64_t y_stride;
+  void* z;
+  int64_t z_stride;
+  float* partials;  // split: [splits][m_tiles * 128][partial_pitch], else null
+  int64_t partial_pitch;
+  int act;
+  int y_tma, z_tma, bias_vec, residual_vec;
+};
+
+__device__ unsigned long long g_timeouts = 0;  // bounded waits that gave up
+
+template <class T, bool LOADER, int BN>
+struct Config {
+  static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+  static constexpr int kABytes = kBM * 128, kBBytes = BN * 128;
+  static constexpr int kStageBytes = kParts * (kABytes + kBBytes);
+  static constexpr int kOutBuffers = BN == 256 || kParts == 3 ? 1 : 2;
+  static constexpr int kOutBytes = kEpilogueWarps * kOutBuffers * 4096;
+  static constexpr int kStagesFit = (kSmemLimit - kOutBytes - 2048) / kStageBytes;
+  static constexpr int kStages = kStagesFit > 6 ? 6 : kStagesFit;
+  static constexpr int kBufferColumns = BN * (kParts == 3 ? 2 : 1);
+  static constexpr int kTmemColumns = 2 * kBufferColumns;
+  static constexpr int kThreads = 32 * (kEpilogueWarps + 2 + (LOADER ? kLoaderWarps - 1 : 0));
+  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kOutBytes + 1024 + 256;
+  static_assert(kStages >= 2 && kTmemColumns <= 512, "tile does not fit");
+};
+
+// act(z) and act'(z).  NaN stays NaN.
+__device__ __forceinline__ float activation(int act, float z) {
+  switch (act) {
+    case NPA_ACTIVATION_RELU: return z < 0.0f ? 0.0f : z;
+    case NPA_ACTIVATION_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case NPA_ACTIVATION_GELU_TANH:
+      return 0.5f * z * (1.0f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
+    case NPA_ACTIVATION_SILU: return z / (1.0f + expf(-z));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float activation_slope(int act, float z) {
+  switch (act) {
+    case NPA_ACTIVATION_RELU: return z <= 0.0f ? 0.0f : 1.0f;
+    case NPA_ACTIVATION_GELU:
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
+             z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case NPA_ACTIVATION_GELU_TANH: {
+      const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
+      return 0.5f * (1.0f + t) +
+             0.5f * z * (1.0f - t * t) * 0.79788456080286536f * (1.0f + 0.134145f * z * z);
+    }
+    case NPA_ACTIVATION_SILU: {
+      const float s = 1.0f / (1.0f + expf(-z));
+      return s * (1.0f + z * (1.0f - s));
+    }
+    default: return 1.0f;
+  }
+}
+
+// The activation of a thread's N values, the choice outside the loop.
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&v)[N]) {
+  switch (act) {
+    case NPA_ACTIVATION_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activation(NPA_ACTIVATION_RELU, v[i]);
+      break;
+    case NPA_ACTIVATION_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activation(NPA_ACTIVATION_GELU, v[i]);
+      break;
+    case NPA_ACTIVATION_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activation(NPA_ACTIVATION_GELU_TANH, v[i]);
+      break;
+    case NPA_ACTIVATION_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activation(NPA_ACTIVATION_SILU, v[i]);
+      break;
+    default: break;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+
+// The shared-memory address of 16-byte chunk c of row r in a tile of 128-byte
+// rows: TMA's 128-byte swizzle.
+__device__ __forceinline__ uint32_t swizzled(int r, int c) {
+  return uint32_t(r * 128 + ((c ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ void store_shared16(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(v.x), "r"(v.y),
+               "r"(v.z), "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// One value of the product by plain f32 steps over [k0, k1).
+template <class T>
+__device__ __noinline__ float plain_dot(const Product& p, int64_t i, int64_t j, int64_t k0, int64_t k1) {
+  const T* a = static_cast<const T*>(p.a.p) + (p.a.mn_major ? i : i * p.a.ld);
+  const T* b = static_cast<const T*>(p.b.p) + (p.b.mn_major ? j : j * p.b.ld);
+  const int64_t sa = p.a.mn_major ? p.a.ld : 1, sb = p.b.mn_major ? p.b.ld : 1;
+  float s = 0.0f;
+  for (int64_t k = k0; k < k1; ++k) s += to_f32(a[k * sa]) * to_f32(b[k * sb]);
+  return s;
+}
+
+// ---- loader warps ----
+// Eight values of a line, zero past `valid`.
+template <class T>
+struct Chunk;
+template <>
+struct alignas(16) Chunk<float> {
+  float v[8];
+};
+template <class T>
+struct Chunk {
+  uint4 v;
+};
+template <class T>
+__device__ __forceinline__ void load_chunk(const T* p, int valid, int vec, Chunk<T>& c) {
+  T* const out = reinterpret_cast<T*>(&c);
+  if (valid >= 8) {
+    constexpr int kMost = 16 / int(sizeof(T));
+    if (vec == kMost) {
+#pragma unroll
+      for (int i = 0; i < 8; i += kMost)
+        *reinterpret_cast<Pack<T, kMost>*>(out + i) = *reinterpret_cast<const Pack<T, kMost>*>(p + i);
+      return;
+    }
+    if (vec >= 2) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2)
+        *reinterpret_cast<Pack<T, 2>*>(out + i) = *reinterpret_cast<const Pack<T, 2>*>(p + i);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[i] = i < valid ? p[i] : T(0.0f);
+}
+__device__ __forceinline__ uint32_t high_halves(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+}
+__device__ __forceinline__ float truncated(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+// Writes the chunk's part(s) at `at`, parts `part_bytes` apart.
+template <class T>
+__device__ __forceinline__ void store_chunk(uint32_t at, uint32_t, const Chunk<T>& c) {
+  store_shared16(at, c.v);
+}
+template <>
+__device__ __forceinline__ void store_chunk<float>(uint32_t at, uint32_t part_bytes,
+                                                   const Chunk<float>& c) {
+  float r1[8], r2[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    r1[i] = c.v[i] - truncated(c.v[i]);
+    r2[i] = r1[i] - truncated(r1[i]);
+  }
+  store_shared16(at, make_uint4(high_halves(c.v[0], c.v[1]), high_halves(c.v[2], c.v[3]),
+                                high_halves(c.v[4], c.v[5]), high_halves(c.v[6], c.v[7])));
+  store_shared16(at + part_bytes, make_uint4(high_halves(r1[0], r1[1]), high_halves(r1[2], r1[3]),
+                                             high_halves(r1[4], r1[5]), high_halves(r1[6], r1[7])));
+  store_shared16(at + 2 * part_bytes,
+                 make_uint4(pack2<__nv_bfloat16>(r2[0], r2[1]), pack2<__nv_bfloat16>(r2[2], r2[3]),
+                            pack2<__nv_bfloat16>(r2[4], r2[5]), pack2<__nv_bfloat16>(r2[6], r2[7])));
+}
+// The chunk `q` of an operand tile that starts at (o0, k0): a tile has lines of
+// 64 values, over k for K-major operands and over m (or n) for MN-major ones.
+template <class T>
+__device__ __forceinline__ void read_tile_chunk(const Operand& o, int vec, int64_t o0, int64_t outer,
+                                                int64_t k0, int64_t k1, int q, Chunk<T>& c) {
+  const int line = q >> 3, e = (q & 7) * 8;
+  int64_t row, col, rows, cols;
+  if (o.mn_major) {
+    row = k0 + (line & 63);
+    col = o0 + (line >> 6) * 64 + e;
+    rows = k1;
+    cols = outer;
+  } else {
+    row = o0 + line;
+    col = k0 + e;
+    rows = outer;
+    cols = k1;
+  }
+  const int64_t left = row < rows ? cols - col : 0;
+  const int valid = left >= 8 ? 8 : left > 0 ? int(left) : 0;
+  load_chunk<T>(static_cast<const T*>(o.p) + (valid ? row * o.ld + col : 0), valid, vec, c);
+}
+
+// ---- epilogue ----
+// One warp's window on an output: 32 rows from row0, a 128-byte group of
+// columns from col0, staged in the warp's shared-memory buffer.
+template <class OUT, int NC>
+__device__ __forceinline__ void stage_values(uint32_t buf, int lane, const float (&v)[NC], int first) {
+  constexpr int kPer = 16 / int(sizeof(OUT));
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint4 u;
+    if constexpr (sizeof(OUT) == 4) {
+      u = make_uint4(__float_as_uint(v[first + c * kPer]), __float_as_uint(v[first + c * kPer + 1]),
+                     __float_as_uint(v[first + c * kPer + 2]),
+                     __float_as_uint(v[first + c * kPer + 3]));
+    } else {
+      u = make_uint4(pack2<OUT>(v[c * kPer], v[c * kPer + 1]),
+                     pack2<OUT>(v[c * kPer + 2], v[c * kPer + 3]),
+                     pack2<OUT>(v[c * kPer + 4], v[c * kPer + 5]),
+                     pack2<OUT>(v[c * kPer + 6], v[c * kPer + 7]));
+    }
+    store_shared16(buf + swizzled(lane, c), u);
+  }
+}
+// The staged group to global memory: by TMA, or row by row where the output's
+// rows do not start on 16 bytes.
+template <class OUT>
+__device__ __forceinline__ void put_group(uint32_t buf, const char* buf_ptr, int lane,
+                                          const CUtensorMap* map, bool tma, int x, int y_tma_row,
+                                          void* out, int64_t stride, int64_t row0, int rows,
+                                          int cols) {
+  constexpr int kCols = 128 / int(sizeof(OUT));
+  if (tma) {
+    tc::fence_async_shared();
+    __syncwarp();
+    if (lane == 0) {
+      tc::tma_store(map, x, y_tma_row, buf);
+      tc::bulk_commit();
+    }
+    return;
+  }
+  __syncwarp();
+  OUT* const base = static_cast<OUT*>(out) + row0 * stride + x;
+  constexpr int kPer = 16 / int(sizeof(OUT));
+  for (int r = 0; r < rows; ++r)
+#pragma unroll
+    for (int c = lane; c < kCols; c += 32)
+      if (c < cols)
+        base[r * stride + c] = reinterpret_cast<const OUT*>(
+            buf_ptr + swizzled(r, c / kPer))[c % kPer];
+}
+
+template <class T, bool LOADER, int BN>
+__global__ void __launch_bounds__((Config<T, LOADER, BN>::kThreads), 1)
+product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z,
+               const __grid_constant__ Product p) {
+  using C = Config<T, LOADER, BN>;
+  constexpr int kGroup = 128 / int(sizeof(T));         // output columns staged at a time
+  constexpr int kGroups = BN / kGroup;
+  constexpr int kGroupsPerWarp = (kGroups + 1) / 2;
+  extern __shared__ char smem_raw[];
+  const uint32_t raw = tc::smem_addr(smem_raw);
+  const uint32_t base = (raw + 1023) & ~1023u;  // the swizzle repeats every 1,024 bytes
+  const uint32_t out_base = base + C::kStages * C::kStageBytes;
+  const uint32_t bars = out_base + C::kOutBytes;
+  const uint32_t full = bars, empty = bars + 8 * C::kStages;
+  const uint32_t acc_full = empty + 8 * C::kStages, acc_empty = acc_full + 16;
+  const uint32_t drain = acc_empty + 16, tmem_at = drain + 8;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kMmaWarp = kEpilogueWarps, kProducerWarp = kEpilogueWarps + 1;
+  const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles * p.splits;
+  const int64_t layer = int64_t(p.m_tiles) * p.n_tiles;
+
+  if (warp == kMmaWarp) {
+    if (lane == 0) {
+      for (int s = 0; s < C::kStages; ++s) {
+        tc::bar_init(full + 8 * s, LOADER ? kLoaderWarps : 1);
+        tc::bar_init(empty + 8 * s, 1);
+      }
+      for (int b = 0; b < 2; ++b) {
+        tc::bar_init(acc_full + 8 * b, 1);
+        tc::bar_init(acc_empty + 8 * b, kEpilogueWarps);
+      }
+      tc::bar_init(drain, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    __syncwarp();
+    tc::tmem_alloc(tmem_at, C::kTmemColumns);
+    tc::fence_before();
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    if (!LOADER) {
+      tc::prefetch_map(&map_a);
+      tc::prefetch_map(&map_b);
+    }
+    if (p.y_tma) tc::prefetch_map(&map_y);
+    if (p.z_tma) tc::prefetch_map(&map_z);
+  }
+  __syncthreads();
+  tc::fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(tmem) : "r"(tmem_at) : "memory");
+  bool ok = true;
+
+  if (warp >= kProducerWarp) {
+    // ---- producers ----
+    if (!LOADER) {
+      if (lane == 0) {
+        uint64_t it = 0;
+        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+          const int split = int(t / layer), in = int(t % layer);
+          const int m0 = in / p.n_tiles * kBM, n0 = in % p.n_tiles * BN;
+          const int kb = split * p.split_blocks;
+          const int ke = min(p.k_blocks, kb + p.split_blocks);
+          for (int kt = kb; kt < ke; ++kt, ++it) {
+            const int s = int(it % C::kStages);
+            ok = tc::bar_wait(empty + 8 * s, uint32_t(it / C::kStages & 1) ^ 1);
+            if (!ok) break;
+            const uint32_t bar = full + 8 * s, a = base + s * C::kStageBytes, b = a + C::kABytes;
+            tc::bar_expect(bar, C::kABytes + C::kBBytes);
+            if (p.a.mn_major) {
+#pragma unroll
+              for (int i = 0; i < kBM / 64; ++i)
+                tc::tma_load(a + i * 8192, &map_a, m0 + i * 64, kt * kBK, bar);
+            } else {
+              tc::tma_load(a, &map_a, kt * kBK, m0, bar);
+            }
+            if (p.b.mn_major) {
+#pragma unroll
+              for (int i = 0; i < BN / 64; ++i)
+                tc::tma_load(b + i * 8192, &map_b, n0 + i * 64, kt * kBK, bar);
+            } else {
+              tc::tma_load(b, &map_b, kt * kBK, n0, bar);
+            }
+          }
+        }
+        if (!ok) {  // copies in flight must land before the block may leave
+          const uint64_t from = it > C::kStages ? it - C::kStages : 0;
+          for (uint64_t j = from; j < it; ++j)
+            tc::bar_wait(full + 8 * int(j % C::kStages), uint32_t(j / C::kStages & 1));
+        }
+      }
+    } else {
+      const int tid = threadIdx.x - kProducerWarp * 32;
+      constexpr int kThreads = kLoaderWarps * 32;
+      constexpr int kPerThread = 1024 / kThreads;  // chunks of 128 lines
+      uint64_t it = 0;
+      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const int split = int(t / layer), in = int(t % layer);
+        const int64_t m0 = int64_t(in / p.n_tiles) * kBM, n0 = int64_t(in % p.n_tiles) * BN;
+        const int kb = split * p.split_blocks;
+        const int ke = min(p.k_blocks, kb + p.split_blocks);
+        for (int kt = kb; kt < ke; ++kt, ++it) {
+          const int s = int(it % C::kStages);
+          const int64_t k0 = int64_t(kt) * kBK;
+          Chunk<T> c[kPerThread];
+#pragma unroll
+          for (int i = 0; i < kPerThread; ++i)
+            read_tile_chunk<T>(p.a, p.a_vec, m0, p.m, k0, p.k, tid + i * kThreads, c[i]);
+          ok = tc::bar_wait(empty + 8 * s, uint32_t(it / C::kStages & 1) ^ 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t a = base + s * C::kStageBytes, b = a + C::kParts * C::kABytes;
+#pragma unroll
+          for (int i = 0; i < kPerThread; ++i) {
+            const int q = tid + i * kThreads;
+            store_chunk<T>(a + swizzled(q >> 3, q & 7), C::kABytes, c[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < BN * 8 / kThreads; ++i)
+            read_tile_chunk<T>(p.b, p.b_vec, n0, p.n, k0, p.k, tid + i * kThreads, c[i]);
+#pragma unroll
+          for (int i = 0; i < BN * 8 / kThreads; ++i) {
+            const int q = tid + i * kThreads;
+            store_chunk<T>(b + swizzled(q >> 3, q & 7), C::kBBytes, c[i]);
+          }
+          tc::fence_async_shared();
+          __syncwarp();
+          if (lane == 0) tc::bar_arrive(full + 8 * s);
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---- the thread that issues the products ----
+    if (lane == 0) {
+      uint64_t it = 0, chunk = 0;
+      const uint32_t a_step = p.a.mn_major ? 2048 : 32, b_step = p.b.mn_major ? 2048 : 32;
+      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const int split = int(t / layer);
+        const int kb = split * p.split_blocks;
+        const int ke = min(p.k_blocks, kb + p.split_blocks);
+        uint32_t d = 0;
+        for (int kt = kb; kt < ke; ++kt, ++it) {
+          const int in_chunk = C::kParts == 3 ? (kt - kb) % kChunkBlocks : kt - kb;
+          if (in_chunk == 0) {
+            const int buf = int(chunk & 1);
+            ok = tc::bar_wait(acc_empty + 8 * buf, uint32_t(chunk / 2 & 1) ^ 1);
+            if (!ok) break;
+            tc::fence_after();
+            d = tmem + buf * C::kBufferColumns;
+          }
+          const int s = int(it % C::kStages);
+          ok = tc::bar_wait(full + 8 * s, uint32_t(it / C::kStages & 1));
+          if (!ok) break;
+          tc::fence_after();
+          const uint32_t a = base + s * C::kStageBytes, b = a + C::kParts * C::kABytes;
+#pragma unroll
+          for (int step = 0; step < kBK / 16; ++step) {
+            const bool more = in_chunk > 0 || step > 0;
+            const uint32_t as = a + step * a_step, bs = b + step * b_step;
+            tc::mma_f16(d, tc::operand_desc(as, p.a.mn_major, 8192),
+                        tc::operand_desc(bs, p.b.mn_major, 8192), p.idesc, more);
+            if constexpr (C::kParts == 3) {
+              constexpr int kA[5] = {0, 1, 1, 0, 2}, kB[5] = {1, 0, 1, 2, 0};
+#pragma unroll
+              for (int j = 0; j < 5; ++j)
+                tc::mma_f16(d + BN,
+                            tc::operand_desc(as + kA[j] * C::kABytes, p.a.mn_major, 8192),
+                            tc::operand_desc(bs + kB[j] * C::kBBytes, p.b.mn_major, 8192), p.idesc,
+                            more || j > 0);
+            }
+          }
+          tc::mma_commit(empty + 8 * s);
+          if (kt + 1 == ke || (C::kParts == 3 && in_chunk + 1 == kChunkBlocks)) {
+            tc::mma_commit(acc_full + 8 * int(chunk & 1));
+            ++chunk;
+          }
+        }
+      }
+      if (!ok) {  // products in flight must end before TMEM is freed
+        tc::mma_commit(drain);
+        tc::bar_wait(drain, 0);
+      }
+    }
+  } else {
+    // ---- epilogue warps: 32 rows each, every other group of columns ----
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const uint32_t bufs = out_base + warp * C::kOutBuffers * 4096;
+    uint32_t turn = 0;
+    uint64_t chunk = 0;
+    // the next staging buffer, free of its last copy
+    auto next_buffer = [&]() -> uint32_t {
+      if (lane == 0) tc::bulk_wait_read<C::kOutBuffers - 1>();
+      __syncwarp();
+      const uint32_t b = bufs + (turn % C::kOutBuffers) * 4096;
+      ++turn;
+      return b;
+    };
+    auto pointer = [&](uint32_t b) -> char* { return smem_raw + (b - raw); };
+    for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int split = int(t / layer), in = int(t % layer);
+      const int m_tile = in / p.n_tiles;
+      const int64_t row0 = int64_t(m_tile) * kBM + quarter * 32;
+      const int n0 = in % p.n_tiles * BN;
+      const int64_t rows_left = int64_t(p.m) - row0;
+      const int rows = rows_left >= 32 ? 32 : rows_left > 0 ? int(rows_left) : 0;
+      float sums[C::kParts == 3 ? kGroupsPerWarp : 1][kGroup];
+      uint32_t d = 0;
+      if constexpr (C::kParts == 3) {
+        const int kb = split * p.split_blocks;
+        const int blocks = min(p.k_blocks, kb + p.split_blocks) - kb;
+        const int chunks = (blocks + kChunkBlocks - 1) / kChunkBlocks;
+#pragma unroll
+        for (int gi = 0; gi < kGroupsPerWarp; ++gi)
+#pragma unroll
+          for (int e = 0; e < kGroup; ++e) sums[gi][e] = 0.0f;
+        for (int ch = 0; ch < chunks; ++ch, ++chunk) {
+          const int buf = int(chunk & 1);
+          ok = tc::bar_wait(acc_full + 8 * buf, uint32_t(chunk / 2 & 1));
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc::fence_after();
+#pragma unroll
+          for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
+            const uint32_t at = tmem + buf * C::kBufferColumns + lanes + (half + 2 * gi) * kGroup;
+            float v[kGroup];
+            tc::tmem_load(at + BN, v);
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) sums[gi][e] += v[e];
+            tc::tmem_load(at, v);
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) sums[gi][e] += v[e];
+          }
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::bar_arrive(acc_empty + 8 * buf);
+        }
+        if (!ok) break;
+      } else {
+        const int buf = int(chunk & 1);
+        ok = tc::bar_wait(acc_full + 8 * buf, uint32_t(chunk / 2 & 1));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after();
+        d = tmem + buf * C::kBufferColumns + lanes;
+      }
+#pragma unroll
+      for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
+        const int g = half + 2 * gi;
+        const int col0 = n0 + g * kGroup;
+        const bool last = gi + 1 == kGroupsPerWarp;
+        const bool mine = g < kGroups && col0 < p.n && rows > 0;
+        const int cols = min(kGroup, p.n - col0);
+        float v[kGroup];
+        // the TMA kernel loads the residual before it reads the accumulators, so
+        // that the loads' latency passes under them; the loader kernel's register
+        // budget (five warps to an SM quarter) has no room for it
+        uint4 res[LOADER ? 1 : 8];
+        const bool res_vec = p.residual_vec && cols == kGroup;
+        auto read_residual = [&](int i) -> uint4 {
+          const int rr = i * 4 + (lane >> 3);
+          const T* const r = static_cast<const T*>(p.residual) + (row0 + rr) * p.residual_stride + col0;
+          return rr < rows ? *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(r) +
+                                                             (lane & 7) * 16)
+                           : make_uint4(0, 0, 0, 0);
+        };
+        if constexpr (!LOADER) {
+          if (mine && !p.partials && p.residual && res_vec) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) res[i] = read_residual(i);
+          }
+        }
+        if constexpr (C::kParts == 3) {
+#pragma unroll
+          for (int e = 0; e < kGroup; ++e) v[e] = sums[gi][e];
+          if (mine && lane < rows) {
+            const int64_t k0 = int64_t(split) * p.split_blocks * kBK;
+            const int64_t k1 = min(int64_t(p.k), k0 + int64_t(p.split_blocks) * kBK);
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e)
+              if (v[e] != v[e] && e < cols) v[e] = plain_dot<T>(p, row0 + lane, col0 + e, k0, k1);
+          }
+          __syncwarp();
+        } else {
+          if (mine) tc::tmem_load(d + g * kGroup, v);
+          if (last) {
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive(acc_empty + 8 * int(chunk & 1));
+            ++chunk;
+          }
+        }
+        if (!mine) continue;
+        if (p.partials) {
+          const int64_t prow = (int64_t(split) * p.m_tiles + m_tile) * kBM + quarter * 32;
+#pragma unroll
+          for (int h = 0; h < kGroup / 32; ++h) {
+            if (h * 32 >= cols) break;
+            const uint32_t b = next_buffer();
+            stage_values<float>(b, lane, v, h * 32);
+            put_group<float>(b, pointer(b), lane, &map_y, true, col0 + h * 32, int(prow), nullptr,
+                             0, 0, 0, 0);
+          }
+          continue;
+        }
+        if (p.bias) {
+          const T* const bias = static_cast<const T*>(p.bias) + col0;
+          constexpr int kPer = 16 / int(sizeof(T));
+          if (p.bias_vec && cols == kGroup) {
+#pragma unroll
+            for (int i = 0; i < kGroup; i += kPer) {
+              const Pack<T, kPer> b = *reinterpret_cast<const Pack<T, kPer>*>(bias + i);
+#pragma unroll
+              for (int j = 0; j < kPer; ++j) v[i + j] += to_f32(b.v[j]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i)
+              if (i < cols) v[i] += to_f32(bias[i]);
+          }
+        }
+        if (p.z) {
+          const uint32_t b = next_buffer();
+          stage_values<T>(b, lane, v, 0);
+          put_group<T>(b, pointer(b), lane, &map_z, p.z_tma, col0, int(row0), p.z, p.z_stride,
+                       row0, rows, cols);
+        }
+        activate(p.act, v);
+        const uint32_t b = next_buffer();
+        if (p.residual) {
+          if (res_vec) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              store_shared16(b + swizzled(i * 4 + (lane >> 3), lane & 7),
+                             LOADER ? read_residual(i) : res[LOADER ? 0 : i]);
+          } else {
+            const T* const r = static_cast<const T*>(p.residual) + row0 * p.residual_stride + col0;
+            constexpr int kPer = 16 / int(sizeof(T));
+            for (int rr = 0; rr < rows; ++rr)
+#pragma unroll
+              for (int c = lane; c < kGroup; c += 32)
+                if (c < cols)
+                  reinterpret_cast<T*>(pointer(b) + swizzled(rr, c / kPer))[c % kPer] =
+                      r[rr * p.residual_stride + c];
+          }
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint4 u = load_shared16(b + swizzled(lane, c));
+            if constexpr (sizeof(T) == 4) {
+              v[c * 4] += __uint_as_float(u.x);
+              v[c * 4 + 1] += __uint_as_float(u.y);
+              v[c * 4 + 2] += __uint_as_float(u.z);
+              v[c * 4 + 3] += __uint_as_float(u.w);
+            } else {
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 f = unpack2<T>(w[j]);
+                v[c * 8 + 2 * j] += f.x;
+                v[c * 8 + 2 * j + 1] += f.y;
+              }
+            }
+          }
+        }
+        stage_values<T>(b, lane, v, 0);
+        put_group<T>(b, pointer(b), lane, &map_y, p.y_tma, col0, int(row0), p.y, p.y_stride, row0,
+                     rows, cols);
+      }
+    }
+    if (lane == 0) tc::bulk_wait_all();
+  }
+  if (!ok && lane == 0) atomicAdd(&g_timeouts, 1ull);
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc::fence_after();
+    tc::tmem_free(tmem, C::kTmemColumns);
+  }
+}
+
+}  // namespace linear_tc
+}  // namespace npa
