@@ -530,7 +530,7 @@ npa_status npa_last_error_detail(npa_error_detail* out) {
 uint64_t npa_kernel_launch_count(void) { return g_launches.load(); }
 
 uint64_t npa_bulk_copy_timeouts(void) {
-  return bulk_copy_timeouts() + ws_step_timeouts() + linear_timeouts();
+  return bulk_copy_timeouts() + ws_step_timeouts() + linear_timeouts() + layer_norm_timeouts();
 }
 
 npa_status npa_prepare_host_tables(int64_t* ln_1p_exceptions) {

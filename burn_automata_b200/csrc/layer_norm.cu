@@ -14,9 +14,22 @@
 // the backward pass keeps each thread's share of dw and db in registers over
 // all rows that it walks; the blocks' shares meet in a second small kernel, in
 // a fixed order.
+//
+// How a row reaches the registers depends on how it lies in memory:
+//  - rows that follow each other without gaps and are short: eight rows are a
+//    whole number of 16-byte units whatever the width, so each warp has a ring
+//    of eight-row tiles in shared memory, filled by bulk copies and (results in
+//    place) emptied by bulk copies.  Odd widths then cost no partial accesses
+//    in global memory.  layer_norm_tiles_kernel, layer_norm_backward_tiles_kernel;
+//  - longer rows that start on 16 bytes: a block per row, whole rows copied
+//    ahead into a ring.  layer_norm_wide_kernel, layer_norm_backward_wide_kernel;
+//  - everything else (column ranges, long odd widths): plain loads.
+//    layer_norm_kernel, layer_norm_backward_kernel, and walks over global memory
+//    past what registers hold.
 #include <algorithm>
 
 #include "layers.h"
+#include "tcgen05.cuh"
 
 namespace npa {
 namespace {
@@ -143,6 +156,580 @@ layer_norm_kernel(LayerNormArgs a, int tpr_) {
     if (lane == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
+    }
+  }
+}
+
+// ---- bulk copies: rows in flight ahead of the arithmetic ----
+__device__ unsigned long long g_timeouts = 0;  // bounded waits that gave up
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(dst), "r"(src),
+               "r"(bytes)
+               : "memory");
+}
+
+// Sums over the tpr lanes of a row.
+__device__ __forceinline__ float lanes_sum(int tpr, float a) {
+  for (int o = tpr >> 1; o > 0; o >>= 1) a += __shfl_xor_sync(kFull, a, o);
+  return a;
+}
+
+constexpr int kTileRows = 8;
+
+// A warp's ring: `stages` slots of `slot` bytes, one barrier each.
+struct WarpRing {
+  uint32_t bars, data, slot;
+  int stages;
+  __device__ __forceinline__ uint32_t bar(int s) const { return bars + 8 * s; }
+  __device__ __forceinline__ uint32_t at(int s) const { return data + s * slot; }
+};
+__device__ __forceinline__ WarpRing warp_ring(char* smem, int stages, uint32_t slot) {
+  // barriers of all warps first, then the slots
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const uint32_t base = tc::smem_addr(smem);
+  WarpRing r;
+  r.bars = base + warp * stages * 8;
+  r.data = base + ((warps * stages * 8 + 127) & ~127) + uint32_t(warp) * stages * slot;
+  r.slot = slot;
+  r.stages = stages;
+  if ((threadIdx.x & 31) == 0) {
+    for (int s = 0; s < stages; ++s) tc::bar_init(r.bar(s), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  __syncwarp();
+  return r;
+}
+
+// Plain copies of a last tile with fewer than eight rows.
+template <class T>
+__device__ __forceinline__ void copy_in(char* dst, const T* src, int count, int lane) {
+  for (int i = lane; i < count; i += 32) reinterpret_cast<T*>(dst)[i] = src[i];
+}
+template <class T>
+__device__ __forceinline__ void copy_out(T* dst, const char* src, int count, int lane) {
+  for (int i = lane; i < count; i += 32) dst[i] = reinterpret_cast<const T*>(src)[i];
+}
+
+template <class T, int VEC, int NV>
+__global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs a, int tpr, int stages) {
+  constexpr int E = NV * VEC;
+  using P = Pack<T, VEC>;
+  extern __shared__ __align__(128) char smem[];
+  const uint32_t base = tc::smem_addr(smem);
+  const uint32_t tile_bytes = kTileRows * a.dims * sizeof(T);
+  const WarpRing ring = warp_ring(smem, stages, (tile_bytes + 127) & ~127u);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = lane & (tpr - 1), group = lane / tpr, at_once = 32 / tpr;
+  const int nvec = a.dims / VEC;
+  const float inv_n = 1.0f / float(a.dims);
+  const int64_t tiles = (a.rows + kTileRows - 1) / kTileRows;
+  const int64_t full_tiles = a.rows / kTileRows;
+  const int64_t first = int64_t(blockIdx.x) * (blockDim.x >> 5) + warp;
+  const int64_t step = int64_t(gridDim.x) * (blockDim.x >> 5);
+  const T* const x = static_cast<const T*>(a.x);
+  T* const y = static_cast<T*>(a.y);
+
+  float w[E], b[E];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int q = sub + k * tpr;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const bool in = q < nvec;
+      w[k * VEC + j] = a.weight && in ? to_f32(static_cast<const T*>(a.weight)[q * VEC + j]) : 1.0f;
+      b[k * VEC + j] = a.bias && in ? to_f32(static_cast<const T*>(a.bias)[q * VEC + j]) : 0.0f;
+    }
+  }
+  auto request = [&](int64_t tile, int slot) {  // lane 0
+    if (tile < full_tiles) {
+      tc::bar_expect(ring.bar(slot), tile_bytes);
+      bulk_load(ring.at(slot), x + tile * kTileRows * a.dims, tile_bytes, ring.bar(slot));
+    }
+  };
+  if (lane == 0)
+    for (int s = 0; s < stages - 1; ++s) request(first + s * step, s);
+  int slot = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int64_t tile = first; tile < tiles; tile += step) {
+    char* const at = smem + (ring.at(slot) - base);
+    const int rows = int(min(int64_t(kTileRows), a.rows - tile * kTileRows));
+    if (rows == kTileRows) {
+      ok = __all_sync(kFull, tc::bar_wait(ring.bar(slot), phase));
+      if (!ok) break;
+    } else {
+      if (lane == 0) tc::bulk_wait_read<0>();
+      __syncwarp();
+      copy_in<T>(at, x + tile * kTileRows * a.dims, rows * a.dims, lane);
+      __syncwarp();
+    }
+    for (int r0 = 0; r0 < kTileRows; r0 += at_once) {
+      const int r = r0 + group;
+      P* const row = reinterpret_cast<P*>(at + size_t(r) * a.dims * sizeof(T));
+      float v[E];
+      float s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int q = sub + k * tpr;
+        if (r < rows && q < nvec) {
+          const P p = row[q];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            v[k * VEC + j] = to_f32(p.v[j]);
+            s += v[k * VEC + j];
+          }
+        }
+      }
+      const float mean = lanes_sum(tpr, s) * inv_n;
+      float var = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (r < rows && sub + k * tpr < nvec) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            v[k * VEC + j] -= mean;
+            var += v[k * VEC + j] * v[k * VEC + j];
+          }
+        }
+      const float rstd = 1.0f / sqrtf(lanes_sum(tpr, var) * inv_n + a.eps);
+      if (r >= rows) continue;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int q = sub + k * tpr;
+        if (q < nvec) {
+          P p;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            p.v[j] = from_f32<T>(v[k * VEC + j] * rstd * w[k * VEC + j] + b[k * VEC + j]);
+          row[q] = p;
+        }
+      }
+      if (sub == 0) {
+        if (a.mean) a.mean[tile * kTileRows + r] = mean;
+        if (a.rstd) a.rstd[tile * kTileRows + r] = rstd;
+      }
+    }
+    if (rows == kTileRows) {
+      tc::fence_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        bulk_store(y + tile * kTileRows * a.dims, ring.at(slot), tile_bytes);
+        tc::bulk_commit();
+        // the slot before this one: its results have left once all groups but
+        // the one just committed have been read
+        tc::bulk_wait_read<1>();
+        request(tile + (stages - 1) * step, slot == 0 ? stages - 1 : slot - 1);
+      }
+    } else {
+      __syncwarp();
+      copy_out<T>(y + tile * kTileRows * a.dims, at, rows * a.dims, lane);
+    }
+    if (++slot == stages) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+  if (lane == 0) tc::bulk_wait_all();
+  if (!ok && lane == 0) {
+    atomicAdd(&g_timeouts, 1ull);
+    // copies in flight must land before the block may leave
+    for (int s = 0; s < stages; ++s) tc::bar_wait(ring.bar(s), s < slot ? phase ^ 1 : phase);
+  }
+}
+
+// The slots of the backward ring: x (dx in place), dy, residual, mean, rstd.
+__host__ __device__ inline uint32_t backward_slot(uint32_t tile_bytes, bool residual) {
+  return ((residual ? 3 : 2) * tile_bytes + 2 * kTileRows * 4 + 127) & ~127u;
+}
+
+template <class T, int VEC, int NV>
+__global__ void __launch_bounds__(256, 2)
+layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, int tpr, int stages) {
+  constexpr int E = NV * VEC;
+  using P = Pack<T, VEC>;
+  extern __shared__ __align__(128) char smem[];
+  const uint32_t base = tc::smem_addr(smem);
+  const uint32_t tile_bytes = kTileRows * a.dims * sizeof(T);
+  const WarpRing ring = warp_ring(smem, stages, backward_slot(tile_bytes, a.residual != nullptr));
+  const uint32_t stats = (a.residual ? 3 : 2) * tile_bytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int sub = lane & (tpr - 1), group = lane / tpr, at_once = 32 / tpr;
+  const int nvec = a.dims / VEC;
+  const float inv_n = 1.0f / float(a.dims);
+  const int64_t tiles = (a.rows + kTileRows - 1) / kTileRows;
+  const int64_t full_tiles = a.rows / kTileRows;
+  const int64_t first = int64_t(blockIdx.x) * warps + warp;
+  const int64_t step = int64_t(gridDim.x) * warps;
+  const T* const x = static_cast<const T*>(a.x);
+  const T* const dy = static_cast<const T*>(a.dy);
+  const T* const res = static_cast<const T*>(a.residual);
+  T* const dx = static_cast<T*>(a.dx);
+
+  float w[E], dw[E], db[E];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int q = sub + k * tpr;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      w[k * VEC + j] =
+          a.weight && q < nvec ? to_f32(static_cast<const T*>(a.weight)[q * VEC + j]) : 1.0f;
+      dw[k * VEC + j] = db[k * VEC + j] = 0.0f;
+    }
+  }
+  auto request = [&](int64_t tile, int slot) {  // lane 0
+    if (tile < full_tiles) {
+      const int64_t row = tile * kTileRows, from = row * a.dims;
+      const uint32_t bar = ring.bar(slot), at = ring.at(slot);
+      tc::bar_expect(bar, stats + 2 * kTileRows * 4);
+      bulk_load(at, x + from, tile_bytes, bar);
+      bulk_load(at + tile_bytes, dy + from, tile_bytes, bar);
+      if (res) bulk_load(at + 2 * tile_bytes, res + from, tile_bytes, bar);
+      bulk_load(at + stats, a.mean + row, kTileRows * 4, bar);
+      bulk_load(at + stats + kTileRows * 4, a.rstd + row, kTileRows * 4, bar);
+    }
+  };
+  if (lane == 0)
+    for (int s = 0; s < stages - 1; ++s) request(first + s * step, s);
+  int slot = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int64_t tile = first; tile < tiles; tile += step) {
+    char* const at = smem + (ring.at(slot) - base);
+    const int64_t from = tile * kTileRows * a.dims;
+    const int rows = int(min(int64_t(kTileRows), a.rows - tile * kTileRows));
+    if (rows == kTileRows) {
+      ok = __all_sync(kFull, tc::bar_wait(ring.bar(slot), phase));
+      if (!ok) break;
+    } else {
+      if (lane == 0) tc::bulk_wait_read<0>();
+      __syncwarp();
+      copy_in<T>(at, x + from, rows * a.dims, lane);
+      copy_in<T>(at + tile_bytes, dy + from, rows * a.dims, lane);
+      if (res) copy_in<T>(at + 2 * tile_bytes, res + from, rows * a.dims, lane);
+      copy_in<float>(at + stats, a.mean + tile * kTileRows, rows, lane);
+      copy_in<float>(at + stats + kTileRows * 4, a.rstd + tile * kTileRows, rows, lane);
+      __syncwarp();
+    }
+    for (int r0 = 0; r0 < kTileRows; r0 += at_once) {
+      const int r = r0 + group;
+      const bool active = r < rows;
+      P* const row = reinterpret_cast<P*>(at + size_t(r) * a.dims * sizeof(T));
+      const P* const grow = reinterpret_cast<const P*>(reinterpret_cast<const char*>(row) + tile_bytes);
+      const float* const st = reinterpret_cast<const float*>(at + stats);
+      const float rstd = active ? st[kTileRows + r] : 0.0f;
+      const float mean = active ? st[r] : 0.0f;
+      float xh[E], g[E];
+      float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int q = sub + k * tpr;
+        if (active && q < nvec) {
+          const P px = row[q], pg = grow[q];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const int e = k * VEC + j;
+            const float d = to_f32(pg.v[j]);
+            xh[e] = (to_f32(px.v[j]) - mean) * rstd;
+            dw[e] += d * xh[e];
+            db[e] += d;
+            g[e] = d * w[e];
+            s1 += g[e];
+            s2 += g[e] * xh[e];
+          }
+        }
+      }
+      for (int o = tpr >> 1; o > 0; o >>= 1) {
+        s1 += __shfl_xor_sync(kFull, s1, o);
+        s2 += __shfl_xor_sync(kFull, s2, o);
+      }
+      s1 *= inv_n;
+      s2 *= inv_n;
+      const P* const rrow =
+          reinterpret_cast<const P*>(reinterpret_cast<const char*>(row) + 2 * tile_bytes);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int q = sub + k * tpr;
+        if (active && q < nvec) {
+          P p, pr;
+          if (res) pr = rrow[q];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const int e = k * VEC + j;
+            float d = rstd * (g[e] - s1 - xh[e] * s2);
+            if (res) d += to_f32(pr.v[j]);
+            p.v[j] = from_f32<T>(d);
+          }
+          row[q] = p;
+        }
+      }
+    }
+    if (rows == kTileRows) {
+      tc::fence_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        if (dx) bulk_store(dx + from, ring.at(slot), tile_bytes);
+        tc::bulk_commit();
+        tc::bulk_wait_read<1>();
+        request(tile + (stages - 1) * step, slot == 0 ? stages - 1 : slot - 1);
+      }
+    } else {
+      __syncwarp();
+      if (dx) copy_out<T>(dx + from, at, rows * a.dims, lane);
+    }
+    if (++slot == stages) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+  if (lane == 0) tc::bulk_wait_all();
+  if (!ok && lane == 0) {
+    atomicAdd(&g_timeouts, 1ull);
+    for (int s = 0; s < stages; ++s) tc::bar_wait(ring.bar(s), s < slot ? phase ^ 1 : phase);
+  }
+  if (!a.partials) return;
+  // the block's dw and db: the row groups add to shared columns in turn
+  __syncthreads();
+  float* const columns = reinterpret_cast<float*>(
+      smem + ((warps * stages * 8 + 127) & ~127));
+  for (int turn = 0; turn < warps * at_once; ++turn) {
+    if (turn == warp * at_once + group) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int q = sub + k * tpr;
+        if (q < nvec) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            float* const c = columns + q * VEC + j;
+            c[0] = turn == 0 ? dw[k * VEC + j] : c[0] + dw[k * VEC + j];
+            c[a.dims] = turn == 0 ? db[k * VEC + j] : c[a.dims] + db[k * VEC + j];
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  float* const part = a.partials + int64_t(blockIdx.x) * 2 * a.dims;
+  for (int i = threadIdx.x; i < 2 * a.dims; i += blockDim.x) part[i] = columns[i];
+}
+
+// ---- wide rows: a block per row, rows copied ahead ----
+template <class T, int NV>
+__global__ void __launch_bounds__(512) layer_norm_wide_kernel(LayerNormArgs a, int stages) {
+  constexpr int VEC = 16 / int(sizeof(T)), E = NV * VEC;
+  using P = Pack<T, VEC>;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ float sums[128];
+  __shared__ uint64_t bars[8];
+  RowSum rs{sums};
+  const int nvec = a.dims / VEC, threads = blockDim.x;
+  const uint32_t row_bytes = a.dims * sizeof(T), slot_bytes = (row_bytes + 127) & ~127u;
+  const uint32_t base = tc::smem_addr(smem), bar0 = tc::smem_addr(bars);
+  const float inv_n = 1.0f / float(a.dims);
+  const T* const x = static_cast<const T*>(a.x);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) tc::bar_init(bar0 + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  __syncthreads();
+  auto request = [&](int64_t row, int slot) {  // thread 0
+    if (row < a.rows) {
+      tc::bar_expect(bar0 + 8 * slot, row_bytes);
+      bulk_load(base + slot * slot_bytes, x + row * a.x_stride, row_bytes, bar0 + 8 * slot);
+    }
+  };
+  if (threadIdx.x == 0)
+    for (int s = 0; s < stages; ++s) request(blockIdx.x + int64_t(s) * gridDim.x, s);
+  int slot = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    ok = tc::bar_wait(bar0 + 8 * slot, phase);
+    ok = __syncthreads_and(ok);
+    if (!ok) break;
+    const P* const in = reinterpret_cast<const P*>(smem + slot * slot_bytes);
+    float v[E];
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = threadIdx.x + k * threads;
+      if (q < nvec) {
+        const P p = in[q];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[k * VEC + j] = to_f32(p.v[j]);
+          s += v[k * VEC + j];
+        }
+      }
+    }
+    const float mean = row_sum<true>(rs, 0, s) * inv_n;
+    // past the barrier in row_sum every thread has read the slot
+    if (threadIdx.x == 0) request(row + int64_t(stages) * gridDim.x, slot);
+    float var = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (int(threadIdx.x) + k * threads < nvec) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[k * VEC + j] -= mean;
+          var += v[k * VEC + j] * v[k * VEC + j];
+        }
+      }
+    const float rstd = 1.0f / sqrtf(row_sum<true>(rs, 0, var) * inv_n + a.eps);
+    P* const out = reinterpret_cast<P*>(static_cast<T*>(a.y) + row * a.y_stride);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = threadIdx.x + k * threads;
+      if (q >= nvec) continue;
+      P p, pw, pb;
+      if (a.weight) pw = static_cast<const P*>(a.weight)[q];
+      if (a.bias) pb = static_cast<const P*>(a.bias)[q];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float o = v[k * VEC + j] * rstd;
+        if (a.weight) o *= to_f32(pw.v[j]);
+        if (a.bias) o += to_f32(pb.v[j]);
+        p.v[j] = from_f32<T>(o);
+      }
+      out[q] = p;
+    }
+    if (threadIdx.x == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+    if (++slot == stages) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+  if (!ok && threadIdx.x == 0) {
+    atomicAdd(&g_timeouts, 1ull);
+    for (int s = 0; s < stages; ++s) tc::bar_wait(bar0 + 8 * s, s < slot ? phase ^ 1 : phase);
+  }
+}
+
+template <class T, int NV, bool PARAMS>
+__global__ void __launch_bounds__(512) layer_norm_backward_wide_kernel(LayerNormBackwardArgs a,
+                                                                       int stages) {
+  constexpr int VEC = 16 / int(sizeof(T)), E = NV * VEC;
+  using P = Pack<T, VEC>;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ float sums[128];
+  __shared__ uint64_t bars[8];
+  RowSum rs{sums};
+  const int nvec = a.dims / VEC, threads = blockDim.x;
+  const uint32_t row_bytes = a.dims * sizeof(T), pitch = (row_bytes + 127) & ~127u;
+  const uint32_t slot_bytes = 2 * pitch;
+  const uint32_t base = tc::smem_addr(smem), bar0 = tc::smem_addr(bars);
+  const float inv_n = 1.0f / float(a.dims);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) tc::bar_init(bar0 + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  __syncthreads();
+  auto request = [&](int64_t row, int slot) {  // thread 0
+    if (row < a.rows) {
+      const uint32_t bar = bar0 + 8 * slot, at = base + slot * slot_bytes;
+      tc::bar_expect(bar, 2 * row_bytes);
+      bulk_load(at, static_cast<const T*>(a.x) + row * a.x_stride, row_bytes, bar);
+      bulk_load(at + pitch, static_cast<const T*>(a.dy) + row * a.dy_stride, row_bytes, bar);
+    }
+  };
+  if (threadIdx.x == 0)
+    for (int s = 0; s < stages; ++s) request(blockIdx.x + int64_t(s) * gridDim.x, s);
+  float dw[E], db[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
+  int slot = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    // loads that do not go through the ring: under the wait
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    P pw[NV], pr[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = threadIdx.x + k * threads;
+      if (q < nvec) {
+        if (a.weight) pw[k] = static_cast<const P*>(a.weight)[q];
+        if (a.residual)
+          pr[k] = reinterpret_cast<const P*>(static_cast<const T*>(a.residual) +
+                                             row * a.residual_stride)[q];
+      }
+    }
+    ok = tc::bar_wait(bar0 + 8 * slot, phase);
+    ok = __syncthreads_and(ok);
+    if (!ok) break;
+    const P* const in = reinterpret_cast<const P*>(smem + slot * slot_bytes);
+    const P* const gin = reinterpret_cast<const P*>(smem + slot * slot_bytes + pitch);
+    float xh[E], g[E];
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = threadIdx.x + k * threads;
+      if (q < nvec) {
+        const P px = in[q], pg = gin[q];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int e = k * VEC + j;
+          xh[e] = (to_f32(px.v[j]) - mean) * rstd;
+          g[e] = to_f32(pg.v[j]);
+          if (PARAMS) {
+            dw[e] += g[e] * xh[e];
+            db[e] += g[e];
+          }
+          if (a.weight) g[e] *= to_f32(pw[k].v[j]);
+          s1 += g[e];
+          s2 += g[e] * xh[e];
+        }
+      }
+    }
+    row_sum2<true>(rs, 0, s1, s2);
+    // past the barrier in row_sum2 every thread has read the slot
+    if (threadIdx.x == 0) request(row + int64_t(stages) * gridDim.x, slot);
+    if (++slot == stages) {
+      slot = 0;
+      phase ^= 1;
+    }
+    if (!a.dx) continue;
+    s1 *= inv_n;
+    s2 *= inv_n;
+    P* const out = reinterpret_cast<P*>(static_cast<T*>(a.dx) + row * a.dx_stride);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = threadIdx.x + k * threads;
+      if (q >= nvec) continue;
+      P p;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int e = k * VEC + j;
+        float d = rstd * (g[e] - s1 - xh[e] * s2);
+        if (a.residual) d += to_f32(pr[k].v[j]);
+        p.v[j] = from_f32<T>(d);
+      }
+      out[q] = p;
+    }
+  }
+  if (!ok && threadIdx.x == 0) {
+    atomicAdd(&g_timeouts, 1ull);
+    for (int s = 0; s < stages; ++s) tc::bar_wait(bar0 + 8 * s, s < slot ? phase ^ 1 : phase);
+  }
+  if (!PARAMS) return;
+  float* const part = a.partials + int64_t(blockIdx.x) * 2 * a.dims;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int q = threadIdx.x + k * threads;
+    if (q >= nvec) continue;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      part[q * VEC + j] = dw[k * VEC + j];
+      part[a.dims + q * VEC + j] = db[k * VEC + j];
     }
   }
 }
@@ -361,45 +948,78 @@ __global__ void __launch_bounds__(256) column_reduce_kernel(const float* __restr
   if (out) out[col < dims ? col : col - dims] = from_f32<T>(s);
 }
 
-// How a row is spread over threads.
+// How a row is spread over threads, in accesses of `vec` values.
 struct RowPlan {
-  int vec;      // values per access
-  int nv;       // accesses per thread (1, 2, 3, 4 or 8); 0: the long kernel
-  int tpr;      // threads per row
-  bool block;   // the whole block has one row
+  int vec;
+  int nv;      // accesses per thread; 0: the long kernel
+  int tpr;     // threads per row
+  bool block;  // the whole block has one row
 };
 
 bool aligned(const void* p, int64_t stride, size_t sz, int vec) {
   return !p || (reinterpret_cast<uintptr_t>(p) % (sz * vec) == 0 && stride % vec == 0);
 }
 
-// The widest access that every buffer allows, then the fewest threads whose
-// registers hold the row: up to `most` values per thread.
-RowPlan plan_row(size_t sz, int dims, int widest, int most) {
+// Accesses per thread at most (16 to 20 values, which the backward kernels hold
+// four times over: xhat, g, dw, db), and the number aimed at where a warp's
+// lanes have a row.
+int aimed_accesses(int vec) { return vec == 8 ? 2 : vec == 4 ? 3 : vec == 2 ? 5 : 9; }
+int most_accesses(int vec) { return vec == 8 ? 2 : vec == 4 ? 5 : vec == 2 ? 9 : 16; }
+
+// Lanes of a warp to a row, or nv = 0 where a warp cannot hold it.  Few lanes
+// with many values each: fewer shuffle steps and address computations per
+// value (130 columns: 8 lanes with nine pairs).
+RowPlan plan_lanes(int dims, int vec) {
   RowPlan p{};
-  p.vec = widest;
-  const int nvec = dims / p.vec;
-  const int nv_most = std::min(8, most / p.vec);
-  auto round_nv = [](int nv) { return nv <= 4 ? nv : 8; };
-  if (nvec <= 32 * nv_most) {
-    int tpr = 4;
-    // a row's threads: about four accesses each while a warp has enough
-    while (tpr < 32 && (nvec + tpr - 1) / tpr > std::min(4, nv_most)) tpr *= 2;
-    p.tpr = tpr;
-    p.nv = round_nv((nvec + tpr - 1) / tpr);
-    return p;
-  }
+  p.vec = vec;
+  const int nvec = dims / vec, most = most_accesses(vec);
+  p.tpr = nvec >= 8 ? 8 : 4;
+  while (p.tpr < 32 && (nvec + p.tpr - 1) / p.tpr > aimed_accesses(vec)) p.tpr *= 2;
+  const int nv = (nvec + p.tpr - 1) / p.tpr;
+  p.nv = nv <= most ? nv : 0;
+  return p;
+}
+// A warp's lanes or a block for rows that are read with plain loads.
+RowPlan plan_row(int dims, int vec) {
+  RowPlan p = plan_lanes(dims, vec);
+  if (p.nv) return p;
   p.block = true;
-  for (int nv : {1, 2, 4, 8}) {
-    if (nv > nv_most) break;
+  const int nvec = dims / vec, most = most_accesses(vec);
+  for (int nv = 1; nv <= most; ++nv) {
     const int threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;
-    if (threads <= 512) {
-      p.nv = nv;
-      p.tpr = threads;
-      if (threads <= 256) break;
-    }
+    if (threads > 512) continue;
+    p.nv = nv;
+    p.tpr = threads;
+    if (threads <= 256) break;
   }
   return p;
+}
+
+// Calls f(integral_constant<VEC>, integral_constant<NV>) with the smallest
+// instance that has room for nv accesses.
+template <class T, class F>
+auto with_row_shape(int vec, int nv, F&& f) {
+  using std::integral_constant;
+  if (vec == 1) {
+    if (nv <= 2) return f(integral_constant<int, 1>(), integral_constant<int, 2>());
+    if (nv <= 5) return f(integral_constant<int, 1>(), integral_constant<int, 5>());
+    if (nv <= 9) return f(integral_constant<int, 1>(), integral_constant<int, 9>());
+    return f(integral_constant<int, 1>(), integral_constant<int, 16>());
+  }
+  if (vec == 2) {
+    if (nv <= 2) return f(integral_constant<int, 2>(), integral_constant<int, 2>());
+    if (nv <= 5) return f(integral_constant<int, 2>(), integral_constant<int, 5>());
+    return f(integral_constant<int, 2>(), integral_constant<int, 9>());
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (vec == 8) {
+      if (nv <= 1) return f(integral_constant<int, 8>(), integral_constant<int, 1>());
+      return f(integral_constant<int, 8>(), integral_constant<int, 2>());
+    }
+  }
+  if (nv <= 2) return f(integral_constant<int, 4>(), integral_constant<int, 2>());
+  if (nv <= 3) return f(integral_constant<int, 4>(), integral_constant<int, 3>());
+  return f(integral_constant<int, 4>(), integral_constant<int, 5>());
 }
 
 int sm_count() {
@@ -432,7 +1052,7 @@ template <class T, int VEC, int NV, bool PARAMS>
 int backward_launch(const LayerNormBackwardArgs& a, const RowPlan& p, cudaStream_t stream) {
   if (p.block) {
     const int64_t grid = std::min<int64_t>(std::min<int64_t>(a.rows, kMaxPartials),
-                                             int64_t(sm_count()) * (1024 / p.tpr));
+                                           int64_t(sm_count()) * (1024 / p.tpr));
     layer_norm_backward_kernel<T, VEC, NV, true, PARAMS>
         <<<unsigned(grid), p.tpr, 0, stream>>>(a, p.tpr);
     return int(grid);
@@ -447,74 +1067,175 @@ int backward_launch(const LayerNormBackwardArgs& a, const RowPlan& p, cudaStream
   return int(grid);
 }
 
-template <class T, int VEC, bool PARAMS>
-int backward_nv(const LayerNormBackwardArgs& a, const RowPlan& p, cudaStream_t s) {
-  switch (p.nv) {
-    case 1: return backward_launch<T, VEC, 1, PARAMS>(a, p, s);
-    case 2: return backward_launch<T, VEC, 2, PARAMS>(a, p, s);
-    default: break;
-  }
-  if constexpr (VEC * 4 <= 16) {
-    switch (p.nv) {
-      case 3: return backward_launch<T, VEC, 3, PARAMS>(a, p, s);
-      case 4: return backward_launch<T, VEC, 4, PARAMS>(a, p, s);
-      default: break;
-    }
-  }
-  if constexpr (VEC * 8 <= 16) return backward_launch<T, VEC, 8, PARAMS>(a, p, s);
-  return 0;
+bool bulk_rows(const void* p, int64_t stride, size_t size) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * int64_t(size) % 16 == 0);
+}
+bool gapless(const void* p, int64_t stride, int64_t rows, int dims) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride == dims || rows <= 1));
 }
 
-template <class T, bool PARAMS>
-int backward_vec(const LayerNormBackwardArgs& a, const RowPlan& p, cudaStream_t s) {
-  switch (p.vec) {
-    case 1: return backward_nv<T, 1, PARAMS>(a, p, s);
-    case 2: return backward_nv<T, 2, PARAMS>(a, p, s);
-    case 4: return backward_nv<T, 4, PARAMS>(a, p, s);
-    default: break;
+constexpr size_t kSmemPerSm = 220 * 1024;
+
+// The tile ring's shape, or row.nv = 0 where a tile has no place.
+struct TilePlan {
+  RowPlan row;
+  int warps, stages;
+  size_t smem;
+};
+TilePlan plan_tiles(size_t size, int dims, int64_t rows, uint32_t slot) {
+  TilePlan p{};
+  int vec = 16 / int(size);
+  while (dims % vec) vec /= 2;
+  RowPlan row = plan_lanes(dims, vec);
+  // few tiles: fewer warps to a block, so that every SM has some
+  const int64_t tiles = (rows + kTileRows - 1) / kTileRows;
+  p.warps = 8;
+  while (p.warps > 1 && tiles < int64_t(p.warps) * 148) p.warps /= 2;
+  // two blocks of eight warps to an SM (their registers allow no more), one
+  // where two slots per warp would not fit otherwise
+  for (int blocks = 2 * (8 / p.warps); blocks >= 1; --blocks) {
+    p.stages = int(std::min<size_t>(4, kSmemPerSm / blocks / (size_t(p.warps) * (slot + 8) + 128)));
+    if (p.stages >= 2) break;
   }
-  if constexpr (sizeof(T) == 2) return backward_nv<T, 8, PARAMS>(a, p, s);
-  return 0;
+  if (p.stages < 2) return p;
+  p.smem = ((size_t(p.warps) * p.stages * 8 + 127) & ~size_t(127)) + size_t(p.warps) * p.stages * slot;
+  p.smem = (p.smem + 4095) & ~size_t(4095);  // few distinct launch shapes
+  p.row = row;
+  return p;
+}
+template <class K>
+npa_status tile_grid(K kernel, const TilePlan& p, int64_t rows, unsigned* grid) {
+  int per_sm = 0, sms = 0;
+  NPA_TRY(kernel_occupancy(reinterpret_cast<const void*>(kernel), p.warps * 32, p.smem, &per_sm, &sms));
+  if (per_sm < 1) return fail(NPA_ERR_UNSUPPORTED, "layer norm kernel cannot be resident");
+  const int64_t tiles = (rows + kTileRows - 1) / kTileRows;
+  *grid = unsigned(std::min<int64_t>(
+      std::min<int64_t>((tiles + p.warps - 1) / p.warps, int64_t(per_sm) * sms), kMaxPartials));
+  return NPA_OK;
 }
 
-template <class T, int VEC>
-void forward_nv(const LayerNormArgs& a, const RowPlan& p, cudaStream_t s) {
-  switch (p.nv) {
-    case 1: return forward_launch<T, VEC, 1>(a, p, s);
-    case 2: return forward_launch<T, VEC, 2>(a, p, s);
-    case 3: return forward_launch<T, VEC, 3>(a, p, s);
-    case 4: return forward_launch<T, VEC, 4>(a, p, s);
-    default: break;
+// Wide rows: 16-byte accesses, NV of them per thread.
+struct WidePlan {
+  int nv, threads, stages;
+  size_t smem;
+};
+WidePlan plan_wide(size_t size, int dims, size_t slot, int most) {
+  WidePlan p{};
+  const int vec = 16 / int(size), nvec = dims / vec;
+  if (dims % vec || nvec < 64) return p;
+  for (int nv = most; nv >= 1; nv /= 2) {
+    p.threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;
+    p.nv = nv;
+    if (p.threads >= 128) break;
   }
-  if constexpr (VEC * 8 <= 32) forward_launch<T, VEC, 8>(a, p, s);
+  if (p.threads > 512) return WidePlan{};
+  const int blocks = std::max(1, 768 / p.threads);
+  p.stages = int(std::min<size_t>(6, std::max<size_t>(2, kSmemPerSm / (blocks * slot))));
+  p.smem = (p.stages * slot + 4095) & ~size_t(4095);  // few distinct launch shapes
+  return p.smem <= kSmemPerSm ? p : WidePlan{};
+}
+template <class K>
+npa_status wide_grid(K kernel, const WidePlan& p, int64_t rows, unsigned* grid) {
+  int per_sm = 0, sms = 0;
+  NPA_TRY(kernel_occupancy(reinterpret_cast<const void*>(kernel), p.threads, p.smem, &per_sm, &sms));
+  if (per_sm < 1) return fail(NPA_ERR_UNSUPPORTED, "layer norm kernel cannot be resident");
+  *grid = unsigned(std::min<int64_t>(std::min<int64_t>(rows, kMaxPartials), int64_t(per_sm) * sms));
+  return NPA_OK;
 }
 
 template <class T>
 npa_status forward_typed(const LayerNormArgs& a, cudaStream_t s) {
+  if (gapless(a.x, a.x_stride, a.rows, a.dims) && gapless(a.y, a.y_stride, a.rows, a.dims)) {
+    const uint32_t slot = (uint32_t(std::min(a.dims, 1 << 16)) * kTileRows * sizeof(T) + 127) & ~127u;
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, slot);
+    if (p.row.nv)
+      return with_row_shape<T>(p.row.vec, p.row.nv, [&](auto vec, auto nv) -> npa_status {
+        const auto kernel = layer_norm_tiles_kernel<T, vec(), nv()>;
+        unsigned grid = 0;
+        NPA_TRY(tile_grid(kernel, p, a.rows, &grid));
+        kernel<<<grid, p.warps * 32, p.smem, s>>>(a, p.row.tpr, p.stages);
+        return after_launch("layer_norm_tiles_kernel");
+      });
+  }
+  if (bulk_rows(a.x, a.x_stride, sizeof(T)) && bulk_rows(a.y, a.y_stride, sizeof(T)) &&
+      bulk_rows(a.weight, 0, sizeof(T)) && bulk_rows(a.bias, 0, sizeof(T))) {
+    const size_t slot = (size_t(a.dims) * sizeof(T) + 127) & ~size_t(127);
+    const WidePlan p = plan_wide(sizeof(T), a.dims, slot, sizeof(T) == 2 ? 2 : 4);
+    if (p.nv) {
+      auto launch = [&](auto kernel) -> npa_status {
+        unsigned grid = 0;
+        NPA_TRY(wide_grid(kernel, p, a.rows, &grid));
+        kernel<<<grid, p.threads, p.smem, s>>>(a, p.stages);
+        return after_launch("layer_norm_wide_kernel");
+      };
+      if (p.nv == 1) return launch(layer_norm_wide_kernel<T, 1>);
+      if (p.nv == 2) return launch(layer_norm_wide_kernel<T, 2>);
+      if constexpr (sizeof(T) == 4) return launch(layer_norm_wide_kernel<T, 4>);
+    }
+  }
   int vec = 16 / int(sizeof(T));
   while (vec > 1 && (a.dims % vec || !aligned(a.x, a.x_stride, sizeof(T), vec) ||
                      !aligned(a.y, a.y_stride, sizeof(T), vec) ||
                      !aligned(a.weight, 0, sizeof(T), vec) || !aligned(a.bias, 0, sizeof(T), vec)))
     vec /= 2;
-  const RowPlan p = plan_row(sizeof(T), a.dims, vec, 32);
+  const RowPlan p = plan_row(a.dims, vec);
   if (p.nv == 0) {
     const int64_t grid = std::min<int64_t>(a.rows, int64_t(sm_count()) * 4);
     layer_norm_long_kernel<T><<<unsigned(grid), 512, 0, s>>>(a);
     return after_launch("layer_norm_long_kernel");
   }
-  switch (p.vec) {
-    case 1: forward_nv<T, 1>(a, p, s); break;
-    case 2: forward_nv<T, 2>(a, p, s); break;
-    case 4: forward_nv<T, 4>(a, p, s); break;
-    default:
-      if constexpr (sizeof(T) == 2) forward_nv<T, 8>(a, p, s);
-  }
+  with_row_shape<T>(p.vec, p.nv, [&](auto v, auto nv) {
+    forward_launch<T, v(), nv()>(a, p, s);
+    return 0;
+  });
   return after_launch("layer_norm_kernel");
 }
 
+// The gradient kernels over the rows; *parts: partial sums left for dw and db.
 template <class T>
-npa_status backward_typed(const LayerNormBackwardArgs& a, cudaStream_t s) {
-  const bool params = a.dweight || a.dbias;
+npa_status backward_rows(const LayerNormBackwardArgs& a, int* parts, cudaStream_t s) {
+  const bool params = a.partials != nullptr;
+  if (gapless(a.x, a.x_stride, a.rows, a.dims) && gapless(a.dy, a.dy_stride, a.rows, a.dims) &&
+      gapless(a.dx, a.dx_stride, a.rows, a.dims) &&
+      gapless(a.residual, a.residual_stride, a.rows, a.dims) && bulk_rows(a.mean, 0, 4) &&
+      bulk_rows(a.rstd, 0, 4)) {
+    const uint32_t slot =
+        backward_slot(uint32_t(std::min(a.dims, 1 << 16)) * kTileRows * sizeof(T), a.residual != nullptr);
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, slot);
+    if (p.row.nv)
+      return with_row_shape<T>(p.row.vec, p.row.nv, [&](auto vec, auto nv) -> npa_status {
+        const auto kernel = layer_norm_backward_tiles_kernel<T, vec(), nv()>;
+        unsigned grid = 0;
+        NPA_TRY(tile_grid(kernel, p, a.rows, &grid));
+        kernel<<<grid, p.warps * 32, p.smem, s>>>(a, p.row.tpr, p.stages);
+        *parts = int(grid);
+        return after_launch("layer_norm_backward_tiles_kernel");
+      });
+  }
+  if (bulk_rows(a.x, a.x_stride, sizeof(T)) && bulk_rows(a.dy, a.dy_stride, sizeof(T)) &&
+      bulk_rows(a.dx, a.dx_stride, sizeof(T)) && bulk_rows(a.weight, 0, sizeof(T)) &&
+      bulk_rows(a.residual, a.residual_stride, sizeof(T))) {
+    const size_t slot = 2 * ((size_t(a.dims) * sizeof(T) + 127) & ~size_t(127));
+    const WidePlan p = plan_wide(sizeof(T), a.dims, slot, sizeof(T) == 2 ? 2 : 4);
+    if (p.nv) {
+      auto launch = [&](auto kernel) -> npa_status {
+        unsigned grid = 0;
+        NPA_TRY(wide_grid(kernel, p, a.rows, &grid));
+        kernel<<<grid, p.threads, p.smem, s>>>(a, p.stages);
+        *parts = int(grid);
+        return after_launch("layer_norm_backward_wide_kernel");
+      };
+      if (p.nv == 1)
+        return params ? launch(layer_norm_backward_wide_kernel<T, 1, true>)
+                      : launch(layer_norm_backward_wide_kernel<T, 1, false>);
+      if (p.nv == 2)
+        return params ? launch(layer_norm_backward_wide_kernel<T, 2, true>)
+                      : launch(layer_norm_backward_wide_kernel<T, 2, false>);
+      if constexpr (sizeof(T) == 4)
+        return params ? launch(layer_norm_backward_wide_kernel<T, 4, true>)
+                      : launch(layer_norm_backward_wide_kernel<T, 4, false>);
+    }
+  }
   int vec = 16 / int(sizeof(T));
   while (vec > 1 &&
          (a.dims % vec || !aligned(a.x, a.x_stride, sizeof(T), vec) ||
@@ -522,26 +1243,36 @@ npa_status backward_typed(const LayerNormBackwardArgs& a, cudaStream_t s) {
           !aligned(a.dx, a.dx_stride, sizeof(T), vec) || !aligned(a.weight, 0, sizeof(T), vec) ||
           !aligned(a.residual, a.residual_stride, sizeof(T), vec)))
     vec /= 2;
-  const RowPlan p = plan_row(sizeof(T), a.dims, vec, 16);
-  int parts = 0;
+  const RowPlan p = plan_row(a.dims, vec);
   if (p.nv == 0) {
-    if (a.dx && a.rows > 0) {
+    if (a.dx) {
       const int64_t grid = std::min<int64_t>(a.rows, int64_t(sm_count()) * 4);
       layer_norm_backward_long_kernel<T><<<unsigned(grid), 512, 0, s>>>(a);
       NPA_TRY(after_launch("layer_norm_backward_long_kernel"));
     }
-    if (params && a.rows > 0) {
-      parts = int(std::min<int64_t>(a.rows, kLongSplits));
-      const int64_t per = (a.rows + parts - 1) / parts;
-      parts = int((a.rows + per - 1) / per);
-      column_partials_kernel<T><<<dim3(unsigned((a.dims + 255) / 256), unsigned(parts)), 256, 0, s>>>(
-          a, per);
+    if (params) {
+      *parts = int(std::min<int64_t>(a.rows, kLongSplits));
+      const int64_t per = (a.rows + *parts - 1) / *parts;
+      *parts = int((a.rows + per - 1) / per);
+      column_partials_kernel<T>
+          <<<dim3(unsigned((a.dims + 255) / 256), unsigned(*parts)), 256, 0, s>>>(a, per);
       NPA_TRY(after_launch("column_partials_kernel"));
     }
-  } else if (a.rows > 0 && (a.dx || params)) {
-    parts = params ? backward_vec<T, true>(a, p, s) : backward_vec<T, false>(a, p, s);
-    NPA_TRY(after_launch("layer_norm_backward_kernel"));
+    return NPA_OK;
   }
+  *parts = with_row_shape<T>(p.vec, p.nv, [&](auto v, auto nv) -> int {
+    return params ? backward_launch<T, v(), nv(), true>(a, p, s)
+                  : backward_launch<T, v(), nv(), false>(a, p, s);
+  });
+  return after_launch("layer_norm_backward_kernel");
+}
+
+template <class T>
+npa_status backward_typed(LayerNormBackwardArgs a, cudaStream_t s) {
+  const bool params = a.dweight || a.dbias;
+  if (!params) a.partials = nullptr;
+  int parts = 0;
+  if (a.rows > 0 && (a.dx || params)) NPA_TRY(backward_rows<T>(a, &parts, s));
   if (!params) return NPA_OK;
   column_reduce_kernel<T><<<unsigned((2 * int64_t(a.dims) + 31) / 32), 256, 0, s>>>(
       a.partials, parts, a.dims, static_cast<T*>(a.dweight), static_cast<T*>(a.dbias));
@@ -570,6 +1301,15 @@ npa_status launch_layer_norm_backward(int dtype, const LayerNormBackwardArgs& a,
     case NPA_DTYPE_F16: return backward_typed<__half>(a, stream);
     default: return backward_typed<__nv_bfloat16>(a, stream);
   }
+}
+
+uint64_t layer_norm_timeouts() {
+  unsigned long long v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_timeouts, sizeof(v)) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return v;
 }
 
 }  // namespace npa

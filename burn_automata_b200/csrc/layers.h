@@ -69,6 +69,8 @@ struct LayerNormBackwardArgs {
   void* dbias;    // optional
   float* partials;
 };
+// Bounded waits of the layer norm kernels that gave up on the current device.
+uint64_t layer_norm_timeouts();
 size_t layer_norm_backward_workspace(int64_t rows, int dims);
 npa_status launch_layer_norm_backward(int dtype, const LayerNormBackwardArgs& a,
                                       cudaStream_t stream);

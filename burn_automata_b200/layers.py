@@ -61,21 +61,25 @@ class LinearGradients:
 
 _torch = None
 _dtypes = {}
+_raw_stream = None
 
 
 def _t():
-    global _torch
+    global _torch, _raw_stream
     if _torch is None:
         import torch
 
         _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        # a stream object costs microseconds; the handle alone does not
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
         _torch = torch
     return _torch
 
 
 def _dtype(x, name: str) -> int:
     """The C ABI's storage type of a CUDA tensor."""
-    torch = _t()
+    torch = _torch or _t()
     if not isinstance(x, torch.Tensor):
         raise InvalidArgument(f"{name} must be a torch tensor")
     code = _dtypes.get(x.dtype)
@@ -89,7 +93,7 @@ def _dtype(x, name: str) -> int:
 
 
 def _like(t, x, name: str):
-    if not isinstance(t, type(x)) and not isinstance(t, _t().Tensor):
+    if not isinstance(t, _torch.Tensor):
         raise InvalidArgument(f"{name} must be a torch tensor")
     if t.dtype != x.dtype or t.device != x.device:
         raise InvalidArgument(f"{name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
@@ -118,47 +122,57 @@ def _vector(t, x, size: int, name: str):
     _like(t, x, name)
     if t.dim() != 1 or t.shape[0] != size:
         raise InvalidArgument(f"{name} has shape {tuple(t.shape)}, expected ({size},)")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _statistic(t, x, name: str):
-    if not isinstance(t, _t().Tensor) or t.dtype != _torch.float32 or t.device != x.device:
+    if not isinstance(t, _torch.Tensor) or t.dtype != _torch.float32 or t.device != x.device:
         raise InvalidArgument(f"{name} must be a float32 tensor on {x.device}")
     if t.shape != x.shape[:-1]:
         raise InvalidArgument(f"{name} has shape {tuple(t.shape)}, expected "
                               f"{tuple(x.shape[:-1])}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _needs(needs, weight_given: bool = True):
+def _needs(needs):
     want = set(needs)
     if not want <= {"x", "weight", "bias"}:
         raise InvalidArgument(f"needs may name x, weight and bias, got {sorted(want)}")
     return want
 
 
-class _on_device:
-    """The launching thread's current device for one call."""
+def _call(entry, device, args, name: str) -> None:
+    """entry(*args, stream) on the device's current stream."""
+    index = device.index
+    if index == _torch.cuda.current_device():
+        status = entry(*args, _raw_stream(index))
+    else:
+        with _torch.cuda.device(index):
+            status = entry(*args, _raw_stream(index))
+    if status:
+        _lib.check(status, name)
 
-    def __init__(self, device):
-        self.device = device
-        self.guard = None
 
-    def __enter__(self):
-        torch = _torch
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
+def _workspace(x, query, args, name: str):
+    """(tensor or None, bytes) of the workspace that the query asks for."""
+    need = ctypes.c_size_t(0)
+    status = query(*args, ctypes.byref(need))
+    if status:
+        _lib.check(status, name)
+    if not need.value:
+        return None, 0
+    return x.new_empty(need.value, dtype=_torch.uint8), need.value
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+
+def _outputs_like(x, shape):
+    """An uninitialised contiguous tensor of x's type."""
+    if x.shape == shape and x.is_contiguous():
+        return _torch.empty_like(x)
+    return x.new_empty(shape)
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> LayerNormOutput:
@@ -169,13 +183,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> LayerNormOutput:
     dims = x.shape[-1]
     w, b = _vector(weight, x, dims, "weight"), _vector(bias, x, dims, "bias")
     xr, xs = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    y = _outputs_like(x, x.shape)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    with _on_device(x.device) as stream:
-        _lib.check(_lib.lib().npa_dev_layer_norm(
-            code, xr.data_ptr(), xs, _ptr(w), _ptr(b), mean.numel(), dims, float(eps),
-            y.data_ptr(), dims, mean.data_ptr(), rstd.data_ptr(), stream), "layer_norm")
+    _call(_lib.lib().npa_dev_layer_norm, x.device,
+          (code, xr.data_ptr(), xs, _ptr(w), _ptr(b), mean.numel(), dims, float(eps),
+           y.data_ptr(), dims, mean.data_ptr(), rstd.data_ptr()), "layer_norm")
     return LayerNormOutput(y, mean, rstd)
 
 
@@ -186,7 +199,6 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, residual_gradient=None,
     added to x's on the way.  `needs` names the gradients to compute: x,
     weight and bias by default, x alone when there is no weight."""
     code = _dtype(x, "x")
-    torch = _torch
     dims = x.shape[-1]
     want = _needs(needs if needs is not None else
                   (("x", "weight", "bias") if weight is not None else ("x",)))
@@ -198,23 +210,19 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, residual_gradient=None,
         residual_gradient, x, x.shape, "residual_gradient")
     if rr is not None and "x" not in want:
         raise InvalidArgument("residual_gradient is added to x's gradient, which is not needed")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if "x" in want else None
-    dw = torch.empty(dims, dtype=x.dtype, device=x.device) if "weight" in want else None
-    db = torch.empty(dims, dtype=x.dtype, device=x.device) if "bias" in want else None
+    dx = _outputs_like(x, x.shape) if "x" in want else None
+    dw = x.new_empty(dims) if "weight" in want else None
+    db = x.new_empty(dims) if "bias" in want else None
     rows = m.numel()
     L = _lib.lib()
-    with _on_device(x.device) as stream:
-        ws, ws_bytes = None, 0
-        if dw is not None or db is not None:
-            need = ctypes.c_size_t(0)
-            _lib.check(L.npa_dev_layer_norm_backward_workspace_size(
-                code, rows, dims, ctypes.byref(need)), "layer_norm_backward")
-            ws_bytes = need.value
-            ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=x.device)
-        _lib.check(L.npa_dev_layer_norm_backward(
-            code, dyr.data_ptr(), dys, xr.data_ptr(), xs, m.data_ptr(), r.data_ptr(), _ptr(w),
-            _ptr(rr), rs, rows, dims, _ptr(dx), dims, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes,
-            stream), "layer_norm_backward")
+    ws, ws_bytes = None, 0
+    if dw is not None or db is not None:
+        ws, ws_bytes = _workspace(x, L.npa_dev_layer_norm_backward_workspace_size,
+                                  (code, rows, dims), "layer_norm_backward")
+    _call(L.npa_dev_layer_norm_backward, x.device,
+          (code, dyr.data_ptr(), dys, xr.data_ptr(), xs, m.data_ptr(), r.data_ptr(), _ptr(w),
+           _ptr(rr), rs, rows, dims, _ptr(dx), dims, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes),
+          "layer_norm_backward")
     return LayerNormGradients(dx, dw, db)
 
 
@@ -240,18 +248,15 @@ def linear(x, weight, bias=None, residual=None, activation: Activation = Activat
     rr, rs = (None, 0) if residual is None else _matrix(residual, x, out_shape, "residual")
     xr, xs = _rows(x)
     rows = x.numel() // inputs if inputs else 0
-    y = torch.empty(out_shape, dtype=x.dtype, device=x.device)
+    y = _outputs_like(x, out_shape)
     z = torch.empty_like(y) if save_pre_activation else None
     L = _lib.lib()
-    with _on_device(x.device) as stream:
-        need = ctypes.c_size_t(0)
-        _lib.check(L.npa_dev_linear_workspace_size(code, rows, inputs, outputs,
-                                                   ctypes.byref(need)), "linear")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
-        _lib.check(L.npa_dev_linear(
-            code, int(activation), xr.data_ptr(), xs, wr.data_ptr(), wstride, _ptr(b), _ptr(rr),
-            rs, rows, inputs, outputs, y.data_ptr(), outputs, _ptr(z), outputs, _ptr(ws),
-            need.value, stream), "linear")
+    ws, ws_bytes = _workspace(x, L.npa_dev_linear_workspace_size, (code, rows, inputs, outputs),
+                              "linear")
+    _call(L.npa_dev_linear, x.device,
+          (code, int(activation), xr.data_ptr(), xs, wr.data_ptr(), wstride, _ptr(b), _ptr(rr), rs,
+           rows, inputs, outputs, y.data_ptr(), outputs, _ptr(z), outputs, _ptr(ws), ws_bytes),
+          "linear")
     return LinearOutput(y, z)
 
 
@@ -262,7 +267,6 @@ def linear_backward(dy, x, weight, pre_activation=None,
     identity) its saved pre-activation.  `needs` names the gradients to
     compute."""
     code = _dtype(x, "x")
-    torch = _torch
     inputs, outputs = _layer_shape(x, weight)
     out_shape = x.shape[:-1] + (outputs,)
     want = _needs(needs)
@@ -275,18 +279,14 @@ def linear_backward(dy, x, weight, pre_activation=None,
         zr, zs = _matrix(pre_activation, x, out_shape, "pre_activation")
     xr, xs = _rows(x)
     rows = x.numel() // inputs if inputs else 0
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if "x" in want else None
-    dw = (torch.empty(weight.shape, dtype=x.dtype, device=x.device) if "weight" in want
-          else None)
-    db = torch.empty(outputs, dtype=x.dtype, device=x.device) if "bias" in want else None
+    dx = _outputs_like(x, x.shape) if "x" in want else None
+    dw = _outputs_like(weight, weight.shape) if "weight" in want else None
+    db = x.new_empty(outputs) if "bias" in want else None
     L = _lib.lib()
-    with _on_device(x.device) as stream:
-        need = ctypes.c_size_t(0)
-        _lib.check(L.npa_dev_linear_backward_workspace_size(
-            code, int(activation), rows, inputs, outputs, ctypes.byref(need)), "linear_backward")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
-        _lib.check(L.npa_dev_linear_backward(
-            code, int(activation), dyr.data_ptr(), dys, xr.data_ptr(), xs, wr.data_ptr(), wstride,
-            _ptr(zr), zs, rows, inputs, outputs, _ptr(dx), inputs, _ptr(dw), _ptr(db), _ptr(ws),
-            need.value, stream), "linear_backward")
+    ws, ws_bytes = _workspace(x, L.npa_dev_linear_backward_workspace_size,
+                              (code, int(activation), rows, inputs, outputs), "linear_backward")
+    _call(L.npa_dev_linear_backward, x.device,
+          (code, int(activation), dyr.data_ptr(), dys, xr.data_ptr(), xs, wr.data_ptr(), wstride,
+           _ptr(zr), zs, rows, inputs, outputs, _ptr(dx), inputs, _ptr(dw), _ptr(db), _ptr(ws),
+           ws_bytes), "linear_backward")
     return LinearGradients(dx, dw, db)
