@@ -938,6 +938,7 @@ __global__ void __launch_bounds__(256) column_reduce_kernel(const float* __restr
   const int64_t col = int64_t(blockIdx.x) * 32 + tx;  // over [2][dims]
   float s = 0.0f;
   if (col < 2 * int64_t(dims))
+#pragma unroll 8
     for (int p = ty; p < count; p += 8) s += partials[int64_t(p) * 2 * dims + col];
   acc[ty][tx] = s;
   __syncthreads();

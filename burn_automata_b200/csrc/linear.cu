@@ -16,30 +16,48 @@ using linear_tc::Operand;
 using linear_tc::Product;
 
 // ---- the split product's layers, summed in order, with the epilogue ----
-// A thread has four columns of a row.
+// A block has 32 groups of four columns; its eight warps each add every eighth
+// layer, and the first adds the eight sums in order.
 template <class T>
 __global__ void __launch_bounds__(256) product_reduce_kernel(const __grid_constant__ Product p) {
+  __shared__ float4 sums[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t quads = (p.n + 3) / 4;
-  const int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (e >= int64_t(p.m) * quads) return;
+  const int64_t e = int64_t(blockIdx.x) * 32 + lane;
+  const bool mine = e < int64_t(p.m) * quads;
   const int64_t row = e / quads, col = e % quads * 4;
   const int64_t layer = int64_t(p.m_tiles) * linear_tc::kBM * p.partial_pitch;
-  const float* at = p.partials + row * p.partial_pitch + col;
-  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.splits; ++s, at += layer) {
-    const float4 f = *reinterpret_cast<const float4*>(at);
-    v[0] += f.x;
-    v[1] += f.y;
-    v[2] += f.z;
-    v[3] += f.w;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (mine) {
+    const float* const at = p.partials + row * p.partial_pitch + col;
+#pragma unroll 8
+    for (int s = warp; s < p.splits; s += 8) {
+      const float4 f = *reinterpret_cast<const float4*>(at + s * layer);
+      v.x += f.x;
+      v.y += f.y;
+      v.z += f.z;
+      v.w += f.w;
+    }
   }
+  sums[warp][lane] = v;
+  __syncthreads();
+  if (warp != 0 || !mine) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) {
+    const float4 f = sums[w][lane];
+    v.x += f.x;
+    v.y += f.y;
+    v.z += f.z;
+    v.w += f.w;
+  }
+  const float total[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (col + j >= p.n) break;
-    float z = v[j];
+    float z = total[j];
     if (p.bias) z += to_f32(static_cast<const T*>(p.bias)[col + j]);
     if (p.z) static_cast<T*>(p.z)[row * p.z_stride + col + j] = from_f32<T>(z);
-    float y = linear_tc::activation(p.act, z);
+    float y = linear_tc::activation<sizeof(T) == 2>(p.act, z);
     if (p.residual)
       y += to_f32(static_cast<const T*>(p.residual)[row * p.residual_stride + col + j]);
     static_cast<T*>(p.y)[row * p.y_stride + col + j] = from_f32<T>(y);
@@ -65,30 +83,50 @@ struct SlopeArgs {
 // the unrounded values.  A thread has VEC columns of every (256 / tx)th row.
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ SlopeArgs a) {
+  using P = Pack<T, VEC>;
   __shared__ float sums[256 * VEC];
+  constexpr int kAhead = sizeof(P) == 16 ? 4 : 8;  // rows in flight per thread
   const int tx = threadIdx.x & (a.tx - 1), ty = threadIdx.x / a.tx, rows_at_once = 256 / a.tx;
   const int64_t col = (int64_t(blockIdx.x) * a.tx + tx) * VEC;
   const bool mine = col < a.outputs;
   const int64_t begin = int64_t(blockIdx.y) * a.rows_per_block;
   const int64_t end = min(begin + a.rows_per_block, a.rows);
+  const T* const dy = static_cast<const T*>(a.dy) + col;
+  const T* const z = static_cast<const T*>(a.z) + col;
+  T* const dz = static_cast<T*>(a.dz) + col;
   float s[VEC] = {};
   if (mine) {
-#pragma unroll 4
-    for (int64_t r = begin + ty; r < end; r += rows_at_once) {
-      const Pack<T, VEC> g =
-          *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + r * a.dy_stride + col);
-      Pack<T, VEC> zz, out;
-      if (a.z)
-        zz = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.z) + r * a.z_stride + col);
+    for (int64_t r0 = begin + ty; r0 < end; r0 += int64_t(kAhead) * rows_at_once) {
+      P g[kAhead], zz[kAhead];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float d = to_f32(g.v[j]);
-        if (a.z) d *= linear_tc::activation_slope(a.act, to_f32(zz.v[j]));
-        s[j] += d;
-        out.v[j] = from_f32<T>(d);
+      for (int i = 0; i < kAhead; ++i) {
+        const int64_t r = r0 + int64_t(i) * rows_at_once;
+        if (r < end) {
+          g[i] = *reinterpret_cast<const P*>(dy + r * a.dy_stride);
+          if (a.z) zz[i] = *reinterpret_cast<const P*>(z + r * a.z_stride);
+        }
       }
-      if (a.dz)
-        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dz) + r * a.dz_stride + col) = out;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int64_t r = r0 + int64_t(i) * rows_at_once;
+        if (r >= end) break;
+        float d[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) d[j] = to_f32(g[i].v[j]);
+        if (a.z) {
+          float zf[VEC];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) zf[j] = to_f32(zz[i].v[j]);
+          linear_tc::times_slope<sizeof(T) == 2>(a.act, d, zf);
+        }
+        P out;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          s[j] += d[j];
+          out.v[j] = from_f32<T>(d[j]);
+        }
+        if (a.dz) *reinterpret_cast<P*>(dz + r * a.dz_stride) = out;
+      }
     }
   }
 #pragma unroll
@@ -110,6 +148,7 @@ __global__ void __launch_bounds__(256) bias_reduce_kernel(const float* __restric
   const int col = blockIdx.x * 32 + tx;
   float s = 0.0f;
   if (col < outputs)
+#pragma unroll 8
     for (int p = ty; p < count; p += 8) s += partials[int64_t(p) * outputs + col];
   acc[ty][tx] = s;
   __syncthreads();
@@ -189,17 +228,28 @@ struct Plan {
 Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
   Plan p{};
   p.m_tiles = ceil_div(m, linear_tc::kBM);
-  // The widest tile moves the fewest operand bytes; narrower ones only where
-  // the widest would leave SMs idle or columns empty.
-  p.bn = size == 2 && tma ? 256 : 128;
-  while (p.bn > 64 && (p.bn / 2 >= n || int64_t(p.m_tiles) * ceil_div(n, p.bn) < kSms)) p.bn /= 2;
-  p.n_tiles = ceil_div(n, p.bn);
   p.k_blocks = ceil_div(k, linear_tc::kBK);
-  const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles;
-  // Few tiles over a long sum: layers of at least four k blocks each.
-  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(kSms / tiles, p.k_blocks / 4)));
-  p.split_blocks = ceil_div(p.k_blocks, p.splits);
-  p.splits = ceil_div(p.k_blocks, p.split_blocks);
+  // The shape with the least work on the fullest SM.  A k block of a tile 256,
+  // 128 or 64 columns wide costs about 8, 5 and 4 units (the narrow tiles
+  // fetch the same rows of A for fewer products), its epilogue as much as two
+  // blocks, and layers of a split sum their traffic: each at least four blocks.
+  int64_t best = INT64_MAX;
+  for (int bn = size == 2 && tma ? 256 : 128; bn >= 64; bn /= 2) {
+    if (bn > 64 && bn / 2 >= n) continue;
+    const int64_t tiles = int64_t(p.m_tiles) * ceil_div(n, bn);
+    int splits = int(std::max<int64_t>(1, std::min<int64_t>(kSms / tiles, p.k_blocks / 4)));
+    const int blocks = ceil_div(p.k_blocks, splits);
+    splits = ceil_div(p.k_blocks, blocks);
+    const int64_t unit = bn == 256 ? 8 : bn == 128 ? 5 : 4;
+    const int64_t cost = ceil_div(tiles * splits, kSms) * (blocks + 2) * unit + (splits > 1 ? 16 : 0);
+    if (cost < best) {
+      best = cost;
+      p.bn = bn;
+      p.n_tiles = ceil_div(n, bn);
+      p.splits = splits;
+      p.split_blocks = blocks;
+    }
+  }
   p.partial_pitch = (n + 3) / 4 * 4;
   return p;
 }
@@ -281,7 +331,7 @@ npa_status run_product(Product p, float* partials, cudaStream_t stream) {
   }
   if (!p.partials) return NPA_OK;
   product_reduce_kernel<T>
-      <<<grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 256), 256, 0, stream>>>(p);
+      <<<grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32), 256, 0, stream>>>(p);
   return after_launch("product_reduce_kernel");
 }
 

@@ -80,30 +80,47 @@ struct Config {
   static_assert(kStages >= 2 && kTmemColumns <= 512, "tile does not fit");
 };
 
-// act(z) and act'(z).  NaN stays NaN.
+// act(z) and act'(z).  NaN stays NaN.  FAST (16-bit storage): exponentials and
+// quotients by the approximate instructions, whose errors of a few 2^-22 vanish
+// in a result that is rounded to 8 or 11 bits; f32 storage takes the library's.
+template <bool FAST>
+__device__ __forceinline__ float exponential(float x) {
+  return FAST ? __expf(x) : expf(x);
+}
+// 1 / (1 + e^-z).  Where e^-z overflows both forms give 0.
+template <bool FAST>
+__device__ __forceinline__ float logistic(float z) {
+  const float d = 1.0f + exponential<FAST>(-z);
+  return FAST ? __fdividef(1.0f, d) : 1.0f / d;
+}
+template <bool FAST>
 __device__ __forceinline__ float activation(int act, float z) {
   switch (act) {
     case NPA_ACTIVATION_RELU: return z < 0.0f ? 0.0f : z;
     case NPA_ACTIVATION_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case NPA_ACTIVATION_GELU_TANH:
-      return 0.5f * z * (1.0f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
-    case NPA_ACTIVATION_SILU: return z / (1.0f + expf(-z));
+    case NPA_ACTIVATION_GELU_TANH: {
+      const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
+      return FAST ? z * logistic<true>(2.0f * u) : 0.5f * z * (1.0f + tanhf(u));
+    }
+    case NPA_ACTIVATION_SILU: return FAST ? z * logistic<true>(z) : z / (1.0f + expf(-z));
     default: return z;
   }
 }
+template <bool FAST>
 __device__ __forceinline__ float activation_slope(int act, float z) {
   switch (act) {
     case NPA_ACTIVATION_RELU: return z <= 0.0f ? 0.0f : 1.0f;
     case NPA_ACTIVATION_GELU:
       return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-             z * 0.39894228040143268f * expf(-0.5f * z * z);
+             z * 0.39894228040143268f * exponential<FAST>(-0.5f * z * z);
     case NPA_ACTIVATION_GELU_TANH: {
-      const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
-      return 0.5f * (1.0f + t) +
-             0.5f * z * (1.0f - t * t) * 0.79788456080286536f * (1.0f + 0.134145f * z * z);
+      // (1 + tanh(u)) / 2 = p = logistic(2u), and its derivative is 2 p (1 - p) u'
+      const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
+      const float p = logistic<FAST>(2.0f * u);
+      return p + 2.0f * z * p * (1.0f - p) * 0.79788456080286536f * (1.0f + 0.134145f * z * z);
     }
     case NPA_ACTIVATION_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
+      const float s = logistic<FAST>(z);
       return s * (1.0f + z * (1.0f - s));
     }
     default: return 1.0f;
@@ -111,24 +128,47 @@ __device__ __forceinline__ float activation_slope(int act, float z) {
 }
 
 // The activation of a thread's N values, the choice outside the loop.
-template <int N>
+template <bool FAST, int N>
 __device__ __forceinline__ void activate(int act, float (&v)[N]) {
   switch (act) {
     case NPA_ACTIVATION_RELU:
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = activation(NPA_ACTIVATION_RELU, v[i]);
+      for (int i = 0; i < N; ++i) v[i] = activation<FAST>(NPA_ACTIVATION_RELU, v[i]);
       break;
     case NPA_ACTIVATION_GELU:
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = activation(NPA_ACTIVATION_GELU, v[i]);
+      for (int i = 0; i < N; ++i) v[i] = activation<FAST>(NPA_ACTIVATION_GELU, v[i]);
       break;
     case NPA_ACTIVATION_GELU_TANH:
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = activation(NPA_ACTIVATION_GELU_TANH, v[i]);
+      for (int i = 0; i < N; ++i) v[i] = activation<FAST>(NPA_ACTIVATION_GELU_TANH, v[i]);
       break;
     case NPA_ACTIVATION_SILU:
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = activation(NPA_ACTIVATION_SILU, v[i]);
+      for (int i = 0; i < N; ++i) v[i] = activation<FAST>(NPA_ACTIVATION_SILU, v[i]);
+      break;
+    default: break;
+  }
+}
+// v[i] *= act'(z[i]).
+template <bool FAST, int N>
+__device__ __forceinline__ void times_slope(int act, float (&v)[N], const float (&z)[N]) {
+  switch (act) {
+    case NPA_ACTIVATION_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] *= activation_slope<FAST>(NPA_ACTIVATION_RELU, z[i]);
+      break;
+    case NPA_ACTIVATION_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] *= activation_slope<FAST>(NPA_ACTIVATION_GELU, z[i]);
+      break;
+    case NPA_ACTIVATION_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] *= activation_slope<FAST>(NPA_ACTIVATION_GELU_TANH, z[i]);
+      break;
+    case NPA_ACTIVATION_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] *= activation_slope<FAST>(NPA_ACTIVATION_SILU, z[i]);
       break;
     default: break;
   }
@@ -648,7 +688,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           put_group<T>(b, pointer(b), lane, &map_z, p.z_tma, col0, int(row0), p.z, p.z_stride,
                        row0, rows, cols);
         }
-        activate(p.act, v);
+        activate<sizeof(T) == 2>(p.act, v);
         const uint32_t b = next_buffer();
         if (p.residual) {
           if (res_vec) {
