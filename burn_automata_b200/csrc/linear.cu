@@ -6,6 +6,7 @@
 // The three products run on product_kernel (linear_product.cuh); the sums over
 // rows that give db, and dz itself, come from slope_kernel.
 #include <algorithm>
+#include <atomic>
 
 #include "linear_product.cuh"
 
@@ -26,7 +27,7 @@ __global__ void __launch_bounds__(256) product_reduce_kernel(const __grid_consta
   const int64_t e = int64_t(blockIdx.x) * 32 + lane;
   const bool mine = e < int64_t(p.m) * quads;
   const int64_t row = e / quads, col = e % quads * 4;
-  const int64_t layer = int64_t(p.m_tiles) * linear_tc::kBM * p.partial_pitch;
+  const int64_t layer = p.layer_rows * p.partial_pitch;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (mine) {
     const float* const at = p.partials + row * p.partial_pitch + col;
@@ -216,41 +217,54 @@ npa_status make_map(CUtensorMap* map, const void* p, int64_t width, int64_t rows
 
 int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
-// Tile width and k splits of an m x n x k product.
+// Tile shape and k splits of an m x n x k product.
 struct Plan {
   int bn;
+  bool pair;
   int m_tiles, n_tiles, k_blocks, splits, split_blocks;
+  int64_t layer_rows, partial_pitch;
   size_t partial_bytes() const {
-    return splits > 1 ? size_t(splits) * m_tiles * linear_tc::kBM * partial_pitch * 4 : 0;
+    return splits > 1 ? size_t(splits) * layer_rows * partial_pitch * 4 : 0;
   }
-  int64_t partial_pitch;
 };
 Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
   Plan p{};
-  p.m_tiles = ceil_div(m, linear_tc::kBM);
   p.k_blocks = ceil_div(k, linear_tc::kBK);
+  p.partial_pitch = (n + 3) / 4 * 4;
   // The shape with the least work on the fullest SM.  A k block of a tile 256,
   // 128 or 64 columns wide costs about 8, 5 and 4 units (the narrow tiles
-  // fetch the same rows of A for fewer products), its epilogue as much as two
-  // blocks, and layers of a split sum their traffic: each at least four blocks.
+  // fetch the same rows of A for fewer products; a pair's fetches less than
+  // its 256 columns would alone: 6), its epilogue as much as two blocks, and
+  // layers of a split sum their traffic: each at least four blocks.
+  struct Shape {
+    int bn, unit;
+    bool pair;
+  };
+  constexpr Shape kShapes[] = {{256, 6, true}, {256, 8, false}, {128, 5, false}, {64, 4, false}};
   int64_t best = INT64_MAX;
-  for (int bn = size == 2 && tma ? 256 : 128; bn >= 64; bn /= 2) {
-    if (bn > 64 && bn / 2 >= n) continue;
-    const int64_t tiles = int64_t(p.m_tiles) * ceil_div(n, bn);
-    int splits = int(std::max<int64_t>(1, std::min<int64_t>(kSms / tiles, p.k_blocks / 4)));
+  for (const Shape& shape : kShapes) {
+    if (shape.bn == 256 && !(size == 2 && tma)) continue;
+    if (shape.bn > 64 && shape.bn / 2 >= n) continue;
+    if (shape.pair && m <= linear_tc::kBM) continue;
+    const int rows = shape.pair ? 2 * linear_tc::kBM : linear_tc::kBM;
+    const int walkers = shape.pair ? kSms / 2 : kSms;
+    const int64_t tiles = int64_t(ceil_div(m, rows)) * ceil_div(n, shape.bn);
+    int splits = int(std::max<int64_t>(1, std::min<int64_t>(walkers / tiles, p.k_blocks / 4)));
     const int blocks = ceil_div(p.k_blocks, splits);
     splits = ceil_div(p.k_blocks, blocks);
-    const int64_t unit = bn == 256 ? 8 : bn == 128 ? 5 : 4;
-    const int64_t cost = ceil_div(tiles * splits, kSms) * (blocks + 2) * unit + (splits > 1 ? 16 : 0);
+    const int64_t cost =
+        ceil_div(tiles * splits, walkers) * (blocks + 2) * shape.unit + (splits > 1 ? 16 : 0);
     if (cost < best) {
       best = cost;
-      p.bn = bn;
-      p.n_tiles = ceil_div(n, bn);
+      p.bn = shape.bn;
+      p.pair = shape.pair;
+      p.m_tiles = ceil_div(m, rows);
+      p.n_tiles = ceil_div(n, shape.bn);
       p.splits = splits;
       p.split_blocks = blocks;
+      p.layer_rows = int64_t(p.m_tiles) * rows;
     }
   }
-  p.partial_pitch = (n + 3) / 4 * 4;
   return p;
 }
 size_t product_workspace(size_t size, int64_t m, int64_t n, int64_t k) {
@@ -267,17 +281,65 @@ int vector_width(const void* p, int64_t stride, int64_t rows) {
   return vec;
 }
 
-template <class T, bool LOADER, int BN>
+// Blocks of the pair kernel that run at once on the current device.
+template <class K>
+npa_status pair_blocks(K kernel, int threads, size_t smem, int sms, int* blocks) {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  NPA_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+  const int known = dev < 64 ? cached[dev].load() : 0;
+  if (known) {
+    *blocks = known;
+    return NPA_OK;
+  }
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(sms / 2 * 2));
+  config.blockDim = dim3(unsigned(threads));
+  config.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  int clusters = 0;
+  NPA_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel, &config),
+           "cudaOccupancyMaxActiveClusters");
+  if (clusters < 1) return fail(NPA_ERR_UNSUPPORTED, "linear pair kernel cannot be resident");
+  *blocks = 2 * clusters;
+  if (dev < 64) cached[dev].store(*blocks);
+  return NPA_OK;
+}
+
+template <class T, bool LOADER, int BN, bool PAIR = false>
 npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, cudaStream_t stream) {
-  using C = linear_tc::Config<T, LOADER, BN>;
-  const auto kernel = linear_tc::product_kernel<T, LOADER, BN>;
+  using C = linear_tc::Config<T, LOADER, BN, PAIR>;
+  const auto kernel = linear_tc::product_kernel<T, LOADER, BN, PAIR>;
   int per_sm = 0, sms = 0;
   NPA_TRY(kernel_occupancy(reinterpret_cast<const void*>(kernel), C::kThreads, C::kSmemBytes,
                            &per_sm, &sms));
   if (per_sm < 1) return fail(NPA_ERR_UNSUPPORTED, "linear kernel cannot be resident");
   const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles * p.splits;
-  kernel<<<unsigned(std::min<int64_t>(tiles, sms)), C::kThreads, C::kSmemBytes, stream>>>(
-      maps[0], maps[1], maps[2], maps[3], p);
+  if constexpr (PAIR) {
+    int blocks = 0;
+    NPA_TRY(pair_blocks(kernel, C::kThreads, C::kSmemBytes, sms, &blocks));
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(unsigned(std::min<int64_t>(2 * tiles, blocks)));
+    config.blockDim = dim3(C::kThreads);
+    config.dynamicSmemBytes = C::kSmemBytes;
+    config.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    NPA_CUDA(cudaLaunchKernelEx(&config, kernel, maps[0], maps[1], maps[2], maps[3], p),
+             "linear product_kernel");
+  } else {
+    kernel<<<unsigned(std::min<int64_t>(tiles, sms)), C::kThreads, C::kSmemBytes, stream>>>(
+        maps[0], maps[1], maps[2], maps[3], p);
+  }
   return after_launch("linear product_kernel");
 }
 
@@ -295,10 +357,11 @@ npa_status run_product(Product p, float* partials, cudaStream_t stream) {
   p.k_blocks = plan.k_blocks;
   p.splits = plan.splits;
   p.split_blocks = plan.split_blocks;
+  p.layer_rows = plan.layer_rows;
   p.partial_pitch = plan.partial_pitch;
   p.partials = plan.splits > 1 ? partials : nullptr;
   p.idesc = tc::instruction_desc(!std::is_same<T, __half>::value, p.a.mn_major, p.b.mn_major,
-                                 linear_tc::kBM, plan.bn);
+                                 plan.pair ? 2 * linear_tc::kBM : linear_tc::kBM, plan.bn);
   p.a_vec = vector_width<T>(p.a.p, p.a.ld, a_rows);
   p.b_vec = vector_width<T>(p.b.p, p.b.ld, b_rows);
   p.y_tma = tma_rows(p.y, p.y_stride, p.m, sizeof(T));
@@ -310,11 +373,12 @@ npa_status run_product(Product p, float* partials, cudaStream_t stream) {
     NPA_TRY(p.a.mn_major ? make_map<T>(&maps[0], p.a.p, p.m, p.k, p.a.ld, linear_tc::kBK)
                          : make_map<T>(&maps[0], p.a.p, p.k, p.m, p.a.ld, linear_tc::kBM));
     NPA_TRY(p.b.mn_major ? make_map<T>(&maps[1], p.b.p, p.n, p.k, p.b.ld, linear_tc::kBK)
-                         : make_map<T>(&maps[1], p.b.p, p.k, p.n, p.b.ld, plan.bn));
+                         : make_map<T>(&maps[1], p.b.p, p.k, p.n, p.b.ld,
+                                       plan.pair ? plan.bn / 2 : plan.bn));
   }
   if (p.partials)
     NPA_TRY(make_map<float>(&maps[2], p.partials, p.n,
-                            int64_t(p.splits) * p.m_tiles * linear_tc::kBM, p.partial_pitch, 32));
+                            int64_t(p.splits) * p.layer_rows, p.partial_pitch, 32));
   else if (p.y_tma)
     NPA_TRY(make_map<T>(&maps[2], p.y, p.n, p.m, p.y_stride, 32));
   if (p.z_tma && !p.partials) NPA_TRY(make_map<T>(&maps[3], p.z, p.n, p.m, p.z_stride, 32));
@@ -322,7 +386,8 @@ npa_status run_product(Product p, float* partials, cudaStream_t stream) {
     NPA_TRY(plan.bn == 128 ? (launch_product<T, true, 128>(maps, p, stream))
                            : (launch_product<T, true, 64>(maps, p, stream)));
   } else if (tma) {
-    NPA_TRY(plan.bn == 256   ? (launch_product<T, false, 256>(maps, p, stream))
+    NPA_TRY(plan.pair        ? (launch_product<T, false, 256, true>(maps, p, stream))
+            : plan.bn == 256 ? (launch_product<T, false, 256>(maps, p, stream))
             : plan.bn == 128 ? (launch_product<T, false, 128>(maps, p, stream))
                              : (launch_product<T, false, 64>(maps, p, stream)));
   } else {

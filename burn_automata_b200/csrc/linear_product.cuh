@@ -56,18 +56,23 @@ struct Product {
   int64_t y_stride;
   void* z;
   int64_t z_stride;
-  float* partials;  // split: [splits][m_tiles * 128][partial_pitch], else null
-  int64_t partial_pitch;
+  float* partials;  // split: [splits][layer_rows][partial_pitch], else null
+  int64_t layer_rows, partial_pitch;
   int act;
   int y_tma, z_tma, bias_vec, residual_vec;
 };
 
 __device__ unsigned long long g_timeouts = 0;  // bounded waits that gave up
 
-template <class T, bool LOADER, int BN>
+// PAIR: two blocks (a cluster) have a tile of 256 rows, each its 128 rows of A
+// and half of B's rows: a block then fetches 32 KB for 512 cycles of products
+// instead of 48 KB, within what L2 delivers.
+template <class T, bool LOADER, int BN, bool PAIR>
 struct Config {
+  static constexpr int kTileRows = PAIR ? 2 * kBM : kBM;
+  static constexpr int kBRows = PAIR ? BN / 2 : BN;  // rows of B in one block
   static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
-  static constexpr int kABytes = kBM * 128, kBBytes = BN * 128;
+  static constexpr int kABytes = kBM * 128, kBBytes = kBRows * 128;
   static constexpr int kStageBytes = kParts * (kABytes + kBBytes);
   static constexpr int kOutBuffers = BN == 256 || kParts == 3 ? 1 : 2;
   static constexpr int kOutBytes = kEpilogueWarps * kOutBuffers * 4096;
@@ -361,12 +366,12 @@ __device__ __forceinline__ void put_group(uint32_t buf, const char* buf_ptr, int
             buf_ptr + swizzled(r, c / kPer))[c % kPer];
 }
 
-template <class T, bool LOADER, int BN>
-__global__ void __launch_bounds__((Config<T, LOADER, BN>::kThreads), 1)
+template <class T, bool LOADER, int BN, bool PAIR>
+__global__ void __launch_bounds__((Config<T, LOADER, BN, PAIR>::kThreads), 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z,
                const __grid_constant__ Product p) {
-  using C = Config<T, LOADER, BN>;
+  using C = Config<T, LOADER, BN, PAIR>;
   constexpr int kGroup = 128 / int(sizeof(T));         // output columns staged at a time
   constexpr int kGroups = BN / kGroup;
   constexpr int kGroupsPerWarp = (kGroups + 1) / 2;
@@ -380,6 +385,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const uint32_t drain = acc_empty + 16, tmem_at = drain + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kMmaWarp = kEpilogueWarps, kProducerWarp = kEpilogueWarps + 1;
+  // a pair walks the tiles together
+  const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
+  const int64_t walker = PAIR ? blockIdx.x / 2 : blockIdx.x;
+  const int64_t walkers = PAIR ? gridDim.x / 2 : gridDim.x;
   const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles * p.splits;
   const int64_t layer = int64_t(p.m_tiles) * p.n_tiles;
 
@@ -391,13 +400,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       }
       for (int b = 0; b < 2; ++b) {
         tc::bar_init(acc_full + 8 * b, 1);
-        tc::bar_init(acc_empty + 8 * b, kEpilogueWarps);
+        tc::bar_init(acc_empty + 8 * b, kEpilogueWarps * (PAIR ? 2 : 1));
       }
       tc::bar_init(drain, 1);
       asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     __syncwarp();
-    tc::tmem_alloc(tmem_at, C::kTmemColumns);
+    tc::tmem_alloc<PAIR>(tmem_at, C::kTmemColumns);
     tc::fence_before();
   }
   if (warp == kProducerWarp && lane == 0) {
@@ -409,6 +418,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (p.z_tma) tc::prefetch_map(&map_z);
   }
   __syncthreads();
+  if (PAIR) tc::cluster_sync();  // the other block's barriers are ready
   tc::fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(tmem) : "r"(tmem_at) : "memory");
@@ -419,34 +429,46 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (!LOADER) {
       if (lane == 0) {
         uint64_t it = 0;
-        for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const uint32_t first_full = PAIR ? tc::in_first_block(full) : full;
+        for (int64_t t = walker; t < tiles && ok; t += walkers) {
           const int split = int(t / layer), in = int(t % layer);
-          const int m0 = in / p.n_tiles * kBM, n0 = in % p.n_tiles * BN;
+          const int m0 = in / p.n_tiles * C::kTileRows + int(rank) * kBM;
+          const int n0 = in % p.n_tiles * BN + int(rank) * C::kBRows;
           const int kb = split * p.split_blocks;
           const int ke = min(p.k_blocks, kb + p.split_blocks);
           for (int kt = kb; kt < ke; ++kt, ++it) {
             const int s = int(it % C::kStages);
             ok = tc::bar_wait(empty + 8 * s, uint32_t(it / C::kStages & 1) ^ 1);
             if (!ok) break;
-            const uint32_t bar = full + 8 * s, a = base + s * C::kStageBytes, b = a + C::kABytes;
-            tc::bar_expect(bar, C::kABytes + C::kBBytes);
+            const uint32_t a = base + s * C::kStageBytes, b = a + C::kABytes;
+            const uint32_t bar = PAIR ? first_full + 8 * s : full + 8 * s;
+            if (rank == 0)
+              tc::bar_expect(full + 8 * s, (C::kABytes + C::kBBytes) * (PAIR ? 2 : 1));
+            auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+              if (PAIR)
+                tc::tma_load_pair(dst, map, x, y, bar);
+              else
+                tc::tma_load(dst, map, x, y, bar);
+            };
             if (p.a.mn_major) {
 #pragma unroll
-              for (int i = 0; i < kBM / 64; ++i)
-                tc::tma_load(a + i * 8192, &map_a, m0 + i * 64, kt * kBK, bar);
+              for (int i = 0; i < kBM / 64; ++i) load(a + i * 8192, &map_a, m0 + i * 64, kt * kBK);
             } else {
-              tc::tma_load(a, &map_a, kt * kBK, m0, bar);
+              load(a, &map_a, kt * kBK, m0);
             }
             if (p.b.mn_major) {
 #pragma unroll
-              for (int i = 0; i < BN / 64; ++i)
-                tc::tma_load(b + i * 8192, &map_b, n0 + i * 64, kt * kBK, bar);
+              for (int i = 0; i < C::kBRows / 64; ++i)
+                load(b + i * 8192, &map_b, n0 + i * 64, kt * kBK);
             } else {
-              tc::tma_load(b, &map_b, kt * kBK, n0, bar);
+              load(b, &map_b, kt * kBK, n0);
             }
           }
         }
-        if (!ok) {  // copies in flight must land before the block may leave
+        // copies in flight must land before the block may leave (the second block
+        // of a pair has no barrier of its own for them: the wait that gave up was
+        // a million times their latency)
+        if (!ok && rank == 0) {
           const uint64_t from = it > C::kStages ? it - C::kStages : 0;
           for (uint64_t j = from; j < it; ++j)
             tc::bar_wait(full + 8 * int(j % C::kStages), uint32_t(j / C::kStages & 1));
@@ -457,7 +479,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       constexpr int kThreads = kLoaderWarps * 32;
       constexpr int kPerThread = 1024 / kThreads;  // chunks of 128 lines
       uint64_t it = 0;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int64_t t = walker; t < tiles && ok; t += walkers) {
         const int split = int(t / layer), in = int(t % layer);
         const int64_t m0 = int64_t(in / p.n_tiles) * kBM, n0 = int64_t(in % p.n_tiles) * BN;
         const int kb = split * p.split_blocks;
@@ -493,11 +515,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       }
     }
   } else if (warp == kMmaWarp) {
-    // ---- the thread that issues the products ----
-    if (lane == 0) {
+    // ---- the thread that issues the products (the pair's first block's) ----
+    if (lane == 0 && rank == 0) {
       uint64_t it = 0, chunk = 0;
       const uint32_t a_step = p.a.mn_major ? 2048 : 32, b_step = p.b.mn_major ? 2048 : 32;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int64_t t = walker; t < tiles && ok; t += walkers) {
         const int split = int(t / layer);
         const int kb = split * p.split_blocks;
         const int ke = min(p.k_blocks, kb + p.split_blocks);
@@ -506,7 +528,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const int in_chunk = C::kParts == 3 ? (kt - kb) % kChunkBlocks : kt - kb;
           if (in_chunk == 0) {
             const int buf = int(chunk & 1);
-            ok = tc::bar_wait(acc_empty + 8 * buf, uint32_t(chunk / 2 & 1) ^ 1);
+            ok = tc::bar_wait<PAIR>(acc_empty + 8 * buf, uint32_t(chunk / 2 & 1) ^ 1);
             if (!ok) break;
             tc::fence_after();
             d = tmem + buf * C::kBufferColumns;
@@ -520,27 +542,27 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           for (int step = 0; step < kBK / 16; ++step) {
             const bool more = in_chunk > 0 || step > 0;
             const uint32_t as = a + step * a_step, bs = b + step * b_step;
-            tc::mma_f16(d, tc::operand_desc(as, p.a.mn_major, 8192),
+            tc::mma_f16<PAIR>(d, tc::operand_desc(as, p.a.mn_major, 8192),
                         tc::operand_desc(bs, p.b.mn_major, 8192), p.idesc, more);
             if constexpr (C::kParts == 3) {
               constexpr int kA[5] = {0, 1, 1, 0, 2}, kB[5] = {1, 0, 1, 2, 0};
 #pragma unroll
               for (int j = 0; j < 5; ++j)
-                tc::mma_f16(d + BN,
+                tc::mma_f16<PAIR>(d + BN,
                             tc::operand_desc(as + kA[j] * C::kABytes, p.a.mn_major, 8192),
                             tc::operand_desc(bs + kB[j] * C::kBBytes, p.b.mn_major, 8192), p.idesc,
                             more || j > 0);
             }
           }
-          tc::mma_commit(empty + 8 * s);
+          tc::mma_commit<PAIR>(empty + 8 * s);
           if (kt + 1 == ke || (C::kParts == 3 && in_chunk + 1 == kChunkBlocks)) {
-            tc::mma_commit(acc_full + 8 * int(chunk & 1));
+            tc::mma_commit<PAIR>(acc_full + 8 * int(chunk & 1));
             ++chunk;
           }
         }
       }
       if (!ok) {  // products in flight must end before TMEM is freed
-        tc::mma_commit(drain);
+        tc::mma_commit<PAIR>(drain);
         tc::bar_wait(drain, 0);
       }
     }
@@ -549,6 +571,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t bufs = out_base + warp * C::kOutBuffers * 4096;
+    const uint32_t first_acc_empty = PAIR ? tc::in_first_block(acc_empty) : acc_empty;
     uint32_t turn = 0;
     uint64_t chunk = 0;
     // the next staging buffer, free of its last copy
@@ -559,11 +582,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       ++turn;
       return b;
     };
+    auto release_accumulators = [&](int buf) {
+      tc::fence_before();
+      __syncwarp();
+      if (lane != 0) return;
+      if (PAIR)
+        tc::bar_arrive_cluster(first_acc_empty + 8 * buf);
+      else
+        tc::bar_arrive(acc_empty + 8 * buf);
+    };
     auto pointer = [&](uint32_t b) -> char* { return smem_raw + (b - raw); };
-    for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int64_t t = walker; t < tiles && ok; t += walkers) {
       const int split = int(t / layer), in = int(t % layer);
       const int m_tile = in / p.n_tiles;
-      const int64_t row0 = int64_t(m_tile) * kBM + quarter * 32;
+      const int64_t row0 = int64_t(m_tile) * C::kTileRows + rank * kBM + quarter * 32;
       const int n0 = in % p.n_tiles * BN;
       const int64_t rows_left = int64_t(p.m) - row0;
       const int rows = rows_left >= 32 ? 32 : rows_left > 0 ? int(rows_left) : 0;
@@ -594,9 +626,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) sums[gi][e] += v[e];
           }
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) tc::bar_arrive(acc_empty + 8 * buf);
+          release_accumulators(buf);
         }
         if (!ok) break;
       } else {
@@ -647,15 +677,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         } else {
           if (mine) tc::tmem_load(d + g * kGroup, v);
           if (last) {
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::bar_arrive(acc_empty + 8 * int(chunk & 1));
+            release_accumulators(int(chunk & 1));
             ++chunk;
           }
         }
         if (!mine) continue;
         if (p.partials) {
-          const int64_t prow = (int64_t(split) * p.m_tiles + m_tile) * kBM + quarter * 32;
+          const int64_t prow = split * p.layer_rows + row0;
 #pragma unroll
           for (int h = 0; h < kGroup / 32; ++h) {
             if (h * 32 >= cols) break;
@@ -735,9 +763,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   }
   if (!ok && lane == 0) atomicAdd(&g_timeouts, 1ull);
   __syncthreads();
+  if (PAIR) tc::cluster_sync();  // neither block leaves while the other may still reach it
   if (warp == kMmaWarp) {
     tc::fence_after();
-    tc::tmem_free(tmem, C::kTmemColumns);
+    tc::tmem_free<PAIR>(tmem, C::kTmemColumns);
   }
 }
 

@@ -35,17 +35,50 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
+// As above where the phase is completed from the other block of a pair.
+__device__ __forceinline__ bool bar_try_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 // Waits for the phase `parity` of the barrier, for at most about two seconds
 // of global time; false when it gave up.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  if (bar_try(bar, parity)) return true;
+  auto done = [&] { return CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity); };
+  if (done()) return true;
   uint64_t t0, t;
   asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t0));
   for (;;) {
-    if (bar_try(bar, parity)) return true;
+    if (done()) return true;
     asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
     if (t - t0 > 2000000000ull) return false;
   }
+}
+
+// ---- block pairs (clusters of two) ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+// Every thread of both blocks.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// The address of this shared-memory location in the pair's first block.
+__device__ __forceinline__ uint32_t in_first_block(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
 
 // ---- TMA ----
@@ -55,6 +88,15 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
       "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
       "[%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+// The same from a block of a pair, signalling the first block's barrier.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                              uint32_t first_block_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".cta_group::2 [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(first_block_bar)
       : "memory");
 }
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, uint32_t src) {
@@ -78,31 +120,62 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 }
 
 // ---- tensor memory and the tensor core ----
-__device__ __forceinline__ void tmem_alloc(uint32_t where, uint32_t columns) {  // one warp
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(where),
-               "r"(columns)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+// One warp (of each block, for a pair) allocates and the same frees.
+template <bool PAIR = false>
+__device__ __forceinline__ void tmem_alloc(uint32_t where, uint32_t columns) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(where),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(where),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+  }
 }
-__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {  // the same warp
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(columns));
+template <bool PAIR = false>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+  if (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(columns));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(columns));
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
-// Arrives on the barrier when this thread's earlier tensor-core work is done.
+// Arrives on the barrier (of both blocks of a pair) when this thread's earlier
+// tensor-core work is done.
+template <bool PAIR = false>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
-      : "memory");
+  if (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;\n" ::"r"(bar),
+        "h"(uint16_t(3))
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
+        : "memory");
 }
 // d (TMEM, f32) = a b (+ d when accumulate): 16-bit operands in shared memory.
+// PAIR: both blocks hold half of a's rows, half of b's rows and half of d.
+template <bool PAIR = false>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                         bool accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
-      : "memory");
+  if (PAIR)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
 }
 // Accumulator columns of this warp's 32 TMEM lanes, one row per thread.  The
 // wait is part of the load: nothing may read the registers before it.
