@@ -232,6 +232,18 @@ __device__ __noinline__ float plain_dot(const Product& p, int64_t i, int64_t j, 
   return s;
 }
 
+// A position in a ring of N slots and the parity of its current phase.
+template <int N>
+struct Cursor {
+  uint32_t slot = 0, parity = 0;
+  __device__ __forceinline__ void advance() {
+    if (++slot == N) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+};
+
 // ---- loader warps ----
 // Eight values of a line, zero past `valid`.
 template <class T>
@@ -428,7 +440,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     // ---- producers ----
     if (!LOADER) {
       if (lane == 0) {
-        uint64_t it = 0;
+        Cursor<C::kStages> at;
+        uint32_t issued = 0;
         const uint32_t first_full = PAIR ? tc::in_first_block(full) : full;
         for (int64_t t = walker; t < tiles && ok; t += walkers) {
           const int split = int(t / layer), in = int(t % layer);
@@ -436,10 +449,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const int n0 = in % p.n_tiles * BN + int(rank) * C::kBRows;
           const int kb = split * p.split_blocks;
           const int ke = min(p.k_blocks, kb + p.split_blocks);
-          for (int kt = kb; kt < ke; ++kt, ++it) {
-            const int s = int(it % C::kStages);
-            ok = tc::bar_wait(empty + 8 * s, uint32_t(it / C::kStages & 1) ^ 1);
+          for (int kt = kb; kt < ke; ++kt, at.advance()) {
+            const uint32_t s = at.slot;
+            ok = tc::bar_wait(empty + 8 * s, at.parity ^ 1);
             if (!ok) break;
+            if (issued < C::kStages) ++issued;
             const uint32_t a = base + s * C::kStageBytes, b = a + C::kABytes;
             const uint32_t bar = PAIR ? first_full + 8 * s : full + 8 * s;
             if (rank == 0)
@@ -469,29 +483,30 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // of a pair has no barrier of its own for them: the wait that gave up was
         // a million times their latency)
         if (!ok && rank == 0) {
-          const uint64_t from = it > C::kStages ? it - C::kStages : 0;
-          for (uint64_t j = from; j < it; ++j)
-            tc::bar_wait(full + 8 * int(j % C::kStages), uint32_t(j / C::kStages & 1));
+          for (uint32_t j = 0; j < issued; ++j) {  // backwards from the slot not filled
+            const uint32_t slot = (at.slot + C::kStages - 1 - j) % C::kStages;
+            tc::bar_wait(full + 8 * slot, slot < at.slot ? at.parity : at.parity ^ 1);
+          }
         }
       }
     } else {
       const int tid = threadIdx.x - kProducerWarp * 32;
       constexpr int kThreads = kLoaderWarps * 32;
       constexpr int kPerThread = 1024 / kThreads;  // chunks of 128 lines
-      uint64_t it = 0;
+      Cursor<C::kStages> at;
       for (int64_t t = walker; t < tiles && ok; t += walkers) {
         const int split = int(t / layer), in = int(t % layer);
         const int64_t m0 = int64_t(in / p.n_tiles) * kBM, n0 = int64_t(in % p.n_tiles) * BN;
         const int kb = split * p.split_blocks;
         const int ke = min(p.k_blocks, kb + p.split_blocks);
-        for (int kt = kb; kt < ke; ++kt, ++it) {
-          const int s = int(it % C::kStages);
+        for (int kt = kb; kt < ke; ++kt, at.advance()) {
+          const uint32_t s = at.slot;
           const int64_t k0 = int64_t(kt) * kBK;
           Chunk<T> c[kPerThread];
 #pragma unroll
           for (int i = 0; i < kPerThread; ++i)
             read_tile_chunk<T>(p.a, p.a_vec, m0, p.m, k0, p.k, tid + i * kThreads, c[i]);
-          ok = tc::bar_wait(empty + 8 * s, uint32_t(it / C::kStages & 1) ^ 1);
+          ok = tc::bar_wait(empty + 8 * s, at.parity ^ 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const uint32_t a = base + s * C::kStageBytes, b = a + C::kParts * C::kABytes;
@@ -517,47 +532,48 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   } else if (warp == kMmaWarp) {
     // ---- the thread that issues the products (the pair's first block's) ----
     if (lane == 0 && rank == 0) {
-      uint64_t it = 0, chunk = 0;
-      const uint32_t a_step = p.a.mn_major ? 2048 : 32, b_step = p.b.mn_major ? 2048 : 32;
+      // One thread issues everything, so its own instructions between two
+      // blocks of k count: cursors step by one and descriptors by additions.
+      Cursor<C::kStages> at;
+      Cursor<2> acc;
+      const uint32_t a_step = (p.a.mn_major ? 2048 : 32) >> 4, b_step = (p.b.mn_major ? 2048 : 32) >> 4;
+      const uint64_t a0 = tc::operand_desc(base, p.a.mn_major, 8192);
+      const uint64_t b0 = tc::operand_desc(base + C::kParts * C::kABytes, p.b.mn_major, 8192);
       for (int64_t t = walker; t < tiles && ok; t += walkers) {
-        const int split = int(t / layer);
+        const int split = p.splits > 1 ? int(t / layer) : 0;
         const int kb = split * p.split_blocks;
-        const int ke = min(p.k_blocks, kb + p.split_blocks);
+        const int blocks = min(p.k_blocks, kb + p.split_blocks) - kb;
         uint32_t d = 0;
-        for (int kt = kb; kt < ke; ++kt, ++it) {
-          const int in_chunk = C::kParts == 3 ? (kt - kb) % kChunkBlocks : kt - kb;
+        int in_chunk = 0;
+        for (int kt = 0; kt < blocks; ++kt, at.advance()) {
           if (in_chunk == 0) {
-            const int buf = int(chunk & 1);
-            ok = tc::bar_wait<PAIR>(acc_empty + 8 * buf, uint32_t(chunk / 2 & 1) ^ 1);
+            ok = tc::bar_wait<PAIR>(acc_empty + 8 * acc.slot, acc.parity ^ 1);
             if (!ok) break;
-            tc::fence_after();
-            d = tmem + buf * C::kBufferColumns;
+            d = tmem + acc.slot * C::kBufferColumns;
           }
-          const int s = int(it % C::kStages);
-          ok = tc::bar_wait(full + 8 * s, uint32_t(it / C::kStages & 1));
+          ok = tc::bar_wait(full + 8 * at.slot, at.parity);
           if (!ok) break;
           tc::fence_after();
-          const uint32_t a = base + s * C::kStageBytes, b = a + C::kParts * C::kABytes;
+          const uint64_t a = a0 + at.slot * (C::kStageBytes >> 4), b = b0 + at.slot * (C::kStageBytes >> 4);
 #pragma unroll
           for (int step = 0; step < kBK / 16; ++step) {
-            const bool more = in_chunk > 0 || step > 0;
-            const uint32_t as = a + step * a_step, bs = b + step * b_step;
-            tc::mma_f16<PAIR>(d, tc::operand_desc(as, p.a.mn_major, 8192),
-                        tc::operand_desc(bs, p.b.mn_major, 8192), p.idesc, more);
+            const bool more = step > 0 || in_chunk > 0;
+            const uint64_t as = a + step * a_step, bs = b + step * b_step;
+            tc::mma_f16<PAIR>(d, as, bs, p.idesc, more);
             if constexpr (C::kParts == 3) {
               constexpr int kA[5] = {0, 1, 1, 0, 2}, kB[5] = {1, 0, 1, 2, 0};
 #pragma unroll
               for (int j = 0; j < 5; ++j)
-                tc::mma_f16<PAIR>(d + BN,
-                            tc::operand_desc(as + kA[j] * C::kABytes, p.a.mn_major, 8192),
-                            tc::operand_desc(bs + kB[j] * C::kBBytes, p.b.mn_major, 8192), p.idesc,
-                            more || j > 0);
+                tc::mma_f16<PAIR>(d + BN, as + kA[j] * (C::kABytes >> 4), bs + kB[j] * (C::kBBytes >> 4),
+                                  p.idesc, more || j > 0);
             }
           }
-          tc::mma_commit<PAIR>(empty + 8 * s);
-          if (kt + 1 == ke || (C::kParts == 3 && in_chunk + 1 == kChunkBlocks)) {
-            tc::mma_commit<PAIR>(acc_full + 8 * int(chunk & 1));
-            ++chunk;
+          tc::mma_commit<PAIR>(empty + 8 * at.slot);
+          ++in_chunk;
+          if (kt + 1 == blocks || (C::kParts == 3 && in_chunk == kChunkBlocks)) {
+            tc::mma_commit<PAIR>(acc_full + 8 * acc.slot);
+            acc.advance();
+            in_chunk = 0;
           }
         }
       }
@@ -573,7 +589,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t bufs = out_base + warp * C::kOutBuffers * 4096;
     const uint32_t first_acc_empty = PAIR ? tc::in_first_block(acc_empty) : acc_empty;
     uint32_t turn = 0;
-    uint64_t chunk = 0;
+    Cursor<2> acc;
     // the next staging buffer, free of its last copy
     auto next_buffer = [&]() -> uint32_t {
       if (lane == 0) tc::bulk_wait_read<C::kOutBuffers - 1>();
@@ -582,7 +598,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       ++turn;
       return b;
     };
-    auto release_accumulators = [&](int buf) {
+    auto release_accumulators = [&](uint32_t buf) {
       tc::fence_before();
       __syncwarp();
       if (lane != 0) return;
@@ -609,9 +625,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         for (int gi = 0; gi < kGroupsPerWarp; ++gi)
 #pragma unroll
           for (int e = 0; e < kGroup; ++e) sums[gi][e] = 0.0f;
-        for (int ch = 0; ch < chunks; ++ch, ++chunk) {
-          const int buf = int(chunk & 1);
-          ok = tc::bar_wait(acc_full + 8 * buf, uint32_t(chunk / 2 & 1));
+        for (int ch = 0; ch < chunks; ++ch, acc.advance()) {
+          const uint32_t buf = acc.slot;
+          ok = tc::bar_wait(acc_full + 8 * buf, acc.parity);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc::fence_after();
@@ -630,8 +646,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         if (!ok) break;
       } else {
-        const int buf = int(chunk & 1);
-        ok = tc::bar_wait(acc_full + 8 * buf, uint32_t(chunk / 2 & 1));
+        const uint32_t buf = acc.slot;
+        ok = tc::bar_wait(acc_full + 8 * buf, acc.parity);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc::fence_after();
@@ -677,8 +693,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         } else {
           if (mine) tc::tmem_load(d + g * kGroup, v);
           if (last) {
-            release_accumulators(int(chunk & 1));
-            ++chunk;
+            release_accumulators(acc.slot);
+            acc.advance();
           }
         }
         if (!mine) continue;
