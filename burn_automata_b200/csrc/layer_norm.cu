@@ -37,11 +37,11 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarpRowThreads = 256;  // threads per block where a warp or less has a row
 
-// Sums `a` and `b` over the row's threads.  WARP: tpr lanes (a power of two)
-// have a row; else the whole block, through shared memory, whose two halves
-// alternate so that one barrier per sum is enough.
+// Sums over a row's threads: tpr lanes of a warp (a power of two), or the whole
+// block through shared memory, whose two halves alternate so that one barrier
+// per sum is enough.
 struct RowSum {
-  float* buf;  // [2][64], block rows only
+  float2* buf;  // [2][16], block rows only
   int phase = 0;
 };
 template <bool BLOCK>
@@ -51,18 +51,16 @@ __device__ __forceinline__ void row_sum2(RowSum& rs, int tpr, float& a, float& b
     b += __shfl_xor_sync(kFull, b, o);
   }
   if (BLOCK) {
-    float* s = rs.buf + rs.phase * 64;
+    float2* const s = rs.buf + rs.phase * 16;
     rs.phase ^= 1;
     const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) {
-      s[warp] = a;
-      s[32 + warp] = b;
-    }
+    if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, b);
     __syncthreads();
     a = b = 0.0f;
     for (int w = 0; w < warps; ++w) {
-      a += s[w];
-      b += s[32 + w];
+      const float2 t = s[w];
+      a += t.x;
+      b += t.y;
     }
   }
 }
@@ -70,40 +68,185 @@ template <bool BLOCK>
 __device__ __forceinline__ float row_sum(RowSum& rs, int tpr, float a) {
   for (int o = (BLOCK ? 32 : tpr) >> 1; o > 0; o >>= 1) a += __shfl_xor_sync(kFull, a, o);
   if (BLOCK) {
-    float* s = rs.buf + rs.phase * 64;
+    float2* const s = rs.buf + rs.phase * 16;
     rs.phase ^= 1;
     const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) s[warp] = a;
+    if ((threadIdx.x & 31) == 0) s[warp].x = a;
     __syncthreads();
     a = 0.0f;
-    for (int w = 0; w < warps; ++w) a += s[w];
+    for (int w = 0; w < warps; ++w) a += s[w].x;
   }
   return a;
 }
 
-// Thread `lane` of a row's `tpr` threads has the vectors lane, lane + tpr, ...
-// of VEC values, NV of them at most.
+// ---- a thread's share of a row ----
+// Thread `lane` of a row's `tpr` threads has the accesses lane, lane + tpr, ...
+// of VEC values, NV of them at most, as E values in pairs.
+template <int VEC, int NV>
+struct Row {
+  static constexpr int E = VEC * NV, kPairs = (E + 1) / 2;
+  F2 v[kPairs];
+};
+// Past nvec (and for `active` false) the values are zero.
 template <class T, int VEC, int NV>
 __device__ __forceinline__ void load_row(const T* row, int lane, int tpr, int nvec, bool active,
-                                         float (&out)[NV * VEC]) {
+                                         Row<VEC, NV>& out) {
+  float f[2 * Row<VEC, NV>::kPairs];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int q = lane + k * tpr;
     if (active && q < nvec) {
       const Pack<T, VEC> p = reinterpret_cast<const Pack<T, VEC>*>(row)[q];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) out[k * VEC + j] = to_f32(p.v[j]);
+      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = to_f32(p.v[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) out[k * VEC + j] = 0.0f;
+      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = 0.0f;
     }
   }
+  if (Row<VEC, NV>::E & 1) f[Row<VEC, NV>::E] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) out.v[i] = f2(f[2 * i], f[2 * i + 1]);
+}
+template <class T, int VEC, int NV>
+__device__ __forceinline__ void store_row(T* row, int lane, int tpr, int nvec, const Row<VEC, NV>& in) {
+  float f[2 * Row<VEC, NV>::kPairs];
+#pragma unroll
+  for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) {
+    const float2 t = values(in.v[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int q = lane + k * tpr;
+    if (q >= nvec) continue;
+    Pack<T, VEC> p;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) p.v[j] = from_f32<T>(f[k * VEC + j]);
+    reinterpret_cast<Pack<T, VEC>*>(row)[q] = p;
+  }
+}
+// A parameter vector's share: `fill` where it is absent.  Scalar loads: read
+// once per thread, and only as aligned as its type.
+template <class T, int VEC, int NV>
+__device__ __forceinline__ void load_parameter(const void* from, int lane, int tpr, int nvec, float fill,
+                                               Row<VEC, NV>& out) {
+  float f[2 * Row<VEC, NV>::kPairs];
+#pragma unroll
+  for (int e = 0; e < 2 * Row<VEC, NV>::kPairs; ++e) {
+    const int q = lane + e / VEC * tpr;
+    f[e] = from && e < VEC * NV && q < nvec ? to_f32(static_cast<const T*>(from)[q * VEC + e % VEC])
+                                            : fill;
+  }
+#pragma unroll
+  for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) out.v[i] = f2(f[2 * i], f[2 * i + 1]);
 }
 
+template <int VEC, int NV>
+__device__ __forceinline__ float forward_sum(const Row<VEC, NV>& x) {
+  F2 s = x.v[0];
+#pragma unroll
+  for (int i = 1; i < Row<VEC, NV>::kPairs; ++i) s = add2(s, x.v[i]);
+  const float2 t = values(s);
+  return t.x + t.y;
+}
+// x - mean in place (zero past nvec), and the sum of its squares.
+template <int VEC, int NV>
+__device__ __forceinline__ float forward_centre(Row<VEC, NV>& x, float mean, int lane, int tpr, int nvec) {
+  F2 s = f2(0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) {
+    const int e0 = 2 * i, e1 = 2 * i + 1;
+    const bool in0 = lane + e0 / VEC * tpr < nvec;
+    const bool in1 = e1 < VEC * NV && lane + e1 / VEC * tpr < nvec;
+    x.v[i] = add2(x.v[i], f2(in0 ? -mean : 0.0f, in1 ? -mean : 0.0f));
+    s = fma2(x.v[i], x.v[i], s);
+  }
+  const float2 t = values(s);
+  return t.x + t.y;
+}
+template <int VEC, int NV>
+__device__ __forceinline__ void forward_out(Row<VEC, NV>& x, float rstd, const Row<VEC, NV>& w,
+                                            const Row<VEC, NV>& b) {
+  const F2 r = f2(rstd, rstd);
+#pragma unroll
+  for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) x.v[i] = fma2(mul2(x.v[i], r), w.v[i], b.v[i]);
+}
+
+// x becomes xhat, g (dy) becomes dy w; dw, db and this thread's share of
+// sum(g) and sum(g xhat) grow.  Values past the row's end are zero in dy, so
+// whatever xhat holds there adds nothing that is stored.  16-bit rows take
+// xhat = x rstd - mean rstd in one step: the rounded product costs 2^-24
+// mean rstd, far below the spacing of the values themselves; f32 rows subtract
+// first.
+template <class T, int VEC, int NV>
+__device__ __forceinline__ void backward_sums(Row<VEC, NV>& x, Row<VEC, NV>& g, const Row<VEC, NV>& w,
+                                              float mean, float rstd, bool params, Row<VEC, NV>& dw,
+                                              Row<VEC, NV>& db, float& s1, float& s2) {
+  const F2 r = f2(rstd, rstd);
+  const float shift = sizeof(T) == 2 ? -mean * rstd : -mean;
+  const F2 m = f2(shift, shift);
+  F2 a = f2(0.0f, 0.0f), b = f2(0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) {
+    x.v[i] = sizeof(T) == 2 ? fma2(x.v[i], r, m) : mul2(add2(x.v[i], m), r);
+    if (params) {
+      dw.v[i] = fma2(g.v[i], x.v[i], dw.v[i]);
+      db.v[i] = add2(db.v[i], g.v[i]);
+    }
+    g.v[i] = mul2(g.v[i], w.v[i]);
+    a = add2(a, g.v[i]);
+    b = fma2(g.v[i], x.v[i], b);
+  }
+  const float2 ta = values(a), tb = values(b);
+  s1 = ta.x + ta.y;
+  s2 = tb.x + tb.y;
+}
+// g becomes dx = rstd (g - s1 - xhat s2), s1 and s2 the means over the row.
+template <int VEC, int NV>
+__device__ __forceinline__ void backward_out(const Row<VEC, NV>& x, Row<VEC, NV>& g, float rstd, float s1,
+                                             float s2) {
+  const F2 r = f2(rstd, rstd), c1 = f2(-rstd * s1, -rstd * s1), c2 = f2(-rstd * s2, -rstd * s2);
+#pragma unroll
+  for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) g.v[i] = fma2(x.v[i], c2, fma2(g.v[i], r, c1));
+}
+template <int VEC, int NV>
+__device__ __forceinline__ void add_row(Row<VEC, NV>& a, const Row<VEC, NV>& b) {
+#pragma unroll
+  for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) a.v[i] = add2(a.v[i], b.v[i]);
+}
+// The block's dw and db into partials[block][2][dims]: row groups that share
+// columns add to shared memory in turn (`turns` groups, this thread's at `turn`).
+template <int VEC, int NV>
+__device__ __forceinline__ void leave_partials(const Row<VEC, NV>& dw, const Row<VEC, NV>& db, int lane,
+                                               int tpr, int nvec, int dims, int turn, int turns,
+                                               float* columns, float* part) {
+  float* const to = turns > 1 ? columns : part;
+  for (int t = 0; t < turns; ++t) {
+    if (t == turn) {
+#pragma unroll
+      for (int e = 0; e < VEC * NV; ++e) {
+        const int q = lane + e / VEC * tpr;
+        if (q >= nvec) continue;
+        const float2 w2 = values(dw.v[e / 2]), b2 = values(db.v[e / 2]);
+        const float w = e & 1 ? w2.y : w2.x, b = e & 1 ? b2.y : b2.x;
+        float* const c = to + q * VEC + e % VEC;
+        c[0] = t == 0 ? w : c[0] + w;
+        c[dims] = t == 0 ? b : c[dims] + b;
+      }
+    }
+    if (turns > 1) __syncthreads();
+  }
+  if (turns > 1)
+    for (int i = threadIdx.x; i < 2 * dims; i += blockDim.x) part[i] = columns[i];
+}
+
+// ---- plain loads ----
 template <class T, int VEC, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 512 : kWarpRowThreads)
 layer_norm_kernel(LayerNormArgs a, int tpr_) {
-  __shared__ float sums[128];
+  __shared__ float2 sums[32];
   RowSum rs{sums};
   const int tpr = BLOCK ? int(blockDim.x) : tpr_;
   const int lane = BLOCK ? int(threadIdx.x) : int(threadIdx.x) & (tpr - 1);
@@ -111,53 +254,65 @@ layer_norm_kernel(LayerNormArgs a, int tpr_) {
   const int in_block = BLOCK ? 0 : int(threadIdx.x) / tpr;
   const int nvec = a.dims / VEC;
   const float inv_n = 1.0f / float(a.dims);
-  const T* const w = static_cast<const T*>(a.weight);
-  const T* const b = static_cast<const T*>(a.bias);
+  Row<VEC, NV> w, b;
+  load_parameter<T>(a.weight, lane, tpr, nvec, 1.0f, w);
+  load_parameter<T>(a.bias, lane, tpr, nvec, 0.0f, b);
   for (int64_t base = int64_t(blockIdx.x) * per_block; base < a.rows;
        base += int64_t(gridDim.x) * per_block) {
     const int64_t row = base + in_block;
     const bool active = row < a.rows;
-    float x[NV * VEC];
-    load_row<T, VEC, NV>(static_cast<const T*>(a.x) + row * a.x_stride, lane, tpr, nvec, active,
-                         x);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < NV * VEC; ++e) s += x[e];
-    const float mean = row_sum<BLOCK>(rs, tpr, s) * inv_n;
-    float v = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (lane + k * tpr < nvec) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float d = x[k * VEC + j] - mean;
-          v += d * d;
-        }
-      }
-    const float rstd = 1.0f / sqrtf(row_sum<BLOCK>(rs, tpr, v) * inv_n + a.eps);
+    Row<VEC, NV> x;
+    load_row<T>(static_cast<const T*>(a.x) + row * a.x_stride, lane, tpr, nvec, active, x);
+    const float mean = row_sum<BLOCK>(rs, tpr, forward_sum(x)) * inv_n;
+    const float var = row_sum<BLOCK>(rs, tpr, forward_centre(x, mean, lane, tpr, nvec)) * inv_n;
+    const float rstd = 1.0f / sqrtf(var + a.eps);
     if (!active) continue;
-    T* const out = static_cast<T*>(a.y) + row * a.y_stride;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = lane + k * tpr;
-      if (q >= nvec) continue;
-      Pack<T, VEC> p, wp, bp;
-      if (w) wp = reinterpret_cast<const Pack<T, VEC>*>(w)[q];
-      if (b) bp = reinterpret_cast<const Pack<T, VEC>*>(b)[q];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float y = (x[k * VEC + j] - mean) * rstd;
-        if (w) y *= to_f32(wp.v[j]);
-        if (b) y += to_f32(bp.v[j]);
-        p.v[j] = from_f32<T>(y);
-      }
-      reinterpret_cast<Pack<T, VEC>*>(out)[q] = p;
-    }
+    forward_out(x, rstd, w, b);
+    store_row<T>(static_cast<T*>(a.y) + row * a.y_stride, lane, tpr, nvec, x);
     if (lane == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
     }
   }
+}
+
+template <class T, int VEC, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : kWarpRowThreads)
+layer_norm_backward_kernel(LayerNormBackwardArgs a, int tpr_) {
+  __shared__ float2 sums[32];
+  extern __shared__ float columns[];  // [2][dims], rows of a warp or less
+  RowSum rs{sums};
+  const int tpr = BLOCK ? int(blockDim.x) : tpr_;
+  const int lane = BLOCK ? int(threadIdx.x) : int(threadIdx.x) & (tpr - 1);
+  const int per_block = BLOCK ? 1 : int(blockDim.x) / tpr;
+  const int in_block = BLOCK ? 0 : int(threadIdx.x) / tpr;
+  const int nvec = a.dims / VEC;
+  const float inv_n = 1.0f / float(a.dims);
+  const bool params = a.partials != nullptr;
+  Row<VEC, NV> w, dw{}, db{};
+  load_parameter<T>(a.weight, lane, tpr, nvec, 1.0f, w);
+  for (int64_t base = int64_t(blockIdx.x) * per_block; base < a.rows;
+       base += int64_t(gridDim.x) * per_block) {
+    const int64_t row = base + in_block;
+    const bool active = row < a.rows;
+    Row<VEC, NV> x, g;
+    load_row<T>(static_cast<const T*>(a.x) + row * a.x_stride, lane, tpr, nvec, active, x);
+    load_row<T>(static_cast<const T*>(a.dy) + row * a.dy_stride, lane, tpr, nvec, active, g);
+    const float mean = active ? a.mean[row] : 0.0f, rstd = active ? a.rstd[row] : 0.0f;
+    float s1, s2;
+    backward_sums<T>(x, g, w, mean, rstd, params, dw, db, s1, s2);
+    row_sum2<BLOCK>(rs, tpr, s1, s2);
+    if (!active || !a.dx) continue;
+    backward_out(x, g, rstd, s1 * inv_n, s2 * inv_n);
+    if (a.residual) {
+      load_row<T>(static_cast<const T*>(a.residual) + row * a.residual_stride, lane, tpr, nvec, true, x);
+      add_row(g, x);
+    }
+    store_row<T>(static_cast<T*>(a.dx) + row * a.dx_stride, lane, tpr, nvec, g);
+  }
+  if (params)
+    leave_partials(dw, db, lane, tpr, nvec, a.dims, in_block, per_block, columns,
+                   a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
 
 // ---- bulk copies: rows in flight ahead of the arithmetic ----
@@ -174,14 +329,6 @@ __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t byt
                "r"(bytes)
                : "memory");
 }
-
-// Sums over the tpr lanes of a row.
-__device__ __forceinline__ float lanes_sum(int tpr, float a) {
-  for (int o = tpr >> 1; o > 0; o >>= 1) a += __shfl_xor_sync(kFull, a, o);
-  return a;
-}
-
-constexpr int kTileRows = 8;
 
 // A warp's ring: `stages` slots of `slot` bytes, one barrier each.
 struct WarpRing {
@@ -217,110 +364,79 @@ __device__ __forceinline__ void copy_out(T* dst, const char* src, int count, int
   for (int i = lane; i < count; i += 32) dst[i] = reinterpret_cast<const T*>(src)[i];
 }
 
+// What one warp of the tile kernels walks: tiles of `rows` (four or eight)
+// rows, a whole number of 16-byte units whatever the width.
+struct TileShape {
+  int tpr, stages, rows;
+};
+
 template <class T, int VEC, int NV>
-__global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs a, int tpr, int stages) {
-  constexpr int E = NV * VEC;
-  using P = Pack<T, VEC>;
+__global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs a, TileShape shape) {
   extern __shared__ __align__(128) char smem[];
+  const int tpr = shape.tpr, stages = shape.stages, tile_rows = shape.rows;
   const uint32_t base = tc::smem_addr(smem);
-  const uint32_t tile_bytes = kTileRows * a.dims * sizeof(T);
+  const uint32_t tile_bytes = tile_rows * a.dims * sizeof(T);
   const WarpRing ring = warp_ring(smem, stages, (tile_bytes + 127) & ~127u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane & (tpr - 1), group = lane / tpr, at_once = 32 / tpr;
   const int nvec = a.dims / VEC;
   const float inv_n = 1.0f / float(a.dims);
-  const int64_t tiles = (a.rows + kTileRows - 1) / kTileRows;
-  const int64_t full_tiles = a.rows / kTileRows;
+  const int64_t tiles = (a.rows + tile_rows - 1) / tile_rows;
+  const int64_t full_tiles = a.rows / tile_rows;
   const int64_t first = int64_t(blockIdx.x) * (blockDim.x >> 5) + warp;
   const int64_t step = int64_t(gridDim.x) * (blockDim.x >> 5);
   const T* const x = static_cast<const T*>(a.x);
   T* const y = static_cast<T*>(a.y);
+  RowSum none{};
 
-  float w[E], b[E];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int q = sub + k * tpr;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const bool in = q < nvec;
-      w[k * VEC + j] = a.weight && in ? to_f32(static_cast<const T*>(a.weight)[q * VEC + j]) : 1.0f;
-      b[k * VEC + j] = a.bias && in ? to_f32(static_cast<const T*>(a.bias)[q * VEC + j]) : 0.0f;
-    }
-  }
   auto request = [&](int64_t tile, int slot) {  // lane 0
     if (tile < full_tiles) {
       tc::bar_expect(ring.bar(slot), tile_bytes);
-      bulk_load(ring.at(slot), x + tile * kTileRows * a.dims, tile_bytes, ring.bar(slot));
+      bulk_load(ring.at(slot), x + tile * tile_rows * a.dims, tile_bytes, ring.bar(slot));
     }
   };
   if (lane == 0)
     for (int s = 0; s < stages - 1; ++s) request(first + s * step, s);
+  Row<VEC, NV> w, b;
+  load_parameter<T>(a.weight, sub, tpr, nvec, 1.0f, w);
+  load_parameter<T>(a.bias, sub, tpr, nvec, 0.0f, b);
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
   for (int64_t tile = first; tile < tiles; tile += step) {
     char* const at = smem + (ring.at(slot) - base);
-    const int rows = int(min(int64_t(kTileRows), a.rows - tile * kTileRows));
-    if (rows == kTileRows) {
+    const int rows = int(min(int64_t(tile_rows), a.rows - tile * tile_rows));
+    if (rows == tile_rows) {
       ok = __all_sync(kFull, tc::bar_wait(ring.bar(slot), phase));
       if (!ok) break;
     } else {
       if (lane == 0) tc::bulk_wait_read<0>();
       __syncwarp();
-      copy_in<T>(at, x + tile * kTileRows * a.dims, rows * a.dims, lane);
+      copy_in<T>(at, x + tile * tile_rows * a.dims, rows * a.dims, lane);
       __syncwarp();
     }
-    for (int r0 = 0; r0 < kTileRows; r0 += at_once) {
+    for (int r0 = 0; r0 < tile_rows; r0 += at_once) {
       const int r = r0 + group;
-      P* const row = reinterpret_cast<P*>(at + size_t(r) * a.dims * sizeof(T));
-      float v[E];
-      float s = 0.0f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int q = sub + k * tpr;
-        if (r < rows && q < nvec) {
-          const P p = row[q];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            v[k * VEC + j] = to_f32(p.v[j]);
-            s += v[k * VEC + j];
-          }
+      T* const row = reinterpret_cast<T*>(at) + r * a.dims;
+      Row<VEC, NV> v;
+      load_row<T>(row, sub, tpr, nvec, r < rows, v);
+      const float mean = row_sum<false>(none, tpr, forward_sum(v)) * inv_n;
+      const float var = row_sum<false>(none, tpr, forward_centre(v, mean, sub, tpr, nvec)) * inv_n;
+      const float rstd = 1.0f / sqrtf(var + a.eps);
+      if (r < rows) {
+        forward_out(v, rstd, w, b);
+        store_row<T>(row, sub, tpr, nvec, v);
+        if (sub == 0) {
+          if (a.mean) a.mean[tile * tile_rows + r] = mean;
+          if (a.rstd) a.rstd[tile * tile_rows + r] = rstd;
         }
-      }
-      const float mean = lanes_sum(tpr, s) * inv_n;
-      float var = 0.0f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-        if (r < rows && sub + k * tpr < nvec) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            v[k * VEC + j] -= mean;
-            var += v[k * VEC + j] * v[k * VEC + j];
-          }
-        }
-      const float rstd = 1.0f / sqrtf(lanes_sum(tpr, var) * inv_n + a.eps);
-      if (r >= rows) continue;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int q = sub + k * tpr;
-        if (q < nvec) {
-          P p;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            p.v[j] = from_f32<T>(v[k * VEC + j] * rstd * w[k * VEC + j] + b[k * VEC + j]);
-          row[q] = p;
-        }
-      }
-      if (sub == 0) {
-        if (a.mean) a.mean[tile * kTileRows + r] = mean;
-        if (a.rstd) a.rstd[tile * kTileRows + r] = rstd;
       }
     }
-    if (rows == kTileRows) {
+    if (rows == tile_rows) {
       tc::fence_async_shared();
       __syncwarp();
       if (lane == 0) {
-        bulk_store(y + tile * kTileRows * a.dims, ring.at(slot), tile_bytes);
+        bulk_store(y + tile * tile_rows * a.dims, ring.at(slot), tile_bytes);
         tc::bulk_commit();
         // the slot before this one: its results have left once all groups but
         // the one just committed have been read
@@ -329,7 +445,7 @@ __global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs 
       }
     } else {
       __syncwarp();
-      copy_out<T>(y + tile * kTileRows * a.dims, at, rows * a.dims, lane);
+      copy_out<T>(y + tile * tile_rows * a.dims, at, rows * a.dims, lane);
     }
     if (++slot == stages) {
       slot = 0;
@@ -345,66 +461,59 @@ __global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs 
 }
 
 // The slots of the backward ring: x (dx in place), dy, residual, mean, rstd.
-__host__ __device__ inline uint32_t backward_slot(uint32_t tile_bytes, bool residual) {
-  return ((residual ? 3 : 2) * tile_bytes + 2 * kTileRows * 4 + 127) & ~127u;
+__host__ __device__ inline uint32_t backward_slot(uint32_t tile_bytes, bool residual, int tile_rows) {
+  return ((residual ? 3 : 2) * tile_bytes + 2 * tile_rows * 4 + 127) & ~127u;
 }
 
 template <class T, int VEC, int NV>
 __global__ void __launch_bounds__(256, 2)
-layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, int tpr, int stages) {
-  constexpr int E = NV * VEC;
-  using P = Pack<T, VEC>;
+layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
   extern __shared__ __align__(128) char smem[];
+  const int tpr = shape.tpr, stages = shape.stages, tile_rows = shape.rows;
   const uint32_t base = tc::smem_addr(smem);
-  const uint32_t tile_bytes = kTileRows * a.dims * sizeof(T);
-  const WarpRing ring = warp_ring(smem, stages, backward_slot(tile_bytes, a.residual != nullptr));
+  const uint32_t tile_bytes = tile_rows * a.dims * sizeof(T);
+  const WarpRing ring =
+      warp_ring(smem, stages, backward_slot(tile_bytes, a.residual != nullptr, tile_rows));
   const uint32_t stats = (a.residual ? 3 : 2) * tile_bytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int sub = lane & (tpr - 1), group = lane / tpr, at_once = 32 / tpr;
   const int nvec = a.dims / VEC;
   const float inv_n = 1.0f / float(a.dims);
-  const int64_t tiles = (a.rows + kTileRows - 1) / kTileRows;
-  const int64_t full_tiles = a.rows / kTileRows;
+  const int64_t tiles = (a.rows + tile_rows - 1) / tile_rows;
+  const int64_t full_tiles = a.rows / tile_rows;
   const int64_t first = int64_t(blockIdx.x) * warps + warp;
   const int64_t step = int64_t(gridDim.x) * warps;
   const T* const x = static_cast<const T*>(a.x);
   const T* const dy = static_cast<const T*>(a.dy);
   const T* const res = static_cast<const T*>(a.residual);
   T* const dx = static_cast<T*>(a.dx);
+  const bool params = a.partials != nullptr;
+  RowSum none{};
 
-  float w[E], dw[E], db[E];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int q = sub + k * tpr;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      w[k * VEC + j] =
-          a.weight && q < nvec ? to_f32(static_cast<const T*>(a.weight)[q * VEC + j]) : 1.0f;
-      dw[k * VEC + j] = db[k * VEC + j] = 0.0f;
-    }
-  }
   auto request = [&](int64_t tile, int slot) {  // lane 0
     if (tile < full_tiles) {
-      const int64_t row = tile * kTileRows, from = row * a.dims;
+      const int64_t row = tile * tile_rows, from = row * a.dims;
       const uint32_t bar = ring.bar(slot), at = ring.at(slot);
-      tc::bar_expect(bar, stats + 2 * kTileRows * 4);
+      tc::bar_expect(bar, stats + 2 * tile_rows * 4);
       bulk_load(at, x + from, tile_bytes, bar);
       bulk_load(at + tile_bytes, dy + from, tile_bytes, bar);
       if (res) bulk_load(at + 2 * tile_bytes, res + from, tile_bytes, bar);
-      bulk_load(at + stats, a.mean + row, kTileRows * 4, bar);
-      bulk_load(at + stats + kTileRows * 4, a.rstd + row, kTileRows * 4, bar);
+      bulk_load(at + stats, a.mean + row, tile_rows * 4, bar);
+      bulk_load(at + stats + tile_rows * 4, a.rstd + row, tile_rows * 4, bar);
     }
   };
   if (lane == 0)
     for (int s = 0; s < stages - 1; ++s) request(first + s * step, s);
+  Row<VEC, NV> w, dw{}, db{};
+  load_parameter<T>(a.weight, sub, tpr, nvec, 1.0f, w);
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
   for (int64_t tile = first; tile < tiles; tile += step) {
     char* const at = smem + (ring.at(slot) - base);
-    const int64_t from = tile * kTileRows * a.dims;
-    const int rows = int(min(int64_t(kTileRows), a.rows - tile * kTileRows));
-    if (rows == kTileRows) {
+    const int64_t from = tile * tile_rows * a.dims;
+    const int rows = int(min(int64_t(tile_rows), a.rows - tile * tile_rows));
+    if (rows == tile_rows) {
       ok = __all_sync(kFull, tc::bar_wait(ring.bar(slot), phase));
       if (!ok) break;
     } else {
@@ -413,64 +522,32 @@ layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, int tpr, int stages) {
       copy_in<T>(at, x + from, rows * a.dims, lane);
       copy_in<T>(at + tile_bytes, dy + from, rows * a.dims, lane);
       if (res) copy_in<T>(at + 2 * tile_bytes, res + from, rows * a.dims, lane);
-      copy_in<float>(at + stats, a.mean + tile * kTileRows, rows, lane);
-      copy_in<float>(at + stats + kTileRows * 4, a.rstd + tile * kTileRows, rows, lane);
+      copy_in<float>(at + stats, a.mean + tile * tile_rows, rows, lane);
+      copy_in<float>(at + stats + tile_rows * 4, a.rstd + tile * tile_rows, rows, lane);
       __syncwarp();
     }
-    for (int r0 = 0; r0 < kTileRows; r0 += at_once) {
+    const float* const st = reinterpret_cast<const float*>(at + stats);
+    for (int r0 = 0; r0 < tile_rows; r0 += at_once) {
       const int r = r0 + group;
       const bool active = r < rows;
-      P* const row = reinterpret_cast<P*>(at + size_t(r) * a.dims * sizeof(T));
-      const P* const grow = reinterpret_cast<const P*>(reinterpret_cast<const char*>(row) + tile_bytes);
-      const float* const st = reinterpret_cast<const float*>(at + stats);
-      const float rstd = active ? st[kTileRows + r] : 0.0f;
-      const float mean = active ? st[r] : 0.0f;
-      float xh[E], g[E];
-      float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int q = sub + k * tpr;
-        if (active && q < nvec) {
-          const P px = row[q], pg = grow[q];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int e = k * VEC + j;
-            const float d = to_f32(pg.v[j]);
-            xh[e] = (to_f32(px.v[j]) - mean) * rstd;
-            dw[e] += d * xh[e];
-            db[e] += d;
-            g[e] = d * w[e];
-            s1 += g[e];
-            s2 += g[e] * xh[e];
-          }
-        }
+      T* const row = reinterpret_cast<T*>(at) + r * a.dims;
+      const T* const grow = row + tile_rows * a.dims;
+      const float mean = active ? st[r] : 0.0f, rstd = active ? st[tile_rows + r] : 0.0f;
+      Row<VEC, NV> xh, g;
+      load_row<T>(row, sub, tpr, nvec, active, xh);
+      load_row<T>(grow, sub, tpr, nvec, active, g);
+      float s1, s2;
+      backward_sums<T>(xh, g, w, mean, rstd, params, dw, db, s1, s2);
+      row_sum2<false>(none, tpr, s1, s2);
+      if (!dx || !active) continue;
+      backward_out(xh, g, rstd, s1 * inv_n, s2 * inv_n);
+      if (res) {
+        load_row<T>(grow + tile_rows * a.dims, sub, tpr, nvec, true, xh);
+        add_row(g, xh);
       }
-      for (int o = tpr >> 1; o > 0; o >>= 1) {
-        s1 += __shfl_xor_sync(kFull, s1, o);
-        s2 += __shfl_xor_sync(kFull, s2, o);
-      }
-      s1 *= inv_n;
-      s2 *= inv_n;
-      const P* const rrow =
-          reinterpret_cast<const P*>(reinterpret_cast<const char*>(row) + 2 * tile_bytes);
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int q = sub + k * tpr;
-        if (active && q < nvec) {
-          P p, pr;
-          if (res) pr = rrow[q];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int e = k * VEC + j;
-            float d = rstd * (g[e] - s1 - xh[e] * s2);
-            if (res) d += to_f32(pr.v[j]);
-            p.v[j] = from_f32<T>(d);
-          }
-          row[q] = p;
-        }
-      }
+      store_row<T>(row, sub, tpr, nvec, g);
     }
-    if (rows == kTileRows) {
+    if (rows == tile_rows) {
       tc::fence_async_shared();
       __syncwarp();
       if (lane == 0) {
@@ -493,47 +570,29 @@ layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, int tpr, int stages) {
     atomicAdd(&g_timeouts, 1ull);
     for (int s = 0; s < stages; ++s) tc::bar_wait(ring.bar(s), s < slot ? phase ^ 1 : phase);
   }
-  if (!a.partials) return;
-  // the block's dw and db: the row groups add to shared columns in turn
-  __syncthreads();
-  float* const columns = reinterpret_cast<float*>(
-      smem + ((warps * stages * 8 + 127) & ~127));
-  for (int turn = 0; turn < warps * at_once; ++turn) {
-    if (turn == warp * at_once + group) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int q = sub + k * tpr;
-        if (q < nvec) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            float* const c = columns + q * VEC + j;
-            c[0] = turn == 0 ? dw[k * VEC + j] : c[0] + dw[k * VEC + j];
-            c[a.dims] = turn == 0 ? db[k * VEC + j] : c[a.dims] + db[k * VEC + j];
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-  float* const part = a.partials + int64_t(blockIdx.x) * 2 * a.dims;
-  for (int i = threadIdx.x; i < 2 * a.dims; i += blockDim.x) part[i] = columns[i];
+  if (!params) return;
+  __syncthreads();  // the ring's memory now holds the block's columns
+  leave_partials(dw, db, sub, tpr, nvec, a.dims, warp * at_once + group, warps * at_once,
+                 reinterpret_cast<float*>(smem + ((warps * stages * 8 + 127) & ~127)),
+                 a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
 
 // ---- wide rows: a block per row, rows copied ahead ----
 template <class T, int NV>
 __global__ void __launch_bounds__(512) layer_norm_wide_kernel(LayerNormArgs a, int stages) {
-  constexpr int VEC = 16 / int(sizeof(T)), E = NV * VEC;
-  using P = Pack<T, VEC>;
+  constexpr int VEC = 16 / int(sizeof(T));
   extern __shared__ __align__(128) char smem[];
-  __shared__ float sums[128];
+  __shared__ float2 sums[32];
   __shared__ uint64_t bars[8];
+  __shared__ int gave_up[2];  // by the parity of the row's turn
   RowSum rs{sums};
-  const int nvec = a.dims / VEC, threads = blockDim.x;
+  const int nvec = a.dims / VEC, threads = blockDim.x, lane = threadIdx.x;
   const uint32_t row_bytes = a.dims * sizeof(T), slot_bytes = (row_bytes + 127) & ~127u;
   const uint32_t base = tc::smem_addr(smem), bar0 = tc::smem_addr(bars);
   const float inv_n = 1.0f / float(a.dims);
   const T* const x = static_cast<const T*>(a.x);
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
+    gave_up[0] = gave_up[1] = 0;
     for (int s = 0; s < stages; ++s) tc::bar_init(bar0 + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -544,91 +603,59 @@ __global__ void __launch_bounds__(512) layer_norm_wide_kernel(LayerNormArgs a, i
       bulk_load(base + slot * slot_bytes, x + row * a.x_stride, row_bytes, bar0 + 8 * slot);
     }
   };
-  if (threadIdx.x == 0)
+  if (lane == 0)
     for (int s = 0; s < stages; ++s) request(blockIdx.x + int64_t(s) * gridDim.x, s);
-  int slot = 0;
+  Row<VEC, NV> w, b;
+  load_parameter<T>(a.weight, lane, threads, nvec, 1.0f, w);
+  load_parameter<T>(a.bias, lane, threads, nvec, 0.0f, b);
+  int slot = 0, turn = 0;
   uint32_t phase = 0;
   bool ok = true;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    ok = tc::bar_wait(bar0 + 8 * slot, phase);
-    ok = __syncthreads_and(ok);
-    if (!ok) break;
-    const P* const in = reinterpret_cast<const P*>(smem + slot * slot_bytes);
-    float v[E];
-    float s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * threads;
-      if (q < nvec) {
-        const P p = in[q];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[k * VEC + j] = to_f32(p.v[j]);
-          s += v[k * VEC + j];
-        }
-      }
-    }
-    const float mean = row_sum<true>(rs, 0, s) * inv_n;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    if (!tc::bar_wait(bar0 + 8 * slot, phase)) gave_up[turn] = 1;
+    Row<VEC, NV> v;
+    load_row<T>(reinterpret_cast<const T*>(smem + slot * slot_bytes), lane, threads, nvec, true, v);
+    const float mean = row_sum<true>(rs, 0, forward_sum(v)) * inv_n;
     // past the barrier in row_sum every thread has read the slot
-    if (threadIdx.x == 0) request(row + int64_t(stages) * gridDim.x, slot);
-    float var = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (int(threadIdx.x) + k * threads < nvec) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[k * VEC + j] -= mean;
-          var += v[k * VEC + j] * v[k * VEC + j];
-        }
-      }
-    const float rstd = 1.0f / sqrtf(row_sum<true>(rs, 0, var) * inv_n + a.eps);
-    P* const out = reinterpret_cast<P*>(static_cast<T*>(a.y) + row * a.y_stride);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * threads;
-      if (q >= nvec) continue;
-      P p, pw, pb;
-      if (a.weight) pw = static_cast<const P*>(a.weight)[q];
-      if (a.bias) pb = static_cast<const P*>(a.bias)[q];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float o = v[k * VEC + j] * rstd;
-        if (a.weight) o *= to_f32(pw.v[j]);
-        if (a.bias) o += to_f32(pb.v[j]);
-        p.v[j] = from_f32<T>(o);
-      }
-      out[q] = p;
-    }
-    if (threadIdx.x == 0) {
-      if (a.mean) a.mean[row] = mean;
-      if (a.rstd) a.rstd[row] = rstd;
-    }
+    ok = gave_up[turn] == 0;
+    if (!ok) break;
+    if (lane == 0) request(row + int64_t(stages) * gridDim.x, slot);
+    const float var = row_sum<true>(rs, 0, forward_centre(v, mean, lane, threads, nvec)) * inv_n;
+    const float rstd = 1.0f / sqrtf(var + a.eps);
     if (++slot == stages) {
       slot = 0;
       phase ^= 1;
     }
+    forward_out(v, rstd, w, b);
+    store_row<T>(static_cast<T*>(a.y) + row * a.y_stride, lane, threads, nvec, v);
+    if (lane == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
   }
-  if (!ok && threadIdx.x == 0) {
+  if (!ok && lane == 0) {
     atomicAdd(&g_timeouts, 1ull);
     for (int s = 0; s < stages; ++s) tc::bar_wait(bar0 + 8 * s, s < slot ? phase ^ 1 : phase);
   }
 }
 
-template <class T, int NV, bool PARAMS>
+template <class T, int NV>
 __global__ void __launch_bounds__(512) layer_norm_backward_wide_kernel(LayerNormBackwardArgs a,
                                                                        int stages) {
-  constexpr int VEC = 16 / int(sizeof(T)), E = NV * VEC;
-  using P = Pack<T, VEC>;
+  constexpr int VEC = 16 / int(sizeof(T));
   extern __shared__ __align__(128) char smem[];
-  __shared__ float sums[128];
+  __shared__ float2 sums[32];
   __shared__ uint64_t bars[8];
+  __shared__ int gave_up[2];  // by the parity of the row's turn
   RowSum rs{sums};
-  const int nvec = a.dims / VEC, threads = blockDim.x;
+  const int nvec = a.dims / VEC, threads = blockDim.x, lane = threadIdx.x;
   const uint32_t row_bytes = a.dims * sizeof(T), pitch = (row_bytes + 127) & ~127u;
-  const uint32_t slot_bytes = 2 * pitch;
+  const uint32_t slot_bytes = (a.residual ? 3 : 2) * pitch;
   const uint32_t base = tc::smem_addr(smem), bar0 = tc::smem_addr(bars);
   const float inv_n = 1.0f / float(a.dims);
-  if (threadIdx.x == 0) {
+  const bool params = a.partials != nullptr;
+  if (lane == 0) {
+    gave_up[0] = gave_up[1] = 0;
     for (int s = 0; s < stages; ++s) tc::bar_init(bar0 + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -636,109 +663,64 @@ __global__ void __launch_bounds__(512) layer_norm_backward_wide_kernel(LayerNorm
   auto request = [&](int64_t row, int slot) {  // thread 0
     if (row < a.rows) {
       const uint32_t bar = bar0 + 8 * slot, at = base + slot * slot_bytes;
-      tc::bar_expect(bar, 2 * row_bytes);
+      tc::bar_expect(bar, (a.residual ? 3 : 2) * row_bytes);
       bulk_load(at, static_cast<const T*>(a.x) + row * a.x_stride, row_bytes, bar);
       bulk_load(at + pitch, static_cast<const T*>(a.dy) + row * a.dy_stride, row_bytes, bar);
+      if (a.residual)
+        bulk_load(at + 2 * pitch, static_cast<const T*>(a.residual) + row * a.residual_stride, row_bytes,
+                  bar);
     }
   };
-  if (threadIdx.x == 0)
+  if (lane == 0)
     for (int s = 0; s < stages; ++s) request(blockIdx.x + int64_t(s) * gridDim.x, s);
-  float dw[E], db[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
-  int slot = 0;
+  Row<VEC, NV> w, dw{}, db{};
+  load_parameter<T>(a.weight, lane, threads, nvec, 1.0f, w);
+  int slot = 0, turn = 0;
   uint32_t phase = 0;
   bool ok = true;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    // loads that do not go through the ring: under the wait
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
     const float mean = a.mean[row], rstd = a.rstd[row];
-    P pw[NV], pr[NV];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * threads;
-      if (q < nvec) {
-        if (a.weight) pw[k] = static_cast<const P*>(a.weight)[q];
-        if (a.residual)
-          pr[k] = reinterpret_cast<const P*>(static_cast<const T*>(a.residual) +
-                                             row * a.residual_stride)[q];
-      }
-    }
-    ok = tc::bar_wait(bar0 + 8 * slot, phase);
-    ok = __syncthreads_and(ok);
-    if (!ok) break;
-    const P* const in = reinterpret_cast<const P*>(smem + slot * slot_bytes);
-    const P* const gin = reinterpret_cast<const P*>(smem + slot * slot_bytes + pitch);
-    float xh[E], g[E];
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * threads;
-      if (q < nvec) {
-        const P px = in[q], pg = gin[q];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const int e = k * VEC + j;
-          xh[e] = (to_f32(px.v[j]) - mean) * rstd;
-          g[e] = to_f32(pg.v[j]);
-          if (PARAMS) {
-            dw[e] += g[e] * xh[e];
-            db[e] += g[e];
-          }
-          if (a.weight) g[e] *= to_f32(pw[k].v[j]);
-          s1 += g[e];
-          s2 += g[e] * xh[e];
-        }
-      }
-    }
+    if (!tc::bar_wait(bar0 + 8 * slot, phase)) gave_up[turn] = 1;
+    const char* const at = smem + slot * slot_bytes;
+    Row<VEC, NV> xh, g;
+    load_row<T>(reinterpret_cast<const T*>(at), lane, threads, nvec, true, xh);
+    load_row<T>(reinterpret_cast<const T*>(at + pitch), lane, threads, nvec, true, g);
+    float s1, s2;
+    backward_sums<T>(xh, g, w, mean, rstd, params, dw, db, s1, s2);
     row_sum2<true>(rs, 0, s1, s2);
-    // past the barrier in row_sum2 every thread has read the slot
-    if (threadIdx.x == 0) request(row + int64_t(stages) * gridDim.x, slot);
+    ok = gave_up[turn] == 0;
+    if (!ok) break;
+    if (a.dx) {
+      backward_out(xh, g, rstd, s1 * inv_n, s2 * inv_n);
+      if (a.residual) {
+        load_row<T>(reinterpret_cast<const T*>(at + 2 * pitch), lane, threads, nvec, true, xh);
+        add_row(g, xh);
+      }
+      store_row<T>(static_cast<T*>(a.dx) + row * a.dx_stride, lane, threads, nvec, g);
+    }
+    // every thread has read x and dy past the barrier in row_sum2, but the
+    // residual only now
+    if (a.residual) __syncthreads();
+    if (lane == 0) request(row + int64_t(stages) * gridDim.x, slot);
     if (++slot == stages) {
       slot = 0;
       phase ^= 1;
     }
-    if (!a.dx) continue;
-    s1 *= inv_n;
-    s2 *= inv_n;
-    P* const out = reinterpret_cast<P*>(static_cast<T*>(a.dx) + row * a.dx_stride);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * threads;
-      if (q >= nvec) continue;
-      P p;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int e = k * VEC + j;
-        float d = rstd * (g[e] - s1 - xh[e] * s2);
-        if (a.residual) d += to_f32(pr[k].v[j]);
-        p.v[j] = from_f32<T>(d);
-      }
-      out[q] = p;
-    }
   }
-  if (!ok && threadIdx.x == 0) {
+  if (!ok && lane == 0) {
     atomicAdd(&g_timeouts, 1ull);
     for (int s = 0; s < stages; ++s) tc::bar_wait(bar0 + 8 * s, s < slot ? phase ^ 1 : phase);
   }
-  if (!PARAMS) return;
-  float* const part = a.partials + int64_t(blockIdx.x) * 2 * a.dims;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int q = threadIdx.x + k * threads;
-    if (q >= nvec) continue;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      part[q * VEC + j] = dw[k * VEC + j];
-      part[a.dims + q * VEC + j] = db[k * VEC + j];
-    }
-  }
+  if (params)
+    leave_partials(dw, db, lane, threads, nvec, a.dims, 0, 1, nullptr,
+                   a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
 
 // Rows too long for registers: a block walks the row three times (the second
 // and third walks find it in L2).
 template <class T>
 __global__ void __launch_bounds__(512) layer_norm_long_kernel(LayerNormArgs a) {
-  __shared__ float sums[128];
+  __shared__ float2 sums[32];
   RowSum rs{sums};
   const float inv_n = 1.0f / float(a.dims);
   const T* const w = static_cast<const T*>(a.weight);
@@ -768,118 +750,11 @@ __global__ void __launch_bounds__(512) layer_norm_long_kernel(LayerNormArgs a) {
   }
 }
 
-// PARAMS: each block leaves its rows' dw and db sums in
-// partials[block][2][dims].
-template <class T, int VEC, int NV, bool BLOCK, bool PARAMS>
-__global__ void __launch_bounds__(BLOCK ? 512 : kWarpRowThreads)
-layer_norm_backward_kernel(LayerNormBackwardArgs a, int tpr_) {
-  constexpr int E = NV * VEC;
-  __shared__ float sums[128];
-  extern __shared__ float columns[];  // [2][dims], warp rows with PARAMS only
-  RowSum rs{sums};
-  const int tpr = BLOCK ? int(blockDim.x) : tpr_;
-  const int lane = BLOCK ? int(threadIdx.x) : int(threadIdx.x) & (tpr - 1);
-  const int per_block = BLOCK ? 1 : int(blockDim.x) / tpr;
-  const int in_block = BLOCK ? 0 : int(threadIdx.x) / tpr;
-  const int nvec = a.dims / VEC;
-  const float inv_n = 1.0f / float(a.dims);
-  const T* const w = static_cast<const T*>(a.weight);
-  float dw[E], db[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
-  for (int64_t base = int64_t(blockIdx.x) * per_block; base < a.rows;
-       base += int64_t(gridDim.x) * per_block) {
-    const int64_t row = base + in_block;
-    const bool active = row < a.rows;
-    float xh[E], g[E];
-    load_row<T, VEC, NV>(static_cast<const T*>(a.x) + row * a.x_stride, lane, tpr, nvec, active,
-                         xh);
-    load_row<T, VEC, NV>(static_cast<const T*>(a.dy) + row * a.dy_stride, lane, tpr, nvec, active,
-                         g);
-    const float mean = active ? a.mean[row] : 0.0f, rstd = active ? a.rstd[row] : 0.0f;
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = lane + k * tpr;
-      if (!active || q >= nvec) continue;
-      Pack<T, VEC> wp;
-      if (w) wp = reinterpret_cast<const Pack<T, VEC>*>(w)[q];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int e = k * VEC + j;
-        xh[e] = (xh[e] - mean) * rstd;
-        if (PARAMS) {
-          dw[e] += g[e] * xh[e];
-          db[e] += g[e];
-        }
-        if (w) g[e] *= to_f32(wp.v[j]);
-        s1 += g[e];
-        s2 += g[e] * xh[e];
-      }
-    }
-    if (!a.dx) continue;
-    row_sum2<BLOCK>(rs, tpr, s1, s2);
-    if (!active) continue;
-    s1 *= inv_n;
-    s2 *= inv_n;
-    T* const out = static_cast<T*>(a.dx) + row * a.dx_stride;
-    const T* const res =
-        a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = lane + k * tpr;
-      if (q >= nvec) continue;
-      Pack<T, VEC> p, rp;
-      if (res) rp = reinterpret_cast<const Pack<T, VEC>*>(res)[q];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int e = k * VEC + j;
-        float d = rstd * (g[e] - s1 - xh[e] * s2);
-        if (res) d += to_f32(rp.v[j]);
-        p.v[j] = from_f32<T>(d);
-      }
-      reinterpret_cast<Pack<T, VEC>*>(out)[q] = p;
-    }
-  }
-  if (!PARAMS) return;
-  float* const part = a.partials + int64_t(blockIdx.x) * 2 * a.dims;
-  if (BLOCK) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = lane + k * tpr;
-      if (q >= nvec) continue;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        part[q * VEC + j] = dw[k * VEC + j];
-        part[a.dims + q * VEC + j] = db[k * VEC + j];
-      }
-    }
-    return;
-  }
-  for (int group = 0; group < per_block; ++group) {
-    if (group == in_block) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int q = lane + k * tpr;
-        if (q >= nvec) continue;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          float* const cw = columns + q * VEC + j;
-          *cw = group == 0 ? dw[k * VEC + j] : *cw + dw[k * VEC + j];
-          cw[a.dims] = group == 0 ? db[k * VEC + j] : cw[a.dims] + db[k * VEC + j];
-        }
-      }
-    }
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < 2 * a.dims; i += blockDim.x) part[i] = columns[i];
-}
-
 // Long rows: dx by a block per row in two walks; dw and db by
 // column_partials_kernel.
 template <class T>
 __global__ void __launch_bounds__(512) layer_norm_backward_long_kernel(LayerNormBackwardArgs a) {
-  __shared__ float sums[128];
+  __shared__ float2 sums[32];
   RowSum rs{sums};
   const float inv_n = 1.0f / float(a.dims);
   const T* const w = static_cast<const T*>(a.weight);
@@ -1049,12 +924,12 @@ void forward_launch(const LayerNormArgs& a, const RowPlan& p, cudaStream_t strea
   }
 }
 
-template <class T, int VEC, int NV, bool PARAMS>
+template <class T, int VEC, int NV>
 int backward_launch(const LayerNormBackwardArgs& a, const RowPlan& p, cudaStream_t stream) {
   if (p.block) {
     const int64_t grid = std::min<int64_t>(std::min<int64_t>(a.rows, kMaxPartials),
                                            int64_t(sm_count()) * (1024 / p.tpr));
-    layer_norm_backward_kernel<T, VEC, NV, true, PARAMS>
+    layer_norm_backward_kernel<T, VEC, NV, true>
         <<<unsigned(grid), p.tpr, 0, stream>>>(a, p.tpr);
     return int(grid);
   }
@@ -1062,8 +937,8 @@ int backward_launch(const LayerNormBackwardArgs& a, const RowPlan& p, cudaStream
   const int64_t grid =
       std::min<int64_t>(std::min<int64_t>((a.rows + per_block - 1) / per_block, kMaxPartials),
                         int64_t(sm_count()) * 4);
-  const size_t smem = PARAMS ? size_t(a.dims) * 2 * sizeof(float) : 0;
-  layer_norm_backward_kernel<T, VEC, NV, false, PARAMS>
+  const size_t smem = a.partials ? size_t(a.dims) * 2 * sizeof(float) : 0;
+  layer_norm_backward_kernel<T, VEC, NV, false>
       <<<unsigned(grid), kWarpRowThreads, smem, stream>>>(a, p.tpr);
   return int(grid);
 }
@@ -1080,28 +955,43 @@ constexpr size_t kSmemPerSm = 220 * 1024;
 // The tile ring's shape, or row.nv = 0 where a tile has no place.
 struct TilePlan {
   RowPlan row;
-  int warps, stages;
+  int warps, stages, tile_rows;
   size_t smem;
+  TileShape shape() const { return {row.tpr, stages, tile_rows}; }
 };
-TilePlan plan_tiles(size_t size, int dims, int64_t rows, uint32_t slot) {
+// slot_of(tile_rows): bytes of one ring slot.
+template <class F>
+TilePlan plan_tiles(size_t size, int dims, int64_t rows, F&& slot_of) {
   TilePlan p{};
   int vec = 16 / int(size);
   while (dims % vec) vec /= 2;
-  RowPlan row = plan_lanes(dims, vec);
-  // few tiles: fewer warps to a block, so that every SM has some
-  const int64_t tiles = (rows + kTileRows - 1) / kTileRows;
-  p.warps = 8;
-  while (p.warps > 1 && tiles < int64_t(p.warps) * 148) p.warps /= 2;
-  // two blocks of eight warps to an SM (their registers allow no more), one
-  // where two slots per warp would not fit otherwise
-  for (int blocks = 2 * (8 / p.warps); blocks >= 1; --blocks) {
-    p.stages = int(std::min<size_t>(4, kSmemPerSm / blocks / (size_t(p.warps) * (slot + 8) + 128)));
-    if (p.stages >= 2) break;
+  const RowPlan row = plan_lanes(dims, vec);
+  if (row.nv == 0) return p;
+  // Two blocks of eight warps fit an SM's registers.  Tiles of eight rows
+  // where their rings leave room for both, else of four where those are whole
+  // 16-byte units and a warp has no more rows at once.
+  for (int tile_rows : {8, 4}) {
+    if (tile_rows == 4 && (size_t(dims) * size * 4 % 16 || row.tpr < 8)) break;
+    const size_t slot = slot_of(tile_rows);
+    // few tiles: fewer warps to a block, so that every SM has some
+    const int64_t tiles = (rows + tile_rows - 1) / tile_rows;
+    int warps = 8;
+    while (warps > 1 && tiles < int64_t(warps) * 148) warps /= 2;
+    for (int blocks = 2 * (8 / warps); blocks >= 1; --blocks) {
+      const int stages =
+          int(std::min<size_t>(4, kSmemPerSm / blocks / (size_t(warps) * (slot + 8) + 128)));
+      if (stages < 2) continue;
+      if (p.row.nv && blocks < 2) break;  // eight rows fit as well as four
+      p.smem = ((size_t(warps) * stages * 8 + 127) & ~size_t(127)) + size_t(warps) * stages * slot;
+      p.smem = (p.smem + 4095) & ~size_t(4095);  // few distinct launch shapes
+      p.row = row;
+      p.warps = warps;
+      p.stages = stages;
+      p.tile_rows = tile_rows;
+      if (blocks >= 2) return p;
+      break;
+    }
   }
-  if (p.stages < 2) return p;
-  p.smem = ((size_t(p.warps) * p.stages * 8 + 127) & ~size_t(127)) + size_t(p.warps) * p.stages * slot;
-  p.smem = (p.smem + 4095) & ~size_t(4095);  // few distinct launch shapes
-  p.row = row;
   return p;
 }
 template <class K>
@@ -1109,7 +999,7 @@ npa_status tile_grid(K kernel, const TilePlan& p, int64_t rows, unsigned* grid) 
   int per_sm = 0, sms = 0;
   NPA_TRY(kernel_occupancy(reinterpret_cast<const void*>(kernel), p.warps * 32, p.smem, &per_sm, &sms));
   if (per_sm < 1) return fail(NPA_ERR_UNSUPPORTED, "layer norm kernel cannot be resident");
-  const int64_t tiles = (rows + kTileRows - 1) / kTileRows;
+  const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   *grid = unsigned(std::min<int64_t>(
       std::min<int64_t>((tiles + p.warps - 1) / p.warps, int64_t(per_sm) * sms), kMaxPartials));
   return NPA_OK;
@@ -1147,14 +1037,15 @@ npa_status wide_grid(K kernel, const WidePlan& p, int64_t rows, unsigned* grid) 
 template <class T>
 npa_status forward_typed(const LayerNormArgs& a, cudaStream_t s) {
   if (gapless(a.x, a.x_stride, a.rows, a.dims) && gapless(a.y, a.y_stride, a.rows, a.dims)) {
-    const uint32_t slot = (uint32_t(std::min(a.dims, 1 << 16)) * kTileRows * sizeof(T) + 127) & ~127u;
-    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, slot);
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, [&](int tile_rows) {
+      return (size_t(a.dims) * tile_rows * sizeof(T) + 127) & ~size_t(127);
+    });
     if (p.row.nv)
       return with_row_shape<T>(p.row.vec, p.row.nv, [&](auto vec, auto nv) -> npa_status {
         const auto kernel = layer_norm_tiles_kernel<T, vec(), nv()>;
         unsigned grid = 0;
         NPA_TRY(tile_grid(kernel, p, a.rows, &grid));
-        kernel<<<grid, p.warps * 32, p.smem, s>>>(a, p.row.tpr, p.stages);
+        kernel<<<grid, p.warps * 32, p.smem, s>>>(a, p.shape());
         return after_launch("layer_norm_tiles_kernel");
       });
   }
@@ -1200,15 +1091,15 @@ npa_status backward_rows(const LayerNormBackwardArgs& a, int* parts, cudaStream_
       gapless(a.dx, a.dx_stride, a.rows, a.dims) &&
       gapless(a.residual, a.residual_stride, a.rows, a.dims) && bulk_rows(a.mean, 0, 4) &&
       bulk_rows(a.rstd, 0, 4)) {
-    const uint32_t slot =
-        backward_slot(uint32_t(std::min(a.dims, 1 << 16)) * kTileRows * sizeof(T), a.residual != nullptr);
-    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, slot);
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, [&](int tile_rows) {
+      return backward_slot(uint32_t(a.dims * tile_rows * sizeof(T)), a.residual != nullptr, tile_rows);
+    });
     if (p.row.nv)
       return with_row_shape<T>(p.row.vec, p.row.nv, [&](auto vec, auto nv) -> npa_status {
         const auto kernel = layer_norm_backward_tiles_kernel<T, vec(), nv()>;
         unsigned grid = 0;
         NPA_TRY(tile_grid(kernel, p, a.rows, &grid));
-        kernel<<<grid, p.warps * 32, p.smem, s>>>(a, p.row.tpr, p.stages);
+        kernel<<<grid, p.warps * 32, p.smem, s>>>(a, p.shape());
         *parts = int(grid);
         return after_launch("layer_norm_backward_tiles_kernel");
       });
@@ -1216,7 +1107,8 @@ npa_status backward_rows(const LayerNormBackwardArgs& a, int* parts, cudaStream_
   if (bulk_rows(a.x, a.x_stride, sizeof(T)) && bulk_rows(a.dy, a.dy_stride, sizeof(T)) &&
       bulk_rows(a.dx, a.dx_stride, sizeof(T)) && bulk_rows(a.weight, 0, sizeof(T)) &&
       bulk_rows(a.residual, a.residual_stride, sizeof(T))) {
-    const size_t slot = 2 * ((size_t(a.dims) * sizeof(T) + 127) & ~size_t(127));
+    const size_t slot =
+        (a.residual ? 3 : 2) * ((size_t(a.dims) * sizeof(T) + 127) & ~size_t(127));
     const WidePlan p = plan_wide(sizeof(T), a.dims, slot, sizeof(T) == 2 ? 2 : 4);
     if (p.nv) {
       auto launch = [&](auto kernel) -> npa_status {
@@ -1226,15 +1118,9 @@ npa_status backward_rows(const LayerNormBackwardArgs& a, int* parts, cudaStream_
         *parts = int(grid);
         return after_launch("layer_norm_backward_wide_kernel");
       };
-      if (p.nv == 1)
-        return params ? launch(layer_norm_backward_wide_kernel<T, 1, true>)
-                      : launch(layer_norm_backward_wide_kernel<T, 1, false>);
-      if (p.nv == 2)
-        return params ? launch(layer_norm_backward_wide_kernel<T, 2, true>)
-                      : launch(layer_norm_backward_wide_kernel<T, 2, false>);
-      if constexpr (sizeof(T) == 4)
-        return params ? launch(layer_norm_backward_wide_kernel<T, 4, true>)
-                      : launch(layer_norm_backward_wide_kernel<T, 4, false>);
+      if (p.nv == 1) return launch(layer_norm_backward_wide_kernel<T, 1>);
+      if (p.nv == 2) return launch(layer_norm_backward_wide_kernel<T, 2>);
+      if constexpr (sizeof(T) == 4) return launch(layer_norm_backward_wide_kernel<T, 4>);
     }
   }
   int vec = 16 / int(sizeof(T));
@@ -1262,8 +1148,7 @@ npa_status backward_rows(const LayerNormBackwardArgs& a, int* parts, cudaStream_
     return NPA_OK;
   }
   *parts = with_row_shape<T>(p.vec, p.nv, [&](auto v, auto nv) -> int {
-    return params ? backward_launch<T, v(), nv(), true>(a, p, s)
-                  : backward_launch<T, v(), nv(), false>(a, p, s);
+    return backward_launch<T, v(), nv()>(a, p, s);
   });
   return after_launch("layer_norm_backward_kernel");
 }
