@@ -216,30 +216,35 @@ __device__ __forceinline__ void add_row(Row<VEC, NV>& a, const Row<VEC, NV>& b) 
 #pragma unroll
   for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) a.v[i] = add2(a.v[i], b.v[i]);
 }
-// The block's dw and db into partials[block][2][dims]: row groups that share
-// columns add to shared memory in turn (`turns` groups, this thread's at `turn`).
+// The block's dw and db into part[2][dims].  Lanes of a warp that share columns
+// add by shuffles, warps through columns[warps][2][dims] in shared memory.
 template <int VEC, int NV>
-__device__ __forceinline__ void leave_partials(const Row<VEC, NV>& dw, const Row<VEC, NV>& db, int lane,
-                                               int tpr, int nvec, int dims, int turn, int turns,
-                                               float* columns, float* part) {
-  float* const to = turns > 1 ? columns : part;
-  for (int t = 0; t < turns; ++t) {
-    if (t == turn) {
+__device__ __forceinline__ void leave_partials(Row<VEC, NV>& dw, Row<VEC, NV>& db, int lane, int tpr,
+                                               int nvec, int dims, float* columns, float* part) {
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  float* const to = tpr <= 32 ? columns + warp * 2 * dims : part;
 #pragma unroll
-      for (int e = 0; e < VEC * NV; ++e) {
-        const int q = lane + e / VEC * tpr;
-        if (q >= nvec) continue;
-        const float2 w2 = values(dw.v[e / 2]), b2 = values(db.v[e / 2]);
-        const float w = e & 1 ? w2.y : w2.x, b = e & 1 ? b2.y : b2.x;
-        float* const c = to + q * VEC + e % VEC;
-        c[0] = t == 0 ? w : c[0] + w;
-        c[dims] = t == 0 ? b : c[dims] + b;
-      }
+  for (int e = 0; e < VEC * NV; ++e) {
+    const float2 w2 = values(dw.v[e / 2]), b2 = values(db.v[e / 2]);
+    float w = e & 1 ? w2.y : w2.x, b = e & 1 ? b2.y : b2.x;
+    for (int o = tpr; o < 32; o <<= 1) {
+      w += __shfl_xor_sync(kFull, w, o);
+      b += __shfl_xor_sync(kFull, b, o);
     }
-    if (turns > 1) __syncthreads();
+    const int q = lane + e / VEC * tpr;
+    if (q < nvec && (tpr > 32 || int(threadIdx.x & 31) < tpr)) {
+      to[q * VEC + e % VEC] = w;
+      to[dims + q * VEC + e % VEC] = b;
+    }
   }
-  if (turns > 1)
-    for (int i = threadIdx.x; i < 2 * dims; i += blockDim.x) part[i] = columns[i];
+  if (tpr > 32) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * dims; i += blockDim.x) {
+    float s = 0.0f;
+#pragma unroll 8
+    for (int w = 0; w < warps; ++w) s += columns[w * 2 * dims + i];
+    part[i] = s;
+  }
 }
 
 // ---- plain loads ----
@@ -280,7 +285,7 @@ template <class T, int VEC, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 512 : kWarpRowThreads)
 layer_norm_backward_kernel(LayerNormBackwardArgs a, int tpr_) {
   __shared__ float2 sums[32];
-  extern __shared__ float columns[];  // [2][dims], rows of a warp or less
+  extern __shared__ float columns[];  // [warps][2][dims], rows of a warp or less
   RowSum rs{sums};
   const int tpr = BLOCK ? int(blockDim.x) : tpr_;
   const int lane = BLOCK ? int(threadIdx.x) : int(threadIdx.x) & (tpr - 1);
@@ -311,7 +316,7 @@ layer_norm_backward_kernel(LayerNormBackwardArgs a, int tpr_) {
     store_row<T>(static_cast<T*>(a.dx) + row * a.dx_stride, lane, tpr, nvec, g);
   }
   if (params)
-    leave_partials(dw, db, lane, tpr, nvec, a.dims, in_block, per_block, columns,
+    leave_partials(dw, db, lane, tpr, nvec, a.dims, columns,
                    a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
 
@@ -572,7 +577,7 @@ layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
   }
   if (!params) return;
   __syncthreads();  // the ring's memory now holds the block's columns
-  leave_partials(dw, db, sub, tpr, nvec, a.dims, warp * at_once + group, warps * at_once,
+  leave_partials(dw, db, sub, tpr, nvec, a.dims,
                  reinterpret_cast<float*>(smem + ((warps * stages * 8 + 127) & ~127)),
                  a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
@@ -712,7 +717,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_wide_kernel(LayerNorm
     for (int s = 0; s < stages; ++s) tc::bar_wait(bar0 + 8 * s, s < slot ? phase ^ 1 : phase);
   }
   if (params)
-    leave_partials(dw, db, lane, threads, nvec, a.dims, 0, 1, nullptr,
+    leave_partials(dw, db, lane, threads, nvec, a.dims, nullptr,
                    a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
 
@@ -802,26 +807,28 @@ __global__ void __launch_bounds__(256) column_partials_kernel(LayerNormBackwardA
   part[a.dims + col] = db;
 }
 
-// dw and db from the blocks' partial sums: 32 columns per block, whose 8 row
-// lanes each add every eighth partial in order and meet in a fixed tree.
+// dw and db from the blocks' partial sums: 32 columns per block, whose 32 row
+// lanes each add every 32nd partial in order; their sums meet in order too.
 template <class T>
-__global__ void __launch_bounds__(256) column_reduce_kernel(const float* __restrict__ partials,
-                                                            int count, int dims, T* dweight,
-                                                            T* dbias) {
-  __shared__ float acc[8][32];
+__global__ void __launch_bounds__(1024) column_reduce_kernel(const float* __restrict__ partials,
+                                                             int count, int dims, T* dweight,
+                                                             T* dbias) {
+  __shared__ float acc[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t col = int64_t(blockIdx.x) * 32 + tx;  // over [2][dims]
   float s = 0.0f;
   if (col < 2 * int64_t(dims))
 #pragma unroll 8
-    for (int p = ty; p < count; p += 8) s += partials[int64_t(p) * 2 * dims + col];
+    for (int p = ty; p < count; p += 32) s += partials[int64_t(p) * 2 * dims + col];
   acc[ty][tx] = s;
   __syncthreads();
-  if (ty != 0 || col >= 2 * int64_t(dims)) return;
-  s = ((acc[0][tx] + acc[1][tx]) + (acc[2][tx] + acc[3][tx])) +
-      ((acc[4][tx] + acc[5][tx]) + (acc[6][tx] + acc[7][tx]));
-  T* const out = col < dims ? dweight : dbias;
-  if (out) out[col < dims ? col : col - dims] = from_f32<T>(s);
+  // warp ty adds column ty's 32 sums
+  s = acc[tx][ty];
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+  const int64_t out_col = int64_t(blockIdx.x) * 32 + ty;
+  if (tx != 0 || out_col >= 2 * int64_t(dims)) return;
+  T* const out = out_col < dims ? dweight : dbias;
+  if (out) out[out_col < dims ? out_col : out_col - dims] = from_f32<T>(s);
 }
 
 // How a row is spread over threads, in accesses of `vec` values.
@@ -937,7 +944,8 @@ int backward_launch(const LayerNormBackwardArgs& a, const RowPlan& p, cudaStream
   const int64_t grid =
       std::min<int64_t>(std::min<int64_t>((a.rows + per_block - 1) / per_block, kMaxPartials),
                         int64_t(sm_count()) * 4);
-  const size_t smem = a.partials ? size_t(a.dims) * 2 * sizeof(float) : 0;
+  const size_t smem =
+      a.partials ? size_t(kWarpRowThreads / 32) * a.dims * 2 * sizeof(float) : 0;
   layer_norm_backward_kernel<T, VEC, NV, false>
       <<<unsigned(grid), kWarpRowThreads, smem, stream>>>(a, p.tpr);
   return int(grid);
@@ -1160,7 +1168,7 @@ npa_status backward_typed(LayerNormBackwardArgs a, cudaStream_t s) {
   int parts = 0;
   if (a.rows > 0 && (a.dx || params)) NPA_TRY(backward_rows<T>(a, &parts, s));
   if (!params) return NPA_OK;
-  column_reduce_kernel<T><<<unsigned((2 * int64_t(a.dims) + 31) / 32), 256, 0, s>>>(
+  column_reduce_kernel<T><<<unsigned((2 * int64_t(a.dims) + 31) / 32), 1024, 0, s>>>(
       a.partials, parts, a.dims, static_cast<T*>(a.dweight), static_cast<T*>(a.dbias));
   return after_launch("column_reduce_kernel");
 }

@@ -65,6 +65,84 @@ __global__ void __launch_bounds__(256) product_reduce_kernel(const __grid_consta
   }
 }
 
+// ---- a few rows: bound by reading the weights once ----
+constexpr int kFewRows = 8;
+
+// A warp has OUTS outputs of all R rows and walks k with 16-byte loads (VEC
+// values; single values where a row does not start on 16 bytes).  Plain f32
+// products: at eight rows a weight read from memory still costs more than its
+// eight multiply-adds.
+template <class T, int R, int OUTS, int VEC>
+__global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ LinearArgs a) {
+  using P = Pack<T, VEC>;
+  const int lane = threadIdx.x & 31;
+  const int64_t first = (int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5)) * OUTS;
+  if (first >= a.outputs) return;
+  const T* const w = static_cast<const T*>(a.weight);
+  const T* const x = static_cast<const T*>(a.x);
+  float acc[R][OUTS];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o) acc[r][o] = 0.0f;
+  const int rows = int(a.rows);
+#pragma unroll 2
+  for (int k = lane * VEC; k < a.inputs; k += 32 * VEC) {
+    P wv[OUTS];
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o)  // past the last output: the last one again
+      wv[o] = *reinterpret_cast<const P*>(w + min(first + o, int64_t(a.outputs) - 1) * a.weight_stride + k);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const P xv = *reinterpret_cast<const P*>(x + int64_t(min(r, rows - 1)) * a.x_stride + k);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float xf = to_f32(xv.v[j]);
+#pragma unroll
+        for (int o = 0; o < OUTS; ++o) acc[r][o] += xf * to_f32(wv[o].v[j]);
+      }
+    }
+  }
+  float mine = 0.0f;  // lane r * OUTS + o keeps (r, o)
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o) {
+      float s = acc[r][o];
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+      if (lane == r * OUTS + o) mine = s;
+    }
+  const int r = lane / OUTS;
+  const int64_t col = first + lane % OUTS;
+  if (r >= R || r >= rows || col >= a.outputs) return;
+  float z = mine;
+  if (a.bias) z += to_f32(static_cast<const T*>(a.bias)[col]);
+  if (a.z) static_cast<T*>(a.z)[r * a.z_stride + col] = from_f32<T>(z);
+  float y = linear_tc::activation<sizeof(T) == 2>(a.activation, z);
+  if (a.residual) y += to_f32(static_cast<const T*>(a.residual)[r * a.residual_stride + col]);
+  static_cast<T*>(a.y)[r * a.y_stride + col] = from_f32<T>(y);
+}
+template <class T, int R>
+npa_status launch_few_rows(const LinearArgs& a, bool vec, cudaStream_t s) {
+  constexpr int kVec = 16 / int(sizeof(T));
+  // four outputs to a warp once that leaves most SMs a block
+  if (a.outputs >= 2048) {
+    const unsigned grid = unsigned((a.outputs + 31) / 32);
+    if (vec)
+      few_rows_kernel<T, R, 4, kVec><<<grid, 256, 0, s>>>(a);
+    else
+      few_rows_kernel<T, R, 4, 1><<<grid, 256, 0, s>>>(a);
+  } else {
+    const unsigned grid = unsigned((a.outputs + 7) / 8);
+    if (vec)
+      few_rows_kernel<T, R, 1, kVec><<<grid, 256, 0, s>>>(a);
+    else
+      few_rows_kernel<T, R, 1, 1><<<grid, 256, 0, s>>>(a);
+  }
+  return after_launch("linear few_rows_kernel");
+}
+
 // ---- dz and the bias gradient ----
 struct SlopeArgs {
   const void* dy;
@@ -426,6 +504,14 @@ BackwardCarve carve_backward(void* ws, int dtype, int activation, int64_t rows, 
 
 template <class T>
 npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
+  if (a.rows <= kFewRows) {
+    constexpr int kVec = 16 / int(sizeof(T));
+    const bool vec = a.inputs % kVec == 0 && vector_width<T>(a.x, a.x_stride, a.rows) == kVec &&
+                     vector_width<T>(a.weight, a.weight_stride, a.outputs) == kVec;
+    if (a.rows == 1) return launch_few_rows<T, 1>(a, vec, s);
+    if (a.rows == 2) return launch_few_rows<T, 2>(a, vec, s);
+    return a.rows <= 4 ? launch_few_rows<T, 4>(a, vec, s) : launch_few_rows<T, 8>(a, vec, s);
+  }
   Product p{};
   p.a = {a.x, a.x_stride, 0};
   p.b = {a.weight, a.weight_stride, 0};
@@ -527,7 +613,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
 }  // namespace
 
 size_t linear_workspace(int dtype, int64_t rows, int inputs, int outputs) {
-  return rows == 0 ? 0 : product_workspace(dtype_bytes(dtype), rows, outputs, inputs);
+  return rows <= kFewRows ? 0 : product_workspace(dtype_bytes(dtype), rows, outputs, inputs);
 }
 
 npa_status launch_linear(int dtype, const LinearArgs& a, void* workspace, cudaStream_t stream) {

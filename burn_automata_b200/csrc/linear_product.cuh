@@ -80,7 +80,8 @@ struct Config {
   static constexpr int kStages = kStagesFit > 6 ? 6 : kStagesFit;
   static constexpr int kBufferColumns = BN * (kParts == 3 ? 2 : 1);
   static constexpr int kTmemColumns = 2 * kBufferColumns;
-  static constexpr int kThreads = 32 * (kEpilogueWarps + 2 + (LOADER ? kLoaderWarps - 1 : 0));
+  // epilogue warps, a warpgroup with the issuing and the TMA warp, loader warps
+  static constexpr int kThreads = 32 * (kEpilogueWarps + 4 + (LOADER ? kLoaderWarps : 0));
   static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kOutBytes + 1024 + 256;
   static_assert(kStages >= 2 && kTmemColumns <= 512, "tile does not fit");
 };
@@ -223,7 +224,7 @@ __device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
 
 // One value of the product by plain f32 steps over [k0, k1).
 template <class T>
-__device__ __noinline__ float plain_dot(const Product& p, int64_t i, int64_t j, int64_t k0, int64_t k1) {
+__device__ __forceinline__ float plain_dot(const Product& p, int64_t i, int64_t j, int64_t k0, int64_t k1) {
   const T* a = static_cast<const T*>(p.a.p) + (p.a.mn_major ? i : i * p.a.ld);
   const T* b = static_cast<const T*>(p.b.p) + (p.b.mn_major ? j : j * p.b.ld);
   const int64_t sa = p.a.mn_major ? p.a.ld : 1, sb = p.b.mn_major ? p.b.ld : 1;
@@ -396,7 +397,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const uint32_t acc_full = empty + 8 * C::kStages, acc_empty = acc_full + 16;
   const uint32_t drain = acc_empty + 16, tmem_at = drain + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kMmaWarp = kEpilogueWarps, kProducerWarp = kEpilogueWarps + 1;
+  constexpr int kMmaWarp = kEpilogueWarps, kTmaWarp = kEpilogueWarps + 1;
+  constexpr int kFirstLoader = kEpilogueWarps + 4;
   // a pair walks the tiles together
   const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
   const int64_t walker = PAIR ? blockIdx.x / 2 : blockIdx.x;
@@ -421,7 +423,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     tc::tmem_alloc<PAIR>(tmem_at, C::kTmemColumns);
     tc::fence_before();
   }
-  if (warp == kProducerWarp && lane == 0) {
+  if (warp == kTmaWarp && lane == 0) {
     if (!LOADER) {
       tc::prefetch_map(&map_a);
       tc::prefetch_map(&map_b);
@@ -436,10 +438,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(tmem) : "r"(tmem_at) : "memory");
   bool ok = true;
 
-  if (warp >= kProducerWarp) {
+  // The loader kernel's 640 threads start with 96 registers each; its control
+  // warpgroup leaves some to the others: 40 + 2 x 96 + 2 x 120 = 472 of the
+  // launch's 480 per thread of each warpgroup.
+  if (warp > kMmaWarp) {
     // ---- producers ----
     if (!LOADER) {
-      if (lane == 0) {
+      if (warp == kTmaWarp && lane == 0) {
         Cursor<C::kStages> at;
         uint32_t issued = 0;
         const uint32_t first_full = PAIR ? tc::in_first_block(full) : full;
@@ -490,47 +495,67 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
       }
     } else {
-      const int tid = threadIdx.x - kProducerWarp * 32;
-      constexpr int kThreads = kLoaderWarps * 32;
-      constexpr int kPerThread = 1024 / kThreads;  // chunks of 128 lines
-      Cursor<C::kStages> at;
-      for (int64_t t = walker; t < tiles && ok; t += walkers) {
-        const int split = int(t / layer), in = int(t % layer);
-        const int64_t m0 = int64_t(in / p.n_tiles) * kBM, n0 = int64_t(in % p.n_tiles) * BN;
-        const int kb = split * p.split_blocks;
-        const int ke = min(p.k_blocks, kb + p.split_blocks);
-        for (int kt = kb; kt < ke; ++kt, at.advance()) {
-          const uint32_t s = at.slot;
-          const int64_t k0 = int64_t(kt) * kBK;
-          Chunk<T> c[kPerThread];
+      if (warp < kFirstLoader) {
+        tc::registers_down<40>();
+      } else {
+        tc::registers_up<120>();
+        // A thread has four chunks of A's tile and up to four of B's.  The loads
+        // of one are in flight while the other is split and written.
+        const int tid = threadIdx.x - kFirstLoader * 32;
+        constexpr int kThreads = kLoaderWarps * 32;
+        constexpr int kAChunks = kBM * 8 / kThreads, kBChunks = BN * 8 / kThreads;
+        Cursor<C::kStages> at;
+        Chunk<T> ca[kAChunks], cb[kBChunks];
+        int64_t t = walker, m0 = 0, n0 = 0;
+        int kt = 0, ke = 0;
+        auto enter_tile = [&]() {
+          const int split = int(t / layer), in = int(t % layer);
+          m0 = int64_t(in / p.n_tiles) * kBM;
+          n0 = int64_t(in % p.n_tiles) * BN;
+          kt = split * p.split_blocks;
+          ke = min(p.k_blocks, kt + p.split_blocks);
+        };
+        auto read_a = [&]() {
 #pragma unroll
-          for (int i = 0; i < kPerThread; ++i)
-            read_tile_chunk<T>(p.a, p.a_vec, m0, p.m, k0, p.k, tid + i * kThreads, c[i]);
-          ok = tc::bar_wait(empty + 8 * s, at.parity ^ 1);
+          for (int i = 0; i < kAChunks; ++i)
+            read_tile_chunk<T>(p.a, p.a_vec, m0, p.m, int64_t(kt) * kBK, p.k, tid + i * kThreads, ca[i]);
+        };
+        if (t < tiles) {
+          enter_tile();
+          read_a();
+        }
+        for (; t < tiles; at.advance()) {
+#pragma unroll
+          for (int i = 0; i < kBChunks; ++i)
+            read_tile_chunk<T>(p.b, p.b_vec, n0, p.n, int64_t(kt) * kBK, p.k, tid + i * kThreads, cb[i]);
+          ok = tc::bar_wait(empty + 8 * at.slot, at.parity ^ 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const uint32_t a = base + s * C::kStageBytes, b = a + C::kParts * C::kABytes;
+          const uint32_t a = base + at.slot * C::kStageBytes, b = a + C::kParts * C::kABytes;
 #pragma unroll
-          for (int i = 0; i < kPerThread; ++i) {
+          for (int i = 0; i < kAChunks; ++i) {
             const int q = tid + i * kThreads;
-            store_chunk<T>(a + swizzled(q >> 3, q & 7), C::kABytes, c[i]);
+            store_chunk<T>(a + swizzled(q >> 3, q & 7), C::kABytes, ca[i]);
           }
+          if (++kt == ke) {
+            t += walkers;
+            if (t < tiles) enter_tile();
+          }
+          if (t < tiles) read_a();
 #pragma unroll
-          for (int i = 0; i < BN * 8 / kThreads; ++i)
-            read_tile_chunk<T>(p.b, p.b_vec, n0, p.n, k0, p.k, tid + i * kThreads, c[i]);
-#pragma unroll
-          for (int i = 0; i < BN * 8 / kThreads; ++i) {
+          for (int i = 0; i < kBChunks; ++i) {
             const int q = tid + i * kThreads;
-            store_chunk<T>(b + swizzled(q >> 3, q & 7), C::kBBytes, c[i]);
+            store_chunk<T>(b + swizzled(q >> 3, q & 7), C::kBBytes, cb[i]);
           }
           tc::fence_async_shared();
           __syncwarp();
-          if (lane == 0) tc::bar_arrive(full + 8 * s);
+          if (lane == 0) tc::bar_arrive(full + 8 * at.slot);
         }
       }
     }
   } else if (warp == kMmaWarp) {
     // ---- the thread that issues the products (the pair's first block's) ----
+    if constexpr (LOADER) tc::registers_down<40>();
     if (lane == 0 && rank == 0) {
       // One thread issues everything, so its own instructions between two
       // blocks of k count: cursors step by one and descriptors by additions.
@@ -634,13 +659,16 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
           for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
             const uint32_t at = tmem + buf * C::kBufferColumns + lanes + (half + 2 * gi) * kGroup;
-            float v[kGroup];
-            tc::tmem_load(at + BN, v);
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e) sums[gi][e] += v[e];
-            tc::tmem_load(at, v);
+            for (int h = 0; h < kGroup; h += 16) {
+              float part[16];
+              tc::tmem_load(at + BN + h, part);
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e) sums[gi][e] += v[e];
+              for (int e = 0; e < 16; ++e) sums[gi][h + e] += part[e];
+              tc::tmem_load(at + h, part);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) sums[gi][h + e] += part[e];
+            }
           }
           release_accumulators(buf);
         }
@@ -653,14 +681,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         tc::fence_after();
         d = tmem + buf * C::kBufferColumns + lanes;
       }
-#pragma unroll
-      for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
+      // One group of columns; v: its sums (f32), or room for its accumulators.
+      auto finish_group = [&](int gi, float (&v)[kGroup]) {
         const int g = half + 2 * gi;
         const int col0 = n0 + g * kGroup;
         const bool last = gi + 1 == kGroupsPerWarp;
         const bool mine = g < kGroups && col0 < p.n && rows > 0;
         const int cols = min(kGroup, p.n - col0);
-        float v[kGroup];
         // the TMA kernel loads the residual before it reads the accumulators, so
         // that the loads' latency passes under them; the loader kernel's register
         // budget (five warps to an SM quarter) has no room for it
@@ -680,16 +707,30 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
         }
         if constexpr (C::kParts == 3) {
+          bool odd = false;
 #pragma unroll
-          for (int e = 0; e < kGroup; ++e) v[e] = sums[gi][e];
-          if (mine && lane < rows) {
-            const int64_t k0 = int64_t(split) * p.split_blocks * kBK;
-            const int64_t k1 = min(int64_t(p.k), k0 + int64_t(p.split_blocks) * kBK);
+          for (int e = 0; e < kGroup; ++e) odd = odd || v[e] != v[e];
+          if (__any_sync(0xffffffffu, mine && lane < rows && odd)) {
+            // through the staging buffer, so that the rare loop needs no registers
+            const uint32_t b = next_buffer();
+            stage_values<float>(b, lane, v, 0);
+            if (mine && lane < rows) {
+              const int64_t k0 = int64_t(split) * p.split_blocks * kBK;
+              const int64_t k1 = min(int64_t(p.k), k0 + int64_t(p.split_blocks) * kBK);
+              for (int e = 0; e < cols; ++e) {
+                float* const at = reinterpret_cast<float*>(pointer(b) + swizzled(lane, e >> 2)) + (e & 3);
+                if (*at != *at) *at = plain_dot<T>(p, row0 + lane, col0 + e, k0, k1);
+              }
+            }
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e)
-              if (v[e] != v[e] && e < cols) v[e] = plain_dot<T>(p, row0 + lane, col0 + e, k0, k1);
+            for (int c = 0; c < 8; ++c) {
+              const uint4 u = load_shared16(b + swizzled(lane, c));
+              v[4 * c] = __uint_as_float(u.x);
+              v[4 * c + 1] = __uint_as_float(u.y);
+              v[4 * c + 2] = __uint_as_float(u.z);
+              v[4 * c + 3] = __uint_as_float(u.w);
+            }
           }
-          __syncwarp();
         } else {
           if (mine) tc::tmem_load(d + g * kGroup, v);
           if (last) {
@@ -697,7 +738,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             acc.advance();
           }
         }
-        if (!mine) continue;
+        if (!mine) return;
         if (p.partials) {
           const int64_t prow = split * p.layer_rows + row0;
 #pragma unroll
@@ -708,7 +749,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             put_group<float>(b, pointer(b), lane, &map_y, true, col0 + h * 32, int(prow), nullptr,
                              0, 0, 0, 0);
           }
-          continue;
+          return;
         }
         if (p.bias) {
           const T* const bias = static_cast<const T*>(p.bias) + col0;
@@ -773,6 +814,15 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         stage_values<T>(b, lane, v, 0);
         put_group<T>(b, pointer(b), lane, &map_y, p.y_tma, col0, int(row0), p.y, p.y_stride, row0,
                      rows, cols);
+      };
+#pragma unroll
+      for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
+        if constexpr (C::kParts == 3) {
+          finish_group(gi, sums[gi]);
+        } else {
+          float v[kGroup];
+          finish_group(gi, v);
+        }
       }
     }
     if (lane == 0) tc::bulk_wait_all();

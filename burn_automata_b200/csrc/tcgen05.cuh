@@ -61,6 +61,16 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   }
 }
 
+// ---- registers between roles: every warp of a warpgroup, shares within the launch's total ----
+template <int REGS>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS));
+}
+
 // ---- block pairs (clusters of two) ----
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -179,6 +189,19 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
 }
 // Accumulator columns of this warp's 32 TMEM lanes, one row per thread.  The
 // wait is part of the load: nothing may read the registers before it.
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      " tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
   uint32_t r[32];
   asm volatile(
