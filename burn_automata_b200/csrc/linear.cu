@@ -8,11 +8,12 @@
 #include <algorithm>
 #include <atomic>
 
-#include "linear_product.cuh"
+#include "linear_backward.cuh"
 
 namespace npa {
 namespace {
 
+using linear_tc::FusedBackward;
 using linear_tc::Operand;
 using linear_tc::Product;
 
@@ -478,6 +479,36 @@ npa_status run_product(Product p, float* partials, cudaStream_t stream) {
   return after_launch("product_reduce_kernel");
 }
 
+// The one-walk backward pass's shape, or stage_bytes = 0 where it has none:
+// 16-bit layers whose weights, two stages of rows and accumulators fit an SM.
+constexpr int64_t kFusedRows = 2048;  // at least: fewer rows leave most SMs idle
+FusedBackward plan_fused(size_t size, int activation, int64_t rows, int inputs, int outputs) {
+  FusedBackward f{};
+  if (size != 2 || rows < kFusedRows || inputs > 256 || outputs > 256) return f;
+  f.rows = rows;
+  f.inputs = inputs;
+  f.outputs = outputs;
+  f.out_blocks = ceil_div(outputs, 64);
+  f.in_blocks = ceil_div(inputs, 64);
+  f.k_pad = ceil_div(outputs, 16) * 16;
+  f.n_pad = ceil_div(inputs, 16) * 16;
+  f.m_blocks = ceil_div(outputs, 128);
+  f.act = activation;
+  f.has_z = activation != NPA_ACTIVATION_IDENTITY;
+  f.stage_bytes = uint32_t(f.out_blocks * (f.has_z ? 2 : 1) + f.in_blocks) * linear_tc::kBM * 128;
+  f.weight_bytes = uint32_t(f.in_blocks) * f.k_pad * 128;
+  f.tmem_columns = 32;
+  while (int(f.tmem_columns) < (f.m_blocks + 2) * f.n_pad) f.tmem_columns *= 2;
+  f.pitch = (int64_t(inputs) + 3) / 4 * 4;
+  return linear_tc::fused_fits(f) ? f : FusedBackward{};
+}
+int fused_blocks(const FusedBackward& f) {
+  return int(std::min<int64_t>(kSms, (f.rows + linear_tc::kBM - 1) / linear_tc::kBM));
+}
+size_t fused_partial_bytes(const FusedBackward& f) {
+  return f.stage_bytes ? size_t(fused_blocks(f)) * f.m_blocks * linear_tc::kBM * f.pitch * 4 : 0;
+}
+
 struct BackwardCarve {
   void* dz;
   int64_t dz_stride;
@@ -495,8 +526,9 @@ BackwardCarve carve_backward(void* ws, int dtype, int activation, int64_t rows, 
              ? static_cast<void*>(c.take<char>(size_t(rows) * b.dz_stride * size))
              : nullptr;
   b.bias_partials = c.take<float>(size_t(kBiasBlocks) * outputs);
-  const size_t partial = std::max(product_workspace(size, rows, inputs, outputs),
+  size_t partial = std::max(product_workspace(size, rows, inputs, outputs),
                                   product_workspace(size, outputs, inputs, rows));
+  partial = std::max(partial, fused_partial_bytes(plan_fused(size, activation, rows, inputs, outputs)));
   b.product_partials = c.take<float>(partial / 4);
   b.bytes = c.used;
   return b;
@@ -545,6 +577,55 @@ npa_status launch_slope(SlopeArgs s, int* parts, cudaStream_t stream) {
 }
 
 template <class T>
+npa_status launch_fused(const LinearBackwardArgs& a, FusedBackward f, const BackwardCarve& ws,
+                        cudaStream_t s) {
+  f.want_dx = a.dx != nullptr;
+  f.want_dw = a.dweight != nullptr;
+  f.want_db = a.dbias != nullptr;
+  f.dw_partials = ws.product_partials;
+  f.db_partials = ws.bias_partials;
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
+  f.dx_idesc = tc::instruction_desc(kBf16, false, true, linear_tc::kBM, f.n_pad);
+  f.dw_idesc = tc::instruction_desc(kBf16, true, true, linear_tc::kBM, f.n_pad);
+  CUtensorMap maps[5] = {};
+  NPA_TRY(make_map<T>(&maps[0], a.dy, a.outputs, a.rows, a.dy_stride, linear_tc::kBM));
+  if (a.z) NPA_TRY(make_map<T>(&maps[1], a.z, a.outputs, a.rows, a.z_stride, linear_tc::kBM));
+  NPA_TRY(make_map<T>(&maps[2], a.x, a.inputs, a.rows, a.x_stride, linear_tc::kBM));
+  NPA_TRY(make_map<T>(&maps[3], a.weight, a.inputs, a.outputs, a.weight_stride, f.k_pad));
+  if (a.dx) NPA_TRY(make_map<T>(&maps[4], a.dx, a.inputs, a.rows, a.dx_stride, 32));
+  const auto kernel = linear_tc::fused_backward_kernel<T>;
+  // the whole of an SM's memory whatever the shape: one launch shape, one block
+  const size_t smem = linear_tc::kSmemLimit - linear_tc::kFusedStaticSmem - 1024;
+  int per_sm = 0, sms = 0;
+  NPA_TRY(kernel_occupancy(reinterpret_cast<const void*>(kernel), linear_tc::kFusedThreads, smem,
+                           &per_sm, &sms));
+  if (per_sm < 1) return fail(NPA_ERR_UNSUPPORTED, "linear backward kernel cannot be resident");
+  const int blocks = fused_blocks(f);
+  kernel<<<unsigned(blocks), linear_tc::kFusedThreads, smem, s>>>(maps[0], maps[1], maps[2], maps[3],
+                                                                  maps[4], f);
+  NPA_TRY(after_launch("linear fused_backward_kernel"));
+  if (a.dbias) {
+    bias_reduce_kernel<T><<<grid_for(a.outputs, 32), 256, 0, s>>>(ws.bias_partials, blocks, a.outputs,
+                                                                  static_cast<T*>(a.dbias));
+    NPA_TRY(after_launch("bias_reduce_kernel"));
+  }
+  if (a.dweight) {
+    Product p{};
+    p.m = a.outputs;
+    p.n = a.inputs;
+    p.splits = blocks;
+    p.layer_rows = int64_t(f.m_blocks) * linear_tc::kBM;
+    p.partial_pitch = f.pitch;
+    p.partials = f.dw_partials;
+    p.y = a.dweight;
+    p.y_stride = a.inputs;
+    product_reduce_kernel<T><<<grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32), 256, 0, s>>>(p);
+    NPA_TRY(after_launch("product_reduce_kernel"));
+  }
+  return NPA_OK;
+}
+
+template <class T>
 npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, cudaStream_t s) {
   if (a.rows == 0) {
     if (a.dweight)
@@ -553,6 +634,15 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     if (a.dbias)
       NPA_CUDA(cudaMemsetAsync(a.dbias, 0, size_t(a.outputs) * sizeof(T), s), "cudaMemsetAsync");
     return NPA_OK;
+  }
+  if constexpr (sizeof(T) == 2) {
+    const FusedBackward f = plan_fused(sizeof(T), a.activation, a.rows, a.inputs, a.outputs);
+    if (f.stage_bytes && (a.dx || a.dweight) && tma_rows(a.dy, a.dy_stride, a.rows, 2) &&
+        (!a.z || tma_rows(a.z, a.z_stride, a.rows, 2)) && a.x &&
+        tma_rows(a.x, a.x_stride, a.rows, 2) && a.weight &&
+        tma_rows(a.weight, a.weight_stride, a.outputs, 2) &&
+        (!a.dx || tma_rows(a.dx, a.dx_stride, a.rows, 2)))
+      return launch_fused<T>(a, f, ws, s);
   }
   const T* dz = static_cast<const T*>(a.dy);
   int64_t dz_stride = a.dy_stride;
