@@ -443,6 +443,9 @@ npa_status run_product(Product p, float* partials, cudaStream_t stream) {
                                  plan.pair ? 2 * linear_tc::kBM : linear_tc::kBM, plan.bn);
   p.a_vec = vector_width<T>(p.a.p, p.a.ld, a_rows);
   p.b_vec = vector_width<T>(p.b.p, p.b.ld, b_rows);
+  constexpr int kWhole = 16 / int(sizeof(T));
+  p.whole_chunks = p.a_vec == kWhole && p.b_vec == kWhole &&
+                   (p.a.mn_major ? p.m : p.k) % kWhole == 0 && (p.b.mn_major ? p.n : p.k) % kWhole == 0;
   p.y_tma = tma_rows(p.y, p.y_stride, p.m, sizeof(T));
   p.z_tma = p.z && tma_rows(p.z, p.z_stride, p.m, sizeof(T));
   p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
