@@ -237,6 +237,54 @@ __global__ void __launch_bounds__(256) bias_reduce_kernel(const float* __restric
                              ((acc[4][tx] + acc[5][tx]) + (acc[6][tx] + acc[7][tx])));
 }
 
+// ---- rows of odd widths, copied to rows that TMA can address ----
+// A thread writes 16 bytes; past the width they are zero.
+template <class T, int VEC>
+__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ from, int64_t stride, int64_t rows,
+                                                   int width, T* __restrict__ to, int64_t pitch) {
+  const int64_t chunks = pitch / 8;
+  const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= rows * chunks) return;
+  const int64_t row = e / chunks;
+  const int col = int(e % chunks) * 8;
+  const T* const at = from + row * stride + col;
+  Pack<T, 8> out;
+#pragma unroll
+  for (int j = 0; j < 8; j += VEC) {
+    Pack<T, VEC> in{};
+    if (col + j + VEC <= width) {
+      in = *reinterpret_cast<const Pack<T, VEC>*>(at + j);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (col + j + i < width) in.v[i] = at[j + i];
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out.v[j + i] = in.v[i];
+  }
+  *reinterpret_cast<Pack<T, 8>*>(to + row * pitch + col) = out;
+}
+template <class T>
+npa_status pack_rows(const void** p, int64_t* stride, int64_t rows, int width, void* to, cudaStream_t s) {
+  const int64_t pitch = (int64_t(width) + 7) / 8 * 8;
+  const T* const from = static_cast<const T*>(*p);
+  const unsigned grid = grid_for(uint64_t(rows) * (pitch / 8), 256);
+  if (*stride % 2 == 0 && reinterpret_cast<uintptr_t>(from) % (2 * sizeof(T)) == 0)
+    pack_kernel<T, 2><<<grid, 256, 0, s>>>(from, *stride, rows, width, static_cast<T*>(to), pitch);
+  else
+    pack_kernel<T, 1><<<grid, 256, 0, s>>>(from, *stride, rows, width, static_cast<T*>(to), pitch);
+  *p = to;
+  *stride = pitch;
+  return after_launch("linear pack_kernel");
+}
+// Whether 16-bit operands with rows of `width` values are packed: where the
+// loader warps would take longer than the copies (65536 x 130 x 128 takes
+// 27 us unpacked and 22 packed, 8192 x 1001 x 1000 190 and 37).
+bool packs(size_t size, int width, int64_t rows, int inputs, int outputs) {
+  return size == 2 && width % 8 != 0 && rows > kFewRows &&
+         double(rows) * inputs * outputs >= double(1 << 29);
+}
+
 // ---- host side ----
 constexpr int kSms = 148;             // the plans' block count: B200's SMs
 constexpr int kBiasBlocks = 4 * kSms;  // blocks of slope_kernel at most
@@ -513,8 +561,9 @@ size_t fused_partial_bytes(const FusedBackward& f) {
 }
 
 struct BackwardCarve {
-  void* dz;
+  void* dz;  // where dz is not dy as it lies
   int64_t dz_stride;
+  void *x, *weight;  // packed, where they are
   float* bias_partials;
   float* product_partials;
   size_t bytes;
@@ -525,9 +574,14 @@ BackwardCarve carve_backward(void* ws, int dtype, int activation, int64_t rows, 
   Carve c(ws, 0);
   BackwardCarve b{};
   b.dz_stride = (int64_t(outputs) + 7) / 8 * 8;  // rows of 16-byte multiples
-  b.dz = activation != NPA_ACTIVATION_IDENTITY
+  b.dz = activation != NPA_ACTIVATION_IDENTITY || packs(size, outputs, rows, inputs, outputs)
              ? static_cast<void*>(c.take<char>(size_t(rows) * b.dz_stride * size))
              : nullptr;
+  if (packs(size, inputs, rows, inputs, outputs)) {
+    const size_t pitch = (size_t(inputs) + 7) / 8 * 8;
+    b.x = c.take<char>(size_t(rows) * pitch * size);
+    b.weight = c.take<char>(size_t(outputs) * pitch * size);
+  }
   b.bias_partials = c.take<float>(size_t(kBiasBlocks) * outputs);
   size_t partial = std::max(product_workspace(size, rows, inputs, outputs),
                                   product_workspace(size, outputs, inputs, rows));
@@ -535,6 +589,24 @@ BackwardCarve carve_backward(void* ws, int dtype, int activation, int64_t rows, 
   b.product_partials = c.take<float>(partial / 4);
   b.bytes = c.used;
   return b;
+}
+
+struct ForwardCarve {
+  void *x, *weight;  // packed, where they are
+  float* product_partials;
+  size_t bytes;
+};
+ForwardCarve carve_forward(void* ws, size_t size, int64_t rows, int inputs, int outputs) {
+  Carve c(ws, 0);
+  ForwardCarve f{};
+  f.product_partials = c.take<float>(product_workspace(size, rows, outputs, inputs) / 4);
+  if (packs(size, inputs, rows, inputs, outputs)) {
+    const size_t pitch = (size_t(inputs) + 7) / 8 * 8;
+    f.x = c.take<char>(size_t(rows) * pitch * size);
+    f.weight = c.take<char>(size_t(outputs) * pitch * size);
+  }
+  f.bytes = c.used;
+  return f;
 }
 
 template <class T>
@@ -561,7 +633,12 @@ npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
   p.z = a.z;
   p.z_stride = a.z_stride;
   p.act = a.activation;
-  return run_product<T>(p, static_cast<float*>(workspace), s);
+  const ForwardCarve ws = carve_forward(workspace, sizeof(T), a.rows, a.inputs, a.outputs);
+  if (ws.x) {
+    NPA_TRY(pack_rows<T>(&p.a.p, &p.a.ld, a.rows, a.inputs, ws.x, s));
+    NPA_TRY(pack_rows<T>(&p.b.p, &p.b.ld, a.outputs, a.inputs, ws.weight, s));
+  }
+  return run_product<T>(p, ws.product_partials, s);
 }
 
 template <class T, int VEC>
@@ -649,7 +726,9 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   }
   const T* dz = static_cast<const T*>(a.dy);
   int64_t dz_stride = a.dy_stride;
-  if (a.dbias || (a.z && (a.dx || a.dweight))) {
+  // dz is written where it is not dy, or where dy's odd rows are worth copying
+  const bool write_dz = ws.dz && (a.dx || a.dweight);
+  if (a.dbias || write_dz) {
     SlopeArgs g{};
     g.dy = a.dy;
     g.dy_stride = a.dy_stride;
@@ -658,7 +737,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     g.rows = a.rows;
     g.outputs = a.outputs;
     g.act = a.activation;
-    g.dz = a.z && (a.dx || a.dweight) ? ws.dz : nullptr;
+    g.dz = write_dz ? ws.dz : nullptr;
     g.dz_stride = ws.dz_stride;
     g.partials = ws.bias_partials;
     int parts = 0;
@@ -678,10 +757,16 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
       dz_stride = ws.dz_stride;
     }
   }
+  const void *x = a.x, *weight = a.weight;
+  int64_t x_stride = a.x_stride, weight_stride = a.weight_stride;
+  if (ws.x) {
+    if (a.dweight) NPA_TRY(pack_rows<T>(&x, &x_stride, a.rows, a.inputs, ws.x, s));
+    if (a.dx) NPA_TRY(pack_rows<T>(&weight, &weight_stride, a.outputs, a.inputs, ws.weight, s));
+  }
   if (a.dx) {
     Product p{};
     p.a = {dz, dz_stride, 0};
-    p.b = {a.weight, a.weight_stride, 1};
+    p.b = {weight, weight_stride, 1};
     p.m = int(a.rows);
     p.n = a.inputs;
     p.k = a.outputs;
@@ -692,7 +777,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   if (a.dweight) {
     Product p{};
     p.a = {dz, dz_stride, 1};
-    p.b = {a.x, a.x_stride, 1};
+    p.b = {x, x_stride, 1};
     p.m = a.outputs;
     p.n = a.inputs;
     p.k = int(a.rows);
@@ -706,7 +791,9 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
 }  // namespace
 
 size_t linear_workspace(int dtype, int64_t rows, int inputs, int outputs) {
-  return rows <= kFewRows ? 0 : product_workspace(dtype_bytes(dtype), rows, outputs, inputs);
+  return rows <= kFewRows
+             ? 0
+             : carve_forward(nullptr, dtype_bytes(dtype), rows, inputs, outputs).bytes;
 }
 
 npa_status launch_linear(int dtype, const LinearArgs& a, void* workspace, cudaStream_t stream) {
