@@ -284,6 +284,7 @@ layer_norm_kernel(LayerNormArgs a, int tpr_) {
 template <class T, int VEC, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 512 : kWarpRowThreads)
 layer_norm_backward_kernel(LayerNormBackwardArgs a, int tpr_) {
+  let_next_launch();
   __shared__ float2 sums[32];
   extern __shared__ float columns[];  // [warps][2][dims], rows of a warp or less
   RowSum rs{sums};
@@ -473,6 +474,7 @@ __host__ __device__ inline uint32_t backward_slot(uint32_t tile_bytes, bool resi
 template <class T, int VEC, int NV>
 __global__ void __launch_bounds__(256, 2)
 layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
+  let_next_launch();
   extern __shared__ __align__(128) char smem[];
   const int tpr = shape.tpr, stages = shape.stages, tile_rows = shape.rows;
   const uint32_t base = tc::smem_addr(smem);
@@ -647,6 +649,7 @@ __global__ void __launch_bounds__(512) layer_norm_wide_kernel(LayerNormArgs a, i
 template <class T, int NV>
 __global__ void __launch_bounds__(512) layer_norm_backward_wide_kernel(LayerNormBackwardArgs a,
                                                                        int stages) {
+  let_next_launch();
   constexpr int VEC = 16 / int(sizeof(T));
   extern __shared__ __align__(128) char smem[];
   __shared__ float2 sums[32];
@@ -790,6 +793,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_long_kernel(LayerNorm
 template <class T>
 __global__ void __launch_bounds__(256) column_partials_kernel(LayerNormBackwardArgs a,
                                                               int64_t rows_per_block) {
+  let_next_launch();
   const int col = blockIdx.x * blockDim.x + threadIdx.x;
   if (col >= a.dims) return;
   const int64_t begin = blockIdx.y * rows_per_block;
@@ -813,6 +817,7 @@ template <class T>
 __global__ void __launch_bounds__(1024) column_reduce_kernel(const float* __restrict__ partials,
                                                              int count, int dims, T* dweight,
                                                              T* dbias) {
+  wait_for_previous();
   __shared__ float acc[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t col = int64_t(blockIdx.x) * 32 + tx;  // over [2][dims]
@@ -1168,8 +1173,11 @@ npa_status backward_typed(LayerNormBackwardArgs a, cudaStream_t s) {
   int parts = 0;
   if (a.rows > 0 && (a.dx || params)) NPA_TRY(backward_rows<T>(a, &parts, s));
   if (!params) return NPA_OK;
-  column_reduce_kernel<T><<<unsigned((2 * int64_t(a.dims) + 31) / 32), 1024, 0, s>>>(
-      a.partials, parts, a.dims, static_cast<T*>(a.dweight), static_cast<T*>(a.dbias));
+  // behind a kernel of this call unless there were no rows
+  NPA_CUDA(launch_kernel(parts > 0, column_reduce_kernel<T>,
+                         dim3(unsigned((2 * int64_t(a.dims) + 31) / 32)), 1024, 0, s, a.partials, parts,
+                         a.dims, static_cast<T*>(a.dweight), static_cast<T*>(a.dbias)),
+           "column_reduce_kernel");
   return after_launch("column_reduce_kernel");
 }
 

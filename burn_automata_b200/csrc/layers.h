@@ -65,6 +65,32 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
+// A call's kernels follow each other with programmatic dependent launches: each
+// lets the next one's blocks in as soon as its own have started, and each waits
+// for the one before to end before it touches memory.  What overlaps is the
+// launch itself and what a kernel sets up for itself.
+__device__ __forceinline__ void let_next_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Launches `kernel` behind the stream's last kernel; `after` = true lets it in
+// early (only behind a kernel of the same call, which lets it).
+template <class... Params, class... Args>
+cudaError_t launch_kernel(bool after, void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                          cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(unsigned(threads));
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = after ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, Params(args)...);
+}
+
 inline size_t dtype_bytes(int dtype) { return dtype == NPA_DTYPE_F32 ? 4 : 2; }
 
 struct LayerNormArgs {

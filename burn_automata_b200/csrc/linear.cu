@@ -22,6 +22,8 @@ using linear_tc::Product;
 // layer, and the first adds the eight sums in order.
 template <class T>
 __global__ void __launch_bounds__(256) product_reduce_kernel(const __grid_constant__ Product p) {
+  let_next_launch();
+  wait_for_previous();
   __shared__ float4 sums[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t quads = (p.n + 3) / 4;
@@ -163,6 +165,8 @@ struct SlopeArgs {
 // the unrounded values.  A thread has VEC columns of every (256 / tx)th row.
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ SlopeArgs a) {
+  let_next_launch();
+  wait_for_previous();
   using P = Pack<T, VEC>;
   __shared__ float sums[256 * VEC];
   constexpr int kAhead = sizeof(P) == 16 ? 4 : 8;  // rows in flight per thread
@@ -223,6 +227,8 @@ __global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ Slop
 template <class T>
 __global__ void __launch_bounds__(256) bias_reduce_kernel(const float* __restrict__ partials,
                                                           int count, int outputs, T* dbias) {
+  let_next_launch();
+  wait_for_previous();
   __shared__ float acc[8][32];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + tx;
@@ -242,6 +248,8 @@ __global__ void __launch_bounds__(256) bias_reduce_kernel(const float* __restric
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ from, int64_t stride, int64_t rows,
                                                    int width, T* __restrict__ to, int64_t pitch) {
+  let_next_launch();
+  wait_for_previous();
   const int64_t chunks = pitch / 8;
   const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (e >= rows * chunks) return;
@@ -265,21 +273,24 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ from, i
   *reinterpret_cast<Pack<T, 8>*>(to + row * pitch + col) = out;
 }
 template <class T>
-npa_status pack_rows(const void** p, int64_t* stride, int64_t rows, int width, void* to, cudaStream_t s) {
+npa_status pack_rows(const void** p, int64_t* stride, int64_t rows, int width, void* to, bool after,
+                     cudaStream_t s) {
   const int64_t pitch = (int64_t(width) + 7) / 8 * 8;
   const T* const from = static_cast<const T*>(*p);
   const unsigned grid = grid_for(uint64_t(rows) * (pitch / 8), 256);
   if (*stride % 2 == 0 && reinterpret_cast<uintptr_t>(from) % (2 * sizeof(T)) == 0)
-    pack_kernel<T, 2><<<grid, 256, 0, s>>>(from, *stride, rows, width, static_cast<T*>(to), pitch);
+    NPA_CUDA(launch_kernel(after, pack_kernel<T, 2>, dim3(grid), 256, 0, s, from, *stride, rows, width,
+                           static_cast<T*>(to), pitch), "linear pack_kernel");
   else
-    pack_kernel<T, 1><<<grid, 256, 0, s>>>(from, *stride, rows, width, static_cast<T*>(to), pitch);
+    NPA_CUDA(launch_kernel(after, pack_kernel<T, 1>, dim3(grid), 256, 0, s, from, *stride, rows, width,
+                           static_cast<T*>(to), pitch), "linear pack_kernel");
   *p = to;
   *stride = pitch;
   return after_launch("linear pack_kernel");
 }
 // Whether 16-bit operands with rows of `width` values are packed: where the
 // loader warps would take longer than the copies (65536 x 130 x 128 takes
-// 27 us unpacked and 22 packed, 8192 x 1001 x 1000 190 and 37).
+// 27 us unpacked and 21 packed, 8192 x 1001 x 1000 190 and 30).
 bool packs(size_t size, int width, int64_t rows, int inputs, int outputs) {
   return size == 2 && width % 8 != 0 && rows > kFewRows &&
          double(rows) * inputs * outputs >= double(1 << 29);
@@ -439,7 +450,8 @@ npa_status pair_blocks(K kernel, int threads, size_t smem, int sms, int* blocks)
 }
 
 template <class T, bool LOADER, int BN, bool PAIR = false>
-npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, cudaStream_t stream) {
+npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, bool after,
+                          cudaStream_t stream) {
   using C = linear_tc::Config<T, LOADER, BN, PAIR>;
   const auto kernel = linear_tc::product_kernel<T, LOADER, BN, PAIR>;
   int per_sm = 0, sms = 0;
@@ -455,24 +467,27 @@ npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, cudaSt
     config.blockDim = dim3(C::kThreads);
     config.dynamicSmemBytes = C::kSmemBytes;
     config.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    config.attrs = &attr;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr;
+    config.numAttrs = after ? 2 : 1;
     NPA_CUDA(cudaLaunchKernelEx(&config, kernel, maps[0], maps[1], maps[2], maps[3], p),
              "linear product_kernel");
   } else {
-    kernel<<<unsigned(std::min<int64_t>(tiles, sms)), C::kThreads, C::kSmemBytes, stream>>>(
-        maps[0], maps[1], maps[2], maps[3], p);
+    NPA_CUDA(launch_kernel(after, kernel, dim3(unsigned(std::min<int64_t>(tiles, sms))), C::kThreads,
+                           C::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], p),
+             "linear product_kernel");
   }
   return after_launch("linear product_kernel");
 }
 
 // Runs the product; p holds operands, sizes and the epilogue's buffers.
 template <class T>
-npa_status run_product(Product p, float* partials, cudaStream_t stream) {
+npa_status run_product(Product p, float* partials, bool after, cudaStream_t stream) {
   constexpr bool kSplitParts = sizeof(T) == 4;
   // rows of an operand as it lies in memory
   const int64_t a_rows = p.a.mn_major ? p.k : p.m, b_rows = p.b.mn_major ? p.k : p.n;
@@ -513,20 +528,21 @@ npa_status run_product(Product p, float* partials, cudaStream_t stream) {
     NPA_TRY(make_map<T>(&maps[2], p.y, p.n, p.m, p.y_stride, 32));
   if (p.z_tma && !p.partials) NPA_TRY(make_map<T>(&maps[3], p.z, p.n, p.m, p.z_stride, 32));
   if constexpr (kSplitParts) {
-    NPA_TRY(plan.bn == 128 ? (launch_product<T, true, 128>(maps, p, stream))
-                           : (launch_product<T, true, 64>(maps, p, stream)));
+    NPA_TRY(plan.bn == 128 ? (launch_product<T, true, 128>(maps, p, after, stream))
+                           : (launch_product<T, true, 64>(maps, p, after, stream)));
   } else if (tma) {
-    NPA_TRY(plan.pair        ? (launch_product<T, false, 256, true>(maps, p, stream))
-            : plan.bn == 256 ? (launch_product<T, false, 256>(maps, p, stream))
-            : plan.bn == 128 ? (launch_product<T, false, 128>(maps, p, stream))
-                             : (launch_product<T, false, 64>(maps, p, stream)));
+    NPA_TRY(plan.pair        ? (launch_product<T, false, 256, true>(maps, p, after, stream))
+            : plan.bn == 256 ? (launch_product<T, false, 256>(maps, p, after, stream))
+            : plan.bn == 128 ? (launch_product<T, false, 128>(maps, p, after, stream))
+                             : (launch_product<T, false, 64>(maps, p, after, stream)));
   } else {
-    NPA_TRY(plan.bn == 128 ? (launch_product<T, true, 128>(maps, p, stream))
-                           : (launch_product<T, true, 64>(maps, p, stream)));
+    NPA_TRY(plan.bn == 128 ? (launch_product<T, true, 128>(maps, p, after, stream))
+                           : (launch_product<T, true, 64>(maps, p, after, stream)));
   }
   if (!p.partials) return NPA_OK;
-  product_reduce_kernel<T>
-      <<<grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32), 256, 0, stream>>>(p);
+  NPA_CUDA(launch_kernel(true, product_reduce_kernel<T>,
+                         dim3(grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32)), 256, 0, stream, p),
+           "product_reduce_kernel");
   return after_launch("product_reduce_kernel");
 }
 
@@ -635,10 +651,10 @@ npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
   p.act = a.activation;
   const ForwardCarve ws = carve_forward(workspace, sizeof(T), a.rows, a.inputs, a.outputs);
   if (ws.x) {
-    NPA_TRY(pack_rows<T>(&p.a.p, &p.a.ld, a.rows, a.inputs, ws.x, s));
-    NPA_TRY(pack_rows<T>(&p.b.p, &p.b.ld, a.outputs, a.inputs, ws.weight, s));
+    NPA_TRY(pack_rows<T>(&p.a.p, &p.a.ld, a.rows, a.inputs, ws.x, false, s));
+    NPA_TRY(pack_rows<T>(&p.b.p, &p.b.ld, a.outputs, a.inputs, ws.weight, true, s));
   }
-  return run_product<T>(p, ws.product_partials, s);
+  return run_product<T>(p, ws.product_partials, ws.x != nullptr, s);
 }
 
 template <class T, int VEC>
@@ -685,8 +701,9 @@ npa_status launch_fused(const LinearBackwardArgs& a, FusedBackward f, const Back
                                                                   maps[4], f);
   NPA_TRY(after_launch("linear fused_backward_kernel"));
   if (a.dbias) {
-    bias_reduce_kernel<T><<<grid_for(a.outputs, 32), 256, 0, s>>>(ws.bias_partials, blocks, a.outputs,
-                                                                  static_cast<T*>(a.dbias));
+    NPA_CUDA(launch_kernel(true, bias_reduce_kernel<T>, dim3(grid_for(a.outputs, 32)), 256, 0, s,
+                           ws.bias_partials, blocks, a.outputs, static_cast<T*>(a.dbias)),
+             "bias_reduce_kernel");
     NPA_TRY(after_launch("bias_reduce_kernel"));
   }
   if (a.dweight) {
@@ -699,7 +716,9 @@ npa_status launch_fused(const LinearBackwardArgs& a, FusedBackward f, const Back
     p.partials = f.dw_partials;
     p.y = a.dweight;
     p.y_stride = a.inputs;
-    product_reduce_kernel<T><<<grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32), 256, 0, s>>>(p);
+    NPA_CUDA(launch_kernel(true, product_reduce_kernel<T>,
+                           dim3(grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32)), 256, 0, s, p),
+             "product_reduce_kernel");
     NPA_TRY(after_launch("product_reduce_kernel"));
   }
   return NPA_OK;
@@ -726,6 +745,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   }
   const T* dz = static_cast<const T*>(a.dy);
   int64_t dz_stride = a.dy_stride;
+  bool after = false;  // a kernel of this call precedes
   // dz is written where it is not dy, or where dy's odd rows are worth copying
   const bool write_dz = ws.dz && (a.dx || a.dweight);
   if (a.dbias || write_dz) {
@@ -747,9 +767,11 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
       NPA_TRY((launch_slope<T, kVec>(g, &parts, s)));
     else
       NPA_TRY((launch_slope<T, 1>(g, &parts, s)));
+    after = true;
     if (a.dbias) {
-      bias_reduce_kernel<T><<<grid_for(a.outputs, 32), 256, 0, s>>>(
-          ws.bias_partials, parts, a.outputs, static_cast<T*>(a.dbias));
+      NPA_CUDA(launch_kernel(true, bias_reduce_kernel<T>, dim3(grid_for(a.outputs, 32)), 256, 0, s,
+                             ws.bias_partials, parts, a.outputs, static_cast<T*>(a.dbias)),
+               "bias_reduce_kernel");
       NPA_TRY(after_launch("bias_reduce_kernel"));
     }
     if (g.dz) {
@@ -760,8 +782,14 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   const void *x = a.x, *weight = a.weight;
   int64_t x_stride = a.x_stride, weight_stride = a.weight_stride;
   if (ws.x) {
-    if (a.dweight) NPA_TRY(pack_rows<T>(&x, &x_stride, a.rows, a.inputs, ws.x, s));
-    if (a.dx) NPA_TRY(pack_rows<T>(&weight, &weight_stride, a.outputs, a.inputs, ws.weight, s));
+    if (a.dweight) {
+      NPA_TRY(pack_rows<T>(&x, &x_stride, a.rows, a.inputs, ws.x, after, s));
+      after = true;
+    }
+    if (a.dx) {
+      NPA_TRY(pack_rows<T>(&weight, &weight_stride, a.outputs, a.inputs, ws.weight, after, s));
+      after = true;
+    }
   }
   if (a.dx) {
     Product p{};
@@ -772,7 +800,8 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     p.k = a.outputs;
     p.y = a.dx;
     p.y_stride = a.dx_stride;
-    NPA_TRY(run_product<T>(p, ws.product_partials, s));
+    NPA_TRY(run_product<T>(p, ws.product_partials, after, s));
+    after = true;
   }
   if (a.dweight) {
     Product p{};
@@ -783,7 +812,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     p.k = int(a.rows);
     p.y = a.dweight;
     p.y_stride = a.inputs;
-    NPA_TRY(run_product<T>(p, ws.product_partials, s));
+    NPA_TRY(run_product<T>(p, ws.product_partials, after, s));
   }
   return NPA_OK;
 }

@@ -71,6 +71,7 @@ fused_backward_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_c
   constexpr int kTma = 4, kMma = 5, kFirstSlope = 8;
   const int64_t tiles = (f.rows + kBM - 1) / kBM;
 
+  let_next_launch();
   if (warp == kMma) {
     if (lane == 0) {
       for (int s = 0; s < kFusedStages; ++s) {

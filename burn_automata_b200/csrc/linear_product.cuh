@@ -454,6 +454,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles * p.splits;
   const int64_t layer = int64_t(p.m_tiles) * p.n_tiles;
 
+  let_next_launch();
   if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int s = 0; s < C::kStages; ++s) {
@@ -485,6 +486,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(tmem) : "r"(tmem_at) : "memory");
   bool ok = true;
+  wait_for_previous();
 
   // The loader kernel's 640 threads start with 96 registers each; its control
   // warpgroup leaves some to the others: 40 + 2 x 96 + 2 x 120 = 472 of the
