@@ -213,6 +213,10 @@ __global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ Slop
       }
     }
   }
+  // the rest of dz's rows is zero (odd widths only: VEC = 1)
+  if (!mine && a.dz && col < a.dz_stride)
+    for (int64_t r = begin + ty; r < end; r += rows_at_once)
+      for (int j = 0; j < VEC; ++j) dz[r * a.dz_stride + j] = from_f32<T>(0.0f);
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sums[j * 256 + threadIdx.x] = s[j];
   __syncthreads();
@@ -489,8 +493,7 @@ npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, bool a
 template <class T>
 npa_status run_product(Product p, float* partials, bool after, cudaStream_t stream) {
   constexpr bool kSplitParts = sizeof(T) == 4;
-  // rows of an operand as it lies in memory
-  const int64_t a_rows = p.a.mn_major ? p.k : p.m, b_rows = p.b.mn_major ? p.k : p.n;
+  const int64_t a_rows = p.a.rows, b_rows = p.b.rows;
   const bool tma = !kSplitParts && tma_rows(p.a.p, p.a.ld, a_rows, sizeof(T)) &&
                    tma_rows(p.b.p, p.b.ld, b_rows, sizeof(T));
   const Plan plan = plan_product(sizeof(T), tma, p.m, p.n, p.k);
@@ -507,8 +510,8 @@ npa_status run_product(Product p, float* partials, bool after, cudaStream_t stre
   p.a_vec = vector_width<T>(p.a.p, p.a.ld, a_rows);
   p.b_vec = vector_width<T>(p.b.p, p.b.ld, b_rows);
   constexpr int kWhole = 16 / int(sizeof(T));
-  p.whole_chunks = p.a_vec == kWhole && p.b_vec == kWhole &&
-                   (p.a.mn_major ? p.m : p.k) % kWhole == 0 && (p.b.mn_major ? p.n : p.k) % kWhole == 0;
+  p.whole_chunks = p.a_vec == kWhole && p.b_vec == kWhole && p.a.width % kWhole == 0 &&
+                   p.b.width % kWhole == 0;
   p.y_tma = tma_rows(p.y, p.y_stride, p.m, sizeof(T));
   p.z_tma = p.z && tma_rows(p.z, p.z_stride, p.m, sizeof(T));
   p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
@@ -590,7 +593,7 @@ BackwardCarve carve_backward(void* ws, int dtype, int activation, int64_t rows, 
   Carve c(ws, 0);
   BackwardCarve b{};
   b.dz_stride = (int64_t(outputs) + 7) / 8 * 8;  // rows of 16-byte multiples
-  b.dz = activation != NPA_ACTIVATION_IDENTITY || packs(size, outputs, rows, inputs, outputs)
+  b.dz = activation != NPA_ACTIVATION_IDENTITY || outputs * size % 16 != 0
              ? static_cast<void*>(c.take<char>(size_t(rows) * b.dz_stride * size))
              : nullptr;
   if (packs(size, inputs, rows, inputs, outputs)) {
@@ -636,8 +639,8 @@ npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
     return a.rows <= 4 ? launch_few_rows<T, 4>(a, vec, s) : launch_few_rows<T, 8>(a, vec, s);
   }
   Product p{};
-  p.a = {a.x, a.x_stride, 0};
-  p.b = {a.weight, a.weight_stride, 0};
+  p.a = {a.x, a.x_stride, 0, int(a.rows), a.inputs};
+  p.b = {a.weight, a.weight_stride, 0, a.outputs, a.inputs};
   p.m = int(a.rows);
   p.n = a.outputs;
   p.k = a.inputs;
@@ -659,7 +662,7 @@ npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
 
 template <class T, int VEC>
 npa_status launch_slope(SlopeArgs s, int* parts, cudaStream_t stream) {
-  const int groups = ceil_div(s.outputs, VEC);
+  const int groups = ceil_div(s.dz ? s.dz_stride : s.outputs, VEC);
   s.tx = 1;
   while (s.tx < 32 && s.tx < groups) s.tx *= 2;
   const int grid_x = ceil_div(groups, s.tx);
@@ -745,9 +748,13 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   }
   const T* dz = static_cast<const T*>(a.dy);
   int64_t dz_stride = a.dy_stride;
+  int dz_width = a.outputs;
   bool after = false;  // a kernel of this call precedes
-  // dz is written where it is not dy, or where dy's odd rows are worth copying
-  const bool write_dz = ws.dz && (a.dx || a.dweight);
+  // dz is written where it is not dy, and where dy's odd rows are worth copying:
+  // by the pass that sums them for dbias, or for much work
+  const bool write_dz =
+      ws.dz && (a.dx || a.dweight) &&
+      (a.z || a.dbias || packs(sizeof(T), a.outputs, a.rows, a.inputs, a.outputs));
   if (a.dbias || write_dz) {
     SlopeArgs g{};
     g.dy = a.dy;
@@ -777,6 +784,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     if (g.dz) {
       dz = static_cast<const T*>(ws.dz);
       dz_stride = ws.dz_stride;
+      dz_width = int((a.outputs + kVec - 1) / kVec * kVec);  // zeros past outputs
     }
   }
   const void *x = a.x, *weight = a.weight;
@@ -793,8 +801,8 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   }
   if (a.dx) {
     Product p{};
-    p.a = {dz, dz_stride, 0};
-    p.b = {weight, weight_stride, 1};
+    p.a = {dz, dz_stride, 0, int(a.rows), dz_width};
+    p.b = {weight, weight_stride, 1, a.outputs, a.inputs};
     p.m = int(a.rows);
     p.n = a.inputs;
     p.k = a.outputs;
@@ -805,8 +813,8 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   }
   if (a.dweight) {
     Product p{};
-    p.a = {dz, dz_stride, 1};
-    p.b = {x, x_stride, 1};
+    p.a = {dz, dz_stride, 1, int(a.rows), dz_width};
+    p.b = {x, x_stride, 1, int(a.rows), a.inputs};
     p.m = a.outputs;
     p.n = a.inputs;
     p.k = int(a.rows);

@@ -40,6 +40,7 @@ struct Operand {
   const void* p;
   int64_t ld;
   int mn_major;
+  int rows, width;  // as it lies in memory; the width may count zeros past k or m
 };
 
 struct Product {
@@ -347,30 +348,27 @@ struct TileReader {
   __device__ __forceinline__ const T* at(int i) const {
     return reinterpret_cast<const T*>(origin + i % kPasses * pass_bytes + i / kPasses * across_bytes);
   }
-  // o_end, k_end: the operand's sizes; vec: values per load that it allows.
-  __device__ __forceinline__ void read(const Operand& o, int o_end, int k_end, int vec, int i,
-                                       Chunk<T>& c) const {
+  // vec: values per load that the operand allows.
+  __device__ __forceinline__ void read(const Operand& o, int vec, int i, Chunk<T>& c) const {
     const int out = outer + (o.mn_major ? i % kPasses : i) * kLines;
     const int in = inner + (o.mn_major ? i / kPasses * 64 : 0);
-    const int left = out < (o.mn_major ? k_end : o_end) ? (o.mn_major ? o_end : k_end) - in : 0;
+    const int left = out < o.rows ? o.width - in : 0;
     load_chunk<T>(left > 0 ? at(i) : reinterpret_cast<const T*>(origin), left, vec, c);
   }
   // Whether all of `passes` chunks lie inside the operand.
-  __device__ __forceinline__ bool inside(const Operand& o, int o_end, int k_end, int passes) const {
+  __device__ __forceinline__ bool inside(const Operand& o, int passes) const {
     const int last_line = (o.mn_major ? kPasses : passes) * kLines - kLines;
     const int last_run = o.mn_major ? (passes / kPasses - 1) * 64 : 0;
-    return outer + last_line < (o.mn_major ? k_end : o_end) &&
-           inner + last_run < (o.mn_major ? o_end : k_end);
+    return outer + last_line < o.rows && inner + last_run < o.width;
   }
   __device__ __forceinline__ void read_inside(int i, Chunk<T>& c) const {
     *reinterpret_cast<uint4*>(c.v) = __ldg(reinterpret_cast<const uint4*>(at(i)));
   }
   // The same where every chunk lies inside or outside the operand, on 16 bytes.
-  __device__ __forceinline__ void read_whole(const Operand& o, int o_end, int k_end, int i,
-                                             Chunk<T>& c) const {
+  __device__ __forceinline__ void read_whole(const Operand& o, int i, Chunk<T>& c) const {
     const int out = outer + (o.mn_major ? i % kPasses : i) * kLines;
     const int in = inner + (o.mn_major ? i / kPasses * 64 : 0);
-    const bool there = out < (o.mn_major ? k_end : o_end) && in < (o.mn_major ? o_end : k_end);
+    const bool there = out < o.rows && in < o.width;
     uint4 u = make_uint4(0, 0, 0, 0);
     if (there) u = __ldg(reinterpret_cast<const uint4*>(at(i)));
     *reinterpret_cast<uint4*>(c.v) = u;
@@ -569,17 +567,17 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         };
         auto read_all = [&]() {
 #pragma unroll
-          for (int i = 0; i < kAChunks; ++i) ra.read(p.a, p.m, p.k, p.a_vec, i, ca[i]);
+          for (int i = 0; i < kAChunks; ++i) ra.read(p.a, p.a_vec, i, ca[i]);
 #pragma unroll
-          for (int i = 0; i < kBChunks; ++i) rb.read(p.b, p.n, p.k, p.b_vec, i, cb[i]);
+          for (int i = 0; i < kBChunks; ++i) rb.read(p.b, p.b_vec, i, cb[i]);
         };
         if (t < tiles) {
           enter_tile();
           if (p.whole_chunks) {
 #pragma unroll
-            for (int i = 0; i < kAChunks; ++i) ra.read_whole(p.a, p.m, p.k, i, ca[i]);
+            for (int i = 0; i < kAChunks; ++i) ra.read_whole(p.a, i, ca[i]);
 #pragma unroll
-            for (int i = 0; i < kBChunks; ++i) rb.read_whole(p.b, p.n, p.k, i, cb[i]);
+            for (int i = 0; i < kBChunks; ++i) rb.read_whole(p.b, i, cb[i]);
           } else {
             read_all();
           }
@@ -603,8 +601,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           // again, for the next stage, as soon as it has been written.  Inside the
           // operands without predicates (8192 x 4096 x 4096 f32: 1.51 ms, 1.81 with).
           if (p.whole_chunks &&
-              __all_sync(0xffffffffu, more && ra.inside(p.a, p.m, p.k, kAChunks) &&
-                                          rb.inside(p.b, p.n, p.k, kBChunks))) {
+              __all_sync(0xffffffffu, more && ra.inside(p.a, kAChunks) && rb.inside(p.b, kBChunks))) {
 #pragma unroll
             for (int i = 0; i < kAChunks; ++i) {
               store_chunk<T>(a + i * Reader::kLines * 128, C::kABytes, ca[i]);
@@ -619,12 +616,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < kAChunks; ++i) {
               store_chunk<T>(a + i * Reader::kLines * 128, C::kABytes, ca[i]);
-              if (more) ra.read_whole(p.a, p.m, p.k, i, ca[i]);
+              if (more) ra.read_whole(p.a, i, ca[i]);
             }
 #pragma unroll
             for (int i = 0; i < kBChunks; ++i) {
               store_chunk<T>(b + i * Reader::kLines * 128, C::kBBytes, cb[i]);
-              if (more) rb.read_whole(p.b, p.n, p.k, i, cb[i]);
+              if (more) rb.read_whole(p.b, i, cb[i]);
             }
           } else {
 #pragma unroll
