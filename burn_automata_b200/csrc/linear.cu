@@ -247,22 +247,23 @@ __global__ void __launch_bounds__(256) bias_reduce_kernel(const float* __restric
                              ((acc[4][tx] + acc[5][tx]) + (acc[6][tx] + acc[7][tx])));
 }
 
-// ---- rows of odd widths, copied to rows that TMA can address ----
+// ---- rows of odd widths, copied to rows that start on 16 bytes ----
 // A thread writes 16 bytes; past the width they are zero.
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ from, int64_t stride, int64_t rows,
                                                    int width, T* __restrict__ to, int64_t pitch) {
+  constexpr int kChunk = 16 / int(sizeof(T));
   let_next_launch();
   wait_for_previous();
-  const int64_t chunks = pitch / 8;
+  const int64_t chunks = pitch / kChunk;
   const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (e >= rows * chunks) return;
   const int64_t row = e / chunks;
-  const int col = int(e % chunks) * 8;
+  const int col = int(e % chunks) * kChunk;
   const T* const at = from + row * stride + col;
-  Pack<T, 8> out;
+  Pack<T, kChunk> out;
 #pragma unroll
-  for (int j = 0; j < 8; j += VEC) {
+  for (int j = 0; j < kChunk; j += VEC) {
     Pack<T, VEC> in{};
     if (col + j + VEC <= width) {
       in = *reinterpret_cast<const Pack<T, VEC>*>(at + j);
@@ -274,30 +275,38 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ from, i
 #pragma unroll
     for (int i = 0; i < VEC; ++i) out.v[j + i] = in.v[i];
   }
-  *reinterpret_cast<Pack<T, 8>*>(to + row * pitch + col) = out;
+  *reinterpret_cast<Pack<T, kChunk>*>(to + row * pitch + col) = out;
 }
+int64_t packed_pitch(int width) { return (int64_t(width) + 7) / 8 * 8; }
+// Replaces an operand's rows by a packed copy in `to`.
 template <class T>
-npa_status pack_rows(const void** p, int64_t* stride, int64_t rows, int width, void* to, bool after,
-                     cudaStream_t s) {
-  const int64_t pitch = (int64_t(width) + 7) / 8 * 8;
-  const T* const from = static_cast<const T*>(*p);
-  const unsigned grid = grid_for(uint64_t(rows) * (pitch / 8), 256);
-  if (*stride % 2 == 0 && reinterpret_cast<uintptr_t>(from) % (2 * sizeof(T)) == 0)
-    NPA_CUDA(launch_kernel(after, pack_kernel<T, 2>, dim3(grid), 256, 0, s, from, *stride, rows, width,
-                           static_cast<T*>(to), pitch), "linear pack_kernel");
+npa_status pack_rows(Operand& o, void* to, bool after, cudaStream_t s) {
+  const int64_t pitch = packed_pitch(o.width), rows = o.rows;
+  const T* const from = static_cast<const T*>(o.p);
+  const dim3 grid(grid_for(uint64_t(rows) * (pitch * sizeof(T) / 16), 256));
+  if (o.ld % 2 == 0 && reinterpret_cast<uintptr_t>(from) % (2 * sizeof(T)) == 0)
+    NPA_CUDA(launch_kernel(after, pack_kernel<T, 2>, grid, 256, 0, s, from, o.ld, rows, o.width,
+                           static_cast<T*>(to), pitch),
+             "linear pack_kernel");
   else
-    NPA_CUDA(launch_kernel(after, pack_kernel<T, 1>, dim3(grid), 256, 0, s, from, *stride, rows, width,
-                           static_cast<T*>(to), pitch), "linear pack_kernel");
-  *p = to;
-  *stride = pitch;
+    NPA_CUDA(launch_kernel(after, pack_kernel<T, 1>, grid, 256, 0, s, from, o.ld, rows, o.width,
+                           static_cast<T*>(to), pitch),
+             "linear pack_kernel");
+  o.p = to;
+  o.ld = pitch;
+  o.width = int(pitch);  // zeros past the width
   return after_launch("linear pack_kernel");
 }
-// Whether 16-bit operands with rows of `width` values are packed: where the
-// loader warps would take longer than the copies (65536 x 130 x 128 takes
-// 27 us unpacked and 21 packed, 8192 x 1001 x 1000 190 and 30).
+// Whether operands with rows of an odd width are packed: where the loader warps
+// would lose more than the copies take.  bf16: 65536 x 130 x 128 takes 27 us
+// unpacked and 21 packed, 8192 x 1001 x 1000 190 and 28.  f32 goes through the
+// loader warps either way and gains only what aligned loads save, once for each
+// tile of outputs: 8192 x 1001 x 1000 takes 203 us unpacked and 135 packed,
+// 70000 x 131 x 600 186 and 146.
 bool packs(size_t size, int width, int64_t rows, int inputs, int outputs) {
-  return size == 2 && width % 8 != 0 && rows > kFewRows &&
-         double(rows) * inputs * outputs >= double(1 << 29);
+  return width * size % 16 != 0 && rows > kFewRows &&
+         double(rows) * inputs * outputs >= double(1 << 29) &&
+         (size == 2 || outputs >= 384);
 }
 
 // ---- host side ----
@@ -597,7 +606,7 @@ BackwardCarve carve_backward(void* ws, int dtype, int activation, int64_t rows, 
              ? static_cast<void*>(c.take<char>(size_t(rows) * b.dz_stride * size))
              : nullptr;
   if (packs(size, inputs, rows, inputs, outputs)) {
-    const size_t pitch = (size_t(inputs) + 7) / 8 * 8;
+    const size_t pitch = size_t(packed_pitch(inputs));
     b.x = c.take<char>(size_t(rows) * pitch * size);
     b.weight = c.take<char>(size_t(outputs) * pitch * size);
   }
@@ -620,7 +629,7 @@ ForwardCarve carve_forward(void* ws, size_t size, int64_t rows, int inputs, int 
   ForwardCarve f{};
   f.product_partials = c.take<float>(product_workspace(size, rows, outputs, inputs) / 4);
   if (packs(size, inputs, rows, inputs, outputs)) {
-    const size_t pitch = (size_t(inputs) + 7) / 8 * 8;
+    const size_t pitch = size_t(packed_pitch(inputs));
     f.x = c.take<char>(size_t(rows) * pitch * size);
     f.weight = c.take<char>(size_t(outputs) * pitch * size);
   }
@@ -654,8 +663,8 @@ npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
   p.act = a.activation;
   const ForwardCarve ws = carve_forward(workspace, sizeof(T), a.rows, a.inputs, a.outputs);
   if (ws.x) {
-    NPA_TRY(pack_rows<T>(&p.a.p, &p.a.ld, a.rows, a.inputs, ws.x, false, s));
-    NPA_TRY(pack_rows<T>(&p.b.p, &p.b.ld, a.outputs, a.inputs, ws.weight, true, s));
+    NPA_TRY(pack_rows<T>(p.a, ws.x, false, s));
+    NPA_TRY(pack_rows<T>(p.b, ws.weight, true, s));
   }
   return run_product<T>(p, ws.product_partials, ws.x != nullptr, s);
 }
@@ -787,22 +796,22 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
       dz_width = int((a.outputs + kVec - 1) / kVec * kVec);  // zeros past outputs
     }
   }
-  const void *x = a.x, *weight = a.weight;
-  int64_t x_stride = a.x_stride, weight_stride = a.weight_stride;
+  Operand weight{a.weight, a.weight_stride, 1, a.outputs, a.inputs};
+  Operand x{a.x, a.x_stride, 1, int(a.rows), a.inputs};
   if (ws.x) {
     if (a.dweight) {
-      NPA_TRY(pack_rows<T>(&x, &x_stride, a.rows, a.inputs, ws.x, after, s));
+      NPA_TRY(pack_rows<T>(x, ws.x, after, s));
       after = true;
     }
     if (a.dx) {
-      NPA_TRY(pack_rows<T>(&weight, &weight_stride, a.outputs, a.inputs, ws.weight, after, s));
+      NPA_TRY(pack_rows<T>(weight, ws.weight, after, s));
       after = true;
     }
   }
   if (a.dx) {
     Product p{};
     p.a = {dz, dz_stride, 0, int(a.rows), dz_width};
-    p.b = {weight, weight_stride, 1, a.outputs, a.inputs};
+    p.b = weight;
     p.m = int(a.rows);
     p.n = a.inputs;
     p.k = a.outputs;
@@ -814,7 +823,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   if (a.dweight) {
     Product p{};
     p.a = {dz, dz_stride, 1, int(a.rows), dz_width};
-    p.b = {x, x_stride, 1, int(a.rows), a.inputs};
+    p.b = x;
     p.m = a.outputs;
     p.n = a.inputs;
     p.k = int(a.rows);

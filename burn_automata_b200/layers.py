@@ -16,6 +16,7 @@ autograd does not see them.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -157,15 +158,18 @@ def _call(entry, device, args, name: str) -> None:
         _lib.check(status, name)
 
 
-def _workspace(x, query, args, name: str):
-    """(tensor or None, bytes) of the workspace that the query asks for."""
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(query: str, *args) -> int:
+    """The workspace size that the C ABI's query gives for these sizes."""
     need = ctypes.c_size_t(0)
-    status = query(*args, ctypes.byref(need))
-    if status:
-        _lib.check(status, name)
-    if not need.value:
-        return None, 0
-    return x.new_empty(need.value, dtype=_torch.uint8), need.value
+    _lib.check(getattr(_lib.lib(), query)(*args, ctypes.byref(need)), query)
+    return need.value
+
+
+def _workspace(x, query: str, *args):
+    """(pointer's owner or None, bytes) of one call's workspace."""
+    need = _workspace_bytes(query, *args)
+    return (x.new_empty(need, dtype=_torch.uint8), need) if need else (None, 0)
 
 
 def _outputs_like(x, shape):
@@ -217,8 +221,8 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, residual_gradient=None,
     L = _lib.lib()
     ws, ws_bytes = None, 0
     if dw is not None or db is not None:
-        ws, ws_bytes = _workspace(x, L.npa_dev_layer_norm_backward_workspace_size,
-                                  (code, rows, dims), "layer_norm_backward")
+        ws, ws_bytes = _workspace(x, "npa_dev_layer_norm_backward_workspace_size", code, rows,
+                                  dims)
     _call(L.npa_dev_layer_norm_backward, x.device,
           (code, dyr.data_ptr(), dys, xr.data_ptr(), xs, m.data_ptr(), r.data_ptr(), _ptr(w),
            _ptr(rr), rs, rows, dims, _ptr(dx), dims, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes),
@@ -251,8 +255,7 @@ def linear(x, weight, bias=None, residual=None, activation: Activation = Activat
     y = _outputs_like(x, out_shape)
     z = torch.empty_like(y) if save_pre_activation else None
     L = _lib.lib()
-    ws, ws_bytes = _workspace(x, L.npa_dev_linear_workspace_size, (code, rows, inputs, outputs),
-                              "linear")
+    ws, ws_bytes = _workspace(x, "npa_dev_linear_workspace_size", code, rows, inputs, outputs)
     _call(L.npa_dev_linear, x.device,
           (code, int(activation), xr.data_ptr(), xs, wr.data_ptr(), wstride, _ptr(b), _ptr(rr), rs,
            rows, inputs, outputs, y.data_ptr(), outputs, _ptr(z), outputs, _ptr(ws), ws_bytes),
@@ -283,8 +286,8 @@ def linear_backward(dy, x, weight, pre_activation=None,
     dw = _outputs_like(weight, weight.shape) if "weight" in want else None
     db = x.new_empty(outputs) if "bias" in want else None
     L = _lib.lib()
-    ws, ws_bytes = _workspace(x, L.npa_dev_linear_backward_workspace_size,
-                              (code, int(activation), rows, inputs, outputs), "linear_backward")
+    ws, ws_bytes = _workspace(x, "npa_dev_linear_backward_workspace_size", code, int(activation), rows,
+                              inputs, outputs)
     _call(L.npa_dev_linear_backward, x.device,
           (code, int(activation), dyr.data_ptr(), dys, xr.data_ptr(), xs, wr.data_ptr(), wstride,
            _ptr(zr), zs, rows, inputs, outputs, _ptr(dx), inputs, _ptr(dw), _ptr(db), _ptr(ws),
