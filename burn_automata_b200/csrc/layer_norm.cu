@@ -91,18 +91,29 @@ struct Row {
 template <class T, int VEC, int NV>
 __device__ __forceinline__ void load_row(const T* row, int lane, int tpr, int nvec, bool active,
                                          Row<VEC, NV>& out) {
+  if constexpr (sizeof(T) == 2 && VEC >= 2) {
+    // whole words: a pair of 16-bit values widens in two instructions
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = lane + k * tpr;
+      Pack<uint32_t, VEC / 2> p{};
+      if (active && q < nvec) p = reinterpret_cast<const Pack<uint32_t, VEC / 2>*>(row)[q];
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) {
+        const float2 t = unpack2<T>(p.v[j]);
+        out.v[k * (VEC / 2) + j] = f2(t.x, t.y);
+      }
+    }
+    return;
+  }
   float f[2 * Row<VEC, NV>::kPairs];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int q = lane + k * tpr;
-    if (active && q < nvec) {
-      const Pack<T, VEC> p = reinterpret_cast<const Pack<T, VEC>*>(row)[q];
+    Pack<T, VEC> p{};
+    if (active && q < nvec) p = reinterpret_cast<const Pack<T, VEC>*>(row)[q];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = to_f32(p.v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = 0.0f;
-    }
+    for (int j = 0; j < VEC; ++j) f[k * VEC + j] = to_f32(p.v[j]);
   }
   if (Row<VEC, NV>::E & 1) f[Row<VEC, NV>::E] = 0.0f;
 #pragma unroll
@@ -110,6 +121,20 @@ __device__ __forceinline__ void load_row(const T* row, int lane, int tpr, int nv
 }
 template <class T, int VEC, int NV>
 __device__ __forceinline__ void store_row(T* row, int lane, int tpr, int nvec, const Row<VEC, NV>& in) {
+  if constexpr (sizeof(T) == 2 && VEC >= 2) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = lane + k * tpr;
+      Pack<uint32_t, VEC / 2> p;
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) {
+        const float2 t = values(in.v[k * (VEC / 2) + j]);
+        p.v[j] = pack2<T>(t.x, t.y);
+      }
+      if (q < nvec) reinterpret_cast<Pack<uint32_t, VEC / 2>*>(row)[q] = p;
+    }
+    return;
+  }
   float f[2 * Row<VEC, NV>::kPairs];
 #pragma unroll
   for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) {
@@ -120,11 +145,10 @@ __device__ __forceinline__ void store_row(T* row, int lane, int tpr, int nvec, c
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int q = lane + k * tpr;
-    if (q >= nvec) continue;
     Pack<T, VEC> p;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) p.v[j] = from_f32<T>(f[k * VEC + j]);
-    reinterpret_cast<Pack<T, VEC>*>(row)[q] = p;
+    if (q < nvec) reinterpret_cast<Pack<T, VEC>*>(row)[q] = p;
   }
 }
 // A parameter vector's share: `fill` where it is absent.  Scalar loads: read
@@ -686,8 +710,15 @@ __global__ void __launch_bounds__(512) layer_norm_backward_wide_kernel(LayerNorm
   int slot = 0, turn = 0;
   uint32_t phase = 0;
   bool ok = true;
+  // the next row's statistics: their latency passes under this row
+  float next_mean = int64_t(blockIdx.x) < a.rows ? a.mean[blockIdx.x] : 0.0f;
+  float next_rstd = int64_t(blockIdx.x) < a.rows ? a.rstd[blockIdx.x] : 0.0f;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-    const float mean = a.mean[row], rstd = a.rstd[row];
+    const float mean = next_mean, rstd = next_rstd;
+    if (row + gridDim.x < a.rows) {
+      next_mean = a.mean[row + gridDim.x];
+      next_rstd = a.rstd[row + gridDim.x];
+    }
     if (!tc::bar_wait(bar0 + 8 * slot, phase)) gave_up[turn] = 1;
     const char* const at = smem + slot * slot_bytes;
     Row<VEC, NV> xh, g;
