@@ -46,10 +46,12 @@ struct RowSum {
 };
 template <bool BLOCK>
 __device__ __forceinline__ void row_sum2(RowSum& rs, int tpr, float& a, float& b) {
-  for (int o = (BLOCK ? 32 : tpr) >> 1; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(kFull, a, o);
-    b += __shfl_xor_sync(kFull, b, o);
-  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (BLOCK || o < tpr) {
+      a += __shfl_xor_sync(kFull, a, o);
+      b += __shfl_xor_sync(kFull, b, o);
+    }
   if (BLOCK) {
     float2* const s = rs.buf + rs.phase * 16;
     rs.phase ^= 1;
@@ -66,7 +68,9 @@ __device__ __forceinline__ void row_sum2(RowSum& rs, int tpr, float& a, float& b
 }
 template <bool BLOCK>
 __device__ __forceinline__ float row_sum(RowSum& rs, int tpr, float a) {
-  for (int o = (BLOCK ? 32 : tpr) >> 1; o > 0; o >>= 1) a += __shfl_xor_sync(kFull, a, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (BLOCK || o < tpr) a += __shfl_xor_sync(kFull, a, o);
   if (BLOCK) {
     float2* const s = rs.buf + rs.phase * 16;
     rs.phase ^= 1;
@@ -439,6 +443,12 @@ __global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs 
     if (rows == tile_rows) {
       ok = __all_sync(kFull, tc::bar_wait(ring.bar(slot), phase));
       if (!ok) break;
+      if (lane == 0) {
+        // the slot before this one, once its results have left, takes a tile
+        // that arrives under this one's arithmetic
+        tc::bulk_wait_read<0>();
+        request(tile + (stages - 1) * step, slot == 0 ? stages - 1 : slot - 1);
+      }
     } else {
       if (lane == 0) tc::bulk_wait_read<0>();
       __syncwarp();
@@ -468,10 +478,6 @@ __global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs 
       if (lane == 0) {
         bulk_store(y + tile * tile_rows * a.dims, ring.at(slot), tile_bytes);
         tc::bulk_commit();
-        // the slot before this one: its results have left once all groups but
-        // the one just committed have been read
-        tc::bulk_wait_read<1>();
-        request(tile + (stages - 1) * step, slot == 0 ? stages - 1 : slot - 1);
       }
     } else {
       __syncwarp();
@@ -495,8 +501,11 @@ __host__ __device__ inline uint32_t backward_slot(uint32_t tile_bytes, bool resi
   return ((residual ? 3 : 2) * tile_bytes + 2 * tile_rows * 4 + 127) & ~127u;
 }
 
+// Blocks of eight warps that an SM's registers are to hold.
+constexpr int backward_blocks(int values) { return values <= 0 ? 3 : 2; }
+
 template <class T, int VEC, int NV>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, backward_blocks(VEC * NV))
 layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
   let_next_launch();
   extern __shared__ __align__(128) char smem[];
@@ -547,6 +556,11 @@ layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
     if (rows == tile_rows) {
       ok = __all_sync(kFull, tc::bar_wait(ring.bar(slot), phase));
       if (!ok) break;
+      if (lane == 0) {
+        // as in the forward kernel
+        tc::bulk_wait_read<0>();
+        request(tile + (stages - 1) * step, slot == 0 ? stages - 1 : slot - 1);
+      }
     } else {
       if (lane == 0) tc::bulk_wait_read<0>();
       __syncwarp();
@@ -584,8 +598,6 @@ layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
       if (lane == 0) {
         if (dx) bulk_store(dx + from, ring.at(slot), tile_bytes);
         tc::bulk_commit();
-        tc::bulk_wait_read<1>();
-        request(tile + (stages - 1) * step, slot == 0 ? stages - 1 : slot - 1);
       }
     } else {
       __syncwarp();
@@ -1005,15 +1017,15 @@ struct TilePlan {
 };
 // slot_of(tile_rows): bytes of one ring slot.
 template <class F>
-TilePlan plan_tiles(size_t size, int dims, int64_t rows, F&& slot_of) {
+TilePlan plan_tiles(size_t size, int dims, int64_t rows, int most_blocks, F&& slot_of) {
   TilePlan p{};
   int vec = 16 / int(size);
   while (dims % vec) vec /= 2;
   const RowPlan row = plan_lanes(dims, vec);
   if (row.nv == 0) return p;
-  // Two blocks of eight warps fit an SM's registers.  Tiles of eight rows
-  // where their rings leave room for both, else of four where those are whole
-  // 16-byte units and a warp has no more rows at once.
+  // most_blocks blocks of eight warps fit an SM's registers.  Tiles of eight
+  // rows where their rings leave room for all, else of four where those are
+  // whole 16-byte units and a warp has no more rows at once.
   for (int tile_rows : {8, 4}) {
     if (tile_rows == 4 && (size_t(dims) * size * 4 % 16 || row.tpr < 8)) break;
     const size_t slot = slot_of(tile_rows);
@@ -1021,18 +1033,18 @@ TilePlan plan_tiles(size_t size, int dims, int64_t rows, F&& slot_of) {
     const int64_t tiles = (rows + tile_rows - 1) / tile_rows;
     int warps = 8;
     while (warps > 1 && tiles < int64_t(warps) * 148) warps /= 2;
-    for (int blocks = 2 * (8 / warps); blocks >= 1; --blocks) {
+    for (int blocks = most_blocks * (8 / warps); blocks >= 1; --blocks) {
       const int stages =
           int(std::min<size_t>(4, kSmemPerSm / blocks / (size_t(warps) * (slot + 8) + 128)));
       if (stages < 2) continue;
-      if (p.row.nv && blocks < 2) break;  // eight rows fit as well as four
+      if (p.row.nv && blocks < most_blocks) break;  // eight rows fit as well as four
       p.smem = ((size_t(warps) * stages * 8 + 127) & ~size_t(127)) + size_t(warps) * stages * slot;
       p.smem = (p.smem + 4095) & ~size_t(4095);  // few distinct launch shapes
       p.row = row;
       p.warps = warps;
       p.stages = stages;
       p.tile_rows = tile_rows;
-      if (blocks >= 2) return p;
+      if (blocks >= most_blocks) return p;
       break;
     }
   }
@@ -1081,7 +1093,7 @@ npa_status wide_grid(K kernel, const WidePlan& p, int64_t rows, unsigned* grid) 
 template <class T>
 npa_status forward_typed(const LayerNormArgs& a, cudaStream_t s) {
   if (gapless(a.x, a.x_stride, a.rows, a.dims) && gapless(a.y, a.y_stride, a.rows, a.dims)) {
-    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, [&](int tile_rows) {
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, 2, [&](int tile_rows) {
       return (size_t(a.dims) * tile_rows * sizeof(T) + 127) & ~size_t(127);
     });
     if (p.row.nv)
@@ -1135,7 +1147,10 @@ npa_status backward_rows(const LayerNormBackwardArgs& a, int* parts, cudaStream_
       gapless(a.dx, a.dx_stride, a.rows, a.dims) &&
       gapless(a.residual, a.residual_stride, a.rows, a.dims) && bulk_rows(a.mean, 0, 4) &&
       bulk_rows(a.rstd, 0, 4)) {
-    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, [&](int tile_rows) {
+    int vec = 16 / int(sizeof(T));
+    while (a.dims % vec) vec /= 2;
+    const int blocks = backward_blocks(vec * plan_lanes(a.dims, vec).nv);
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, blocks, [&](int tile_rows) {
       return backward_slot(uint32_t(a.dims * tile_rows * sizeof(T)), a.residual != nullptr, tile_rows);
     });
     if (p.row.nv)
