@@ -84,22 +84,28 @@ __device__ __forceinline__ float row_sum(RowSum& rs, int tpr, float a) {
 }
 
 // ---- a thread's share of a row ----
-// Thread `lane` of a row's `tpr` threads has the accesses lane, lane + tpr, ...
-// of VEC values, NV of them at most, as E values in pairs.
+// A thread has the accesses first, first + step, ... of VEC values, NV of them
+// at most, as E values in pairs.  In global memory a row's threads lie side by
+// side (first = lane, step = threads per row).  In a warp's shared-memory tile
+// a thread's accesses follow each other (first = lane * NV, step = Next, known
+// to the compiler): the offsets are immediates, and odd NV meet all banks.
+struct Next {
+  __device__ __forceinline__ constexpr operator int() const { return 1; }
+};
 template <int VEC, int NV>
 struct Row {
   static constexpr int E = VEC * NV, kPairs = (E + 1) / 2;
   F2 v[kPairs];
 };
 // Past nvec (and for `active` false) the values are zero.
-template <class T, int VEC, int NV>
-__device__ __forceinline__ void load_row(const T* row, int lane, int tpr, int nvec, bool active,
+template <class T, int VEC, int NV, class Step>
+__device__ __forceinline__ void load_row(const T* row, int first, Step step, int nvec, bool active,
                                          Row<VEC, NV>& out) {
   if constexpr (sizeof(T) == 2 && VEC >= 2) {
     // whole words: a pair of 16-bit values widens in two instructions
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int q = lane + k * tpr;
+      const int q = first + k * step;
       Pack<uint32_t, VEC / 2> p{};
       if (active && q < nvec) p = reinterpret_cast<const Pack<uint32_t, VEC / 2>*>(row)[q];
 #pragma unroll
@@ -113,7 +119,7 @@ __device__ __forceinline__ void load_row(const T* row, int lane, int tpr, int nv
   float f[2 * Row<VEC, NV>::kPairs];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int q = lane + k * tpr;
+    const int q = first + k * step;
     Pack<T, VEC> p{};
     if (active && q < nvec) p = reinterpret_cast<const Pack<T, VEC>*>(row)[q];
 #pragma unroll
@@ -123,12 +129,12 @@ __device__ __forceinline__ void load_row(const T* row, int lane, int tpr, int nv
 #pragma unroll
   for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) out.v[i] = f2(f[2 * i], f[2 * i + 1]);
 }
-template <class T, int VEC, int NV>
-__device__ __forceinline__ void store_row(T* row, int lane, int tpr, int nvec, const Row<VEC, NV>& in) {
+template <class T, int VEC, int NV, class Step>
+__device__ __forceinline__ void store_row(T* row, int first, Step step, int nvec, const Row<VEC, NV>& in) {
   if constexpr (sizeof(T) == 2 && VEC >= 2) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int q = lane + k * tpr;
+      const int q = first + k * step;
       Pack<uint32_t, VEC / 2> p;
 #pragma unroll
       for (int j = 0; j < VEC / 2; ++j) {
@@ -148,7 +154,7 @@ __device__ __forceinline__ void store_row(T* row, int lane, int tpr, int nvec, c
   }
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int q = lane + k * tpr;
+    const int q = first + k * step;
     Pack<T, VEC> p;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) p.v[j] = from_f32<T>(f[k * VEC + j]);
@@ -157,13 +163,13 @@ __device__ __forceinline__ void store_row(T* row, int lane, int tpr, int nvec, c
 }
 // A parameter vector's share: `fill` where it is absent.  Scalar loads: read
 // once per thread, and only as aligned as its type.
-template <class T, int VEC, int NV>
-__device__ __forceinline__ void load_parameter(const void* from, int lane, int tpr, int nvec, float fill,
+template <class T, int VEC, int NV, class Step>
+__device__ __forceinline__ void load_parameter(const void* from, int first, Step step, int nvec, float fill,
                                                Row<VEC, NV>& out) {
   float f[2 * Row<VEC, NV>::kPairs];
 #pragma unroll
   for (int e = 0; e < 2 * Row<VEC, NV>::kPairs; ++e) {
-    const int q = lane + e / VEC * tpr;
+    const int q = first + e / VEC * step;
     f[e] = from && e < VEC * NV && q < nvec ? to_f32(static_cast<const T*>(from)[q * VEC + e % VEC])
                                             : fill;
   }
@@ -180,14 +186,14 @@ __device__ __forceinline__ float forward_sum(const Row<VEC, NV>& x) {
   return t.x + t.y;
 }
 // x - mean in place (zero past nvec), and the sum of its squares.
-template <int VEC, int NV>
-__device__ __forceinline__ float forward_centre(Row<VEC, NV>& x, float mean, int lane, int tpr, int nvec) {
+template <int VEC, int NV, class Step>
+__device__ __forceinline__ float forward_centre(Row<VEC, NV>& x, float mean, int first, Step step, int nvec) {
   F2 s = f2(0.0f, 0.0f);
 #pragma unroll
   for (int i = 0; i < Row<VEC, NV>::kPairs; ++i) {
     const int e0 = 2 * i, e1 = 2 * i + 1;
-    const bool in0 = lane + e0 / VEC * tpr < nvec;
-    const bool in1 = e1 < VEC * NV && lane + e1 / VEC * tpr < nvec;
+    const bool in0 = first + e0 / VEC * step < nvec;
+    const bool in1 = e1 < VEC * NV && first + e1 / VEC * step < nvec;
     x.v[i] = add2(x.v[i], f2(in0 ? -mean : 0.0f, in1 ? -mean : 0.0f));
     s = fma2(x.v[i], x.v[i], s);
   }
@@ -246,9 +252,9 @@ __device__ __forceinline__ void add_row(Row<VEC, NV>& a, const Row<VEC, NV>& b) 
 }
 // The block's dw and db into part[2][dims].  Lanes of a warp that share columns
 // add by shuffles, warps through columns[warps][2][dims] in shared memory.
-template <int VEC, int NV>
-__device__ __forceinline__ void leave_partials(Row<VEC, NV>& dw, Row<VEC, NV>& db, int lane, int tpr,
-                                               int nvec, int dims, float* columns, float* part) {
+template <int VEC, int NV, class Step>
+__device__ __forceinline__ void leave_partials(Row<VEC, NV>& dw, Row<VEC, NV>& db, int first, Step step,
+                                               int tpr, int nvec, int dims, float* columns, float* part) {
   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   float* const to = tpr <= 32 ? columns + warp * 2 * dims : part;
 #pragma unroll
@@ -259,7 +265,7 @@ __device__ __forceinline__ void leave_partials(Row<VEC, NV>& dw, Row<VEC, NV>& d
       w += __shfl_xor_sync(kFull, w, o);
       b += __shfl_xor_sync(kFull, b, o);
     }
-    const int q = lane + e / VEC * tpr;
+    const int q = first + e / VEC * step;
     if (q < nvec && (tpr > 32 || int(threadIdx.x & 31) < tpr)) {
       to[q * VEC + e % VEC] = w;
       to[dims + q * VEC + e % VEC] = b;
@@ -345,7 +351,7 @@ layer_norm_backward_kernel(LayerNormBackwardArgs a, int tpr_) {
     store_row<T>(static_cast<T*>(a.dx) + row * a.dx_stride, lane, tpr, nvec, g);
   }
   if (params)
-    leave_partials(dw, db, lane, tpr, nvec, a.dims, columns,
+    leave_partials(dw, db, lane, tpr, tpr, nvec, a.dims, columns,
                    a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
 
@@ -432,8 +438,8 @@ __global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs 
   if (lane == 0)
     for (int s = 0; s < stages - 1; ++s) request(first + s * step, s);
   Row<VEC, NV> w, b;
-  load_parameter<T>(a.weight, sub, tpr, nvec, 1.0f, w);
-  load_parameter<T>(a.bias, sub, tpr, nvec, 0.0f, b);
+  load_parameter<T>(a.weight, sub * NV, Next(), nvec, 1.0f, w);
+  load_parameter<T>(a.bias, sub * NV, Next(), nvec, 0.0f, b);
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -459,13 +465,13 @@ __global__ void __launch_bounds__(256, 2) layer_norm_tiles_kernel(LayerNormArgs 
       const int r = r0 + group;
       T* const row = reinterpret_cast<T*>(at) + r * a.dims;
       Row<VEC, NV> v;
-      load_row<T>(row, sub, tpr, nvec, r < rows, v);
+      load_row<T>(row, sub * NV, Next(), nvec, r < rows, v);
       const float mean = row_sum<false>(none, tpr, forward_sum(v)) * inv_n;
-      const float var = row_sum<false>(none, tpr, forward_centre(v, mean, sub, tpr, nvec)) * inv_n;
+      const float var = row_sum<false>(none, tpr, forward_centre(v, mean, sub * NV, Next(), nvec)) * inv_n;
       const float rstd = 1.0f / sqrtf(var + a.eps);
       if (r < rows) {
         forward_out(v, rstd, w, b);
-        store_row<T>(row, sub, tpr, nvec, v);
+        store_row<T>(row, sub * NV, Next(), nvec, v);
         if (sub == 0) {
           if (a.mean) a.mean[tile * tile_rows + r] = mean;
           if (a.rstd) a.rstd[tile * tile_rows + r] = rstd;
@@ -545,7 +551,7 @@ layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
   if (lane == 0)
     for (int s = 0; s < stages - 1; ++s) request(first + s * step, s);
   Row<VEC, NV> w, dw{}, db{};
-  load_parameter<T>(a.weight, sub, tpr, nvec, 1.0f, w);
+  load_parameter<T>(a.weight, sub * NV, Next(), nvec, 1.0f, w);
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -579,18 +585,18 @@ layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
       const T* const grow = row + tile_rows * a.dims;
       const float mean = active ? st[r] : 0.0f, rstd = active ? st[tile_rows + r] : 0.0f;
       Row<VEC, NV> xh, g;
-      load_row<T>(row, sub, tpr, nvec, active, xh);
-      load_row<T>(grow, sub, tpr, nvec, active, g);
+      load_row<T>(row, sub * NV, Next(), nvec, active, xh);
+      load_row<T>(grow, sub * NV, Next(), nvec, active, g);
       float s1, s2;
       backward_sums<T>(xh, g, w, mean, rstd, params, dw, db, s1, s2);
       row_sum2<false>(none, tpr, s1, s2);
       if (!dx || !active) continue;
       backward_out(xh, g, rstd, s1 * inv_n, s2 * inv_n);
       if (res) {
-        load_row<T>(grow + tile_rows * a.dims, sub, tpr, nvec, true, xh);
+        load_row<T>(grow + tile_rows * a.dims, sub * NV, Next(), nvec, true, xh);
         add_row(g, xh);
       }
-      store_row<T>(row, sub, tpr, nvec, g);
+      store_row<T>(row, sub * NV, Next(), nvec, g);
     }
     if (rows == tile_rows) {
       tc::fence_async_shared();
@@ -615,7 +621,7 @@ layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
   }
   if (!params) return;
   __syncthreads();  // the ring's memory now holds the block's columns
-  leave_partials(dw, db, sub, tpr, nvec, a.dims,
+  leave_partials(dw, db, sub * NV, Next(), tpr, nvec, a.dims,
                  reinterpret_cast<float*>(smem + ((warps * stages * 8 + 127) & ~127)),
                  a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
@@ -763,7 +769,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_wide_kernel(LayerNorm
     for (int s = 0; s < stages; ++s) tc::bar_wait(bar0 + 8 * s, s < slot ? phase ^ 1 : phase);
   }
   if (params)
-    leave_partials(dw, db, lane, threads, nvec, a.dims, nullptr,
+    leave_partials(dw, db, lane, threads, threads, nvec, a.dims, nullptr,
                    a.partials + int64_t(blockIdx.x) * 2 * a.dims);
 }
 
