@@ -17,6 +17,7 @@ from .layers import (LayerNormGradients, LayerNormOutput, LinearGradients, Linea
                      layer_norm, layer_norm_backward, linear, linear_backward)
 from .model import (CudaAutomataExecutor, NpaModel, NpaWeights, RolloutConfig, RolloutTrace,
                     StepOutput, rollout_update_masks, run_rollout_from_particles)
+from .update_network import UpdateBlock, UpdateNetwork
 from . import bpk
 from ._lib import build as build_library, lib as load_library
 
@@ -28,6 +29,7 @@ __all__ = [
     "perceive_with_options", "CudaAutomataExecutor", "NpaModel", "NpaWeights", "RolloutConfig",
     "RolloutTrace", "StepOutput", "rollout_update_masks", "run_rollout_from_particles",
     "Activation", "LayerNormGradients", "LayerNormOutput", "LinearGradients", "LinearOutput",
-    "layer_norm", "layer_norm_backward", "linear", "linear_backward",
+    "layer_norm", "layer_norm_backward", "linear", "linear_backward", "UpdateBlock",
+    "UpdateNetwork",
     "build_library", "load_library",
 ]

@@ -427,3 +427,25 @@ def test_shapes_types_and_devices_that_do_not_fit():
             call()
     with pytest.raises(ba.config.InvalidEps):
         ba.layer_norm(x, eps=0.0)
+
+
+# Shapes at which the linear layer changes its way of working: odd widths with
+# enough work to be packed, tiles of block pairs with ragged edges, small layers
+# over many rows (the one-walk backward pass), every count of few rows.
+WAYS = [  # rows, inputs, outputs
+    (9000, 251, 240), (4200, 513, 384), (2100, 515, 1000), (2049, 1024, 1030), (300, 264, 4104),
+    (257, 4096, 520), (2048, 64, 192), (5001, 160, 64), (2500, 256, 64), (3333, 96, 256),
+    (6000, 200, 16), (10000, 8, 8), (4444, 72, 120),
+] + [(r, 1000, 2100) for r in range(1, 10)] + [(r, 77, 50) for r in (3, 5, 8)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,inputs,outputs", WAYS)
+def test_linear_at_its_ways_borders(rows, inputs, outputs, dtype):
+    test_linear(rows, inputs, outputs, 0, 0, dtype)
+    test_linear_backward(rows, inputs, outputs, 0, 0, dtype)
+
+
+def test_waits_all_end():
+    """No bounded wait of the kernels above has given up."""
+    assert ba.load_library().npa_bulk_copy_timeouts() == 0
