@@ -14,6 +14,7 @@ namespace npa {
 namespace {
 
 using linear_tc::FusedBackward;
+using linear_tc::load_ragged;
 using linear_tc::Operand;
 using linear_tc::Product;
 
@@ -146,6 +147,108 @@ npa_status launch_few_rows(const LinearArgs& a, bool vec, cudaStream_t s) {
   return after_launch("linear few_rows_kernel");
 }
 
+// The backward pass of a few rows as one kernel.  A block has a slab of inputs
+// and all outputs: LANES threads side by side have the slab (VEC inputs each),
+// the block's groups of them share the outputs out.  W's slab is read once (dx)
+// and dW's written on the way; the groups' shares of dx meet in shared memory.
+template <class T, int R, int VEC, int LANES>
+__global__ void __launch_bounds__(256) few_rows_backward_kernel(const __grid_constant__ LinearBackwardArgs a) {
+  using P = Pack<T, VEC>;
+  constexpr int kGroups = 256 / LANES, kSlab = LANES * VEC;
+  __shared__ float sums[8][R][kSlab];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int in_group = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int64_t col = int64_t(blockIdx.x) * kSlab + in_group * VEC;
+  const bool mine = col < a.inputs;
+  const int rows = int(a.rows);
+  const T* const w = static_cast<const T*>(a.weight);
+  float acc[R][VEC];
+  P x[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[r][j] = 0.0f;
+    x[r] = P{};
+    if (a.dweight && mine && r < rows)
+      x[r] = *reinterpret_cast<const P*>(static_cast<const T*>(a.x) + r * a.x_stride + col);
+  }
+  // every lane of a warp makes the same number of turns: they exchange dz
+#pragma unroll 2
+  for (int o0 = 0; o0 < a.outputs; o0 += kGroups) {
+    const int64_t o = o0 + group;
+    const bool there = o < a.outputs;
+    P wv{};
+    if (a.dx && there && mine) wv = *reinterpret_cast<const P*>(w + o * a.weight_stride + col);
+    // lane r of every eight has row r's dz
+    float d = 0.0f;
+    if (there && (lane & 7) < rows) {
+      const int64_t r = lane & 7;
+      d = to_f32(static_cast<const T*>(a.dy)[r * a.dy_stride + o]);
+      if (a.z)
+        d *= linear_tc::activation_slope<sizeof(T) == 2>(
+            a.activation, to_f32(static_cast<const T*>(a.z)[r * a.z_stride + o]));
+    }
+    float dw[VEC], db = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) dw[j] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float dr = __shfl_sync(0xffffffffu, d, (lane & ~7) | r);
+      if (r < rows) {
+        db += dr;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          acc[r][j] += dr * to_f32(wv.v[j]);
+          dw[j] += dr * to_f32(x[r].v[j]);
+        }
+      }
+    }
+    if (there && mine && a.dweight) {
+      P out;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) out.v[j] = from_f32<T>(dw[j]);
+      *reinterpret_cast<P*>(static_cast<T*>(a.dweight) + o * a.inputs + col) = out;
+    }
+    if (there && a.dbias && blockIdx.x == 0 && in_group == 0)
+      static_cast<T*>(a.dbias)[o] = from_f32<T>(db);
+  }
+  if (!a.dx) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      float s = acc[r][j];
+#pragma unroll
+      for (int d = LANES; d < 32; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+      if (lane < LANES) sums[warp][r][in_group * VEC + j] = s;
+    }
+  __syncthreads();
+  for (int e = threadIdx.x; e < R * kSlab; e += 256) {
+    const int r = e / kSlab, c = e % kSlab;
+    const int64_t at = int64_t(blockIdx.x) * kSlab + c;
+    if (r >= rows || at >= a.inputs) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) s += sums[q][r][c];
+    static_cast<T*>(a.dx)[r * a.dx_stride + at] = from_f32<T>(s);
+  }
+}
+template <class T, int R>
+npa_status launch_few_rows_backward(const LinearBackwardArgs& a, bool vec, cudaStream_t s) {
+  constexpr int kVec = 16 / int(sizeof(T));
+  if (vec)
+    few_rows_backward_kernel<T, R, kVec, 8>
+        <<<unsigned((a.inputs + 8 * kVec - 1) / (8 * kVec)), 256, 0, s>>>(a);
+  else
+    few_rows_backward_kernel<T, R, 1, 32><<<unsigned((a.inputs + 31) / 32), 256, 0, s>>>(a);
+  return after_launch("linear few_rows_backward_kernel");
+}
+// Few enough that a block's walk over all outputs stays short (a kernel or
+// three less to launch than the tiles' way, which is what such calls cost).
+bool few_rows_backward(int64_t rows, int outputs) {
+  return rows <= kFewRows && rows * outputs <= 4096;
+}
+
 // ---- dz and the bias gradient ----
 struct SlopeArgs {
   const void* dy;
@@ -162,22 +265,30 @@ struct SlopeArgs {
   int tx;           // column groups per block, a power of two
 };
 // dz = dy act'(z) rounded to the storage type, and each block's column sums of
-// the unrounded values.  A thread has VEC columns of every (256 / tx)th row.
-template <class T, int VEC>
+// the unrounded values.  A thread has 16 bytes of every (256 / tx)th row; RAGGED:
+// of rows that start anywhere or end within them (dz's rows are whole, zero past
+// the outputs).
+template <class T, bool RAGGED>
 __global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ SlopeArgs a) {
   let_next_launch();
   wait_for_previous();
+  constexpr int VEC = 16 / int(sizeof(T));
   using P = Pack<T, VEC>;
   __shared__ float sums[256 * VEC];
-  constexpr int kAhead = sizeof(P) == 16 ? 4 : 8;  // rows in flight per thread
+  constexpr int kAhead = RAGGED ? 2 : 4;  // rows in flight per thread
   const int tx = threadIdx.x & (a.tx - 1), ty = threadIdx.x / a.tx, rows_at_once = 256 / a.tx;
   const int64_t col = (int64_t(blockIdx.x) * a.tx + tx) * VEC;
   const bool mine = col < a.outputs;
+  const int valid = mine ? int(min(int64_t(VEC), a.outputs - col)) : 0;
   const int64_t begin = int64_t(blockIdx.y) * a.rows_per_block;
   const int64_t end = min(begin + a.rows_per_block, a.rows);
   const T* const dy = static_cast<const T*>(a.dy) + col;
   const T* const z = static_cast<const T*>(a.z) + col;
   T* const dz = static_cast<T*>(a.dz) + col;
+  auto read = [&](const T* p, int64_t r) -> P {
+    if (!RAGGED) return *reinterpret_cast<const P*>(p);
+    return load_ragged<T>(p, valid, (r > 0 || col > 0) && r + 1 < a.rows);
+  };
   float s[VEC] = {};
   if (mine) {
     for (int64_t r0 = begin + ty; r0 < end; r0 += int64_t(kAhead) * rows_at_once) {
@@ -186,8 +297,8 @@ __global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ Slop
       for (int i = 0; i < kAhead; ++i) {
         const int64_t r = r0 + int64_t(i) * rows_at_once;
         if (r < end) {
-          g[i] = *reinterpret_cast<const P*>(dy + r * a.dy_stride);
-          if (a.z) zz[i] = *reinterpret_cast<const P*>(z + r * a.z_stride);
+          g[i] = read(dy + r * a.dy_stride, r);
+          if (a.z) zz[i] = read(z + r * a.z_stride, r);
         }
       }
 #pragma unroll
@@ -213,10 +324,6 @@ __global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ Slop
       }
     }
   }
-  // the rest of dz's rows is zero (odd widths only: VEC = 1)
-  if (!mine && a.dz && col < a.dz_stride)
-    for (int64_t r = begin + ty; r < end; r += rows_at_once)
-      for (int j = 0; j < VEC; ++j) dz[r * a.dz_stride + j] = from_f32<T>(0.0f);
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sums[j * 256 + threadIdx.x] = s[j];
   __syncthreads();
@@ -249,7 +356,7 @@ __global__ void __launch_bounds__(256) bias_reduce_kernel(const float* __restric
 
 // ---- rows of odd widths, copied to rows that start on 16 bytes ----
 // A thread writes 16 bytes; past the width they are zero.
-template <class T, int VEC>
+template <class T>
 __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ from, int64_t stride, int64_t rows,
                                                    int width, T* __restrict__ to, int64_t pitch) {
   constexpr int kChunk = 16 / int(sizeof(T));
@@ -260,21 +367,10 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ from, i
   if (e >= rows * chunks) return;
   const int64_t row = e / chunks;
   const int col = int(e % chunks) * kChunk;
-  const T* const at = from + row * stride + col;
-  Pack<T, kChunk> out;
-#pragma unroll
-  for (int j = 0; j < kChunk; j += VEC) {
-    Pack<T, VEC> in{};
-    if (col + j + VEC <= width) {
-      in = *reinterpret_cast<const Pack<T, VEC>*>(at + j);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (col + j + i < width) in.v[i] = at[j + i];
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out.v[j + i] = in.v[i];
-  }
+  Pack<T, kChunk> out{};
+  if (col < width)
+    out = load_ragged<T>(from + row * stride + col, min(kChunk, width - col),
+                         (row > 0 || col > 0) && row + 1 < rows);
   *reinterpret_cast<Pack<T, kChunk>*>(to + row * pitch + col) = out;
 }
 int64_t packed_pitch(int width) { return (int64_t(width) + 7) / 8 * 8; }
@@ -284,14 +380,9 @@ npa_status pack_rows(Operand& o, void* to, bool after, cudaStream_t s) {
   const int64_t pitch = packed_pitch(o.width), rows = o.rows;
   const T* const from = static_cast<const T*>(o.p);
   const dim3 grid(grid_for(uint64_t(rows) * (pitch * sizeof(T) / 16), 256));
-  if (o.ld % 2 == 0 && reinterpret_cast<uintptr_t>(from) % (2 * sizeof(T)) == 0)
-    NPA_CUDA(launch_kernel(after, pack_kernel<T, 2>, grid, 256, 0, s, from, o.ld, rows, o.width,
-                           static_cast<T*>(to), pitch),
-             "linear pack_kernel");
-  else
-    NPA_CUDA(launch_kernel(after, pack_kernel<T, 1>, grid, 256, 0, s, from, o.ld, rows, o.width,
-                           static_cast<T*>(to), pitch),
-             "linear pack_kernel");
+  NPA_CUDA(launch_kernel(after, pack_kernel<T>, grid, 256, 0, s, from, o.ld, rows, o.width,
+                         static_cast<T*>(to), pitch),
+           "linear pack_kernel");
   o.p = to;
   o.ld = pitch;
   o.width = int(pitch);  // zeros past the width
@@ -669,9 +760,9 @@ npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
   return run_product<T>(p, ws.product_partials, ws.x != nullptr, s);
 }
 
-template <class T, int VEC>
+template <class T, bool RAGGED>
 npa_status launch_slope(SlopeArgs s, int* parts, cudaStream_t stream) {
-  const int groups = ceil_div(s.dz ? s.dz_stride : s.outputs, VEC);
+  const int groups = ceil_div(s.outputs, 16 / int(sizeof(T)));
   s.tx = 1;
   while (s.tx < 32 && s.tx < groups) s.tx *= 2;
   const int grid_x = ceil_div(groups, s.tx);
@@ -680,7 +771,7 @@ npa_status launch_slope(SlopeArgs s, int* parts, cudaStream_t stream) {
   *parts = int(std::max<int64_t>(1, std::min<int64_t>(most, (s.rows + at_once * 4 - 1) / (at_once * 4))));
   s.rows_per_block = (s.rows + *parts - 1) / *parts;
   *parts = int((s.rows + s.rows_per_block - 1) / s.rows_per_block);
-  slope_kernel<T, VEC><<<dim3(unsigned(grid_x), unsigned(*parts)), 256, 0, stream>>>(s);
+  slope_kernel<T, RAGGED><<<dim3(unsigned(grid_x), unsigned(*parts)), 256, 0, stream>>>(s);
   return after_launch("slope_kernel");
 }
 
@@ -746,6 +837,19 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
       NPA_CUDA(cudaMemsetAsync(a.dbias, 0, size_t(a.outputs) * sizeof(T), s), "cudaMemsetAsync");
     return NPA_OK;
   }
+  if (few_rows_backward(a.rows, a.outputs)) {
+    if (!a.dx && !a.dweight && !a.dbias) return NPA_OK;
+    constexpr int kVec = 16 / int(sizeof(T));
+    const bool vec = a.inputs % kVec == 0 &&
+                     (!a.dx || (vector_width<T>(a.weight, a.weight_stride, a.outputs) == kVec &&
+                                vector_width<T>(a.dx, a.dx_stride, a.rows) == kVec)) &&
+                     (!a.dweight || (vector_width<T>(a.x, a.x_stride, a.rows) == kVec &&
+                                     vector_width<T>(a.dweight, a.inputs, a.outputs) == kVec));
+    if (a.rows == 1) return launch_few_rows_backward<T, 1>(a, vec, s);
+    if (a.rows == 2) return launch_few_rows_backward<T, 2>(a, vec, s);
+    return a.rows <= 4 ? launch_few_rows_backward<T, 4>(a, vec, s)
+                       : launch_few_rows_backward<T, 8>(a, vec, s);
+  }
   if constexpr (sizeof(T) == 2) {
     const FusedBackward f = plan_fused(sizeof(T), a.activation, a.rows, a.inputs, a.outputs);
     if (f.stage_bytes && (a.dx || a.dweight) && tma_rows(a.dy, a.dy_stride, a.rows, 2) &&
@@ -780,9 +884,9 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     constexpr int kVec = 16 / int(sizeof(T));
     if (a.outputs % kVec == 0 && vector_width<T>(a.dy, a.dy_stride, a.rows) == kVec &&
         (!a.z || vector_width<T>(a.z, a.z_stride, a.rows) == kVec))
-      NPA_TRY((launch_slope<T, kVec>(g, &parts, s)));
+      NPA_TRY((launch_slope<T, false>(g, &parts, s)));
     else
-      NPA_TRY((launch_slope<T, 1>(g, &parts, s)));
+      NPA_TRY((launch_slope<T, true>(g, &parts, s)));
     after = true;
     if (a.dbias) {
       NPA_CUDA(launch_kernel(true, bias_reduce_kernel<T>, dim3(grid_for(a.outputs, 32)), 256, 0, s,
@@ -851,14 +955,15 @@ npa_status launch_linear(int dtype, const LinearArgs& a, void* workspace, cudaSt
 }
 
 size_t linear_backward_workspace(int dtype, int activation, int64_t rows, int inputs, int outputs) {
-  if (rows == 0) return 0;
+  if (rows == 0 || few_rows_backward(rows, outputs)) return 0;
   return carve_backward(nullptr, dtype, activation, rows, inputs, outputs).bytes;
 }
 
 npa_status launch_linear_backward(int dtype, const LinearBackwardArgs& a, void* workspace,
                                   cudaStream_t stream) {
   const BackwardCarve ws =
-      a.rows == 0 ? BackwardCarve{}
+      a.rows == 0 || few_rows_backward(a.rows, a.outputs)
+          ? BackwardCarve{}
                   : carve_backward(workspace, dtype, a.activation, a.rows, a.inputs, a.outputs);
   switch (dtype) {
     case NPA_DTYPE_F32: return backward_typed<float>(a, ws, stream);

@@ -76,7 +76,9 @@ struct Config {
   static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   static constexpr int kABytes = kBM * 128, kBBytes = kBRows * 128;
   static constexpr int kStageBytes = kParts * (kABytes + kBBytes);
-  static constexpr int kOutBuffers = BN == 256 || kParts == 3 ? 1 : 2;
+  // Two staging buffers to an epilogue warp where they fit: the next group is
+  // written while TMA reads the last.
+  static constexpr int kOutBuffers = (BN == 256 && !PAIR) || kParts == 3 ? 1 : 2;
   static constexpr int kOutBytes = kEpilogueWarps * kOutBuffers * 4096;
   static constexpr int kStagesFit = (kSmemLimit - kOutBytes - 2048) / kStageBytes;
   static constexpr int kStages = kStagesFit > 6 ? 6 : kStagesFit;
@@ -89,24 +91,49 @@ struct Config {
 };
 
 // act(z) and act'(z).  NaN stays NaN.  FAST (16-bit storage): exponentials and
-// quotients by the approximate instructions, whose errors of a few 2^-22 vanish
-// in a result that is rounded to 8 or 11 bits; f32 storage takes the library's.
+// reciprocals by the approximate instructions, without the library's handling of
+// subnormal values, and erf by a short formula: errors of 2^-22 or so of the
+// largest term, which vanish in a result that is rounded to 8 or 11 bits.  f32
+// storage takes the library's functions.
 template <bool FAST>
 __device__ __forceinline__ float exponential(float x) {
-  return FAST ? __expf(x) : expf(x);
+  if (!FAST) return expf(x);
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
 }
 // 1 / (1 + e^-z).  Where e^-z overflows both forms give 0.
+__device__ __forceinline__ float fast_reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 template <bool FAST>
 __device__ __forceinline__ float logistic(float z) {
   const float d = 1.0f + exponential<FAST>(-z);
-  return FAST ? __fdividef(1.0f, d) : 1.0f / d;
+  return FAST ? fast_reciprocal(d) : 1.0f / d;
+}
+// The normal distribution function at z, with e = exp(-z^2 / 2): Abramowitz and
+// Stegun's 7.1.26, 1 - erf(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x),
+// off by 1.5e-7 at most, at x = |z| / sqrt(2).
+__device__ __forceinline__ float fast_normal(float z, float e) {
+  const float t = fast_reciprocal(fmaf(0.23164190f, fabsf(z), 1.0f));
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f);
+  q = 0.5f * t * q * e;
+  return z < 0.0f ? q : 1.0f - q;
 }
 template <bool FAST>
 __device__ __forceinline__ float activation(int act, float z) {
   switch (act) {
     case NPA_ACTIVATION_RELU: return z < 0.0f ? 0.0f : z;
-    case NPA_ACTIVATION_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case NPA_ACTIVATION_GELU:
+      return FAST ? z * fast_normal(z, exponential<true>(-0.5f * z * z))
+                  : 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
     case NPA_ACTIVATION_GELU_TANH: {
+      // (1 + tanh(u)) / 2 = logistic(2u)
       const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
       return FAST ? z * logistic<true>(2.0f * u) : 0.5f * z * (1.0f + tanhf(u));
     }
@@ -118,11 +145,13 @@ template <bool FAST>
 __device__ __forceinline__ float activation_slope(int act, float z) {
   switch (act) {
     case NPA_ACTIVATION_RELU: return z <= 0.0f ? 0.0f : 1.0f;
-    case NPA_ACTIVATION_GELU:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-             z * 0.39894228040143268f * exponential<FAST>(-0.5f * z * z);
+    case NPA_ACTIVATION_GELU: {
+      const float e = exponential<FAST>(-0.5f * z * z);
+      const float cdf = FAST ? fast_normal(z, e) : 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+      return cdf + z * 0.39894228040143268f * e;
+    }
     case NPA_ACTIVATION_GELU_TANH: {
-      // (1 + tanh(u)) / 2 = p = logistic(2u), and its derivative is 2 p (1 - p) u'
+      // p = logistic(2u), and its derivative is 2 p (1 - p) u'
       const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
       const float p = logistic<FAST>(2.0f * u);
       return p + 2.0f * z * p * (1.0f - p) * 0.79788456080286536f * (1.0f + 0.134145f * z * z);
@@ -352,6 +381,38 @@ struct TileReader {
   }
 };
 
+// ---- rows that do not start on 16 bytes ----
+// `valid` (1 to N) values from any address, zero past them, N of them 16 bytes.
+// 16-bit values come as the aligned words that hold them, `inside` saying that
+// the value before and the value after the N also belong to the buffer; at the
+// buffer's ends one by one.
+template <class T>
+__device__ __forceinline__ Pack<T, 16 / int(sizeof(T))> load_ragged(const T* p, int valid, bool inside) {
+  constexpr int N = 16 / int(sizeof(T));
+  Pack<T, N> out{};
+  if constexpr (sizeof(T) == 2) {
+    if (inside && valid == N) {
+      const uint32_t* const w =
+          reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+      uint32_t v[N / 2 + 1];
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) v[i] = w[i];
+      if (reinterpret_cast<uintptr_t>(p) & 2) {
+        v[N / 2] = w[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) v[i] = __byte_perm(v[i], v[i + 1], 0x5432);
+      }
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) reinterpret_cast<uint32_t*>(out.v)[i] = v[i];
+      return out;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < valid) out.v[i] = p[i];
+  return out;
+}
+
 // ---- epilogue ----
 // One warp's window on an output: 32 rows from row0, a 128-byte group of
 // columns from col0, staged in the warp's shared-memory buffer.
@@ -377,11 +438,10 @@ __device__ __forceinline__ void stage_values(uint32_t buf, int lane, const float
 // The staged group to global memory: by TMA, or row by row where the output's
 // rows do not start on 16 bytes.
 template <class OUT>
-__device__ __forceinline__ void put_group(uint32_t buf, const char* buf_ptr, int lane,
+__device__ __forceinline__ void put_group(uint32_t buf, int lane,
                                           const CUtensorMap* map, bool tma, int x, int y_tma_row,
                                           void* out, int64_t stride, int64_t row0, int rows,
                                           int cols) {
-  constexpr int kCols = 128 / int(sizeof(OUT));
   if (tma) {
     tc::fence_async_shared();
     __syncwarp();
@@ -392,14 +452,38 @@ __device__ __forceinline__ void put_group(uint32_t buf, const char* buf_ptr, int
     return;
   }
   __syncwarp();
-  OUT* const base = static_cast<OUT*>(out) + row0 * stride + x;
-  constexpr int kPer = 16 / int(sizeof(OUT));
-  for (int r = 0; r < rows; ++r)
+  // A lane has columns lane and lane + 32 of every row; eight rows are read from
+  // shared memory before the first is written.
+  constexpr int kPer = 16 / int(sizeof(OUT)), kAcross = 4 / int(sizeof(OUT));
+  OUT* to = static_cast<OUT*>(out) + row0 * stride + x + lane;
+  const int e = lane % kPer * int(sizeof(OUT));
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    uint32_t v[8][kAcross];
 #pragma unroll
-    for (int c = lane; c < kCols; c += 32)
-      if (c < cols)
-        base[r * stride + c] = reinterpret_cast<const OUT*>(
-            buf_ptr + swizzled(r, c / kPer))[c % kPer];
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int h = 0; h < kAcross; ++h) {
+        const uint32_t at = buf + swizzled(r0 + r, (lane + 32 * h) / kPer) + e;
+        if constexpr (sizeof(OUT) == 4)
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[r][h]) : "r"(at));
+        else
+          asm volatile("{ .reg .b16 t; ld.shared.b16 t, [%1]; cvt.u32.u16 %0, t; }"
+                       : "=r"(v[r][h])
+                       : "r"(at));
+      }
+#pragma unroll
+    for (int r = 0; r < 8; ++r, to += stride) {
+      if (r0 + r >= rows) break;
+#pragma unroll
+      for (int h = 0; h < kAcross; ++h)
+        if (lane + 32 * h < cols) {
+          if constexpr (sizeof(OUT) == 4)
+            to[32 * h] = __uint_as_float(v[r][h]);
+          else
+            reinterpret_cast<uint16_t*>(to)[32 * h] = uint16_t(v[r][h]);
+        }
+    }
+  }
 }
 
 template <class T, bool LOADER, int BN, bool PAIR>
@@ -756,16 +840,24 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // that the loads' latency passes under them; the loader kernel's register
         // budget (five warps to an SM quarter) has no room for it
         uint4 res[LOADER ? 1 : 8];
-        const bool res_vec = p.residual_vec && cols == kGroup;
-        auto read_residual = [&](int i) -> uint4 {
-          const int rr = i * 4 + (lane >> 3);
-          const T* const r = static_cast<const T*>(p.residual) + (row0 + rr) * p.residual_stride + col0;
-          return rr < rows ? *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(r) +
-                                                             (lane & 7) * 16)
-                           : make_uint4(0, 0, 0, 0);
+        auto read_residual = [&](int i) -> uint4 {  // 16 bytes of row i * 4 + lane / 8
+          constexpr int kPer = 16 / int(sizeof(T));
+          const int64_t row = row0 + i * 4 + (lane >> 3);
+          const int c = (lane & 7) * kPer;
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (row >= p.m || c >= cols) return u;
+          const T* const r = static_cast<const T*>(p.residual) + row * p.residual_stride + col0 + c;
+          if (p.residual_vec && c + kPer <= cols) {
+            u = *reinterpret_cast<const uint4*>(r);
+          } else {
+            const Pack<T, kPer> v = load_ragged<T>(r, min(kPer, cols - c),
+                                                   (row > 0 || col0 + c > 0) && row + 1 < p.m);
+            u = *reinterpret_cast<const uint4*>(&v);
+          }
+          return u;
         };
         if constexpr (!LOADER) {
-          if (mine && !p.partials && p.residual && res_vec) {
+          if (mine && !p.partials && p.residual) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) res[i] = read_residual(i);
           }
@@ -810,7 +902,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (h * 32 >= cols) break;
             const uint32_t b = next_buffer();
             stage_values<float>(b, lane, v, h * 32);
-            put_group<float>(b, pointer(b), lane, &map_y, true, col0 + h * 32, int(prow), nullptr,
+            put_group<float>(b, lane, &map_y, true, col0 + h * 32, int(prow), nullptr,
                              0, 0, 0, 0);
           }
           return;
@@ -834,27 +926,16 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (p.z) {
           const uint32_t b = next_buffer();
           stage_values<T>(b, lane, v, 0);
-          put_group<T>(b, pointer(b), lane, &map_z, p.z_tma, col0, int(row0), p.z, p.z_stride,
+          put_group<T>(b, lane, &map_z, p.z_tma, col0, int(row0), p.z, p.z_stride,
                        row0, rows, cols);
         }
         activate<sizeof(T) == 2>(p.act, v);
         const uint32_t b = next_buffer();
         if (p.residual) {
-          if (res_vec) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              store_shared16(b + swizzled(i * 4 + (lane >> 3), lane & 7),
-                             LOADER ? read_residual(i) : res[LOADER ? 0 : i]);
-          } else {
-            const T* const r = static_cast<const T*>(p.residual) + row0 * p.residual_stride + col0;
-            constexpr int kPer = 16 / int(sizeof(T));
-            for (int rr = 0; rr < rows; ++rr)
-#pragma unroll
-              for (int c = lane; c < kGroup; c += 32)
-                if (c < cols)
-                  reinterpret_cast<T*>(pointer(b) + swizzled(rr, c / kPer))[c % kPer] =
-                      r[rr * p.residual_stride + c];
-          }
+          for (int i = 0; i < 8; ++i)
+            store_shared16(b + swizzled(i * 4 + (lane >> 3), lane & 7),
+                           LOADER ? read_residual(i) : res[LOADER ? 0 : i]);
           __syncwarp();
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
@@ -876,7 +957,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
         }
         stage_values<T>(b, lane, v, 0);
-        put_group<T>(b, pointer(b), lane, &map_y, p.y_tma, col0, int(row0), p.y, p.y_stride, row0,
+        put_group<T>(b, lane, &map_y, p.y_tma, col0, int(row0), p.y, p.y_stride, row0,
                      rows, cols);
       };
 #pragma unroll

@@ -110,6 +110,18 @@ def _rows(t):
     return t.contiguous(), t.shape[-1]
 
 
+def _aligned_rows(t):
+    """As _rows for the linear layer's operands: a large range of columns whose
+    rows do not start on 16 bytes, but would by themselves, is copied.  The
+    products read such rows several times, by TMA only when aligned."""
+    t, stride = _rows(t)
+    size = t.element_size()
+    if ((stride * size) % 16 and t.shape[0] > 1 and t.shape[-1] * size % 16 == 0
+            and t.numel() >= 1 << 19):
+        return t.contiguous(), t.shape[-1]
+    return t, stride
+
+
 def _matrix(t, x, shape, name: str):
     _like(t, x, name)
     if t.shape != shape:
@@ -247,10 +259,11 @@ def linear(x, weight, bias=None, residual=None, activation: Activation = Activat
     torch = _torch
     inputs, outputs = _layer_shape(x, weight)
     out_shape = x.shape[:-1] + (outputs,)
-    wr, wstride = _matrix(weight, x, weight.shape, "weight")
+    _like(weight, x, "weight")
+    wr, wstride = _aligned_rows(weight)
     b = _vector(bias, x, outputs, "bias")
     rr, rs = (None, 0) if residual is None else _matrix(residual, x, out_shape, "residual")
-    xr, xs = _rows(x)
+    xr, xs = _aligned_rows(x)
     rows = x.numel() // inputs if inputs else 0
     y = _outputs_like(x, out_shape)
     z = torch.empty_like(y) if save_pre_activation else None
@@ -273,14 +286,15 @@ def linear_backward(dy, x, weight, pre_activation=None,
     inputs, outputs = _layer_shape(x, weight)
     out_shape = x.shape[:-1] + (outputs,)
     want = _needs(needs)
-    wr, wstride = _matrix(weight, x, weight.shape, "weight")
+    _like(weight, x, "weight")
+    wr, wstride = _aligned_rows(weight)
     dyr, dys = _matrix(dy, x, out_shape, "dy")
     zr, zs = None, 0
     if int(activation) != Activation.Identity:
         if pre_activation is None:
             raise InvalidArgument("this activation's gradient needs pre_activation")
         zr, zs = _matrix(pre_activation, x, out_shape, "pre_activation")
-    xr, xs = _rows(x)
+    xr, xs = _aligned_rows(x)
     rows = x.numel() // inputs if inputs else 0
     dx = _outputs_like(x, x.shape) if "x" in want else None
     dw = _outputs_like(weight, weight.shape) if "weight" in want else None

@@ -597,8 +597,8 @@ npa_status npa_dev_linear_backward_workspace_size(int32_t dtype, int32_t activat
  *   dx = dz weight,  dweight = dz^T x [outputs][inputs],  dbias = sum over
  *   rows of dz.  The residual's gradient is dy itself.
  * Each output is optional; weight is read for dx only and x for dweight only.
- * 16-bit types round dz to the storage type for the two products (their sums
- * stay in 32 bits); dbias sums dz unrounded. */
+ * 16-bit types round dz to the storage type for the two products of more than a
+ * few rows (their sums stay in 32 bits); dbias sums dz unrounded. */
 npa_status npa_dev_linear_backward(int32_t dtype, int32_t activation, const void* d_dy,
                                    int64_t dy_stride, const void* d_x, int64_t x_stride,
                                    const void* d_weight, int64_t weight_stride,
