@@ -473,19 +473,23 @@ Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
   Plan p{};
   p.k_blocks = ceil_div(k, linear_tc::kBK);
   p.partial_pitch = (n + 3) / 4 * 4;
-  // The shape with the least work on the fullest SM.  A k block of a tile 256,
-  // 128 or 64 columns wide costs about 8, 5 and 4 units (the narrow tiles
-  // fetch the same rows of A for fewer products; a pair's fetches less than
-  // its 256 columns would alone: 6), its epilogue as much as two blocks, and
-  // layers of a split sum their traffic: each at least four blocks.
+  // The shape with the least time on the fullest SM, in units of 100 cycles: a
+  // tile takes its k blocks or its epilogue, whichever is longer, as measured
+  // (8192 x 4096 x 4096: 7 units a block in a pair's tile; 607399 x 48 x 192:
+  // 109 us in pairs' tiles of 256 columns, 98 in tiles of 128), and a split sum
+  // another pass.  The loader warps' blocks cost more than their products.
   struct Shape {
-    int bn, unit;
+    int bn, block, epilogue;
     bool pair;
   };
-  constexpr Shape kShapes[] = {{256, 6, true}, {256, 8, false}, {128, 5, false}, {64, 4, false}};
+  constexpr Shape kTmaShapes[] = {{256, 7, 66, true}, {256, 10, 70, false}, {128, 5, 28, false}, {64, 4, 16, false}};
+  constexpr Shape kF32Shapes[] = {{128, 30, 35, false}, {64, 20, 20, false}};
+  constexpr Shape kLoaderShapes[] = {{128, 40, 28, false}, {64, 26, 16, false}};
+  const Shape* shapes = size == 4 ? kF32Shapes : tma ? kTmaShapes : kLoaderShapes;
+  const int shape_count = size == 2 && tma ? 4 : 2;
   int64_t best = INT64_MAX;
-  for (const Shape& shape : kShapes) {
-    if (shape.bn == 256 && !(size == 2 && tma)) continue;
+  for (int i = 0; i < shape_count; ++i) {
+    const Shape& shape = shapes[i];
     if (shape.bn > 64 && shape.bn / 2 >= n) continue;
     if (shape.pair && m <= linear_tc::kBM) continue;
     const int rows = shape.pair ? 2 * linear_tc::kBM : linear_tc::kBM;
@@ -495,7 +499,8 @@ Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
     const int blocks = ceil_div(p.k_blocks, splits);
     splits = ceil_div(p.k_blocks, blocks);
     const int64_t cost =
-        ceil_div(tiles * splits, walkers) * (blocks + 2) * shape.unit + (splits > 1 ? 16 : 0);
+        int64_t(ceil_div(tiles * splits, walkers)) * (std::max(blocks * shape.block, shape.epilogue) + 8) +
+        (splits > 1 ? 40 : 0);
     if (cost < best) {
       best = cost;
       p.bn = shape.bn;
@@ -670,7 +675,9 @@ FusedBackward plan_fused(size_t size, int activation, int64_t rows, int inputs, 
   f.tmem_columns = 32;
   while (int(f.tmem_columns) < (f.m_blocks + 2) * f.n_pad) f.tmem_columns *= 2;
   f.pitch = (int64_t(inputs) + 3) / 4 * 4;
-  return linear_tc::fused_fits(f) ? f : FusedBackward{};
+  for (f.stages = linear_tc::kFusedStages; f.stages >= 1; --f.stages)
+    if (linear_tc::fused_fits(f)) return f;
+  return FusedBackward{};
 }
 int fused_blocks(const FusedBackward& f) {
   return int(std::min<int64_t>(kSms, (f.rows + linear_tc::kBM - 1) / linear_tc::kBM));

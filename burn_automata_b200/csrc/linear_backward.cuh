@@ -19,7 +19,19 @@ namespace npa {
 namespace linear_tc {
 
 constexpr int kFusedThreads = 512;     // 4 dx warps, 4 control, 8 for dz
-constexpr int kFusedStages = 2;
+constexpr int kFusedStages = 2;  // at most
+
+// A position in a ring of `slots` slots and the parity of its current phase.
+struct RingCursor {
+  int slots;
+  uint32_t slot = 0, parity = 0;
+  __device__ __forceinline__ void advance() {
+    if (++slot == uint32_t(slots)) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+};
 
 struct FusedBackward {
   int64_t rows;
@@ -27,6 +39,7 @@ struct FusedBackward {
   int out_blocks, in_blocks;  // of 64 columns
   int k_pad, n_pad;           // outputs and inputs in whole 16s
   int m_blocks;               // of 128 outputs
+  int stages;  // two where they fit, else one
   uint32_t stage_bytes, weight_bytes;
   uint32_t tmem_columns;
   uint32_t dx_idesc, dw_idesc;
@@ -39,7 +52,7 @@ struct FusedBackward {
 // Shared memory of a block: the stages (dy, z, x), the weights, dx's staging
 // buffers and the barriers.
 inline size_t fused_smem(const FusedBackward& f) {
-  return size_t(kFusedStages) * f.stage_bytes + f.weight_bytes + 4 * 4096 + 1024 + 256;
+  return size_t(f.stages) * f.stage_bytes + f.weight_bytes + 4 * 4096 + 1024 + 256;
 }
 // Static shared memory beside it (the column sums).
 constexpr size_t kFusedStaticSmem = kLoaderWarps * 32 * 8 * sizeof(float);
@@ -58,7 +71,7 @@ fused_backward_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_c
   __shared__ float db_sums[kLoaderWarps * 32 * 8];
   const uint32_t raw = tc::smem_addr(smem_raw);
   const uint32_t base = (raw + 1023) & ~1023u;
-  const uint32_t weights = base + kFusedStages * f.stage_bytes;
+  const uint32_t weights = base + f.stages * f.stage_bytes;
   const uint32_t out_base = weights + f.weight_bytes;
   const uint32_t full = out_base + 4 * 4096, ready = full + 8 * kFusedStages;
   const uint32_t empty = ready + 8 * kFusedStages, acc_full = empty + 8 * kFusedStages;
@@ -103,12 +116,12 @@ fused_backward_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_c
         for (int i = 0; i < f.in_blocks; ++i)
           tc::tma_load(weights + i * f.k_pad * 128, &map_w, i * 64, 0, weights_full);
       }
-      Cursor<kFusedStages> at;
+      RingCursor at{f.stages};
       uint32_t issued = 0;
       for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, at.advance()) {
         ok = tc::bar_wait(empty + 8 * at.slot, at.parity ^ 1);
         if (!ok) break;
-        if (issued < kFusedStages) ++issued;
+        if (issued < uint32_t(f.stages)) ++issued;
         const uint32_t bar = full + 8 * at.slot, stage = base + at.slot * f.stage_bytes;
         const int row = int(t * kBM);
         tc::bar_expect(bar, f.stage_bytes);
@@ -121,13 +134,13 @@ fused_backward_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_c
       }
       if (!ok)  // copies in flight must land before the block may leave
         for (uint32_t j = 0; j < issued; ++j) {
-          const uint32_t slot = (at.slot + kFusedStages - 1 - j) % kFusedStages;
+          const uint32_t slot = (at.slot + f.stages - 1 - j) % f.stages;
           tc::bar_wait(full + 8 * slot, slot < at.slot ? at.parity : at.parity ^ 1);
         }
     }
   } else if (warp == kMma) {
     if (lane == 0) {
-      Cursor<kFusedStages> at;
+      RingCursor at{f.stages};
       Cursor<2> acc;
       if (f.want_dx) ok = tc::bar_wait(weights_full, 0);
       bool first = true;
@@ -172,7 +185,7 @@ fused_backward_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_c
     const int chunk = tid % chunks, row0 = tid / chunks;
     const uint32_t column = (chunk >> 3) * kBlockBytes;
     float sums[8] = {};
-    Cursor<kFusedStages> at;
+    RingCursor at{f.stages};
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, at.advance()) {
       ok = __all_sync(0xffffffffu, tc::bar_wait(full + 8 * at.slot, at.parity));
       if (!ok) break;

@@ -840,26 +840,58 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // that the loads' latency passes under them; the loader kernel's register
         // budget (five warps to an SM quarter) has no room for it
         uint4 res[LOADER ? 1 : 8];
-        auto read_residual = [&](int i) -> uint4 {  // 16 bytes of row i * 4 + lane / 8
-          constexpr int kPer = 16 / int(sizeof(T));
-          const int64_t row = row0 + i * 4 + (lane >> 3);
-          const int c = (lane & 7) * kPer;
+        // 16 bytes of row i * 4 + lane / 8; or, where rows do not start on 16 bytes,
+        // words i * 4 .. + 3 of the lane's columns lane and lane + 32 of half the
+        // rows: with hardly any L1 beside the stages an access has to take all of
+        // what it touches
+        const bool res_vec = p.residual_vec && cols * int(sizeof(T)) % 16 == 0;
+        auto read_residual = [&](int i, int half_rows) -> uint4 {
           uint4 u = make_uint4(0, 0, 0, 0);
-          if (row >= p.m || c >= cols) return u;
-          const T* const r = static_cast<const T*>(p.residual) + row * p.residual_stride + col0 + c;
-          if (p.residual_vec && c + kPer <= cols) {
-            u = *reinterpret_cast<const uint4*>(r);
-          } else {
-            const Pack<T, kPer> v = load_ragged<T>(r, min(kPer, cols - c),
-                                                   (row > 0 || col0 + c > 0) && row + 1 < p.m);
-            u = *reinterpret_cast<const uint4*>(&v);
+          if (res_vec) {
+            const int rr = i * 4 + (lane >> 3), c = (lane & 7) * (16 / int(sizeof(T)));
+            if (rr < rows && c < cols)
+              u = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) +
+                                                  (row0 + rr) * p.residual_stride + col0 + c);
+            return u;
           }
-          return u;
+          constexpr int kAcross = kGroup / 32;
+          uint32_t w[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int rr = half_rows + (i * 4 + q) / kAcross, c = lane + 32 * ((i * 4 + q) % kAcross);
+            w[q] = 0;
+            if (rr < rows && c < cols) {
+              const T* const r = static_cast<const T*>(p.residual) + (row0 + rr) * p.residual_stride + col0 + c;
+              if constexpr (sizeof(T) == 4)
+                w[q] = *reinterpret_cast<const uint32_t*>(r);
+              else
+                w[q] = *reinterpret_cast<const uint16_t*>(r);
+            }
+          }
+          return make_uint4(w[0], w[1], w[2], w[3]);
+        };
+        auto stage_residual = [&](uint32_t b, int i, int half_rows, uint4 u) {
+          if (res_vec) {
+            store_shared16(b + swizzled(i * 4 + (lane >> 3), lane & 7), u);
+            return;
+          }
+          constexpr int kAcross = kGroup / 32, kPer = 16 / int(sizeof(T));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int rr = half_rows + (i * 4 + q) / kAcross, c = lane + 32 * ((i * 4 + q) % kAcross);
+            const uint32_t at = b + swizzled(rr, c / kPer) + c % kPer * int(sizeof(T));
+            if constexpr (sizeof(T) == 4)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(w[q]) : "memory");
+            else
+              asm volatile("{ .reg .b16 t; cvt.u16.u32 t, %1; st.shared.b16 [%0], t; }" ::"r"(at), "r"(w[q])
+                           : "memory");
+          }
         };
         if constexpr (!LOADER) {
           if (mine && !p.partials && p.residual) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) res[i] = read_residual(i);
+            for (int i = 0; i < 8; ++i) res[i] = read_residual(i, 0);
           }
         }
         if constexpr (C::kParts == 3) {
@@ -932,10 +964,25 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         activate<sizeof(T) == 2>(p.act, v);
         const uint32_t b = next_buffer();
         if (p.residual) {
+          if constexpr (LOADER) {
+            for (int i = 0; i < 8; ++i) stage_residual(b, i, 0, read_residual(i, 0));
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            store_shared16(b + swizzled(i * 4 + (lane >> 3), lane & 7),
-                           LOADER ? read_residual(i) : res[LOADER ? 0 : i]);
+            for (int i = 0; i < 8; ++i) stage_residual(b, i, 0, res[i]);
+          }
+          // 32 single values per lane are all of 32 f32 columns, and half of the
+          // rows of 64 columns
+          if (kGroup == 64 && !res_vec) {
+            constexpr int kAt = 16;
+            if constexpr (LOADER) {
+              for (int i = 0; i < 8; ++i) stage_residual(b, i, kAt, read_residual(i, kAt));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) res[i] = read_residual(i, kAt);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) stage_residual(b, i, kAt, res[i]);
+            }
+          }
           __syncwarp();
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
