@@ -269,7 +269,7 @@ struct SlopeArgs {
 // of rows that start anywhere or end within them (dz's rows are whole, zero past
 // the outputs).
 template <class T, bool RAGGED>
-__global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ SlopeArgs a) {
+__global__ void __launch_bounds__(256, 3) slope_kernel(const __grid_constant__ SlopeArgs a) {
   let_next_launch();
   wait_for_previous();
   constexpr int VEC = 16 / int(sizeof(T));
@@ -402,7 +402,9 @@ bool packs(size_t size, int width, int64_t rows, int inputs, int outputs) {
 
 // ---- host side ----
 constexpr int kSms = 148;             // the plans' block count: B200's SMs
-constexpr int kBiasBlocks = 4 * kSms;  // blocks of slope_kernel at most
+// Blocks of slope_kernel at most: the three to an SM that its registers allow, in
+// one wave (16384 x 4096 f16 silu: 119 us with four, which take a second wave).
+constexpr int kBiasBlocks = 3 * kSms;
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
