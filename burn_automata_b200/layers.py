@@ -242,6 +242,15 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, residual_gradient=None,
     return LayerNormGradients(dx, dw, db)
 
 
+def _activation(activation) -> int:
+    if type(activation) is not Activation:
+        try:
+            activation = Activation(activation)
+        except ValueError:
+            raise InvalidArgument(f"unknown activation {activation!r}") from None
+    return int(activation)
+
+
 def _layer_shape(x, weight):
     if not isinstance(weight, _t().Tensor) or weight.dim() != 2:
         raise InvalidArgument("weight must be a 2-D tensor [outputs, inputs]")
@@ -255,7 +264,7 @@ def linear(x, weight, bias=None, residual=None, activation: Activation = Activat
     """activation(x weight^T + bias) + residual, weight [outputs, inputs].
     save_pre_activation also returns z = x weight^T + bias, which
     linear_backward reads for every activation but the identity."""
-    code = _dtype(x, "x")
+    code, act = _dtype(x, "x"), _activation(activation)
     torch = _torch
     inputs, outputs = _layer_shape(x, weight)
     out_shape = x.shape[:-1] + (outputs,)
@@ -270,7 +279,7 @@ def linear(x, weight, bias=None, residual=None, activation: Activation = Activat
     L = _lib.lib()
     ws, ws_bytes = _workspace(x, "npa_dev_linear_workspace_size", code, rows, inputs, outputs)
     _call(L.npa_dev_linear, x.device,
-          (code, int(activation), xr.data_ptr(), xs, wr.data_ptr(), wstride, _ptr(b), _ptr(rr), rs,
+          (code, act, xr.data_ptr(), xs, wr.data_ptr(), wstride, _ptr(b), _ptr(rr), rs,
            rows, inputs, outputs, y.data_ptr(), outputs, _ptr(z), outputs, _ptr(ws), ws_bytes),
           "linear")
     return LinearOutput(y, z)
@@ -282,7 +291,7 @@ def linear_backward(dy, x, weight, pre_activation=None,
     """The gradients of linear given dy and (for every activation but the
     identity) its saved pre-activation.  `needs` names the gradients to
     compute."""
-    code = _dtype(x, "x")
+    code, act = _dtype(x, "x"), _activation(activation)
     inputs, outputs = _layer_shape(x, weight)
     out_shape = x.shape[:-1] + (outputs,)
     want = _needs(needs)
@@ -290,7 +299,7 @@ def linear_backward(dy, x, weight, pre_activation=None,
     wr, wstride = _aligned_rows(weight)
     dyr, dys = _matrix(dy, x, out_shape, "dy")
     zr, zs = None, 0
-    if int(activation) != Activation.Identity:
+    if act != Activation.Identity:
         if pre_activation is None:
             raise InvalidArgument("this activation's gradient needs pre_activation")
         zr, zs = _matrix(pre_activation, x, out_shape, "pre_activation")
@@ -300,10 +309,10 @@ def linear_backward(dy, x, weight, pre_activation=None,
     dw = _outputs_like(weight, weight.shape) if "weight" in want else None
     db = x.new_empty(outputs) if "bias" in want else None
     L = _lib.lib()
-    ws, ws_bytes = _workspace(x, "npa_dev_linear_backward_workspace_size", code, int(activation), rows,
+    ws, ws_bytes = _workspace(x, "npa_dev_linear_backward_workspace_size", code, act, rows,
                               inputs, outputs)
     _call(L.npa_dev_linear_backward, x.device,
-          (code, int(activation), dyr.data_ptr(), dys, xr.data_ptr(), xs, wr.data_ptr(), wstride,
+          (code, act, dyr.data_ptr(), dys, xr.data_ptr(), xs, wr.data_ptr(), wstride,
            _ptr(zr), zs, rows, inputs, outputs, _ptr(dx), inputs, _ptr(dw), _ptr(db), _ptr(ws),
            ws_bytes), "linear_backward")
     return LinearGradients(dx, dw, db)
