@@ -561,11 +561,11 @@ npa_status pair_blocks(K kernel, int threads, size_t smem, int sms, int* blocks)
   return NPA_OK;
 }
 
-template <class T, bool LOADER, int BN, bool PAIR = false>
-npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, bool after,
+template <class T, bool LOADER, int BN, bool PAIR, bool RAGGED>
+npa_status launch_product_as(const CUtensorMap (&maps)[4], const Product& p, bool after,
                           cudaStream_t stream) {
   using C = linear_tc::Config<T, LOADER, BN, PAIR>;
-  const auto kernel = linear_tc::product_kernel<T, LOADER, BN, PAIR>;
+  const auto kernel = linear_tc::product_kernel<T, LOADER, BN, PAIR, RAGGED>;
   int per_sm = 0, sms = 0;
   NPA_TRY(kernel_occupancy(reinterpret_cast<const void*>(kernel), C::kThreads, C::kSmemBytes,
                            &per_sm, &sms));
@@ -595,6 +595,15 @@ npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, bool a
              "linear product_kernel");
   }
   return after_launch("linear product_kernel");
+}
+
+template <class T, bool LOADER, int BN, bool PAIR = false>
+npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, bool after,
+                          cudaStream_t stream) {
+  const bool whole = p.partials || (p.y_tma && (!p.z || p.z_tma) &&
+                                    (!p.residual || (p.residual_vec && p.n * sizeof(T) % 16 == 0)));
+  return whole ? launch_product_as<T, LOADER, BN, PAIR, false>(maps, p, after, stream)
+               : launch_product_as<T, LOADER, BN, PAIR, true>(maps, p, after, stream);
 }
 
 // Runs the product; p holds operands, sizes and the epilogue's buffers.

@@ -446,12 +446,12 @@ __device__ __forceinline__ void stage_values(uint32_t buf, int lane, const float
 }
 // The staged group to global memory: by TMA, or row by row where the output's
 // rows do not start on 16 bytes.
-template <class OUT>
+template <class OUT, bool RAGGED>
 __device__ __forceinline__ void put_group(uint32_t buf, int lane,
                                           const CUtensorMap* map, bool tma, int x, int y_tma_row,
                                           void* out, int64_t stride, int64_t row0, int rows,
                                           int cols) {
-  if (tma) {
+  if (!RAGGED || tma) {
     tc::fence_async_shared();
     __syncwarp();
     if (lane == 0) {
@@ -495,7 +495,10 @@ __device__ __forceinline__ void put_group(uint32_t buf, int lane,
   }
 }
 
-template <class T, bool LOADER, int BN, bool PAIR>
+// RAGGED: outputs or a residual whose rows do not start on 16 bytes.  The common
+// case does without that code: its size alone costs (1048576 x 64 x 128 bf16: 126
+// us with it, 117 without).
+template <class T, bool LOADER, int BN, bool PAIR, bool RAGGED>
 __global__ void __launch_bounds__((Config<T, LOADER, BN, PAIR>::kThreads), 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z,
@@ -853,7 +856,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // words i * 4 .. + 3 of the lane's columns lane and lane + 32 of half the
         // rows: with hardly any L1 beside the stages an access has to take all of
         // what it touches
-        const bool res_vec = p.residual_vec && cols * int(sizeof(T)) % 16 == 0;
+        const bool res_vec = !RAGGED || (p.residual_vec && cols * int(sizeof(T)) % 16 == 0);
         auto read_residual = [&](int i, int half_rows) -> uint4 {
           uint4 u = make_uint4(0, 0, 0, 0);
           if (res_vec) {
@@ -943,7 +946,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (h * 32 >= cols) break;
             const uint32_t b = next_buffer();
             stage_values<float>(b, lane, v, h * 32);
-            put_group<float>(b, lane, &map_y, true, col0 + h * 32, int(prow), nullptr,
+            put_group<float, false>(b, lane, &map_y, true, col0 + h * 32, int(prow), nullptr,
                              0, 0, 0, 0);
           }
           return;
@@ -967,7 +970,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (p.z) {
           const uint32_t b = next_buffer();
           stage_values<T>(b, lane, v, 0);
-          put_group<T>(b, lane, &map_z, p.z_tma, col0, int(row0), p.z, p.z_stride,
+          put_group<T, RAGGED>(b, lane, &map_z, p.z_tma, col0, int(row0), p.z, p.z_stride,
                        row0, rows, cols);
         }
         activate<sizeof(T) == 2>(p.act, v);
@@ -981,7 +984,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
           // 32 single values per lane are all of 32 f32 columns, and half of the
           // rows of 64 columns
-          if (kGroup == 64 && !res_vec) {
+          if (RAGGED && kGroup == 64 && !res_vec) {
             constexpr int kAt = 16;
             if constexpr (LOADER) {
               for (int i = 0; i < 8; ++i) stage_residual(b, i, kAt, read_residual(i, kAt));
@@ -1013,7 +1016,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
         }
         stage_values<T>(b, lane, v, 0);
-        put_group<T>(b, lane, &map_y, p.y_tma, col0, int(row0), p.y, p.y_stride, row0,
+        put_group<T, RAGGED>(b, lane, &map_y, p.y_tma, col0, int(row0), p.y, p.y_stride, row0,
                      rows, cols);
       };
 #pragma unroll
