@@ -19,12 +19,41 @@ using linear_tc::Operand;
 using linear_tc::Product;
 
 // ---- the split product's layers, summed in order, with the epilogue ----
-// A block has 32 groups of four columns; its eight warps each add every eighth
-// layer, and the first adds the eight sums in order.
+// Column sums that wait to be added: [count][outputs].
+struct BiasSums {
+  const float* partials;  // null: none
+  int count, outputs;
+  void* dbias;
+};
+// 32 outputs by a block; its eight warps each add every eighth partial in order.
 template <class T>
-__global__ void __launch_bounds__(256) product_reduce_kernel(const __grid_constant__ Product p) {
+__device__ __forceinline__ void reduce_bias(const BiasSums& b, int block) {
+  __shared__ float acc[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int col = block * 32 + tx;
+  float s = 0.0f;
+  if (col < b.outputs)
+#pragma unroll 8
+    for (int p = ty; p < b.count; p += 8) s += b.partials[int64_t(p) * b.outputs + col];
+  acc[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && col < b.outputs)
+    static_cast<T*>(b.dbias)[col] =
+        from_f32<T>(((acc[0][tx] + acc[1][tx]) + (acc[2][tx] + acc[3][tx])) +
+                    ((acc[4][tx] + acc[5][tx]) + (acc[6][tx] + acc[7][tx])));
+}
+// A block has 32 groups of four columns; its eight warps each add every eighth
+// layer, and the first adds the eight sums in order.  The blocks past `blocks`
+// add a bias gradient on the way: a launch less.
+template <class T>
+__global__ void __launch_bounds__(256) product_reduce_kernel(const __grid_constant__ Product p, int blocks,
+                                                             const __grid_constant__ BiasSums bias) {
   let_next_launch();
   wait_for_previous();
+  if (int(blockIdx.x) >= blocks) {
+    reduce_bias<T>(bias, int(blockIdx.x) - blocks);
+    return;
+  }
   __shared__ float4 sums[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t quads = (p.n + 3) / 4;
@@ -337,22 +366,24 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const __grid_constant__ S
   }
 }
 template <class T>
-__global__ void __launch_bounds__(256) bias_reduce_kernel(const float* __restrict__ partials,
-                                                          int count, int outputs, T* dbias) {
+__global__ void __launch_bounds__(256) bias_reduce_kernel(const __grid_constant__ BiasSums bias) {
   let_next_launch();
   wait_for_previous();
-  __shared__ float acc[8][32];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + tx;
-  float s = 0.0f;
-  if (col < outputs)
-#pragma unroll 8
-    for (int p = ty; p < count; p += 8) s += partials[int64_t(p) * outputs + col];
-  acc[ty][tx] = s;
-  __syncthreads();
-  if (ty == 0 && col < outputs)
-    dbias[col] = from_f32<T>(((acc[0][tx] + acc[1][tx]) + (acc[2][tx] + acc[3][tx])) +
-                             ((acc[4][tx] + acc[5][tx]) + (acc[6][tx] + acc[7][tx])));
+  reduce_bias<T>(bias, int(blockIdx.x));
+}
+template <class T>
+npa_status launch_bias_reduce(const BiasSums& b, cudaStream_t s) {
+  NPA_CUDA(launch_kernel(true, bias_reduce_kernel<T>, dim3(grid_for(b.outputs, 32)), 256, 0, s, b),
+           "bias_reduce_kernel");
+  return after_launch("bias_reduce_kernel");
+}
+template <class T>
+npa_status launch_product_reduce(const Product& p, const BiasSums& b, cudaStream_t s) {
+  const unsigned blocks = grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32);
+  const unsigned more = b.partials ? grid_for(b.outputs, 32) : 0;
+  NPA_CUDA(launch_kernel(true, product_reduce_kernel<T>, dim3(blocks + more), 256, 0, s, p, int(blocks), b),
+           "product_reduce_kernel");
+  return after_launch("product_reduce_kernel");
 }
 
 // ---- rows of odd widths, copied to rows that start on 16 bytes ----
@@ -606,9 +637,10 @@ npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, bool a
                : launch_product_as<T, LOADER, BN, PAIR, true>(maps, p, after, stream);
 }
 
-// Runs the product; p holds operands, sizes and the epilogue's buffers.
+// Runs the product; p holds operands, sizes and the epilogue's buffers.  A bias
+// gradient that waits is added behind it.
 template <class T>
-npa_status run_product(Product p, float* partials, bool after, cudaStream_t stream) {
+npa_status run_product(Product p, float* partials, bool after, BiasSums bias, cudaStream_t stream) {
   constexpr bool kSplitParts = sizeof(T) == 4;
   const int64_t a_rows = p.a.rows, b_rows = p.b.rows;
   const bool tma = !kSplitParts && tma_rows(p.a.p, p.a.ld, a_rows, sizeof(T)) &&
@@ -659,11 +691,8 @@ npa_status run_product(Product p, float* partials, bool after, cudaStream_t stre
     NPA_TRY(plan.bn == 128 ? (launch_product<T, true, 128>(maps, p, after, stream))
                            : (launch_product<T, true, 64>(maps, p, after, stream)));
   }
-  if (!p.partials) return NPA_OK;
-  NPA_CUDA(launch_kernel(true, product_reduce_kernel<T>,
-                         dim3(grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32)), 256, 0, stream, p),
-           "product_reduce_kernel");
-  return after_launch("product_reduce_kernel");
+  if (p.partials) return launch_product_reduce<T>(p, bias, stream);
+  return bias.partials ? launch_bias_reduce<T>(bias, stream) : NPA_OK;
 }
 
 // The one-walk backward pass's shape, or stage_bytes = 0 where it has none:
@@ -776,7 +805,7 @@ npa_status forward_typed(const LinearArgs& a, void* workspace, cudaStream_t s) {
     NPA_TRY(pack_rows<T>(p.a, ws.x, false, s));
     NPA_TRY(pack_rows<T>(p.b, ws.weight, true, s));
   }
-  return run_product<T>(p, ws.product_partials, ws.x != nullptr, s);
+  return run_product<T>(p, ws.product_partials, ws.x != nullptr, {}, s);
 }
 
 template <class T, bool RAGGED>
@@ -822,12 +851,8 @@ npa_status launch_fused(const LinearBackwardArgs& a, FusedBackward f, const Back
   kernel<<<unsigned(blocks), linear_tc::kFusedThreads, smem, s>>>(maps[0], maps[1], maps[2], maps[3],
                                                                   maps[4], f);
   NPA_TRY(after_launch("linear fused_backward_kernel"));
-  if (a.dbias) {
-    NPA_CUDA(launch_kernel(true, bias_reduce_kernel<T>, dim3(grid_for(a.outputs, 32)), 256, 0, s,
-                           ws.bias_partials, blocks, a.outputs, static_cast<T*>(a.dbias)),
-             "bias_reduce_kernel");
-    NPA_TRY(after_launch("bias_reduce_kernel"));
-  }
+  BiasSums bias{};
+  if (a.dbias) bias = {ws.bias_partials, blocks, a.outputs, a.dbias};
   if (a.dweight) {
     Product p{};
     p.m = a.outputs;
@@ -838,11 +863,9 @@ npa_status launch_fused(const LinearBackwardArgs& a, FusedBackward f, const Back
     p.partials = f.dw_partials;
     p.y = a.dweight;
     p.y_stride = a.inputs;
-    NPA_CUDA(launch_kernel(true, product_reduce_kernel<T>,
-                           dim3(grid_for(uint64_t(p.m) * ((p.n + 3) / 4), 32)), 256, 0, s, p),
-             "product_reduce_kernel");
-    NPA_TRY(after_launch("product_reduce_kernel"));
+    return launch_product_reduce<T>(p, bias, s);
   }
+  if (a.dbias) return launch_bias_reduce<T>(bias, s);
   return NPA_OK;
 }
 
@@ -882,6 +905,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
   int64_t dz_stride = a.dy_stride;
   int dz_width = a.outputs;
   bool after = false;  // a kernel of this call precedes
+  BiasSums bias{};     // waits for the last product
   // dz is written where it is not dy, and where dy's odd rows are worth copying:
   // by the pass that sums them for dbias, or for much work
   const bool write_dz =
@@ -907,12 +931,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     else
       NPA_TRY((launch_slope<T, true>(g, &parts, s)));
     after = true;
-    if (a.dbias) {
-      NPA_CUDA(launch_kernel(true, bias_reduce_kernel<T>, dim3(grid_for(a.outputs, 32)), 256, 0, s,
-                             ws.bias_partials, parts, a.outputs, static_cast<T*>(a.dbias)),
-               "bias_reduce_kernel");
-      NPA_TRY(after_launch("bias_reduce_kernel"));
-    }
+    if (a.dbias) bias = {ws.bias_partials, parts, a.outputs, a.dbias};
     if (g.dz) {
       dz = static_cast<const T*>(ws.dz);
       dz_stride = ws.dz_stride;
@@ -940,7 +959,7 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     p.k = a.outputs;
     p.y = a.dx;
     p.y_stride = a.dx_stride;
-    NPA_TRY(run_product<T>(p, ws.product_partials, after, s));
+    NPA_TRY(run_product<T>(p, ws.product_partials, after, a.dweight ? BiasSums{} : bias, s));
     after = true;
   }
   if (a.dweight) {
@@ -952,9 +971,9 @@ npa_status backward_typed(const LinearBackwardArgs& a, const BackwardCarve& ws, 
     p.k = int(a.rows);
     p.y = a.dweight;
     p.y_stride = a.inputs;
-    NPA_TRY(run_product<T>(p, ws.product_partials, after, s));
+    return run_product<T>(p, ws.product_partials, after, bias, s);
   }
-  return NPA_OK;
+  return !a.dx && bias.partials ? launch_bias_reduce<T>(bias, s) : NPA_OK;
 }
 
 }  // namespace
