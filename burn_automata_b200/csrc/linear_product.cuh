@@ -103,7 +103,7 @@ struct Config {
 // reciprocals by the approximate instructions, without the library's handling of
 // subnormal values, and erf by a short formula: errors of 2^-22 or so of the
 // largest term, which vanish in a result that is rounded to 8 or 11 bits.  f32
-// storage takes the library's functions.
+// storage takes the library's exp and erf.
 template <bool FAST>
 __device__ __forceinline__ float exponential(float x) {
   if (!FAST) return expf(x);
@@ -119,8 +119,12 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
 }
 template <bool FAST>
 __device__ __forceinline__ float logistic(float z) {
-  const float d = 1.0f + exponential<FAST>(-z);
-  return FAST ? fast_reciprocal(d) : 1.0f / d;
+  if (FAST) return fast_reciprocal(1.0f + exponential<true>(-z));
+  // one Newton step from the approximate reciprocal: within an ulp or two, at a
+  // fifth of the division's instructions.  d = 1e38 stands for all beyond.
+  const float d = fminf(1.0f + expf(-z), 1e38f);
+  const float r = fast_reciprocal(d);
+  return fmaf(r, fmaf(-d, r, 1.0f), r);
 }
 // The normal distribution function at z, with e = exp(-z^2 / 2): Abramowitz and
 // Stegun's 7.1.26, 1 - erf(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x),
@@ -144,9 +148,9 @@ __device__ __forceinline__ float activation(int act, float z) {
     case NPA_ACTIVATION_GELU_TANH: {
       // (1 + tanh(u)) / 2 = logistic(2u)
       const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-      return FAST ? z * logistic<true>(2.0f * u) : 0.5f * z * (1.0f + tanhf(u));
+      return z * logistic<FAST>(2.0f * u);
     }
-    case NPA_ACTIVATION_SILU: return FAST ? z * logistic<true>(z) : z / (1.0f + expf(-z));
+    case NPA_ACTIVATION_SILU: return z * logistic<FAST>(z);
     default: return z;
   }
 }
@@ -740,8 +744,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (LOADER) tc::fence_async_shared();  // the loaders' writes, ordered by the barrier
           tc::fence_after();
           const uint64_t a = a0 + at.slot * (C::kStageBytes >> 4), b = b0 + at.slot * (C::kStageBytes >> 4);
+          const int k_left = p.k - (kb + kt) * kBK;  // a last block may end early
 #pragma unroll
           for (int step = 0; step < kBK / 16; ++step) {
+            if (step * 16 >= k_left) break;
             const bool more = step > 0 || in_chunk > 0;
             const uint64_t as = a + step * a_step, bs = b + step * b_step;
             tc::mma_f16<PAIR>(d, as, bs, p.idesc, more);
