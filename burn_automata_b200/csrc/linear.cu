@@ -646,6 +646,8 @@ npa_status run_product(Product p, float* partials, bool after, BiasSums bias, cu
   const bool tma = !kSplitParts && tma_rows(p.a.p, p.a.ld, a_rows, sizeof(T)) &&
                    tma_rows(p.b.p, p.b.ld, b_rows, sizeof(T));
   const Plan plan = plan_product(sizeof(T), tma, p.m, p.n, p.k);
+  if (int64_t(plan.m_tiles) * plan.n_tiles * plan.splits >= int64_t(1) << 31)
+    return fail(NPA_ERR_UNSUPPORTED, "linear product of 2^31 tiles or more");
   p.m_tiles = plan.m_tiles;
   p.n_tiles = plan.n_tiles;
   p.k_blocks = plan.k_blocks;
@@ -663,7 +665,6 @@ npa_status run_product(Product p, float* partials, bool after, BiasSums bias, cu
                    p.b.width % kWhole == 0;
   p.y_tma = tma_rows(p.y, p.y_stride, p.m, sizeof(T));
   p.z_tma = p.z && tma_rows(p.z, p.z_stride, p.m, sizeof(T));
-  p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
   p.residual_vec = p.residual && tma_rows(p.residual, p.residual_stride, p.m, sizeof(T));
   CUtensorMap maps[4] = {};
   if (tma) {

@@ -141,45 +141,44 @@ fused_backward_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_c
         }
     }
   } else if (warp == kMma) {
-    if (lane == 0) {
-      RingCursor at{f.stages};
-      Cursor<2> acc;
-      if (f.want_dx) ok = tc::bar_wait(weights_full, 0);
-      bool first = true;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, at.advance()) {
-        ok = tc::bar_wait(ready + 8 * at.slot, at.parity);
+    const uint32_t issue = tc::elected();
+    RingCursor at{f.stages};
+    Cursor<2> acc;
+    if (f.want_dx) ok = __all_sync(0xffffffffu, tc::bar_wait(weights_full, 0));
+    bool first = true;
+    for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, at.advance()) {
+      ok = __all_sync(0xffffffffu, tc::bar_wait(ready + 8 * at.slot, at.parity));
+      if (!ok) break;
+      tc::fence_after();
+      const uint32_t dz = base + at.slot * f.stage_bytes, x = dz + x_off;
+      if (f.want_dx) {
+        ok = __all_sync(0xffffffffu, tc::bar_wait(acc_empty + 8 * acc.slot, acc.parity ^ 1));
         if (!ok) break;
         tc::fence_after();
-        const uint32_t dz = base + at.slot * f.stage_bytes, x = dz + x_off;
-        if (f.want_dx) {
-          ok = tc::bar_wait(acc_empty + 8 * acc.slot, acc.parity ^ 1);
-          if (!ok) break;
-          tc::fence_after();
-          const uint64_t a0 = tc::operand_desc(dz, false, 0);
-          const uint64_t b0 = tc::operand_desc(weights, true, f.k_pad * 128);
-          for (int k = 0; k < f.k_pad / 16; ++k)
-            tc::mma_f16(tmem_dx + acc.slot * f.n_pad, a0 + ((k / 4 * kBlockBytes + k % 4 * 32) >> 4),
-                        b0 + (k * 2048 >> 4), f.dx_idesc, k > 0);
-          tc::mma_commit(acc_full + 8 * acc.slot);
-          acc.advance();
-        }
-        if (f.want_dw) {
-          const uint64_t b0 = tc::operand_desc(x, true, kBlockBytes);
-          for (int m = 0; m < f.m_blocks; ++m) {
-            const uint64_t a0 = tc::operand_desc(dz + m * 2 * kBlockBytes, true, kBlockBytes);
-#pragma unroll
-            for (int k = 0; k < kBM / 16; ++k)
-              tc::mma_f16(tmem + m * f.n_pad, a0 + (k * 2048 >> 4), b0 + (k * 2048 >> 4), f.dw_idesc,
-                          !first || k > 0);
-          }
-        }
-        first = false;
-        tc::mma_commit(empty + 8 * at.slot);
+        const uint64_t a0 = tc::operand_desc(dz, false, 0);
+        const uint64_t b0 = tc::operand_desc(weights, true, f.k_pad * 128);
+        for (int k = 0; k < f.k_pad / 16; ++k)
+          tc::mma_f16(tmem_dx + acc.slot * f.n_pad, a0 + ((k / 4 * kBlockBytes + k % 4 * 32) >> 4),
+                      b0 + (k * 2048 >> 4), f.dx_idesc, k > 0, issue);
+        tc::mma_commit(acc_full + 8 * acc.slot, issue);
+        acc.advance();
       }
-      // dW is whole (and nothing is in flight) when this completes
-      tc::mma_commit(dw_done);
-      if (!tc::bar_wait(dw_done, 0)) ok = false;
+      if (f.want_dw) {
+        const uint64_t b0 = tc::operand_desc(x, true, kBlockBytes);
+        for (int m = 0; m < f.m_blocks; ++m) {
+          const uint64_t a0 = tc::operand_desc(dz + m * 2 * kBlockBytes, true, kBlockBytes);
+#pragma unroll
+          for (int k = 0; k < kBM / 16; ++k)
+            tc::mma_f16(tmem + m * f.n_pad, a0 + (k * 2048 >> 4), b0 + (k * 2048 >> 4), f.dw_idesc,
+                        !first || k > 0, issue);
+        }
+      }
+      first = false;
+      tc::mma_commit(empty + 8 * at.slot, issue);
     }
+    // dW is whole (and nothing is in flight) when this completes
+    tc::mma_commit(dw_done, issue);
+    if (!__all_sync(0xffffffffu, tc::bar_wait(dw_done, 0))) ok = false;
   } else if (warp >= kFirstSlope) {
     // dz in place of dy, and the columns' sums: a thread keeps eight columns
     const int tid = threadIdx.x - kFirstSlope * 32;

@@ -70,7 +70,7 @@ struct Product {
   float* partials;  // split: [splits][layer_rows][partial_pitch], else null
   int64_t layer_rows, partial_pitch;
   int act;
-  int y_tma, z_tma, bias_vec, residual_vec;
+  int y_tma, z_tma, residual_vec;
 };
 
 __device__ unsigned long long g_timeouts = 0;  // bounded waits that gave up
@@ -89,13 +89,13 @@ struct Config {
   // written while TMA reads the last.
   static constexpr int kOutBuffers = (BN == 256 && !PAIR) || kParts == 3 ? 1 : 2;
   static constexpr int kOutBytes = kEpilogueWarps * kOutBuffers * 4096;
-  static constexpr int kStagesFit = (kSmemLimit - kOutBytes - 2048) / kStageBytes;
+  static constexpr int kStagesFit = (kSmemLimit - kOutBytes - 2048 - 256) / kStageBytes;
   static constexpr int kStages = kStagesFit > 6 ? 6 : kStagesFit;
   static constexpr int kBufferColumns = BN * (kParts == 3 ? 2 : 1);
   static constexpr int kTmemColumns = 2 * kBufferColumns;
   // epilogue warps, a warpgroup with the issuing and the TMA warp, loader warps
   static constexpr int kThreads = 32 * (kEpilogueWarps + 4 + (LOADER ? kLoaderWarps : 0));
-  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kOutBytes + 1024 + 256;
+  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kOutBytes + 2048 + 256;
   static_assert(kStages >= 2 && kTmemColumns <= 512, "tile does not fit");
 };
 
@@ -515,7 +515,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const uint32_t raw = tc::smem_addr(smem_raw);
   const uint32_t base = (raw + 1023) & ~1023u;  // the swizzle repeats every 1,024 bytes
   const uint32_t out_base = base + C::kStages * C::kStageBytes;
-  const uint32_t bars = out_base + C::kOutBytes;
+  const uint32_t bias_base = out_base + C::kOutBytes;  // 128 bytes per epilogue warp
+  const uint32_t bars = bias_base + kEpilogueWarps * 128;
   const uint32_t full = bars, empty = bars + 8 * C::kStages;
   const uint32_t acc_full = empty + 8 * C::kStages, acc_empty = acc_full + 16;
   const uint32_t drain = acc_empty + 16, tmem_at = drain + 8;
@@ -524,10 +525,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   constexpr int kFirstLoader = kEpilogueWarps + 4;
   // a pair walks the tiles together
   const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
-  const int64_t walker = PAIR ? blockIdx.x / 2 : blockIdx.x;
-  const int64_t walkers = PAIR ? gridDim.x / 2 : gridDim.x;
-  const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles * p.splits;
-  const int64_t layer = int64_t(p.m_tiles) * p.n_tiles;
+  const uint32_t walker = PAIR ? blockIdx.x / 2 : blockIdx.x;
+  const uint32_t walkers = PAIR ? gridDim.x / 2 : gridDim.x;
+  const uint32_t layer = uint32_t(p.m_tiles) * p.n_tiles;  // the host keeps tiles below 2^31
+  const uint32_t tiles = layer * p.splits;
 
   let_next_launch();
   if (warp == kMmaWarp) {
@@ -573,8 +574,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         Cursor<C::kStages> at;
         uint32_t issued = 0;
         const uint32_t first_full = PAIR ? tc::in_first_block(full) : full;
-        for (int64_t t = walker; t < tiles && ok; t += walkers) {
-          const int split = int(t / layer), in = int(t % layer);
+        for (uint32_t t = walker; t < tiles && ok; t += walkers) {
+          const int split = p.splits > 1 ? int(t / layer) : 0, in = int(t - split * layer);
           const int m0 = in / p.n_tiles * C::kTileRows + int(rank) * kBM;
           const int n0 = in % p.n_tiles * BN + int(rank) * C::kBRows;
           const int kb = split * p.split_blocks;
@@ -632,7 +633,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         Cursor<C::kStages> at;
         Chunk<T> ca[kAChunks], cb[kBChunks];
         Reader ra, rb;
-        int64_t t = walker;
+        uint32_t t = walker;
         int blocks_left = 0;
         auto enter_tile = [&]() {
           const int split = p.splits > 1 ? int(t / layer) : 0, in = int(t - split * layer);
@@ -717,59 +718,65 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       }
     }
   } else if (warp == kMmaWarp) {
-    // ---- the thread that issues the products (the pair's first block's) ----
+    // ---- the warp that issues the products (the pair's first block's) ----
     if constexpr (LOADER) tc::registers_down<40>();
-    if (lane == 0 && rank == 0) {
-      // One thread issues everything, so its own instructions between two
-      // blocks of k count: cursors step by one and descriptors by additions.
+    if (rank == 0) {
+      // One lane issues everything, so what lies between two blocks of k counts:
+      // the warp runs whole, cursors step by one and descriptors by additions.
+      const uint32_t issue = tc::elected();
       Cursor<C::kStages> at;
       Cursor<2> acc;
       const uint32_t a_step = (p.a.mn_major ? 2048 : 32) >> 4, b_step = (p.b.mn_major ? 2048 : 32) >> 4;
       const uint64_t a0 = tc::operand_desc(base, p.a.mn_major, 8192);
       const uint64_t b0 = tc::operand_desc(base + C::kParts * C::kABytes, p.b.mn_major, 8192);
-      for (int64_t t = walker; t < tiles && ok; t += walkers) {
+      for (uint32_t t = walker; t < tiles && ok; t += walkers) {
         const int split = p.splits > 1 ? int(t / layer) : 0;
         const int kb = split * p.split_blocks;
         const int blocks = min(p.k_blocks, kb + p.split_blocks) - kb;
+        // a last block may end early: steps past k's end are left out
+        const int last_steps = min(kBK / 16, (p.k - (kb + blocks - 1) * kBK + 15) / 16);
         uint32_t d = 0;
         int in_chunk = 0;
         for (int kt = 0; kt < blocks; ++kt, at.advance()) {
           if (in_chunk == 0) {
-            ok = tc::bar_wait<PAIR>(acc_empty + 8 * acc.slot, acc.parity ^ 1);
+            ok = __all_sync(0xffffffffu, tc::bar_wait<PAIR>(acc_empty + 8 * acc.slot, acc.parity ^ 1));
             if (!ok) break;
             d = tmem + acc.slot * C::kBufferColumns;
           }
-          ok = tc::bar_wait(full + 8 * at.slot, at.parity);
+          ok = __all_sync(0xffffffffu, tc::bar_wait(full + 8 * at.slot, at.parity));
           if (!ok) break;
           if (LOADER) tc::fence_async_shared();  // the loaders' writes, ordered by the barrier
           tc::fence_after();
           const uint64_t a = a0 + at.slot * (C::kStageBytes >> 4), b = b0 + at.slot * (C::kStageBytes >> 4);
-          const int k_left = p.k - (kb + kt) * kBK;  // a last block may end early
-#pragma unroll
-          for (int step = 0; step < kBK / 16; ++step) {
-            if (step * 16 >= k_left) break;
+          auto products = [&](int step) {
             const bool more = step > 0 || in_chunk > 0;
             const uint64_t as = a + step * a_step, bs = b + step * b_step;
-            tc::mma_f16<PAIR>(d, as, bs, p.idesc, more);
+            tc::mma_f16<PAIR>(d, as, bs, p.idesc, more, issue);
             if constexpr (C::kParts == 3) {
               constexpr int kA[5] = {0, 1, 1, 0, 2}, kB[5] = {1, 0, 1, 2, 0};
 #pragma unroll
               for (int j = 0; j < 5; ++j)
                 tc::mma_f16<PAIR>(d + BN, as + kA[j] * (C::kABytes >> 4), bs + kB[j] * (C::kBBytes >> 4),
-                                  p.idesc, more || j > 0);
+                                  p.idesc, more || j > 0, issue);
             }
+          };
+          if (kt + 1 < blocks || last_steps == kBK / 16) {
+#pragma unroll
+            for (int step = 0; step < kBK / 16; ++step) products(step);
+          } else {
+            for (int step = 0; step < last_steps; ++step) products(step);
           }
-          tc::mma_commit<PAIR>(empty + 8 * at.slot);
+          tc::mma_commit<PAIR>(empty + 8 * at.slot, issue);
           ++in_chunk;
           if (kt + 1 == blocks || (C::kParts == 3 && in_chunk == kChunkBlocks)) {
-            tc::mma_commit<PAIR>(acc_full + 8 * acc.slot);
+            tc::mma_commit<PAIR>(acc_full + 8 * acc.slot, issue);
             acc.advance();
             in_chunk = 0;
           }
         }
       }
       if (!ok) {  // products in flight must end before TMEM is freed
-        tc::mma_commit<PAIR>(drain);
+        tc::mma_commit<PAIR>(drain, issue);
         tc::bar_wait(drain, 0);
       }
     }
@@ -799,8 +806,24 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         tc::bar_arrive(acc_empty + 8 * buf);
     };
     auto pointer = [&](uint32_t b) -> char* { return smem_raw + (b - raw); };
-    for (int64_t t = walker; t < tiles && ok; t += walkers) {
-      const int split = int(t / layer), in = int(t % layer);
+    T* const bias_row = reinterpret_cast<T*>(pointer(bias_base + warp * 128));
+    // The bias of the next group, a value or two per lane, loaded a group ahead:
+    // there is hardly any L1 beside the stages, so even what all rows share comes
+    // from L2 each time, 600 cycles away and more.
+    T bias_values[kGroup / 32];
+    auto prefetch_bias = [&](uint32_t tile, int gi) {
+      if (!p.bias || p.partials || tile >= tiles) return;
+      const int in = int(p.splits > 1 ? tile % layer : tile);
+      const int col0 = in % p.n_tiles * BN + (half + 2 * gi) * kGroup;
+#pragma unroll
+      for (int h = 0; h < kGroup / 32; ++h) {
+        const int c = col0 + lane + 32 * h;
+        bias_values[h] = c < p.n ? static_cast<const T*>(p.bias)[c] : T(0.0f);
+      }
+    };
+    prefetch_bias(walker, 0);
+    for (uint32_t t = walker; t < tiles && ok; t += walkers) {
+      const int split = p.splits > 1 ? int(t / layer) : 0, in = int(t - split * layer);
       const int m_tile = in / p.n_tiles;
       const int64_t row0 = int64_t(m_tile) * C::kTileRows + rank * kBM + quarter * 32;
       const int n0 = in % p.n_tiles * BN;
@@ -808,6 +831,50 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       const int rows = rows_left >= 32 ? 32 : rows_left > 0 ? int(rows_left) : 0;
       float sums[C::kParts == 3 ? kGroupsPerWarp : 1][kGroup];
       uint32_t d = 0;
+      // The TMA kernels ask for the residual before the wait for the accumulators
+      // (the first group) or before they read them; the loader kernels' register
+      // budget (five warps to an SM quarter) has no room for it.
+      uint4 res[LOADER ? 1 : 8];
+      // 16 bytes of row i * 4 + lane / 8; or, where rows do not start on 16 bytes,
+      // words i * 4 .. + 3 of the lane's columns lane and lane + 32 of half the
+      // rows: an access has to take all of what it touches
+      auto residual_at = [&](int col0, int cols, int i, int half_rows) -> uint4 {
+        const bool res_vec = !RAGGED || (p.residual_vec && cols * int(sizeof(T)) % 16 == 0);
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (res_vec) {
+          const int rr = i * 4 + (lane >> 3), c = (lane & 7) * (16 / int(sizeof(T)));
+          if (rr < rows && c < cols)
+            u = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) +
+                                                (row0 + rr) * p.residual_stride + col0 + c);
+          return u;
+        }
+        constexpr int kAcross = kGroup / 32;
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int rr = half_rows + (i * 4 + q) / kAcross, c = lane + 32 * ((i * 4 + q) % kAcross);
+          w[q] = 0;
+          if (rr < rows && c < cols) {
+            const T* const r = static_cast<const T*>(p.residual) + (row0 + rr) * p.residual_stride + col0 + c;
+            if constexpr (sizeof(T) == 4)
+              w[q] = *reinterpret_cast<const uint32_t*>(r);
+            else
+              w[q] = *reinterpret_cast<const uint16_t*>(r);
+          }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+      };
+      auto prefetch = [&](int gi) {
+        const int g = half + 2 * gi, col0 = n0 + g * kGroup, cols = min(kGroup, p.n - col0);
+        if (g >= kGroups || col0 >= p.n || rows <= 0 || p.partials) return;
+        if constexpr (!LOADER) {
+          if (p.residual) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) res[i] = residual_at(col0, cols, i, 0);
+          }
+        }
+      };
+      prefetch(0);
       if constexpr (C::kParts == 3) {
         const int kb = split * p.split_blocks;
         const int blocks = min(p.k_blocks, kb + p.split_blocks) - kb;
@@ -854,40 +921,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const bool last = gi + 1 == kGroupsPerWarp;
         const bool mine = g < kGroups && col0 < p.n && rows > 0;
         const int cols = min(kGroup, p.n - col0);
-        // the TMA kernel loads the residual before it reads the accumulators, so
-        // that the loads' latency passes under them; the loader kernel's register
-        // budget (five warps to an SM quarter) has no room for it
-        uint4 res[LOADER ? 1 : 8];
-        // 16 bytes of row i * 4 + lane / 8; or, where rows do not start on 16 bytes,
-        // words i * 4 .. + 3 of the lane's columns lane and lane + 32 of half the
-        // rows: with hardly any L1 beside the stages an access has to take all of
-        // what it touches
         const bool res_vec = !RAGGED || (p.residual_vec && cols * int(sizeof(T)) % 16 == 0);
-        auto read_residual = [&](int i, int half_rows) -> uint4 {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (res_vec) {
-            const int rr = i * 4 + (lane >> 3), c = (lane & 7) * (16 / int(sizeof(T)));
-            if (rr < rows && c < cols)
-              u = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) +
-                                                  (row0 + rr) * p.residual_stride + col0 + c);
-            return u;
-          }
-          constexpr int kAcross = kGroup / 32;
-          uint32_t w[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int rr = half_rows + (i * 4 + q) / kAcross, c = lane + 32 * ((i * 4 + q) % kAcross);
-            w[q] = 0;
-            if (rr < rows && c < cols) {
-              const T* const r = static_cast<const T*>(p.residual) + (row0 + rr) * p.residual_stride + col0 + c;
-              if constexpr (sizeof(T) == 4)
-                w[q] = *reinterpret_cast<const uint32_t*>(r);
-              else
-                w[q] = *reinterpret_cast<const uint16_t*>(r);
-            }
-          }
-          return make_uint4(w[0], w[1], w[2], w[3]);
-        };
+        auto read_residual = [&](int i, int half_rows) { return residual_at(col0, cols, i, half_rows); };
         auto stage_residual = [&](uint32_t b, int i, int half_rows, uint4 u) {
           if (res_vec) {
             store_shared16(b + swizzled(i * 4 + (lane >> 3), lane & 7), u);
@@ -906,12 +941,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                            : "memory");
           }
         };
-        if constexpr (!LOADER) {
-          if (mine && !p.partials && p.residual) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) res[i] = read_residual(i, 0);
-          }
-        }
+        if (gi > 0) prefetch(gi);
         if constexpr (C::kParts == 3) {
           bool odd = false;
 #pragma unroll
@@ -944,7 +974,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             acc.advance();
           }
         }
-        if (!mine) return;
+        if (!mine) {
+          if (last) prefetch_bias(t + walkers, 0);
+          return;
+        }
         if (p.partials) {
           const int64_t prow = split * p.layer_rows + row0;
 #pragma unroll
@@ -958,19 +991,21 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           return;
         }
         if (p.bias) {
-          const T* const bias = static_cast<const T*>(p.bias) + col0;
-          constexpr int kPer = 16 / int(sizeof(T));
-          if (p.bias_vec && cols == kGroup) {
+          // through shared memory to all lanes: each has a row of its own
+          __syncwarp();
 #pragma unroll
-            for (int i = 0; i < kGroup; i += kPer) {
-              const Pack<T, kPer> b = *reinterpret_cast<const Pack<T, kPer>*>(bias + i);
+          for (int h = 0; h < kGroup / 32; ++h) bias_row[lane + 32 * h] = bias_values[h];
+          __syncwarp();
+          if (last)
+            prefetch_bias(t + walkers, 0);
+          else
+            prefetch_bias(t, gi + 1);
 #pragma unroll
-              for (int j = 0; j < kPer; ++j) v[i + j] += to_f32(b.v[j]);
-            }
-          } else {
+          for (int c = 0; c < 8; ++c) {
+            constexpr int kPer = 16 / int(sizeof(T));
+            const Pack<T, kPer> b = reinterpret_cast<const Pack<T, kPer>*>(bias_row)[c];
 #pragma unroll
-            for (int i = 0; i < kGroup; ++i)
-              if (i < cols) v[i] += to_f32(bias[i]);
+            for (int j = 0; j < kPer; ++j) v[c * kPer + j] += to_f32(b.v[j]);
           }
         }
         if (p.z) {

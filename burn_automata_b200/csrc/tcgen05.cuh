@@ -154,37 +154,51 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
-// Arrives on the barrier (of both blocks of a pair) when this thread's earlier
-// tensor-core work is done.
+// One lane of a converged warp.  The instructions below take their operands
+// from uniform registers: a warp that runs them whole, masked to this lane,
+// keeps its addresses there, where a single thread's branch would move every one
+// of them over for each instruction.
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t is;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(is));
+  return is;
+}
+// Arrives on the barrier (of both blocks of a pair) when the issuing thread's
+// earlier tensor-core work is done.
 template <bool PAIR = false>
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t issue) {
   if (PAIR)
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-        "[%0], %1;\n" ::"r"(bar),
-        "h"(uint16_t(3))
+        "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+        " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;\n}\n" ::"r"(bar),
+        "h"(uint16_t(3)), "r"(issue)
         : "memory");
   else
     asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+        "r"(issue)
         : "memory");
 }
 // d (TMEM, f32) = a b (+ d when accumulate): 16-bit operands in shared memory.
 // PAIR: both blocks hold half of a's rows, half of b's rows and half of d.
 template <bool PAIR = false>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                        bool accumulate) {
+                                        bool accumulate, uint32_t issue) {
   if (PAIR)
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(issue)
         : "memory");
   else
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(issue)
         : "memory");
 }
 // Accumulator columns of this warp's 32 TMEM lanes, one row per thread.  The
