@@ -565,7 +565,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   wait_for_previous();
 
   // The loader kernel's 640 threads start with 96 registers each; its control
-  // warpgroup leaves some to the others: 40 + 2 x 96 + 2 x 120 = 472 of the
+  // warpgroup leaves some to the others: 56 + 2 x 96 + 2 x 112 = 472 of the
   // launch's 480 per thread of each warpgroup.
   if (warp > kMmaWarp) {
     // ---- producers ----
@@ -622,9 +622,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       }
     } else {
       if (warp < kFirstLoader) {
-        tc::registers_down<40>();
+        tc::registers_down<56>();
       } else {
-        tc::registers_up<120>();
+        tc::registers_up<112>();
         // A thread has up to 32 registers of A's tile and of B's, loaded a stage
         // ahead of their use.
         const int tid = threadIdx.x - kFirstLoader * 32;
@@ -719,7 +719,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
   } else if (warp == kMmaWarp) {
     // ---- the warp that issues the products (the pair's first block's) ----
-    if constexpr (LOADER) tc::registers_down<40>();
+    if constexpr (LOADER) tc::registers_down<56>();
     if (rank == 0) {
       // One lane issues everything, so what lies between two blocks of k counts:
       // the warp runs whole, cursors step by one and descriptors by additions.
@@ -807,8 +807,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     };
     auto pointer = [&](uint32_t b) -> char* { return smem_raw + (b - raw); };
     T* const bias_row = reinterpret_cast<T*>(pointer(bias_base + warp * 128));
-    // The bias of the next group, a value or two per lane, loaded a group ahead:
-    // there is hardly any L1 beside the stages, so even what all rows share comes
+    // The bias of the next group, a value or two per lane, loaded a group ahead in
+    // the TMA kernels: there is hardly any L1 beside the stages, so even what all rows share comes
     // from L2 each time, 600 cycles away and more.
     T bias_values[kGroup / 32];
     auto prefetch_bias = [&](uint32_t tile, int gi) {
@@ -821,7 +821,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         bias_values[h] = c < p.n ? static_cast<const T*>(p.bias)[c] : T(0.0f);
       }
     };
-    prefetch_bias(walker, 0);
+    if (!LOADER) prefetch_bias(walker, 0);
     for (uint32_t t = walker; t < tiles && ok; t += walkers) {
       const int split = p.splits > 1 ? int(t / layer) : 0, in = int(t - split * layer);
       const int m_tile = in / p.n_tiles;
@@ -942,6 +942,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
         };
         if (gi > 0) prefetch(gi);
+        if (LOADER) prefetch_bias(t, gi);
         if constexpr (C::kParts == 3) {
           bool odd = false;
 #pragma unroll
@@ -975,7 +976,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
         }
         if (!mine) {
-          if (last) prefetch_bias(t + walkers, 0);
+          if (!LOADER && last) prefetch_bias(t + walkers, 0);
           return;
         }
         if (p.partials) {
@@ -996,10 +997,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
           for (int h = 0; h < kGroup / 32; ++h) bias_row[lane + 32 * h] = bias_values[h];
           __syncwarp();
-          if (last)
-            prefetch_bias(t + walkers, 0);
-          else
-            prefetch_bias(t, gi + 1);
+          if (!LOADER) prefetch_bias(last ? t + walkers : t, last ? 0 : gi + 1);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             constexpr int kPer = 16 / int(sizeof(T));
