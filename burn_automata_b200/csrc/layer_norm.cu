@@ -28,7 +28,7 @@
 //    past what registers hold.
 //
 // Measured on one B200, beside a copy's 6.45 TB/s: forward 1048576 x 130 f32
-// 180 us (6.1 TB/s); backward with a residual 1048576 x 130 bf16 209 us (5.3
+// 178 us (6.1 TB/s); backward with a residual 1048576 x 130 bf16 209 us (5.3
 // TB/s, instruction issue at 70 %), 16384 x 4096 f16 83 us (4.8 TB/s); the plain
 // loads of unaligned rows reach about a quarter (52529 x 1599 f16, odd pitch:
 // 400 us), bound by their two-byte accesses.
@@ -1029,7 +1029,7 @@ struct TilePlan {
 };
 // slot_of(tile_rows): bytes of one ring slot.
 template <class F>
-TilePlan plan_tiles(size_t size, int dims, int64_t rows, int most_blocks, F&& slot_of) {
+TilePlan plan_tiles(size_t size, int dims, int64_t rows, int most_blocks, bool deep, F&& slot_of) {
   TilePlan p{};
   int vec = 16 / int(size);
   while (dims % vec) vec /= 2;
@@ -1042,8 +1042,10 @@ TilePlan plan_tiles(size_t size, int dims, int64_t rows, int most_blocks, F&& sl
   // (885704 x 8 bf16 backward: 61 us with tiles of 128 bytes).
   int whole = 8;
   while (whole < 64 && size_t(dims) * size * whole < 2048 && rows / (2 * whole) >= 148 * 16) whole *= 2;
-  for (int tile_rows : {whole, 4}) {
-    if (tile_rows == 4 && (size_t(dims) * size * 4 % 16 || row.tpr < 8)) break;
+  const int most_stages = deep ? 5 : 4;
+  const bool four_first = deep && size_t(dims) * size * 4 >= 2048;
+  for (int tile_rows : {four_first ? 4 : whole, four_first ? whole : 4}) {
+    if (tile_rows == 4 && (size_t(dims) * size * 4 % 16 || row.tpr < 8)) continue;
     const size_t slot = slot_of(tile_rows);
     // few tiles: fewer warps to a block, so that every SM has some
     const int64_t tiles = (rows + tile_rows - 1) / tile_rows;
@@ -1051,7 +1053,7 @@ TilePlan plan_tiles(size_t size, int dims, int64_t rows, int most_blocks, F&& sl
     while (warps > 1 && tiles < int64_t(warps) * 148) warps /= 2;
     for (int blocks = most_blocks * (8 / warps); blocks >= 1; --blocks) {
       const int stages =
-          int(std::min<size_t>(4, kSmemPerSm / blocks / (size_t(warps) * (slot + 8) + 128)));
+          int(std::min<size_t>(most_stages, kSmemPerSm / blocks / (size_t(warps) * (slot + 8) + 128)));
       if (stages < 2) continue;
       if (p.row.nv && blocks < most_blocks) break;  // eight rows fit as well as four
       p.smem = ((size_t(warps) * stages * 8 + 127) & ~size_t(127)) + size_t(warps) * stages * slot;
@@ -1109,7 +1111,14 @@ npa_status wide_grid(K kernel, const WidePlan& p, int64_t rows, unsigned* grid) 
 template <class T>
 npa_status forward_typed(const LayerNormArgs& a, cudaStream_t s) {
   if (gapless(a.x, a.x_stride, a.rows, a.dims) && gapless(a.y, a.y_stride, a.rows, a.dims)) {
-    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, 2, [&](int tile_rows) {
+    // f32 rows of 256 to 576 bytes keep five tiles to a ring, of four rows from 2 KB
+    // on (536 MB of x, us before and with it: 64 values 207, 168; 128 197, 178; 130
+    // 203, 173; 136 204, 165; 144 202, 194; 68 193, 198).  Elsewhere this loses: 32
+    // f32 values 208, 256; 192 186, 194; 64 16-bit values 213, 262; 129, an odd
+    // width, 169, 192.
+    const size_t row_bytes = size_t(a.dims) * sizeof(T);
+    const bool deep = sizeof(T) == 4 && a.dims % 2 == 0 && row_bytes >= 256 && row_bytes <= 576;
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, 2, deep, [&](int tile_rows) {
       return (size_t(a.dims) * tile_rows * sizeof(T) + 127) & ~size_t(127);
     });
     if (p.row.nv)
@@ -1166,7 +1175,7 @@ npa_status backward_rows(const LayerNormBackwardArgs& a, int* parts, cudaStream_
     int vec = 16 / int(sizeof(T));
     while (a.dims % vec) vec /= 2;
     const int blocks = backward_blocks(vec * plan_lanes(a.dims, vec).nv);
-    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, blocks, [&](int tile_rows) {
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, blocks, false, [&](int tile_rows) {
       return backward_slot(uint32_t(a.dims * tile_rows * sizeof(T)), a.residual != nullptr, tile_rows);
     });
     if (p.row.nv)

@@ -90,6 +90,13 @@ def test_layer_norm(rows, dims, pitch, offset, dtype):
     close(out.rstd, rstd[:, 0], e * rstd[:, 0] * (1 + size[:, 0]), "rstd")
 
 
+@pytest.mark.parametrize("dims", [62, 64, 128, 130, 144, 146])
+def test_layer_norm_rings_of_every_depth(dims):
+    """f32 widths on both sides of the forward ring's choices of tile and depth;
+    enough rows that a ring turns, and a last tile that is not whole."""
+    test_layer_norm(75779, dims, 0, 0, next(k for k, v in TYPES.items() if v == torch.float32))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("rows,dims,pitch,offset", NORMS)
 def test_layer_norm_backward(rows, dims, pitch, offset, dtype):
