@@ -11,8 +11,9 @@
 // (outputs x rows, k across lines) for dW, so it is written once.  dW stays in
 // TMEM over all tiles of the block; the blocks' sums meet in
 // product_reduce_kernel in a fixed order.
-// 1048576 rows of a 64 -> 128 relu layer in bf16: 140 us, 5.7 TB/s (separate
-// passes for dz, dx and dW take 131 + 67 + 63).
+// 1048576 rows of a 64 -> 128 relu layer in bf16: 139 us, 5.8 TB/s; the
+// whole call, with the sums' kernel, 152 (separate passes for dz, dx and dW
+// take 131 + 67 + 63).
 #pragma once
 
 #include "linear_product.cuh"

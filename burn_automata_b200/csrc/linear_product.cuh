@@ -21,14 +21,17 @@
 // f32 sums in registers.  An infinite value has no such parts (its rest is
 // NaN): outputs that come out NaN are recomputed from their rows.
 //
-// Measured on one B200.  bf16 8192 x 4096 x 4096 in pairs' tiles: 197 us, the
-// library's product 184; with the tanh gelu and a residual 213, and 250 back to
-// back, where the power limit lowers the clock (a bound of shared memory: a k
-// block's 512 cycles of products move 64 KB of operands in and out of it).  With
+// Measured on one B200.  bf16 8192 x 4096 x 4096 in pairs' tiles: 170 us, the
+// library's product 180; with the tanh gelu and a residual 185, and 220 back to
+// back, where the power limit lowers the clock (tensor pipe 81 % busy).  With
 // little k the epilogue and DRAM bound: 1048576 x 64 x 128 with relu and the
-// pre-activation kept takes 119 us, 5.6 TB/s.  f32 8192 x 4096 x 4096 takes 1.5
-// ms, 181 TFLOP/s (the library's f32 product 54), bound by 24 products of 128
-// columns per k block at 112 cycles each.
+// pre-activation kept takes 116 us, 5.8 TB/s.  f32 8192 x 4096 x 4096 takes 1.5
+// ms, 180 TFLOP/s (the library's f32 product 54): a k block's 24 products of 128
+// columns and the loader warps' splits of its values take about as long.
+//
+// The issuing warp runs whole and one lane's products are let through: with
+// loop state and descriptors in uniform registers a k block costs it few
+// instructions.  A branch to one thread instead took 222 us for the first shape.
 #pragma once
 
 #include "layers.h"
@@ -808,8 +811,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     auto pointer = [&](uint32_t b) -> char* { return smem_raw + (b - raw); };
     T* const bias_row = reinterpret_cast<T*>(pointer(bias_base + warp * 128));
     // The bias of the next group, a value or two per lane, loaded a group ahead in
-    // the TMA kernels: there is hardly any L1 beside the stages, so even what all rows share comes
-    // from L2 each time, 600 cycles away and more.
+    // the TMA kernels: there is hardly any L1 beside the stages, so even what all
+    // rows share comes from L2 each time, 600 cycles away and more.  The loader
+    // kernels read it in place: their epilogue warps have no registers for it
+    // (858187 x 64 x 48 f32: 102 us, 118 ahead).
     T bias_values[kGroup / 32];
     auto prefetch_bias = [&](uint32_t tile, int gi) {
       if (!p.bias || p.partials || tile >= tiles) return;

@@ -158,7 +158,8 @@ uint64_t npa_kernel_launch_count(void);
 /* Diagnostic: feature-tile bulk copies of the MLP step kernel, and feature-tile
  * hand-overs of the warp-specialised step, that did not complete within their
  * bounded wait on the current device (0 in a healthy run; a block that gives
- * up leaves its remaining tiles undone).  The
+ * up leaves its remaining tiles undone).  The waits of the layer norm and
+ * linear kernels count here too.  The
  * synchronising host calls (npa_model_step, npa_model_run_rollout*,
  * npa_executor_read_state) return NPA_ERR_TIMEOUT when this device's count
  * has grown since the last such check on the device. */
@@ -533,7 +534,8 @@ npa_status npa_dev_model_step(npa_model* model, const npa_grid_config* grid,
  * passed.  Every matrix and vector of a call has the storage type `dtype`;
  * sums, statistics and products are held in 32 bits and results are rounded
  * once.  NULL leaves an optional buffer out.  Outputs must not overlap inputs
- * or each other.  rows = 0 is valid (gradients over rows are then zero).
+ * or each other.  A workspace starts on 256 bytes and serves calls that follow
+ * each other on a stream.  rows = 0 is valid (gradients over rows are then zero).
  * Results do not depend on timing: no sum goes through atomics. */
 enum { NPA_DTYPE_F32 = 0, NPA_DTYPE_F16 = 1, NPA_DTYPE_BF16 = 2 };
 
