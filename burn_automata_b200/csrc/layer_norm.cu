@@ -28,8 +28,8 @@
 //    past what registers hold.
 //
 // Measured on one B200, beside a copy's 6.45 TB/s: forward 1048576 x 130 f32
-// 178 us (6.1 TB/s); backward with a residual 1048576 x 130 bf16 209 us (5.3
-// TB/s, instruction issue at 70 %), 16384 x 4096 f16 83 us (4.8 TB/s); the plain
+// 178 us (6.1 TB/s; 194 on inputs that change from call to call); backward with a
+// residual 1048576 x 130 bf16 209 us (5.3 TB/s, instruction issue at 70 %), 16384 x 4096 f16 83 us (4.8 TB/s); the plain
 // loads of unaligned rows reach about a quarter (52529 x 1599 f16, odd pitch:
 // 400 us), bound by their two-byte accesses.
 #include <algorithm>
