@@ -1,0 +1,102 @@
+"""Layer norm and the linear layer where values, lengths and addresses are out
+of the ordinary: infinities and NaN over long sums, sums of many thousand terms
+of one sign, activations far out on their tails, views that start anywhere.
+
+The tolerances are those of test_layers_gpu.py unless a test derives its own.
+"""
+
+import pytest
+
+import burn_automata_b200 as ba
+from burn_automata_b200 import Activation
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+INF, NAN = float("inf"), float("nan")
+
+
+def normal(shape, dtype, seed, scale=1.0, shift=0.0):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    return torch.empty(shape, device="cuda").normal_(shift, scale, generator=gen).to(dtype)
+
+
+def uniform(shape, dtype, seed, low, high):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    return torch.empty(shape, device="cuda").uniform_(low, high, generator=gen).to(dtype)
+
+
+def waits_that_gave_up():
+    torch.cuda.synchronize()
+    return ba.load_library().npa_bulk_copy_timeouts()
+
+
+# ------------------------------------------------- infinities and NaN in f32
+def test_f32_weight_gradient_of_a_diverged_step():
+    """Every gradient NaN, or infinite, over a long sum: the same walk as for
+    finite values, with no wait that gives up."""
+    rows, inputs, outputs = 300000, 640, 520
+    x, w = normal((rows, inputs), F32, 1), normal((outputs, inputs), F32, 2, 0.05)
+    before = waits_that_gave_up()
+    for value in (NAN, INF, -INF):
+        dy = torch.full((rows, outputs), value, device="cuda")
+        g = ba.linear_backward(dy, x, w)
+        # x and w have both signs: infinities of both signs meet in every sum
+        assert bool(g.weight.isnan().all()) and bool(g.x.isnan().all())
+        assert bool(g.bias.isnan().all()) if value != value else bool((g.bias == value).all())
+    assert waits_that_gave_up() == before
+
+
+def test_f32_infinities_at_the_end_of_a_long_sum():
+    rows, inputs, outputs = 200003, 96, 72
+    x, w = normal((rows, inputs), F32, 1), normal((outputs, inputs), F32, 2, 0.1)
+    dy = normal((rows, outputs), F32, 3)
+    dy = torch.where(dy == 0, torch.ones_like(dy), dy)
+    clean = ba.linear_backward(dy, x, w).weight
+    x[-1, 3] = INF                      # one infinite term: its sign
+    x[-2, 7], x[5, 7] = INF, NAN        # a NaN wins
+    x[1000, 11], x[-7, 11] = INF, -INF  # sign by the gradients' signs, NaN where they meet
+    dy[-1, 9] = 0.0                     # an infinity times zero
+    got = ba.linear_backward(dy, x, w).weight
+    assert torch.equal(got[:9, 3], dy[-1, :9] * INF) and torch.equal(got[10:, 3], dy[-1, 10:] * INF)
+    assert bool(got[9, 3].isnan())
+    assert bool(got[:, 7].isnan().all())
+    want = dy[1000] * INF + dy[-7] * -INF
+    assert torch.equal(got[:, 11].isnan(), want.isnan())
+    assert torch.equal(got[:, 11].nan_to_num(0.0, INF, -INF), want.nan_to_num(0.0, INF, -INF))
+    other = [c for c in range(inputs) if c not in (3, 7, 11)]
+    keep = [r for r in range(outputs) if r != 9]
+    assert torch.equal(got[keep][:, other], clean[keep][:, other])
+
+
+@pytest.mark.parametrize("rows", [200, 3000])
+@pytest.mark.parametrize("inputs", [16, 97, 1000])
+def test_f32_infinities_and_nan_where_64_bits_have_them(rows, inputs):
+    """Against 64-bit products, entry by entry; a payload in a NaN's low bits
+    alone, which a cut to 16 bits would lose, among them."""
+    x, w = normal((rows, inputs), F32, 1), normal((40, inputs), F32, 2, 0.2)
+    w[3] = 1.0  # whole in 16 bits: nothing is left for its second and third part
+    w[5, 4], w[6, 4] = 0.0, INF
+    x[1, 4], x[2, 4], x[4, inputs - 1] = INF, -INF, NAN
+    x[7, 2], x[7, 9] = INF, -INF
+    x.view(torch.int32)[9, 3] = 0x7F800001
+    x.view(torch.int32)[10, 3] = 0x7F800001 - (1 << 31)
+    got, ref = ba.linear(x, w).y.double(), x.double() @ w.double().t()
+    ref[9:11] = NAN
+    assert torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got.isinf() & (got > 0), ref.isinf() & (ref > 0))
+    assert torch.equal(got.isinf() & (got < 0), ref.isinf() & (ref < 0))
+
+
+def test_f32_largest_values():
+    """Values up to the largest f32 stay finite where their products are."""
+    x, w = torch.zeros((150, 64), device="cuda"), torch.zeros((40, 64), device="cuda")
+    top = torch.finfo(F32).max
+    x[:, 5], w[:, 5] = top, 0.5
+    x[3, 5], w[7, 5] = -top, -1.0
+    ref = x.double() @ w.double().t()
+    got = ba.linear(x, w).y.double()
+    assert bool(((got - ref).abs() <= 2.0 ** -22 * ref.abs()).all())
