@@ -433,7 +433,7 @@ bool packs(size_t size, int width, int64_t rows, int inputs, int outputs) {
 }
 
 // ---- host side ----
-constexpr int kSms = 148;             // the plans' block count: B200's SMs
+constexpr int kSms = linear_tc::kMaxBlocks;  // the plans' block count
 // Blocks of slope_kernel at most: the three to an SM that its registers allow, in
 // one wave (16384 x 4096 f16 silu: 88 us; 119 with four, which take a second wave).
 constexpr int kBiasBlocks = 3 * kSms;
@@ -502,6 +502,11 @@ struct Plan {
   size_t partial_bytes() const {
     return splits > 1 ? size_t(splits) * layer_rows * partial_pitch * 4 : 0;
   }
+  // f32 operands keep their sums in registers
+  size_t running_bytes(size_t size) const {
+    return size == 2 && split_blocks > linear_tc::kLongBlocks ? linear_tc::running_bytes(bn) : 0;
+  }
+  size_t bytes(size_t size) const { return partial_bytes() + running_bytes(size); }
 };
 Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
   Plan p{};
@@ -549,8 +554,8 @@ Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
   return p;
 }
 size_t product_workspace(size_t size, int64_t m, int64_t n, int64_t k) {
-  return std::max(plan_product(size, true, m, n, k).partial_bytes(),
-                  plan_product(size, false, m, n, k).partial_bytes());
+  return std::max(plan_product(size, true, m, n, k).bytes(size),
+                  plan_product(size, false, m, n, k).bytes(size));
 }
 
 template <class T>
@@ -592,11 +597,11 @@ npa_status pair_blocks(K kernel, int threads, size_t smem, int sms, int* blocks)
   return NPA_OK;
 }
 
-template <class T, bool LOADER, int BN, bool PAIR, bool RAGGED>
+template <class T, bool LOADER, int BN, bool PAIR, linear_tc::Form FORM>
 npa_status launch_product_as(const CUtensorMap (&maps)[4], const Product& p, bool after,
                           cudaStream_t stream) {
   using C = linear_tc::Config<T, LOADER, BN, PAIR>;
-  const auto kernel = linear_tc::product_kernel<T, LOADER, BN, PAIR, RAGGED>;
+  const auto kernel = linear_tc::product_kernel<T, LOADER, BN, PAIR, FORM>;
   int per_sm = 0, sms = 0;
   NPA_TRY(kernel_occupancy(reinterpret_cast<const void*>(kernel), C::kThreads, C::kSmemBytes,
                            &per_sm, &sms));
@@ -606,7 +611,7 @@ npa_status launch_product_as(const CUtensorMap (&maps)[4], const Product& p, boo
     int blocks = 0;
     NPA_TRY(pair_blocks(kernel, C::kThreads, C::kSmemBytes, sms, &blocks));
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(unsigned(std::min<int64_t>(2 * tiles, blocks)));
+    config.gridDim = dim3(unsigned(std::min<int64_t>({2 * tiles, blocks, kSms})));
     config.blockDim = dim3(C::kThreads);
     config.dynamicSmemBytes = C::kSmemBytes;
     config.stream = stream;
@@ -621,7 +626,7 @@ npa_status launch_product_as(const CUtensorMap (&maps)[4], const Product& p, boo
     NPA_CUDA(cudaLaunchKernelEx(&config, kernel, maps[0], maps[1], maps[2], maps[3], p),
              "linear product_kernel");
   } else {
-    NPA_CUDA(launch_kernel(after, kernel, dim3(unsigned(std::min<int64_t>(tiles, sms))), C::kThreads,
+    NPA_CUDA(launch_kernel(after, kernel, dim3(unsigned(std::min<int64_t>({tiles, sms, kSms}))), C::kThreads,
                            C::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], p),
              "linear product_kernel");
   }
@@ -631,10 +636,13 @@ npa_status launch_product_as(const CUtensorMap (&maps)[4], const Product& p, boo
 template <class T, bool LOADER, int BN, bool PAIR = false>
 npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, bool after,
                           cudaStream_t stream) {
+  using linear_tc::kLong, linear_tc::kRagged, linear_tc::kWhole;
+  if constexpr (sizeof(T) == 2)
+    if (p.running) return launch_product_as<T, LOADER, BN, PAIR, kLong>(maps, p, after, stream);
   const bool whole = p.partials || (p.y_tma && (!p.z || p.z_tma) &&
                                     (!p.residual || (p.residual_vec && p.n * sizeof(T) % 16 == 0)));
-  return whole ? launch_product_as<T, LOADER, BN, PAIR, false>(maps, p, after, stream)
-               : launch_product_as<T, LOADER, BN, PAIR, true>(maps, p, after, stream);
+  return whole ? launch_product_as<T, LOADER, BN, PAIR, kWhole>(maps, p, after, stream)
+               : launch_product_as<T, LOADER, BN, PAIR, kRagged>(maps, p, after, stream);
 }
 
 // Runs the product; p holds operands, sizes and the epilogue's buffers.  A bias
@@ -656,6 +664,9 @@ npa_status run_product(Product p, float* partials, bool after, BiasSums bias, cu
   p.layer_rows = plan.layer_rows;
   p.partial_pitch = plan.partial_pitch;
   p.partials = plan.splits > 1 ? partials : nullptr;
+  p.running = plan.running_bytes(sizeof(T))
+                  ? reinterpret_cast<float4*>(partials + plan.partial_bytes() / 4)
+                  : nullptr;
   p.idesc = tc::instruction_desc(!std::is_same<T, __half>::value, p.a.mn_major, p.b.mn_major,
                                  plan.pair ? 2 * linear_tc::kBM : linear_tc::kBM, plan.bn);
   p.a_vec = vector_width<T>(p.a.p, p.a.ld, a_rows);

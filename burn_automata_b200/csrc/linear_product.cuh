@@ -24,6 +24,14 @@
 // first part is zero, gives NaN.)  Such values cost no time: a backward pass of
 // 16384 x 1024 x 1024 takes 434 us, and 425 with every gradient NaN.
 //
+// 16-bit operands sum all of a tile's k in TMEM up to 128 blocks of k, 512
+// accumulating steps.  Terms of one sign lose 1.1e-7 of their sum at each
+// (measured with f16 over 65,536 to 1,048,576 values of k), so 512 steps stay
+// below 2^-14, an eighth of f16's rounding.  A longer k moves its sums every
+// 128 blocks to rounded f32 ones in the workspace, each in the thread that
+// finishes it, under the next blocks' products: unmoved, a weight gradient over
+// 1,048,576 rows came out 0.7 % low.
+//
 // Measured on one B200.  bf16 8192 x 4096 x 4096 in pairs' tiles: 170 us, the
 // library's product 180; with the tanh gelu and a residual 185, and 220 back to
 // back, where the power limit lowers the clock (tensor pipe 81 % busy).  With
@@ -48,6 +56,8 @@ constexpr int kBK = 64;                  // k values per stage: one 128-byte swi
 constexpr int kEpilogueWarps = 8;        // two per 32 TMEM lanes
 constexpr int kLoaderWarps = 8;
 constexpr int kChunkBlocks = 4;          // k blocks between f32 moves out of TMEM
+constexpr int kLongBlocks = 128;         // the same for 16-bit operands
+constexpr int kMaxBlocks = 148;          // of a launch: B200's SMs
 constexpr int kSmemLimit = 227 * 1024;
 
 // One operand: value (i, k) at i * ld + k, or at k * ld + i when MN-major.
@@ -74,10 +84,17 @@ struct Product {
   void* z;
   int64_t z_stride;
   float* partials;  // split: [splits][layer_rows][partial_pitch], else null
+  float4* running;  // long k: each thread's sums, running_bytes() of them
   int64_t layer_rows, partial_pitch;
   int act;
   int y_tma, z_tma, residual_vec;
 };
+
+// The sums of a launch with tiles of bn columns: an epilogue thread's 64 columns
+// of every second group.
+constexpr size_t running_bytes(int bn) {
+  return size_t(kMaxBlocks) * ((bn + 127) / 128) * kEpilogueWarps * 32 * 64 * sizeof(float);
+}
 
 __device__ unsigned long long g_timeouts = 0;  // bounded waits that gave up
 
@@ -503,15 +520,19 @@ __device__ __forceinline__ void put_group(uint32_t buf, int lane,
   }
 }
 
-// RAGGED: outputs or a residual whose rows do not start on 16 bytes.  The common
-// case does without that code: its size alone costs (1048576 x 64 x 128 bf16: 126
-// us with it, 117 without).
-template <class T, bool LOADER, int BN, bool PAIR, bool RAGGED>
+// kRagged: outputs or a residual whose rows do not start on 16 bytes.  kLong: the
+// same, and more than kLongBlocks of k (16-bit operands).  The common case does
+// without that code: its size alone costs (1048576 x 64 x 128 bf16: 126 us with
+// the ragged epilogue, 117 without; 607399 x 48 -> 179: 269 us with the long
+// k's sums, 259 without).
+enum Form { kWhole, kRagged, kLong };
+template <class T, bool LOADER, int BN, bool PAIR, Form FORM>
 __global__ void __launch_bounds__((Config<T, LOADER, BN, PAIR>::kThreads), 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z,
                const __grid_constant__ Product p) {
   using C = Config<T, LOADER, BN, PAIR>;
+  constexpr bool RAGGED = FORM != kWhole, LONG = FORM == kLong;
   constexpr int kGroup = 128 / int(sizeof(T));         // output columns staged at a time
   constexpr int kGroups = BN / kGroup;
   constexpr int kGroupsPerWarp = (kGroups + 1) / 2;
@@ -772,7 +793,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
           tc::mma_commit<PAIR>(empty + 8 * at.slot, issue);
           ++in_chunk;
-          if (kt + 1 == blocks || (C::kParts == 3 && in_chunk == kChunkBlocks)) {
+          constexpr int kMoved = C::kParts == 3 ? kChunkBlocks : LONG ? kLongBlocks : 0;
+          if (kt + 1 == blocks || (kMoved > 0 && in_chunk == kMoved)) {
             tc::mma_commit<PAIR>(acc_full + 8 * acc.slot, issue);
             acc.advance();
             in_chunk = 0;
@@ -809,6 +831,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       else
         tc::bar_arrive(acc_empty + 8 * buf);
     };
+    // four of this thread's sums in p.running: a warp's lie side by side
+    [[maybe_unused]] auto running_at = [&](int gi, int quad) -> float4* {
+      return p.running + ((blockIdx.x * kGroupsPerWarp + gi) * (kGroup / 4) + quad) * (kEpilogueWarps * 32) +
+             warp * 32 + lane;
+    };
     auto pointer = [&](uint32_t b) -> char* { return smem_raw + (b - raw); };
     T* const bias_row = reinterpret_cast<T*>(pointer(bias_base + warp * 128));
     // The bias of the next group, a value or two per lane, loaded a group ahead in
@@ -837,6 +864,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       const int rows = rows_left >= 32 ? 32 : rows_left > 0 ? int(rows_left) : 0;
       float sums[C::kParts == 3 ? kGroupsPerWarp : 1][kGroup];
       uint32_t d = 0;
+      [[maybe_unused]] bool moved = false;  // sums of earlier blocks of k are in p.running
       // The TMA kernels ask for the residual before the wait for the accumulators
       // (the first group) or before they read them; the loader kernels' register
       // budget (five warps to an SM quarter) has no room for it.
@@ -930,6 +958,38 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         if (!ok) break;
       } else {
+        if constexpr (LONG) {
+          const int kb = split * p.split_blocks;
+          for (int left = min(p.k_blocks, kb + p.split_blocks) - kb; left > kLongBlocks;
+               left -= kLongBlocks, acc.advance()) {
+            ok = __all_sync(0xffffffffu, tc::bar_wait(acc_full + 8 * acc.slot, acc.parity));
+            if (!ok) break;
+            tc::fence_after();
+#pragma unroll
+            for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
+              const int g = half + 2 * gi;
+              if (g >= kGroups || n0 + g * kGroup >= p.n) continue;
+#pragma unroll
+              for (int h = 0; h < kGroup; h += 16) {
+                float part[16];
+                tc::tmem_load(tmem + acc.slot * C::kBufferColumns + lanes + g * kGroup + h, part);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  float4* const at = running_at(gi, h / 4 + q);
+                  float4 f = moved ? *at : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                  f.x += part[4 * q];
+                  f.y += part[4 * q + 1];
+                  f.z += part[4 * q + 2];
+                  f.w += part[4 * q + 3];
+                  *at = f;
+                }
+              }
+            }
+            release_accumulators(acc.slot);
+            moved = true;
+          }
+          if (!ok) break;
+        }
         const uint32_t buf = acc.slot;
         ok = tc::bar_wait(acc_full + 8 * buf, acc.parity);
         ok = __all_sync(0xffffffffu, ok);
@@ -971,6 +1031,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (last) {
             release_accumulators(acc.slot);
             acc.advance();
+          }
+          if constexpr (LONG) {
+            if (mine && moved) {
+#pragma unroll
+              for (int q = 0; q < kGroup / 4; ++q) {
+                // not all loads at once: there are no registers for them
+                if (q % (LOADER ? 2 : 8) == 0) asm volatile("" ::: "memory");
+                const float4 f = *running_at(gi, q);
+                v[4 * q] += f.x;
+                v[4 * q + 1] += f.y;
+                v[4 * q + 2] += f.z;
+                v[4 * q + 3] += f.w;
+              }
+            }
           }
         }
         if (!mine) {

@@ -100,3 +100,48 @@ def test_f32_largest_values():
     ref = x.double() @ w.double().t()
     got = ba.linear(x, w).y.double()
     assert bool(((got - ref).abs() <= 2.0 ** -22 * ref.abs()).all())
+
+
+# ------------------------------------------- long sums of terms of one sign
+def one_sign_error(k):
+    """What a 16-bit product's sum of k terms of one sign may lose, relative to
+    their sum: 512 accumulating steps of the tensor core with a unit of 2^-23
+    each, and the f32 sum of the parts."""
+    return 2.0 ** -14 + (k / 4096) ** 0.5 * 2.0 ** -24
+
+
+LONG = [  # rows, inputs, outputs: products whose k (the rows) is split or not
+    (131149, 2048, 1280),  # pairs' tiles, k in one piece
+    (262144, 1024, 512),   # pairs' tiles, split k
+    (1000003, 9, 7),       # odd widths: loader warps
+    (700001, 264, 24),     # one narrow tile, split k
+    (70000, 1000, 2056),   # ragged tiles
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("rows,inputs,outputs", LONG)
+def test_weight_gradient_of_many_rows_of_one_sign(rows, inputs, outputs, dtype):
+    top = (40000.0 / rows) ** 0.5  # the sums stay inside f16
+    x = uniform((rows, inputs), dtype, 1, top / 2, top)
+    dy = uniform((rows, outputs), dtype, 2, top / 2, top)
+    w = torch.zeros((outputs, inputs), dtype=dtype, device="cuda")
+    got = ba.linear_backward(dy, x, w, needs=("weight",)).weight.double()
+    ref = dy.double().t() @ x.double()
+    unit = 2.0 ** -11 if dtype == F16 else 2.0 ** -8
+    assert float(((got - ref).abs() / ref).max()) <= unit + one_sign_error(rows)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("rows,inputs,outputs", [(2048, 9000, 4096), (2100, 4160, 4099), (300, 40008, 136),
+                                                 (1000, 4097, 40)])
+def test_linear_of_many_inputs_of_one_sign(rows, inputs, outputs, dtype):
+    """The same over many inputs, with the whole epilogue behind it."""
+    top = (2000.0 / inputs) ** 0.5
+    x, w = uniform((rows, inputs), dtype, 1, top / 2, top), uniform((outputs, inputs), dtype, 2, top / 2, top)
+    b, res = uniform((outputs,), dtype, 3, 1, 2), uniform((rows, outputs), dtype, 4, 1, 2)
+    out = ba.linear(x, w, b, residual=res, activation=Activation.Relu, save_pre_activation=True)
+    z = x.double() @ w.double().t() + b.double()
+    unit = 2.0 ** -11 if dtype == F16 else 2.0 ** -8
+    for got, ref in ((out.pre_activation, z), (out.y, z + res.double())):
+        assert float(((got.double() - ref).abs() / ref).max()) <= unit + one_sign_error(inputs)
