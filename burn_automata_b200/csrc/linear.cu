@@ -732,8 +732,13 @@ FusedBackward plan_fused(size_t size, int activation, int64_t rows, int inputs, 
     if (linear_tc::fused_fits(f)) return f;
   return FusedBackward{};
 }
+// A block for each SM, or several one after another where a block would walk more
+// than kFusedTiles tiles: dW's accumulator takes a step for every 16 rows (each
+// start costs about 7 us: 1300000 x 64 x 128 186 us, 174 in one walk whose sums
+// would lose up to 6e-5 of them).
 int fused_blocks(const FusedBackward& f) {
-  return int(std::min<int64_t>(kSms, (f.rows + linear_tc::kBM - 1) / linear_tc::kBM));
+  const int64_t tiles = (f.rows + linear_tc::kBM - 1) / linear_tc::kBM, a_wave = kSms * linear_tc::kFusedTiles;
+  return int(std::min<int64_t>(tiles, kSms * ((tiles + a_wave - 1) / a_wave)));
 }
 size_t fused_partial_bytes(const FusedBackward& f) {
   return f.stage_bytes ? size_t(fused_blocks(f)) * f.m_blocks * linear_tc::kBM * f.pitch * 4 : 0;
@@ -761,10 +766,11 @@ BackwardCarve carve_backward(void* ws, int dtype, int activation, int64_t rows, 
     b.x = c.take<char>(size_t(rows) * pitch * size);
     b.weight = c.take<char>(size_t(outputs) * pitch * size);
   }
-  b.bias_partials = c.take<float>(size_t(kBiasBlocks) * outputs);
+  const FusedBackward fused = plan_fused(size, activation, rows, inputs, outputs);
+  b.bias_partials = c.take<float>(size_t(std::max(kBiasBlocks, fused.stage_bytes ? fused_blocks(fused) : 0)) * outputs);
   size_t partial = std::max(product_workspace(size, rows, inputs, outputs),
                                   product_workspace(size, outputs, inputs, rows));
-  partial = std::max(partial, fused_partial_bytes(plan_fused(size, activation, rows, inputs, outputs)));
+  partial = std::max(partial, fused_partial_bytes(fused));
   b.product_partials = c.take<float>(partial / 4);
   b.bytes = c.used;
   return b;

@@ -23,6 +23,9 @@ namespace linear_tc {
 
 constexpr int kFusedThreads = 512;     // 4 dx warps, 4 control, 8 for dz
 constexpr int kFusedStages = 2;  // at most
+// Tiles to a block at most: 512 accumulating steps of dW, as long as any sum
+// stays in one accumulator (terms of one sign lose 1.1e-7 of it at each).
+constexpr int kFusedTiles = kLongBlocks * kBK / kBM;
 
 // A position in a ring of `slots` slots and the parity of its current phase.
 struct RingCursor {

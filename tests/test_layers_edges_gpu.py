@@ -145,3 +145,21 @@ def test_linear_of_many_inputs_of_one_sign(rows, inputs, outputs, dtype):
     unit = 2.0 ** -11 if dtype == F16 else 2.0 ** -8
     for got, ref in ((out.pre_activation, z), (out.y, z + res.double())):
         assert float(((got.double() - ref).abs() / ref).max()) <= unit + one_sign_error(inputs)
+
+
+def test_one_walk_backward_of_many_rows_of_one_sign():
+    """Few weights and so many rows that a block's walk over them has to end
+    more than once."""
+    rows, inputs, outputs = 20000003, 16, 8
+    top = (40000.0 / rows) ** 0.5
+    x = uniform((rows, inputs), F16, 1, top / 2, top)
+    dy = uniform((rows, outputs), F16, 2, top / 2, top)
+    w = normal((outputs, inputs), F16, 3)
+    g = ba.linear_backward(dy, x, w)
+    ref = dy.double().t() @ x.double()
+    assert float(((g.weight.double() - ref).abs() / ref).max()) <= 2.0 ** -11 + one_sign_error(rows)
+    assert bool(g.bias.isinf().all())  # 670,000: beyond f16
+    some = slice(0, rows, 99991)
+    ref = dy[some].double() @ w.double()
+    size = dy[some].double().abs() @ w.double().abs()
+    assert bool(((g.x[some].double() - ref).abs() <= 2.0 ** -11 * ref.abs() + 2.0 ** -20 * size + 2.0 ** -24).all())
