@@ -14,7 +14,7 @@ from .kernels import (DevicePerception, Gaussian3d, HashGridSnapshot, Perception
                       perceive_adjoint_with_options, perceive_state_adjoint_with_options,
                       perceive_with_options, splat_particles_2d)
 from .layers import (LayerNormGradients, LayerNormOutput, LinearGradients, LinearOutput,
-                     layer_norm, layer_norm_backward, linear, linear_backward)
+                     check_layer_waits, layer_norm, layer_norm_backward, linear, linear_backward)
 from .model import (CudaAutomataExecutor, NpaModel, NpaWeights, RolloutConfig, RolloutTrace,
                     StepOutput, rollout_update_masks, run_rollout_from_particles)
 from .update_network import UpdateBlock, UpdateNetwork
@@ -29,7 +29,7 @@ __all__ = [
     "perceive_with_options", "CudaAutomataExecutor", "NpaModel", "NpaWeights", "RolloutConfig",
     "RolloutTrace", "StepOutput", "rollout_update_masks", "run_rollout_from_particles",
     "Activation", "LayerNormGradients", "LayerNormOutput", "LinearGradients", "LinearOutput",
-    "layer_norm", "layer_norm_backward", "linear", "linear_backward", "UpdateBlock",
+    "check_layer_waits", "layer_norm", "layer_norm_backward", "linear", "linear_backward", "UpdateBlock",
     "UpdateNetwork",
     "build_library", "load_library",
 ]

@@ -163,6 +163,7 @@ SIGNATURES = [
     ("npa_dev_linear_backward", c_i32,
      [c_i32, c_i32, vp, c_i64, vp, c_i64, vp, c_i64, vp, c_i64, c_i64, c_i64, c_i64, vp, c_i64,
       vp, vp, vp, ctypes.c_size_t, vp]),
+    ("npa_dev_check_layer_waits", c_i32, [vp]),
     ("npa_executor_create", c_i32, [vp, P(GridConfigC), c_i64, c_i64, P(vp)]),
     ("npa_executor_destroy", None, [vp]),
     ("npa_executor_upload_state", c_i32, [vp, f32p, f32p]),

@@ -17,6 +17,7 @@
 #include <string>
 #include <vector>
 
+#include "host_state.h"
 #include "layers.h"
 
 namespace npa {
@@ -866,16 +867,11 @@ npa_status npa_model_forward_update_from_features(npa_model* m, const float* fea
 // device: NPA_ERR_TIMEOUT when that device's count of feature-tile copies that
 // missed their bounded wait has grown since the last check on that device
 // (those blocks left their tiles undone).  One watermark per device ordinal.
-static std::mutex g_bulk_mu;
-static std::vector<uint64_t> g_bulk_timeouts_seen;
+static Watermarks g_bulk_timeouts_seen;
 static npa_status check_bulk_copies() {
   int dev = 0;
   NPA_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
-  const uint64_t now = bulk_copy_timeouts() + ws_step_timeouts();
-  std::lock_guard<std::mutex> lock(g_bulk_mu);
-  if (dev >= int(g_bulk_timeouts_seen.size())) g_bulk_timeouts_seen.resize(dev + 1, 0);
-  if (now <= g_bulk_timeouts_seen[dev]) return NPA_OK;
-  g_bulk_timeouts_seen[dev] = now;
+  if (!g_bulk_timeouts_seen.grown(dev, bulk_copy_timeouts() + ws_step_timeouts())) return NPA_OK;
   return fail(NPA_ERR_TIMEOUT,
               "a bounded wait of the step kernels (an MLP feature-tile copy or a feature-tile "
               "hand-over) gave up");

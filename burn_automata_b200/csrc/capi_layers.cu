@@ -3,6 +3,7 @@
 #include <cmath>
 #include <new>
 
+#include "host_state.h"
 #include "layers.h"
 
 using namespace npa;
@@ -78,6 +79,8 @@ npa_status guarded(F&& body) {
     return NPA_ERR_INVALID_ARGUMENT;
   }
 }
+
+Watermarks g_layer_timeouts_seen;
 
 npa_status check_norm_shape(int32_t dtype, int64_t rows, int64_t dims) {
   NPA_TRY(check_dtype(dtype));
@@ -243,6 +246,18 @@ npa_status npa_dev_linear_backward(int32_t dtype, int32_t activation, const void
                                rows, int(inputs), int(outputs), d_dx, dx_stride, d_dweight,
                                d_dbias, activation};
     return launch_linear_backward(dtype, a, d_workspace, static_cast<cudaStream_t>(stream));
+  });
+}
+
+npa_status npa_dev_check_layer_waits(void* stream) {
+  return guarded([&]() -> npa_status {
+    int dev = 0;
+    NPA_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+    NPA_CUDA(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)), "cudaStreamSynchronize");
+    if (!g_layer_timeouts_seen.grown(dev, layer_norm_timeouts() + linear_timeouts())) return NPA_OK;
+    return fail(NPA_ERR_TIMEOUT,
+                "a bounded wait of the layer norm or linear kernels gave up; outputs of calls since the "
+                "last check may be unwritten");
   });
 }
 

@@ -242,6 +242,20 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, residual_gradient=None,
     return LayerNormGradients(dx, dw, db)
 
 
+def check_layer_waits(device=None) -> None:
+    """Waits for the device's current stream and raises DeviceTimeout if a bounded
+    wait of the kernels behind this module's calls has given up on the device
+    since the last such check: the calls return before their kernels run, and a
+    kernel that gives up leaves outputs unwritten.  Once for a training step or a
+    batch of requests."""
+    torch = _torch or _t()
+    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    with torch.cuda.device(index):
+        status = _lib.lib().npa_dev_check_layer_waits(
+            _raw_stream(torch.cuda.current_device()))
+    _lib.check(status, "check_layer_waits")
+
+
 def _activation(activation) -> int:
     if type(activation) is not Activation:
         try:

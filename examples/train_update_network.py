@@ -60,6 +60,7 @@ def train(particles: int = 4096, steps: int = 60, dtype=torch.bfloat16, hidden: 
         # the gradient of the summed squares per particle, averaged over particles
         dy = (error * (2.0 / particles)).to(dtype)
         _, _, gradients = net.backward(dy, saved)
+        ba.check_layer_waits()  # a step whose kernels gave up must not reach the weights
         net.sgd_step(gradients, learning_rate)
         if log and (step % 10 == 0 or step + 1 == steps):
             log(f"step {step:4d}  mean squared error {losses[-1]:.5f}")

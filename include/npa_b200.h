@@ -155,14 +155,14 @@ const char* npa_last_error_message(void);
 /* Number of kernels this library has launched in this process (all devices). */
 uint64_t npa_kernel_launch_count(void);
 
-/* Diagnostic: feature-tile bulk copies of the MLP step kernel, and feature-tile
- * hand-overs of the warp-specialised step, that did not complete within their
- * bounded wait on the current device (0 in a healthy run; a block that gives
- * up leaves its remaining tiles undone).  The waits of the layer norm and
- * linear kernels count here too.  The
- * synchronising host calls (npa_model_step, npa_model_run_rollout*,
- * npa_executor_read_state) return NPA_ERR_TIMEOUT when this device's count
- * has grown since the last such check on the device. */
+/* Diagnostic: bounded waits that gave up on the current device (0 in a healthy
+ * run; a block that gives up leaves its remaining tiles undone).  It counts the
+ * feature-tile bulk copies of the MLP step kernel and the feature-tile
+ * hand-overs of the warp-specialised step, which the synchronising host calls
+ * (npa_model_step, npa_model_run_rollout*, npa_executor_read_state) report as
+ * NPA_ERR_TIMEOUT when they have grown since the last such call on the device;
+ * and the waits of the layer norm and linear kernels, which
+ * npa_dev_check_layer_waits reports. */
 uint64_t npa_bulk_copy_timeouts(void);
 
 /* The payload of the last error on the calling thread, as the reference's
@@ -608,6 +608,14 @@ npa_status npa_dev_linear_backward(int32_t dtype, int32_t activation, const void
                                    int64_t rows, int64_t inputs, int64_t outputs, void* d_dx,
                                    int64_t dx_stride, void* d_dweight, void* d_dbias,
                                    void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Waits for `stream`, then returns NPA_ERR_TIMEOUT if a bounded wait of the layer
+ * norm and linear kernels has given up on the current device since the last
+ * such check: the calls above return before their kernels run, and a kernel that
+ * gives up (after two seconds; it does not happen in a healthy run) leaves
+ * outputs unwritten.  Once for a training step or a batch of requests, not for
+ * every call; not while the stream is being captured. */
+npa_status npa_dev_check_layer_waits(void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Executor: resident rollout state (the CUDA counterpart of            */

@@ -163,3 +163,18 @@ def test_one_walk_backward_of_many_rows_of_one_sign():
     ref = dy[some].double() @ w.double()
     size = dy[some].double().abs() @ w.double().abs()
     assert bool(((g.x[some].double() - ref).abs() <= 2.0 ** -11 * ref.abs() + 2.0 ** -20 * size + 2.0 ** -24).all())
+
+
+# ------------------------------------------------------------------- waits
+def test_check_of_waits_after_healthy_calls():
+    """Nothing gave up: the check waits for the stream and returns, however the
+    device is named."""
+    x, w = normal((300, 64), F16, 1), normal((32, 64), F16, 2)
+    ba.linear(x, w)
+    ba.check_layer_waits()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ba.layer_norm(x)
+        ba.check_layer_waits("cuda:0")
+        assert side.query()  # it waited
+    ba.check_layer_waits(torch.device("cuda"))
