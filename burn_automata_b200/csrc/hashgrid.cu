@@ -23,6 +23,7 @@
 
 #include <cuda.h>
 
+#include "host_state.h"
 #include "npa_internal.h"
 
 namespace npa {
@@ -599,61 +600,41 @@ npa_status static_scratch_address(void** out) {
 // host step makes tens of launches, and these runtime calls cost as much host
 // time as the launches themselves.
 namespace {
-struct PlanKey {
-  int device;
-  CUcontext ctx;
-  const void* kernel;
-  int threads;
-  size_t smem;
-  int per_sm;
-  int sms;
-};
-std::mutex g_plan_mu;
-std::vector<PlanKey> g_plans;
+LaunchPlans g_plans;
 }  // namespace
 
 npa_status kernel_occupancy(const void* kernel, int threads, size_t smem, int* per_sm, int* sms) {
-  int dev = 0;
-  NPA_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+  LaunchPlan plan{};
+  NPA_CUDA(cudaGetDevice(&plan.device), "cudaGetDevice");
   CUcontext ctx = nullptr;
   NPA_TRY(current_context(&ctx));
-  {
-    std::lock_guard<std::mutex> lock(g_plan_mu);
-    if (ctx)
-      for (const PlanKey& k : g_plans)
-        if (k.device == dev && k.ctx == ctx && k.kernel == kernel && k.threads == threads &&
-            k.smem == smem) {
-          *per_sm = k.per_sm;
-          *sms = k.sms;
-          return NPA_OK;
-        }
+  plan.ctx = ctx;
+  plan.kernel = kernel;
+  plan.threads = threads;
+  plan.smem = smem;
+  if (!g_plans.find(&plan)) {
+    int max_optin = 0;
+    NPA_CUDA(cudaDeviceGetAttribute(&max_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, plan.device),
+             "cudaDeviceGetAttribute");
+    NPA_CUDA(cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, plan.device),
+             "cudaDeviceGetAttribute");
+    if (smem > size_t(max_optin))
+      return fail(NPA_ERR_UNSUPPORTED, "kernel needs more shared memory than a block has");
+    if (!ctx) {  // the runtime makes the device's context current
+      NPA_CUDA(cudaFree(nullptr), "cudaFree");
+      NPA_TRY(current_context(&ctx));
+      plan.ctx = ctx;
+    }
+    NPA_TRY(g_plans.add(&plan, [&](size_t limit, LaunchPlan* p) -> npa_status {
+      NPA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(limit)),
+               "cudaFuncSetAttribute");
+      NPA_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&p->per_sm, kernel, threads, smem),
+               "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
+      return NPA_OK;
+    }));
   }
-  int max_optin = 0, count = 0, blocks = 0;
-  NPA_CUDA(cudaDeviceGetAttribute(&max_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev),
-           "cudaDeviceGetAttribute");
-  NPA_CUDA(cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev),
-           "cudaDeviceGetAttribute");
-  if (smem > size_t(max_optin))
-    return fail(NPA_ERR_UNSUPPORTED, "kernel needs more shared memory than a block has");
-  // The limit only ever rises: launches planned earlier with more shared
-  // memory keep theirs.
-  size_t limit = smem;
-  {
-    std::lock_guard<std::mutex> lock(g_plan_mu);
-    for (const PlanKey& k : g_plans)
-      if (k.device == dev && k.ctx == ctx && k.kernel == kernel) limit = std::max(limit, k.smem);
-  }
-  NPA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(limit)),
-           "cudaFuncSetAttribute");
-  NPA_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, smem),
-           "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
-  NPA_TRY(current_context(&ctx));
-  {
-    std::lock_guard<std::mutex> lock(g_plan_mu);
-    g_plans.push_back(PlanKey{dev, ctx, kernel, threads, smem, blocks, count});
-  }
-  *per_sm = blocks;
-  *sms = count;
+  *per_sm = plan.per_sm;
+  *sms = plan.sms;
   return NPA_OK;
 }
 

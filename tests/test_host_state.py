@@ -11,6 +11,8 @@ import pytest
 CSRC = Path(__file__).resolve().parents[1] / "burn_automata_b200" / "csrc"
 
 SOURCE = r"""
+#include <atomic>
+#include <chrono>
 #include <thread>
 #include <vector>
 #include "host_state.h"
@@ -33,6 +35,44 @@ int watermarks_race(void* w, int device, uint64_t now) {
   for (int r : reports) n += r;
   return n;
 }
+
+// Two threads plan one kernel with different amounts, the smaller one slow to
+// set its limit; the limit that the kernel is left with, and each plan's answer.
+size_t plans_race(size_t slow, size_t fast, int* found) {
+  npa::LaunchPlans plans;
+  std::atomic<size_t> attribute{0};  // the device's side
+  std::atomic<bool> started{false};
+  int kernel = 0, ctx = 0;
+  auto plan = [&](size_t smem, int ms) {
+    npa::LaunchPlan p{0, &ctx, &kernel, 256, smem, 0, 0};
+    if (plans.find(&p)) return;
+    plans.add(&p, [&](size_t limit, npa::LaunchPlan* q) {
+      started = true;
+      std::this_thread::sleep_for(std::chrono::milliseconds(ms));
+      attribute = limit;
+      q->per_sm = int(smem / 1000);
+      return 0;
+    });
+  };
+  std::thread a([&] { plan(slow, 100); });
+  while (!started) std::this_thread::yield();
+  std::thread b([&] { plan(fast, 0); });
+  a.join();
+  b.join();
+  npa::LaunchPlan p{0, &ctx, &kernel, 256, slow, 0, 0}, q{0, &ctx, &kernel, 256, fast, 0, 0};
+  npa::LaunchPlan other{0, &ctx, &kernel, 128, fast, 0, 0}, device{1, &ctx, &kernel, 256, fast, 0, 0};
+  *found = plans.find(&p) && plans.find(&q) && p.per_sm == int(slow / 1000) &&
+           q.per_sm == int(fast / 1000) && !plans.find(&other) && !plans.find(&device);
+  return attribute;
+}
+// A plan that could not be set is not kept.
+int plans_failed() {
+  npa::LaunchPlans plans;
+  int kernel = 0, ctx = 0;
+  npa::LaunchPlan p{0, &ctx, &kernel, 256, 1000, 0, 0};
+  const int status = plans.add(&p, [](size_t, npa::LaunchPlan*) { return 5; });
+  return status == 5 && !plans.find(&p);
+}
 }
 """
 
@@ -51,6 +91,8 @@ def lib(tmp_path_factory):
     lib.watermarks_new.restype = ctypes.c_void_p
     lib.watermarks_grown.argtypes = lib.watermarks_race.argtypes = [
         ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64]
+    lib.plans_race.restype = ctypes.c_size_t
+    lib.plans_race.argtypes = [ctypes.c_size_t, ctypes.c_size_t, ctypes.POINTER(ctypes.c_int)]
     return lib
 
 
@@ -67,6 +109,17 @@ def test_a_grown_count_is_reported_once_per_device(lib):
 
 def test_threads_report_one_growth_once(lib):
     assert lib.watermarks_race(lib.watermarks_new(), 1, 7) == 1
+
+
+@pytest.mark.parametrize("slow,fast", [(100000, 200000), (200000, 100000), (50000, 50000)])
+def test_threads_that_plan_one_kernel_leave_the_largest_limit(lib, slow, fast):
+    found = ctypes.c_int(0)
+    assert lib.plans_race(slow, fast, ctypes.byref(found)) == max(slow, fast)
+    assert found.value == 1
+
+
+def test_a_plan_that_failed_is_not_kept(lib):
+    assert lib.plans_failed() == 1
 
 
 def test_the_layers_waits_are_reported_by_an_entry_point(npa_lib):

@@ -178,3 +178,35 @@ def test_check_of_waits_after_healthy_calls():
         ba.check_layer_waits("cuda:0")
         assert side.query()  # it waited
     ba.check_layer_waits(torch.device("cuda"))
+
+
+def test_threads_with_new_shapes():
+    """Threads whose first calls of a kernel come with different shapes, and so
+    with different amounts of shared memory."""
+    import threading
+
+    widths = [64 + 4 * i for i in range(24)]
+    x = {d: normal((5000, d), F32, d) for d in widths}
+    w = normal((64, 64), BF16, 1)
+    want = {d: torch.nn.functional.layer_norm(x[d].double(), (d,)) for d in widths}
+    errors = []
+
+    def work(part):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for d in part:
+                    o = ba.layer_norm(x[d])
+                    ba.layer_norm_backward(x[d], x[d], o.mean, o.rstd)
+                    ba.linear(x[d][:, :64].bfloat16(), w)
+                    assert float((o.y.double() - want[d]).abs().max()) < 1e-4
+        except BaseException as e:  # noqa: BLE001 -- reported by the test's own thread
+            errors.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(widths[i::6],)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
