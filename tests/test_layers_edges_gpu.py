@@ -210,3 +210,42 @@ def test_threads_with_new_shapes():
         t.join()
     torch.cuda.synchronize()
     assert not errors, errors
+
+
+# ------------------------------------------------------- activations' tails
+def through_linear(z, act, rows):
+    """act at the values z (one per output), through products of one-hot rows."""
+    x, w = torch.zeros((rows, 16), dtype=z.dtype, device="cuda"), torch.zeros((z.numel(), 16), dtype=z.dtype,
+                                                                              device="cuda")
+    x[:, 0], w[:, 0] = 1, z
+    return ba.linear(x, w, activation=act).y[rows - 1].double()
+
+
+def slope_through_backward(z, act, rows):
+    """act' at z as the bias gradient of one row of ones, and as an x gradient."""
+    dy = torch.zeros((rows, z.numel()), dtype=z.dtype, device="cuda")
+    dy[rows - 1] = 1
+    x = torch.zeros((rows, 16), dtype=z.dtype, device="cuda")
+    w = torch.zeros((z.numel(), 16), dtype=z.dtype, device="cuda")
+    g = ba.linear_backward(dy, x, w, z.expand(rows, -1).contiguous(), activation=act, needs=("bias",))
+    return g.bias.double()
+
+
+def normal_cdf_and_density(z):
+    # ndtr cancels below zero as 1 + erf does
+    return torch.special.erfc(-z / 2 ** 0.5) / 2, torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_f32_gelu_tail(rows):
+    """z Phi(z) down to -12 with a relative error: the argument's two roundings
+    move erfc by z^2 2^-23 of itself, the function and the products err by a few
+    2^-23."""
+    z = torch.linspace(-12, 8, 4001, device="cuda")
+    cdf, density = normal_cdf_and_density(z.double())
+    bound = 2.0 ** -20 + z.double() ** 2 * 2.0 ** -22
+    got = through_linear(z, Activation.Gelu, rows)
+    assert float(((got - z.double() * cdf).abs() / (z.double() * cdf).abs().clamp(min=1e-45) / bound).max()) <= 1
+    got = slope_through_backward(z, Activation.Gelu, rows)
+    size = cdf + z.double().abs() * density
+    assert float(((got - (cdf + z.double() * density)).abs() / size / bound).max()) <= 1
