@@ -249,3 +249,34 @@ def test_f32_gelu_tail(rows):
     got = slope_through_backward(z, Activation.Gelu, rows)
     size = cdf + z.double().abs() * density
     assert float(((got - (cdf + z.double() * density)).abs() / size / bound).max()) <= 1
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_16_bit_activations_tails(dtype, rows):
+    """Relative to the result: one rounding, and 2^-13 for the short forms of the
+    exponential, the reciprocal and Phi.  What these forms flush to zero, below
+    2^-126, comes into a result times z, or times its factors in a slope."""
+    unit, least = (2.0 ** -11, 2.0 ** -24) if dtype == F16 else (2.0 ** -8, 2.0 ** -126)
+    z = torch.linspace(-12.5, 8, 2001, device="cuda").to(dtype)
+    zd = z.double()
+    cdf, density = normal_cdf_and_density(zd)
+    logistic = torch.sigmoid(zd)
+    inner = 2 * (2 / torch.pi) ** 0.5 * (zd + 0.044715 * zd ** 3)
+    p = torch.sigmoid(inner)
+    slope_of_inner = 2 * (2 / torch.pi) ** 0.5 * (1 + 3 * 0.044715 * zd ** 2)
+    cases = {
+        Activation.Gelu: (zd * cdf, [cdf, zd * density]),
+        Activation.Silu: (zd * logistic, [logistic, zd * logistic * torch.sigmoid(-zd)]),
+        Activation.GeluTanh: (zd * p, [p, zd * p * torch.sigmoid(-inner) * slope_of_inner]),
+    }
+    for act, (value, terms) in cases.items():
+        # the exponential's argument is rounded: 2^-22 of it moves the result
+        moved = 2.0 ** -13 + 2.0 ** -22 * inner.abs().clamp(min=1) if act == Activation.GeluTanh else 2.0 ** -13
+        got = through_linear(z, act, rows)
+        flushed = least + zd.abs() * 2.0 ** -126
+        assert bool(((got - value).abs() <= (unit + moved) * value.abs() + flushed).all()), act
+        got = slope_through_backward(z, act, rows)
+        ref, size = sum(terms), sum(t.abs() for t in terms)
+        flushed = least + (1 + zd.abs() * slope_of_inner) * 2.0 ** -126
+        assert bool(((got - ref).abs() <= unit * ref.abs() + moved * size + flushed).all()), act
