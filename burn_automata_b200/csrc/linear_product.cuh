@@ -210,10 +210,13 @@ __device__ __forceinline__ float activation_slope(int act, float z) {
       return normal<FAST>(z, e) + z * 0.39894228040143268f * e;
     }
     case NPA_ACTIVATION_GELU_TANH: {
-      // p = logistic(2u), and its derivative is 2 p (1 - p) u'
+      // p = logistic(2u), and its derivative is 2 p (1 - p) u'.  p (1 - p) is zero
+      // from |z| = 11 on, and its products with z one by one stay zero up to the
+      // largest f32, where z^2 would be infinite
       const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
       const float p = logistic<FAST>(2.0f * u);
-      return p + 2.0f * z * p * (1.0f - p) * 0.79788456080286536f * (1.0f + 0.134145f * z * z);
+      const float d = p * (1.0f - p) * z;
+      return p + 1.59576912160573071f * (d + d * z * (0.134145f * z));
     }
     case NPA_ACTIVATION_SILU: {
       const float s = logistic<FAST>(z);

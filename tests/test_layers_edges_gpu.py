@@ -280,3 +280,34 @@ def test_16_bit_activations_tails(dtype, rows):
         ref, size = sum(terms), sum(t.abs() for t in terms)
         flushed = least + (1 + zd.abs() * slope_of_inner) * 2.0 ** -126
         assert bool(((got - ref).abs() <= unit * ref.abs() + moved * size + flushed).all()), act
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("act", list(Activation))
+def test_activations_at_the_largest_values(act, dtype, rows):
+    """Far out every activation is z or zero and its slope one or zero, exactly, up
+    to the type's largest value; infinities and NaN give what the formula gives."""
+    top = torch.finfo(dtype).max
+    for size in (50.0, 300.0, 6e4, 1e10, 5e19, 1e25, top):
+        if size > top:
+            continue
+        z = torch.tensor([size, -size] * 8, device="cuda").to(dtype)
+        value = z.double() if act == Activation.Identity else z.double().clamp(min=0)
+        slope = torch.ones_like(value) if act == Activation.Identity else (z > 0).double()
+        # silu at -50 is 1e-20 yet, and its slope
+        near = 1e-18 if size == 50.0 and act in (Activation.Silu, Activation.Gelu, Activation.GeluTanh) else 0.0
+        assert float((through_linear(z, act, rows) - value).abs().max()) <= near, size
+        if act != Activation.Identity:
+            assert float((slope_through_backward(z, act, rows) - slope).abs().max()) <= near, size
+    z = torch.tensor([INF, NAN, -INF] * 5 + [NAN], device="cuda").to(dtype)
+    got = ba.linear(torch.zeros((rows, 8), dtype=dtype, device="cuda"),
+                    torch.zeros((16, 8), dtype=dtype, device="cuda"), z, activation=act).y[rows - 1]
+    assert bool((got[0::3][:5] == INF).all()) and bool(got[1::3].isnan().all())
+    below = got[2::3]
+    if act == Activation.Identity:
+        assert bool((below == -INF).all())
+    elif act == Activation.Relu:
+        assert bool((below == 0).all())
+    else:
+        assert bool(below.isnan().all())  # -infinity times zero
