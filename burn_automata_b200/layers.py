@@ -110,15 +110,22 @@ def _rows(t):
     return t.contiguous(), t.shape[-1]
 
 
-def _aligned_rows(t):
-    """As _rows for the linear layer's operands: a large range of columns whose
-    rows do not start on 16 bytes, but would by themselves, is copied.  The
-    products read such rows several times, by TMA only when aligned."""
+def _aligned_rows(t, work: int, reuse: int):
+    """As _rows for a product's operand: one whose rows do not all start on 16
+    bytes (by its stride or by its address), but would in a copy of its own, is
+    copied where that pays.  `work` is the product's multiplications, `reuse` how
+    many of them a value takes part in.  16 bits: TMA reads aligned rows only, and
+    the loader warps that read others lose more than a copy takes from 2^30 on (x
+    one value off, forward, us without and with it: 16384 x 512 -> 2048 262 and 46,
+    300000 x 64 -> 128 64 and 50; 2^29: 16384 x 256 -> 128 15 and 24).  f32 goes
+    through them either way and gains on values that are read often (65536 x 128 ->
+    1024 187 and 142; 65536 x 1024 -> 128 194 and 221)."""
     t, stride = _rows(t)
     size = t.element_size()
-    if ((stride * size) % 16 and t.shape[0] > 1 and t.shape[-1] * size % 16 == 0
-            and t.numel() >= 1 << 19):
-        return t.contiguous(), t.shape[-1]
+    if ((t.data_ptr() % 16 or (stride * size) % 16 and t.shape[0] > 1)
+            and t.shape[-1] * size % 16 == 0 and work >= 1 << 30
+            and (size == 2 or reuse >= 384)):
+        return t.clone(memory_format=_t().contiguous_format), t.shape[-1]
     return t, stride
 
 
@@ -283,11 +290,12 @@ def linear(x, weight, bias=None, residual=None, activation: Activation = Activat
     inputs, outputs = _layer_shape(x, weight)
     out_shape = x.shape[:-1] + (outputs,)
     _like(weight, x, "weight")
-    wr, wstride = _aligned_rows(weight)
+    rows = x.numel() // inputs if inputs else 0
+    work = rows * inputs * outputs
+    wr, wstride = _aligned_rows(weight, work, rows)
     b = _vector(bias, x, outputs, "bias")
     rr, rs = (None, 0) if residual is None else _matrix(residual, x, out_shape, "residual")
-    xr, xs = _aligned_rows(x)
-    rows = x.numel() // inputs if inputs else 0
+    xr, xs = _aligned_rows(x, work, outputs)
     y = _outputs_like(x, out_shape)
     z = torch.empty_like(y) if save_pre_activation else None
     L = _lib.lib()
@@ -310,15 +318,19 @@ def linear_backward(dy, x, weight, pre_activation=None,
     out_shape = x.shape[:-1] + (outputs,)
     want = _needs(needs)
     _like(weight, x, "weight")
-    wr, wstride = _aligned_rows(weight)
+    rows = x.numel() // inputs if inputs else 0
+    work = rows * inputs * outputs
+    wr, wstride = _aligned_rows(weight, work, rows)
     dyr, dys = _matrix(dy, x, out_shape, "dy")
     zr, zs = None, 0
     if act != Activation.Identity:
         if pre_activation is None:
             raise InvalidArgument("this activation's gradient needs pre_activation")
         zr, zs = _matrix(pre_activation, x, out_shape, "pre_activation")
-    xr, xs = _aligned_rows(x)
-    rows = x.numel() // inputs if inputs else 0
+    else:
+        # dy itself is the products' operand; with an activation a pass makes dz of it
+        dyr, dys = _aligned_rows(dyr, work, inputs)
+    xr, xs = _aligned_rows(x, work, outputs)
     dx = _outputs_like(x, x.shape) if "x" in want else None
     dw = _outputs_like(weight, weight.shape) if "weight" in want else None
     db = x.new_empty(outputs) if "bias" in want else None

@@ -107,3 +107,32 @@ def test_python_layer_refuses_what_it_cannot_take():
             call()
     assert Activation.Silu == 4
     assert _lib.lib().npa_abi_version() == 1
+
+
+def test_operands_off_16_bytes_are_copied_where_it_pays():
+    """By the stride and by the address alike; small products, f32 operands that
+    few outputs read and rows that a copy would not align stay in place."""
+    torch = pytest.importorskip("torch")
+    big = 1 << 30
+
+    def at(rows, width, offset, pitch, dtype):
+        # a start on 16 bytes, whatever the allocator gives
+        flat = torch.zeros(rows * (width + pitch) + offset + 16, dtype=dtype)
+        start = -flat.data_ptr() % 16 // flat.element_size() + offset
+        return flat[start:start + rows * (width + pitch)].view(rows, width + pitch)[:, :width]
+
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        for offset, pitch, copied in ((0, 0, False), (1, 0, True), (0, 1, True), (3, 8, True),
+                                      (0, 8, False), (8, 0, False)):
+            t = at(64, 32, offset, pitch, dtype)
+            t += torch.arange(64 * 32).view(64, 32).to(dtype) / 64
+            got, stride = layers._aligned_rows(t, big, 1024)
+            assert (got.data_ptr() != t.data_ptr()) == copied, (dtype, offset, pitch)
+            assert torch.equal(got, t) and stride == (32 if copied else 32 + pitch)
+            if copied:
+                assert got.data_ptr() % 16 == 0 and got.is_contiguous()
+            assert layers._aligned_rows(t, big - 1, 1024)[0].data_ptr() == t.data_ptr()
+            few = layers._aligned_rows(t, big, 128)[0]
+            assert (few.data_ptr() != t.data_ptr()) == (copied and dtype != torch.float32)
+    odd = at(64, 33, 1, 0, torch.bfloat16)
+    assert layers._aligned_rows(odd, big, 1024)[0].data_ptr() == odd.data_ptr()

@@ -311,3 +311,28 @@ def test_activations_at_the_largest_values(act, dtype, rows):
         assert bool((below == 0).all())
     else:
         assert bool(below.isnan().all())  # -infinity times zero
+
+
+# ------------------------------------------------- views that start anywhere
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,inputs,outputs", [(8192, 512, 384), (40000, 64, 128)])
+@pytest.mark.parametrize("act", [Activation.Identity, Activation.Silu])
+def test_large_views_off_16_bytes(act, rows, inputs, outputs, dtype):
+    """Operands whose first value is one past a 16-byte boundary, or whose rows
+    are, give what aligned copies of them give, up to the order of sums."""
+    def view(width, seed, offset, pitch):
+        flat = normal((rows * (width + pitch) + offset,), dtype, seed)
+        return flat[offset:].view(rows, width + pitch)[:, :width]
+
+    w, b = normal((outputs, inputs), dtype, 1, 0.1), normal((outputs,), dtype, 2)
+    unit = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}[dtype]
+    for offset, pitch in ((1, 0), (0, 3)):
+        x, dy, z = view(inputs, 3, offset, pitch), view(outputs, 4, offset, pitch), view(outputs, 5, offset, pitch)
+        xc, dyc, zc = x.clone(), dy.clone(), z.clone()
+        for got, want, size in (
+                (ba.linear(x, w, b, activation=act).y, ba.linear(xc, w, b, activation=act).y, inputs),
+                *zip(vars(ba.linear_backward(dy, x, w, z, activation=act)).values(),
+                     vars(ba.linear_backward(dyc, xc, w, zc, activation=act)).values(), (outputs, rows, rows))):
+            # two roundings of the result and of dz, and sums of `size` terms of order one
+            error = (got.double() - want.double()).norm() / want.double().norm()
+            assert float(error) <= 4 * unit + (size ** 0.5 + 16) * 2.0 ** -22
