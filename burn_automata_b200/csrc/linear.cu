@@ -567,9 +567,10 @@ int vector_width(const void* p, int64_t stride, int64_t rows) {
   return vec;
 }
 
-// Blocks of the pair kernel that run at once on the current device.
-template <class K>
-npa_status pair_blocks(K kernel, int threads, size_t smem, int sms, int* blocks) {
+// Blocks of the pair kernel KERNEL that run at once on the current device; one
+// answer per kernel and device is kept.
+template <auto KERNEL>
+npa_status pair_blocks(int threads, size_t smem, int sms, int* blocks) {
   static std::atomic<int> cached[64];
   int dev = 0;
   NPA_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
@@ -589,7 +590,7 @@ npa_status pair_blocks(K kernel, int threads, size_t smem, int sms, int* blocks)
   config.attrs = &attr;
   config.numAttrs = 1;
   int clusters = 0;
-  NPA_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel, &config),
+  NPA_CUDA(cudaOccupancyMaxActiveClusters(&clusters, KERNEL, &config),
            "cudaOccupancyMaxActiveClusters");
   if (clusters < 1) return fail(NPA_ERR_UNSUPPORTED, "linear pair kernel cannot be resident");
   *blocks = 2 * clusters;
@@ -609,7 +610,8 @@ npa_status launch_product_as(const CUtensorMap (&maps)[4], const Product& p, boo
   const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles * p.splits;
   if constexpr (PAIR) {
     int blocks = 0;
-    NPA_TRY(pair_blocks(kernel, C::kThreads, C::kSmemBytes, sms, &blocks));
+    NPA_TRY((pair_blocks<linear_tc::product_kernel<T, LOADER, BN, PAIR, FORM>>(C::kThreads, C::kSmemBytes, sms,
+                                                                             &blocks)));
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(unsigned(std::min<int64_t>({2 * tiles, blocks, kSms})));
     config.blockDim = dim3(C::kThreads);
