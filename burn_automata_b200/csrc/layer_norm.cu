@@ -514,10 +514,10 @@ __host__ __device__ inline uint32_t backward_slot(uint32_t tile_bytes, bool resi
 }
 
 // Blocks of eight warps that an SM's registers are to hold.
-constexpr int backward_blocks(int values) { return values <= 0 ? 3 : 2; }
+constexpr int kBackwardBlocks = 2;
 
 template <class T, int VEC, int NV>
-__global__ void __launch_bounds__(256, backward_blocks(VEC * NV))
+__global__ void __launch_bounds__(256, kBackwardBlocks)
 layer_norm_backward_tiles_kernel(LayerNormBackwardArgs a, TileShape shape) {
   let_next_launch();
   extern __shared__ __align__(128) char smem[];
@@ -1172,10 +1172,7 @@ npa_status backward_rows(const LayerNormBackwardArgs& a, int* parts, cudaStream_
       gapless(a.dx, a.dx_stride, a.rows, a.dims) &&
       gapless(a.residual, a.residual_stride, a.rows, a.dims) && bulk_rows(a.mean, 0, 4) &&
       bulk_rows(a.rstd, 0, 4)) {
-    int vec = 16 / int(sizeof(T));
-    while (a.dims % vec) vec /= 2;
-    const int blocks = backward_blocks(vec * plan_lanes(a.dims, vec).nv);
-    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, blocks, false, [&](int tile_rows) {
+    const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, kBackwardBlocks, false, [&](int tile_rows) {
       return backward_slot(uint32_t(a.dims * tile_rows * sizeof(T)), a.residual != nullptr, tile_rows);
     });
     if (p.row.nv)
