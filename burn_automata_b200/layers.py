@@ -121,10 +121,11 @@ def _aligned_rows(t, work: int, reuse: int):
     through them either way and gains on values that are read often (65536 x 128 ->
     1024 187 and 142; 65536 x 1024 -> 128 194 and 221)."""
     t, stride = _rows(t)
+    if work < 1 << 30:
+        return t, stride
     size = t.element_size()
     if ((t.data_ptr() % 16 or (stride * size) % 16 and t.shape[0] > 1)
-            and t.shape[-1] * size % 16 == 0 and work >= 1 << 30
-            and (size == 2 or reuse >= 384)):
+            and t.shape[-1] * size % 16 == 0 and (size == 2 or reuse >= 384)):
         return t.clone(memory_format=_t().contiguous_format), t.shape[-1]
     return t, stride
 
