@@ -104,8 +104,8 @@ constexpr int kFewRows = 8;
 // A warp has OUTS outputs of all R rows and walks k with 16-byte loads (VEC
 // values; single values where a row does not start on 16 bytes).  Plain f32
 // products: at eight rows a weight read from memory still costs more than its
-// eight multiply-adds.  One row of a 1024 -> 4096 bf16 layer: 3.7 us on the device
-// against 8.2 for split tiles and their sum.
+// eight multiply-adds.  One row of a 1024 -> 4096 bf16 layer: 4.0 us on the device
+// with the weights in memory, against 8.2 for split tiles and their sum.
 template <class T, int R, int OUTS, int VEC>
 __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ LinearArgs a) {
   using P = Pack<T, VEC>;
@@ -160,8 +160,20 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ L
 template <class T, int R>
 npa_status launch_few_rows(const LinearArgs& a, bool vec, cudaStream_t s) {
   constexpr int kVec = 16 / int(sizeof(T));
-  // four outputs to a warp once that leaves most SMs a block
-  if (a.outputs >= 2048) {
+  // One output to a warp, or four for two rows or more whose outputs would take
+  // more than three quarters of a wave of such warps: a weight is then read for
+  // several rows, and x for four outputs at once (bf16 2 x 1024 -> 4096 4.9 us, four
+  // 5.2; -> 8192 8.1 and 6.4; 8 x 1024 -> 2560 7.0 and 7.4; -> 3584 8.8 and 7.5; but
+  // 1 x 1024 -> 4096 4.0 and 6.3, -> 32768 14.2 and 15.4).
+  bool four = false;
+  if (R > 1 && a.outputs > 2048) {
+    int per_sm = 0, sms = 0;
+    const void* const one = vec ? reinterpret_cast<const void*>(few_rows_kernel<T, R, 1, kVec>)
+                                : reinterpret_cast<const void*>(few_rows_kernel<T, R, 1, 1>);
+    NPA_TRY(kernel_occupancy(one, 256, 0, &per_sm, &sms));
+    four = a.outputs > int64_t(per_sm) * sms * 8 * 3 / 4;
+  }
+  if (four) {
     const unsigned grid = unsigned((a.outputs + 31) / 32);
     if (vec)
       few_rows_kernel<T, R, 4, kVec><<<grid, 256, 0, s>>>(a);

@@ -336,3 +336,23 @@ def test_large_views_off_16_bytes(act, rows, inputs, outputs, dtype):
             # two roundings of the result and of dz, and sums of `size` terms of order one
             error = (got.double() - want.double()).norm() / want.double().norm()
             assert float(error) <= 4 * unit + (size ** 0.5 + 16) * 2.0 ** -22
+
+
+# ------------------------------------------------ a few rows and many outputs
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 2, 4, 7])
+def test_few_rows_do_not_depend_on_the_outputs_beside_them(rows, dtype):
+    """One output to a warp or four: each is the same sum."""
+    x, w = normal((rows, 264), dtype, 1), normal((16001, 264), dtype, 2, 0.1)
+    b, res = normal((16001,), dtype, 3), normal((rows, 16001), dtype, 4)
+    whole = ba.linear(x, w, b, residual=res, activation=Activation.Silu, save_pre_activation=True)
+    for n in (1, 2047, 2049, 3553, 3600, 9473, 16000):
+        part = ba.linear(x, w[:n], b[:n], residual=res[:, :n], activation=Activation.Silu,
+                         save_pre_activation=True)
+        assert torch.equal(part.y, whole.y[:, :n])
+        assert torch.equal(part.pre_activation, whole.pre_activation[:, :n])
+    ref = x.double() @ w.double().t() + b.double()
+    unit = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}[dtype]
+    size = x.double().abs() @ w.double().abs().t() + b.double().abs()
+    bound = unit * ref.abs() + (264 ** 0.5 + 16) * 2.0 ** -22 * size + 2.0 ** -24
+    assert bool(((whole.pre_activation.double() - ref).abs() <= bound).all())
