@@ -310,8 +310,14 @@ struct SlopeArgs {
 // the unrounded values.  A thread has 16 bytes of every (256 / tx)th row; RAGGED:
 // of rows that start anywhere or end within them (dz's rows are whole, zero past
 // the outputs).
+// Blocks to an SM, all in one wave: three, but two of the aligned bf16 kernel, which
+// spills at 80 registers (16384 x 1024 -> 4096 backward, us with three and two: bf16
+// silu 321 and 275, gelu 372 and 333, relu 342 and 304; f16 silu 315 and 321; with
+// four f16 took a second wave, 31 more).
 template <class T, bool RAGGED>
-__global__ void __launch_bounds__(256, 3) slope_kernel(const __grid_constant__ SlopeArgs a) {
+constexpr int kSlopeBlocks = std::is_same<T, __nv_bfloat16>::value && !RAGGED ? 2 : 3;
+template <class T, bool RAGGED>
+__global__ void __launch_bounds__(256, (kSlopeBlocks<T, RAGGED>)) slope_kernel(const __grid_constant__ SlopeArgs a) {
   let_next_launch();
   wait_for_previous();
   constexpr int VEC = 16 / int(sizeof(T));
@@ -446,9 +452,7 @@ bool packs(size_t size, int width, int64_t rows, int inputs, int outputs) {
 
 // ---- host side ----
 constexpr int kSms = linear_tc::kMaxBlocks;  // the plans' block count
-// Blocks of slope_kernel at most: the three to an SM that its registers allow, in
-// one wave (16384 x 4096 f16 silu: 88 us; 119 with four, which take a second wave).
-constexpr int kBiasBlocks = 3 * kSms;
+constexpr int kBiasBlocks = 3 * kSms;  // of slope_kernel at most
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -847,7 +851,7 @@ npa_status launch_slope(SlopeArgs s, int* parts, cudaStream_t stream) {
   while (s.tx < 32 && s.tx < groups) s.tx *= 2;
   const int grid_x = ceil_div(groups, s.tx);
   const int64_t at_once = 256 / s.tx;
-  const int64_t most = std::max(1, kBiasBlocks / grid_x);
+  const int64_t most = std::max(1, kSlopeBlocks<T, RAGGED> * kSms / grid_x);
   *parts = int(std::max<int64_t>(1, std::min<int64_t>(most, (s.rows + at_once * 4 - 1) / (at_once * 4))));
   s.rows_per_block = (s.rows + *parts - 1) / *parts;
   *parts = int((s.rows + s.rows_per_block - 1) / s.rows_per_block);
