@@ -451,7 +451,7 @@ bool packs(size_t size, int width, int64_t rows, int inputs, int outputs) {
 }
 
 // ---- host side ----
-constexpr int kSms = linear_tc::kMaxBlocks;  // the plans' block count
+constexpr int kSms = 148;             // the plans' block count: B200's SMs
 constexpr int kBiasBlocks = 3 * kSms;  // of slope_kernel at most
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -518,11 +518,6 @@ struct Plan {
   size_t partial_bytes() const {
     return splits > 1 ? size_t(splits) * layer_rows * partial_pitch * 4 : 0;
   }
-  // f32 operands keep their sums in registers
-  size_t running_bytes(size_t size) const {
-    return size == 2 && split_blocks > linear_tc::kLongBlocks ? linear_tc::running_bytes(bn) : 0;
-  }
-  size_t bytes(size_t size) const { return partial_bytes() + running_bytes(size); }
 };
 Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
   Plan p{};
@@ -570,8 +565,8 @@ Plan plan_product(size_t size, bool tma, int64_t m, int64_t n, int64_t k) {
   return p;
 }
 size_t product_workspace(size_t size, int64_t m, int64_t n, int64_t k) {
-  return std::max(plan_product(size, true, m, n, k).bytes(size),
-                  plan_product(size, false, m, n, k).bytes(size));
+  return std::max(plan_product(size, true, m, n, k).partial_bytes(),
+                  plan_product(size, false, m, n, k).partial_bytes());
 }
 
 template <class T>
@@ -629,7 +624,7 @@ npa_status launch_product_as(const CUtensorMap (&maps)[4], const Product& p, boo
     NPA_TRY((pair_blocks<linear_tc::product_kernel<T, LOADER, BN, PAIR, FORM>>(C::kThreads, C::kSmemBytes, sms,
                                                                              &blocks)));
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(unsigned(std::min<int64_t>({2 * tiles, blocks, kSms})));
+    config.gridDim = dim3(unsigned(std::min<int64_t>(2 * tiles, blocks)));
     config.blockDim = dim3(C::kThreads);
     config.dynamicSmemBytes = C::kSmemBytes;
     config.stream = stream;
@@ -644,7 +639,7 @@ npa_status launch_product_as(const CUtensorMap (&maps)[4], const Product& p, boo
     NPA_CUDA(cudaLaunchKernelEx(&config, kernel, maps[0], maps[1], maps[2], maps[3], p),
              "linear product_kernel");
   } else {
-    NPA_CUDA(launch_kernel(after, kernel, dim3(unsigned(std::min<int64_t>({tiles, sms, kSms}))), C::kThreads,
+    NPA_CUDA(launch_kernel(after, kernel, dim3(unsigned(std::min<int64_t>(tiles, sms))), C::kThreads,
                            C::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], p),
              "linear product_kernel");
   }
@@ -656,7 +651,7 @@ npa_status launch_product(const CUtensorMap (&maps)[4], const Product& p, bool a
                           cudaStream_t stream) {
   using linear_tc::kLong, linear_tc::kRagged, linear_tc::kWhole;
   if constexpr (sizeof(T) == 2)
-    if (p.running) return launch_product_as<T, LOADER, BN, PAIR, kLong>(maps, p, after, stream);
+    if (p.long_k) return launch_product_as<T, LOADER, BN, PAIR, kLong>(maps, p, after, stream);
   const bool whole = p.partials || (p.y_tma && (!p.z || p.z_tma) &&
                                     (!p.residual || (p.residual_vec && p.n * sizeof(T) % 16 == 0)));
   return whole ? launch_product_as<T, LOADER, BN, PAIR, kWhole>(maps, p, after, stream)
@@ -682,9 +677,7 @@ npa_status run_product(Product p, float* partials, bool after, BiasSums bias, cu
   p.layer_rows = plan.layer_rows;
   p.partial_pitch = plan.partial_pitch;
   p.partials = plan.splits > 1 ? partials : nullptr;
-  p.running = plan.running_bytes(sizeof(T))
-                  ? reinterpret_cast<float4*>(partials + plan.partial_bytes() / 4)
-                  : nullptr;
+  p.long_k = sizeof(T) == 2 && plan.split_blocks > linear_tc::kLongBlocks;
   p.idesc = tc::instruction_desc(!std::is_same<T, __half>::value, p.a.mn_major, p.b.mn_major,
                                  plan.pair ? 2 * linear_tc::kBM : linear_tc::kBM, plan.bn);
   p.a_vec = vector_width<T>(p.a.p, p.a.ld, a_rows);

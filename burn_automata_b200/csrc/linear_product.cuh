@@ -28,8 +28,7 @@
 // accumulating steps.  Terms of one sign lose 1.1e-7 of their sum at each
 // (measured with f16 over 65,536 to 1,048,576 values of k), so 512 steps stay
 // below 2^-14, an eighth of f16's rounding.  A longer k moves its sums every
-// 128 blocks to rounded f32 ones in the workspace, each in the thread that
-// finishes it, under the next blocks' products: unmoved, a weight gradient over
+// 128 blocks to registers as f32 operands do: unmoved, a weight gradient over
 // 1,048,576 rows came out 0.7 % low.
 //
 // Measured on one B200.  bf16 8192 x 4096 x 4096 in pairs' tiles: 170 us, the
@@ -57,7 +56,6 @@ constexpr int kEpilogueWarps = 8;        // two per 32 TMEM lanes
 constexpr int kLoaderWarps = 8;
 constexpr int kChunkBlocks = 4;          // k blocks between f32 moves out of TMEM
 constexpr int kLongBlocks = 128;         // the same for 16-bit operands
-constexpr int kMaxBlocks = 148;          // of a launch: B200's SMs
 constexpr int kSmemLimit = 227 * 1024;
 
 // One operand: value (i, k) at i * ld + k, or at k * ld + i when MN-major.
@@ -84,17 +82,11 @@ struct Product {
   void* z;
   int64_t z_stride;
   float* partials;  // split: [splits][layer_rows][partial_pitch], else null
-  float4* running;  // long k: each thread's sums, running_bytes() of them
+  int long_k;  // 16-bit operands: more than kLongBlocks in a split
   int64_t layer_rows, partial_pitch;
   int act;
   int y_tma, z_tma, residual_vec;
 };
-
-// The sums of a launch with tiles of bn columns: an epilogue thread's 64 columns
-// of every second group.
-constexpr size_t running_bytes(int bn) {
-  return size_t(kMaxBlocks) * ((bn + 127) / 128) * kEpilogueWarps * 32 * 64 * sizeof(float);
-}
 
 __device__ unsigned long long g_timeouts = 0;  // bounded waits that gave up
 
@@ -549,8 +541,7 @@ __device__ __forceinline__ void put_group(uint32_t buf, int lane,
 // kRagged: outputs or a residual whose rows do not start on 16 bytes.  kLong: the
 // same, and more than kLongBlocks of k (16-bit operands).  The common case does
 // without that code: its size alone costs (1048576 x 64 x 128 bf16: 126 us with
-// the ragged epilogue, 117 without; 607399 x 48 -> 179: 269 us with the long
-// k's sums, 259 without).
+// the ragged epilogue, 117 without).
 enum Form { kWhole, kRagged, kLong };
 template <class T, bool LOADER, int BN, bool PAIR, Form FORM>
 __global__ void __launch_bounds__((Config<T, LOADER, BN, PAIR>::kThreads), 1)
@@ -562,6 +553,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   constexpr int kGroup = 128 / int(sizeof(T));         // output columns staged at a time
   constexpr int kGroups = BN / kGroup;
   constexpr int kGroupsPerWarp = (kGroups + 1) / 2;
+  // k blocks between moves out of TMEM, 0: none before the tile's end
+  constexpr int kMoved = C::kParts == 3 ? kChunkBlocks : LONG ? kLongBlocks : 0;
   extern __shared__ char smem_raw[];
   const uint32_t raw = tc::smem_addr(smem_raw);
   const uint32_t base = (raw + 1023) & ~1023u;  // the swizzle repeats every 1,024 bytes
@@ -617,10 +610,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 
   // The loader kernel's 640 threads start with 96 registers each; its control
   // warpgroup leaves some to the others: 56 + 2 x 96 + 2 x 112 = 472 of the
-  // launch's 480 per thread of each warpgroup.
+  // launch's 480 per thread of each warpgroup.  The TMA kernels' 384 threads start
+  // with 168; where sums stay in registers over a long k the two epilogue
+  // warpgroups get 224 each and the control warpgroup keeps 56: all 504.
   if (warp > kMmaWarp) {
     // ---- producers ----
     if (!LOADER) {
+      if constexpr (LONG) tc::registers_down<56>();
       if (warp == kTmaWarp && lane == 0) {
         Cursor<C::kStages> at;
         uint32_t issued = 0;
@@ -770,7 +766,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
   } else if (warp == kMmaWarp) {
     // ---- the warp that issues the products (the pair's first block's) ----
-    if constexpr (LOADER) tc::registers_down<56>();
+    if constexpr (LOADER || LONG) tc::registers_down<56>();
     if (rank == 0) {
       // One lane issues everything, so what lies between two blocks of k counts:
       // the warp runs whole, cursors step by one and descriptors by additions.
@@ -819,7 +815,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
           tc::mma_commit<PAIR>(empty + 8 * at.slot, issue);
           ++in_chunk;
-          constexpr int kMoved = C::kParts == 3 ? kChunkBlocks : LONG ? kLongBlocks : 0;
           if (kt + 1 == blocks || (kMoved > 0 && in_chunk == kMoved)) {
             tc::mma_commit<PAIR>(acc_full + 8 * acc.slot, issue);
             acc.advance();
@@ -834,6 +829,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
   } else {
     // ---- epilogue warps: 32 rows each, every other group of columns ----
+    if constexpr (LONG && !LOADER) tc::registers_up<224>();
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t bufs = out_base + warp * C::kOutBuffers * 4096;
@@ -856,11 +852,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         tc::bar_arrive_cluster(first_acc_empty + 8 * buf);
       else
         tc::bar_arrive(acc_empty + 8 * buf);
-    };
-    // four of this thread's sums in p.running: a warp's lie side by side
-    [[maybe_unused]] auto running_at = [&](int gi, int quad) -> float4* {
-      return p.running + ((blockIdx.x * kGroupsPerWarp + gi) * (kGroup / 4) + quad) * (kEpilogueWarps * 32) +
-             warp * 32 + lane;
     };
     auto pointer = [&](uint32_t b) -> char* { return smem_raw + (b - raw); };
     T* const bias_row = reinterpret_cast<T*>(pointer(bias_base + warp * 128));
@@ -888,9 +879,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       const int n0 = in % p.n_tiles * BN;
       const int64_t rows_left = int64_t(p.m) - row0;
       const int rows = rows_left >= 32 ? 32 : rows_left > 0 ? int(rows_left) : 0;
-      float sums[C::kParts == 3 ? kGroupsPerWarp : 1][kGroup];
+      float sums[kMoved > 0 ? kGroupsPerWarp : 1][kGroup];
       uint32_t d = 0;
-      [[maybe_unused]] bool moved = false;  // sums of earlier blocks of k are in p.running
       // The TMA kernels ask for the residual before the wait for the accumulators
       // (the first group) or before they read them; the loader kernels' register
       // budget (five warps to an SM quarter) has no room for it.
@@ -935,10 +925,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
       };
       prefetch(0);
-      if constexpr (C::kParts == 3) {
+      if constexpr (kMoved > 0) {
         const int kb = split * p.split_blocks;
         const int blocks = min(p.k_blocks, kb + p.split_blocks) - kb;
-        const int chunks = (blocks + kChunkBlocks - 1) / kChunkBlocks;
+        const int chunks = (blocks + kMoved - 1) / kMoved;
 #pragma unroll
         for (int gi = 0; gi < kGroupsPerWarp; ++gi)
 #pragma unroll
@@ -951,6 +941,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           tc::fence_after();
 #pragma unroll
           for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
+            if constexpr (kGroups % 2 != 0)
+              if (half + 2 * gi >= kGroups) continue;
             const uint32_t at = tmem + buf * C::kBufferColumns + lanes + (half + 2 * gi) * kGroup;
 #pragma unroll
             for (int h = 0; h < kGroup; h += 16) {
@@ -958,6 +950,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
               tc::tmem_load(at + h, part);
 #pragma unroll
               for (int e = 0; e < 16; ++e) sums[gi][h + e] += part[e];
+              if constexpr (C::kParts == 1) continue;
               tc::tmem_load(at + BN + h, part);
               if constexpr (RAGGED) {
                 // value by value: this kernel spills with the other form (backward
@@ -984,38 +977,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         if (!ok) break;
       } else {
-        if constexpr (LONG) {
-          const int kb = split * p.split_blocks;
-          for (int left = min(p.k_blocks, kb + p.split_blocks) - kb; left > kLongBlocks;
-               left -= kLongBlocks, acc.advance()) {
-            ok = __all_sync(0xffffffffu, tc::bar_wait(acc_full + 8 * acc.slot, acc.parity));
-            if (!ok) break;
-            tc::fence_after();
-#pragma unroll
-            for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
-              const int g = half + 2 * gi;
-              if (g >= kGroups || n0 + g * kGroup >= p.n) continue;
-#pragma unroll
-              for (int h = 0; h < kGroup; h += 16) {
-                float part[16];
-                tc::tmem_load(tmem + acc.slot * C::kBufferColumns + lanes + g * kGroup + h, part);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  float4* const at = running_at(gi, h / 4 + q);
-                  float4 f = moved ? *at : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                  f.x += part[4 * q];
-                  f.y += part[4 * q + 1];
-                  f.z += part[4 * q + 2];
-                  f.w += part[4 * q + 3];
-                  *at = f;
-                }
-              }
-            }
-            release_accumulators(acc.slot);
-            moved = true;
-          }
-          if (!ok) break;
-        }
         const uint32_t buf = acc.slot;
         ok = tc::bar_wait(acc_full + 8 * buf, acc.parity);
         ok = __all_sync(0xffffffffu, ok);
@@ -1023,7 +984,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         tc::fence_after();
         d = tmem + buf * C::kBufferColumns + lanes;
       }
-      // One group of columns; v: its sums (f32), or room for its accumulators.
+      // One group of columns; v: its sums, or room for its accumulators.
       auto finish_group = [&](int gi, float (&v)[kGroup]) {
         const int g = half + 2 * gi;
         const int col0 = n0 + g * kGroup;
@@ -1052,25 +1013,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         };
         if (gi > 0) prefetch(gi);
         if (LOADER) prefetch_bias(t, gi);
-        if constexpr (C::kParts != 3) {
+        if constexpr (kMoved == 0) {
           if (mine) tc::tmem_load(d + g * kGroup, v);
           if (last) {
             release_accumulators(acc.slot);
             acc.advance();
-          }
-          if constexpr (LONG) {
-            if (mine && moved) {
-#pragma unroll
-              for (int q = 0; q < kGroup / 4; ++q) {
-                // not all loads at once: there are no registers for them
-                if (q % (LOADER ? 2 : 8) == 0) asm volatile("" ::: "memory");
-                const float4 f = *running_at(gi, q);
-                v[4 * q] += f.x;
-                v[4 * q + 1] += f.y;
-                v[4 * q + 2] += f.z;
-                v[4 * q + 3] += f.w;
-              }
-            }
           }
         }
         if (!mine) {
@@ -1158,7 +1105,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       };
 #pragma unroll
       for (int gi = 0; gi < kGroupsPerWarp; ++gi) {
-        if constexpr (C::kParts == 3) {
+        if constexpr (kMoved > 0) {
           finish_group(gi, sums[gi]);
         } else {
           float v[kGroup];
