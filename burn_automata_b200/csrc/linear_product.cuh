@@ -13,12 +13,18 @@
 // alignment they have and write the same swizzled tiles.
 //
 // f32 values are split into three bf16 parts, x = x0 + x1 + x2 exactly but for
-// 2^-24 |x|, and six of the nine part products are summed in f32:
-//   x w ~ x0 w0 + (x0 w1 + x1 w0 + x1 w1 + x0 w2 + x2 w0),
-// the rest is below 2^-24 |x w|.  The tensor core truncates as it accumulates,
-// so the leading products and the five small ones have accumulators of their
-// own, and every 256 values of k the epilogue warps move both into rounded
-// f32 sums in registers.  An infinite or NaN value is whole in its first part
+// 2^-24 |x| (2^-134 for the smallest), and six of the nine part products are
+// summed in f32:
+//   x w ~ x0 w0 + (x0 w1 + x1 w0 + x1 w1 + x0 w2 + x2 w0).
+// The first two parts are cut and not rounded, so the rest, x1 w2 + x2 w1, has the
+// product's sign: up to 2^-21 |x w|, 0.7 x 2^-24 in the mean over normal values.
+// Sums of 256 to 4,096 terms of one sign come out 6e-8 low, 2.5e-7 off at most (the
+// library's f32 product 1e-6).  Rounded parts cost the loader warps 5 to 15 %
+// (8192 x 4096 x 4096 1.55 ms, 1.48).
+// The tensor core truncates as it accumulates, so the leading products and the
+// five small ones have accumulators of their own, and every 256 values of k the
+// epilogue warps move both into rounded f32 sums in registers.
+// An infinite or NaN value is whole in its first part
 // and its rest is NaN: where the leading sum is not finite it is the result, and
 // the small one is left out.  (An infinity times an f32 below 2^-133, whose
 // first part is zero, gives NaN.)  Such values cost no time: a backward pass of

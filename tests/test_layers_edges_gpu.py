@@ -356,3 +356,38 @@ def test_few_rows_do_not_depend_on_the_outputs_beside_them(rows, dtype):
     size = x.double().abs() @ w.double().abs().t() + b.double().abs()
     bound = unit * ref.abs() + (264 ** 0.5 + 16) * 2.0 ** -22 * size + 2.0 ** -24
     assert bool(((whole.pre_activation.double() - ref).abs() <= bound).all())
+
+
+# --------------------------------------------------- f32 products' last bits
+@pytest.mark.parametrize("inputs", [16, 250, 1000, 4096, 70001])
+def test_f32_products_of_one_sign_keep_all_three_parts(inputs):
+    """Relative to the sum: 2^-21 for the part products that are left out, 16
+    accumulating steps of 2^-23 before sums move to registers, and the roundings
+    there.  Without the third parts a product is 2^-16 low in the mean."""
+    x, w = uniform((300, inputs), F32, 1, 0.5, 1), uniform((72, inputs), F32, 2, 0.5, 1)
+    bound = 2.0 ** -21 + 2.0 ** -19 + (inputs / 256) ** 0.5 * 2.0 ** -24
+    ref = x.double() @ w.double().t()
+    assert float(((ba.linear(x, w).y.double() - ref).abs() / ref).max()) <= bound
+    dy = uniform((300, 72), F32, 3, 0.5, 1)
+    ref = dy.double().t() @ x.double()
+    assert float(((ba.linear_backward(dy, x, w).weight.double() - ref).abs() / ref).max()) <= bound
+
+
+# --------------------------------------------------- one output, many rows
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("inputs,outputs", [(40, 1), (1, 40), (1, 1), (300, 1), (1, 300)])
+def test_backward_of_one_input_or_output_over_many_rows(inputs, outputs, dtype):
+    """A sum of n products in f32 errs by (sqrt(n) + 16) 2^-22 of the terms'
+    magnitudes, 16-bit storage rounds dz and the result once each."""
+    rows = 100003
+    x, w = normal((rows, inputs), dtype, 1), normal((outputs, inputs), dtype, 2)
+    dy, z = normal((rows, outputs), dtype, 3), normal((rows, outputs), dtype, 4)
+    unit = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}[dtype]
+    g = ba.linear_backward(dy, x, w, z, activation=Activation.Relu)
+    dz = dy.double() * (z > 0).double()
+    for got, ref, size, n in (
+            (g.x, dz @ w.double(), dz.abs() @ w.double().abs(), outputs),
+            (g.weight, dz.t() @ x.double(), dz.abs().t() @ x.double().abs(), rows),
+            (g.bias, dz.sum(0), dz.abs().sum(0), rows)):
+        bound = unit * ref.abs() + (n ** 0.5 + 16) * 2.0 ** -22 * size + 2.0 ** -24
+        assert bool(((got.double() - ref).abs() <= bound).all())
