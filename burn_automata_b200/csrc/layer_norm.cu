@@ -30,8 +30,9 @@
 // Measured on one B200, beside a copy's 6.45 TB/s: forward 1048576 x 130 f32
 // 178 us (6.1 TB/s; 194 on inputs that change from call to call); backward with a
 // residual 1048576 x 130 bf16 209 us (5.3 TB/s, instruction issue at 70 %), 16384 x 4096 f16 83 us (4.8 TB/s); the plain
-// loads of unaligned rows reach about a quarter (52529 x 1599 f16, odd pitch:
-// 400 us), bound by their two-byte accesses.
+// loads of unaligned rows reach a quarter to a third (52529 x 1599 f16, odd pitch:
+// forward 173 us, backward 279, with a residual 397), bound by their two-byte
+// accesses.
 #include <algorithm>
 
 #include "layers.h"
@@ -218,8 +219,10 @@ __device__ __forceinline__ void forward_out(Row<VEC, NV>& x, float rstd, const R
 // sum(g) and sum(g xhat) grow.  Values past the row's end are zero in dy, so
 // whatever xhat holds there adds nothing that is stored.  16-bit rows take
 // xhat = x rstd - mean rstd in one step: the rounded product costs 2^-24
-// mean rstd, far below the spacing of the values themselves; f32 rows subtract
-// first.
+// mean rstd, as much as the rounding of the saved mean and far below the spacing
+// of the values themselves (rows of one value far from zero get that in place of
+// zeros; subtracting first would cost 1048576 x 130 bf16 209 us, 191 like this);
+// f32 rows subtract first.
 template <class T, int VEC, int NV>
 __device__ __forceinline__ void backward_sums(Row<VEC, NV>& x, Row<VEC, NV>& g, const Row<VEC, NV>& w,
                                               float mean, float rstd, bool params, Row<VEC, NV>& dw,
@@ -1111,11 +1114,12 @@ npa_status wide_grid(K kernel, const WidePlan& p, int64_t rows, unsigned* grid) 
 template <class T>
 npa_status forward_typed(const LayerNormArgs& a, cudaStream_t s) {
   if (gapless(a.x, a.x_stride, a.rows, a.dims) && gapless(a.y, a.y_stride, a.rows, a.dims)) {
-    // f32 rows of 256 to 576 bytes keep five tiles to a ring, of four rows from 2 KB
-    // on (536 MB of x, us before and with it: 64 values 207, 168; 128 197, 178; 130
-    // 203, 173; 136 204, 165; 144 202, 194; 68 193, 198).  Elsewhere this loses: 32
-    // f32 values 208, 256; 192 186, 194; 64 16-bit values 213, 262; 129, an odd
-    // width, 169, 192.
+    // f32 rows of 256 to 576 bytes keep five tiles to a ring, of four rows from 512
+    // bytes on (536 MB of x in six places each, median us without and with it: 64
+    // values 209, 171; 66 179, 177; 68 194, 198; 72 to 120 the same within 0.5 %; 128
+    // 199, 181; 130 204, 175; 136 205, 168; 144 205, 195).  Elsewhere this loses: 32
+    // f32 values 208, 256; 152 201, 202; 176 194, 201; 192 188, 197; 64 16-bit values
+    // 213, 262; 129, an odd width, 169, 192.
     const size_t row_bytes = size_t(a.dims) * sizeof(T);
     const bool deep = sizeof(T) == 4 && a.dims % 2 == 0 && row_bytes >= 256 && row_bytes <= 576;
     const TilePlan p = plan_tiles(sizeof(T), a.dims, a.rows, 2, deep, [&](int tile_rows) {
